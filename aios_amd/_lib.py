@@ -21,6 +21,8 @@ AIOS_ERR_LAUNCH = 4
 
 PHASE_PREFILL = 0
 PHASE_DECODE = 1
+PHASE_PREFILL8 = 2  # a plan's phase for the 8-bit cache
+PHASE_DECODE8 = 3
 PROLOGUE_NONE = 0
 PROLOGUE_ADD_RMSNORM = 1
 EPILOGUE_NONE = 0
@@ -62,6 +64,15 @@ EXPORTED_SYMBOLS = (
     "aios_sample",
     "aios_sample_workspace",
     "aios_sample_ws",
+    "aios_kv8_append",
+    "aios_qk_norm_rope_append8",
+    "aios_attn_plan8",
+    "aios_attn_prefill8",
+    "aios_attn_decode8",
+    "aios_attn_append_decode8",
+    "aios_attn_append_decode_rope8",
+    "aios_token_logprobs_workspace",
+    "aios_token_logprobs",
 )
 
 
@@ -207,6 +218,40 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.aios_sample_ws.restype = ctypes.c_int
     lib.aios_sample_ws.argtypes = [_vp, _i64, _i32, _i32, _i32, _f32, _i32, _f32, _vp, _i64, _i32,
                                    _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _vp]
+    lib.aios_kv8_append.restype = ctypes.c_int
+    lib.aios_kv8_append.argtypes = [_vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp, _i64,
+                                    _i64, _vp]
+    lib.aios_qk_norm_rope_append8.restype = ctypes.c_int
+    lib.aios_qk_norm_rope_append8.argtypes = [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp,
+                                              _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _f32,
+                                              _vp]
+    lib.aios_attn_plan8.restype = ctypes.c_int
+    lib.aios_attn_plan8.argtypes = lib.aios_attn_plan.argtypes
+    lib.aios_attn_prefill8.restype = ctypes.c_int
+    lib.aios_attn_prefill8.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64,
+        _f32, _vp,
+    ]
+    lib.aios_attn_decode8.restype = ctypes.c_int
+    lib.aios_attn_decode8.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _f32,
+        _vp,
+    ]
+    lib.aios_attn_append_decode8.restype = ctypes.c_int
+    lib.aios_attn_append_decode8.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
+        _vp, _vp, _vp, _i64, _f32, _vp,
+    ]
+    lib.aios_attn_append_decode_rope8.restype = ctypes.c_int
+    lib.aios_attn_append_decode_rope8.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
+        _vp, _vp, _vp, _vp, _vp, _i64, _vp, _f32, _vp, _vp, _i64, _f32, _vp,
+    ]
+    lib.aios_token_logprobs_workspace.restype = _i64
+    lib.aios_token_logprobs_workspace.argtypes = [_i64, _i32, _i32]
+    lib.aios_token_logprobs.restype = ctypes.c_int
+    lib.aios_token_logprobs.argtypes = [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
+                                        _vp, _i64, _vp]
     lib.aios_attnres_mix.restype = ctypes.c_int
     lib.aios_attnres_mix.argtypes = [_vp, _i32, _i64, _i32, _vp, _vp, _f32, _vp, _vp, _vp]
     lib.aios_attnres_mix_ex.restype = ctypes.c_int

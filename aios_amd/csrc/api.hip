@@ -218,10 +218,10 @@ int aios_kv_append(void* k_cache, void* v_cache, int64_t num_slots, int64_t cach
   return check_hip(e, "kv_append launch");
 }
 
-int aios_attn_plan(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
-                   int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
-                   int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
-                   aios_attn_plan_t* p) {
+// The checks and the batch's sizes, common to both caches' plans.
+static int plan_sizes(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
+                      int32_t hq, int32_t hkv, int32_t d, int32_t page_size,
+                      aios_attn_plan_t* p) {
   if (!p) return fail(AIOS_ERR_INVALID, "plan: null plan");
   memset(p, 0, sizeof(*p));
   if (phase != AIOS_PHASE_PREFILL && phase != AIOS_PHASE_DECODE)
@@ -259,16 +259,26 @@ int aios_attn_plan(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int3
   p->max_q_len = max_q;
   p->max_kv_len = max_kv;
   p->min_kv_len = min_kv;
-  const int cus = device_cus();
-
   if (phase == AIOS_PHASE_PREFILL) {
     // 128 MFMA rows per workgroup = q_tile tokens x G heads.
-    const int32_t q_tile = 128 / G;
-    p->prefill_q_tile = q_tile;
-    p->num_q_tiles = max_q > 0 ? cdiv(max_q, q_tile) : 0;
+    p->prefill_q_tile = 128 / G;
+    p->num_q_tiles = max_q > 0 ? cdiv(max_q, p->prefill_q_tile) : 0;
+  }
+  return AIOS_OK;
+}
+
+int aios_attn_plan(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
+                   int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
+                   int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
+                   aios_attn_plan_t* p) {
+  const int rc = plan_sizes(phase, cu_q, cu_k, batch, hq, hkv, d, page_size, p);
+  if (rc) return rc;
+  const int cus = device_cus();
+  if (phase == AIOS_PHASE_PREFILL) {
     plan_prefill_parts(p, cu_q, cu_k, cus, ws_bytes);
     return AIOS_OK;
   }
+  const int32_t G = p->group, max_kv = p->max_kv_len, min_kv = p->min_kv_len;
 
   // ---- decode ----------------------------------------------------------------
   if (shared_prefix < 0 || shared_prefix > min_kv)
@@ -367,6 +377,89 @@ int aios_attn_plan(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int3
     p->ws_parts_o = 0;
     p->ws_parts_lse = align_up((int64_t)batch * hkv * n_parts * G * d * 2, 256);
     p->ws_bytes = p->ws_parts_lse + align_up((int64_t)batch * hkv * n_parts * G * 4, 256);
+  }
+  if (p->ws_bytes > ws_bytes)
+    return fail(AIOS_ERR_WORKSPACE, "plan: workspace of %lld bytes is smaller than the %lld needed",
+                (long long)ws_bytes, (long long)p->ws_bytes);
+  return AIOS_OK;
+}
+
+int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
+                    int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
+                    int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
+                    aios_attn_plan_t* p) {
+  const int rc = plan_sizes(phase, cu_q, cu_k, batch, hq, hkv, d, page_size, p);
+  if (rc) return rc;
+  const int32_t cus = device_cus();
+  p->phase = phase == AIOS_PHASE_PREFILL ? AIOS_PHASE_PREFILL8 : AIOS_PHASE_DECODE8;
+  if (phase == AIOS_PHASE_PREFILL) {
+    plan_prefill_parts(p, cu_q, cu_k, cus, ws_bytes);
+    return AIOS_OK;
+  }
+  if (shared_prefix < 0 || shared_prefix > p->min_kv_len)
+    return fail(AIOS_ERR_INVALID,
+                "plan: shared_prefix_len %d exceeds the shortest row (%d KV positions)",
+                shared_prefix, p->min_kv_len);
+  const int32_t G = p->group, m_rows = batch * G;
+  const bool cascade = shared_prefix > 0 && batch > 1 && m_rows >= 16 &&
+                       (prefix_chunk_len > 0 || shared_prefix >= kMinCascadePrefix);
+  const int32_t P = cascade ? shared_prefix : 0;
+  int32_t chunk = 0, n_chunks = 0, mgroups = 0;
+  if (cascade) {
+    mgroups = cdiv(m_rows, 128);
+    if (prefix_chunk_len > 0) {
+      chunk = (int32_t)align_up(prefix_chunk_len, 32);
+    } else {
+      // About one prefix workgroup per compute unit, in whole staging steps.
+      int32_t want = cdiv(cus, hkv * mgroups);
+      if (want < 1) want = 1;
+      chunk = (int32_t)align_up(cdiv(P, want), 64);
+    }
+    n_chunks = cdiv(P, chunk);
+  }
+  const int32_t max_suffix = p->max_kv_len - P;
+  const int32_t pass = aios::kSuffixPass;
+  int32_t split;
+  if (suffix_split_len > 0) {
+    split = suffix_split_len;
+  } else if (cascade) {
+    split = pass;
+  } else if (max_suffix <= 2 * pass) {
+    split = max_suffix > 0 ? max_suffix : 1;
+  } else {
+    // Rows of their own: about four items per compute unit.
+    const int64_t items = (int64_t)batch * hkv;
+    const int32_t want = (int32_t)((4ll * cus + items - 1) / items);
+    split = (int32_t)align_up(cdiv(max_suffix, want), pass);
+  }
+  int32_t n_splits = max_suffix > 0 ? cdiv(max_suffix, split) : 1;
+  while (n_chunks + n_splits > kMaxParts) {
+    if (n_splits > n_chunks) {
+      split *= 2;
+      n_splits = max_suffix > 0 ? cdiv(max_suffix, split) : 1;
+    } else {
+      chunk = (int32_t)align_up((int64_t)chunk * 2, 32);
+      n_chunks = cdiv(P, chunk);
+    }
+  }
+  const int32_t per_item =
+      (cascade && n_chunks + n_splits * aios::kSuffixWaves <= kMaxParts) ? aios::kSuffixWaves : 1;
+  const int32_t n_parts = n_chunks + n_splits * per_item;
+  p->suffix_parts_per_item = per_item;
+  p->prefix_len = P;
+  p->prefix_chunk_len = chunk;
+  p->num_prefix_chunks = n_chunks;
+  p->cascade_rows = m_rows;
+  p->cascade_mgroups = mgroups;
+  p->suffix_split_len = split;
+  p->num_suffix_splits = n_splits;
+  p->suffix_tpg = pass / 4;
+  p->num_parts = n_parts;
+  if (n_parts > 1) {
+    const int64_t states = (int64_t)batch * hkv * n_parts * G;
+    p->ws_parts_o = 0;
+    p->ws_parts_lse = align_up(states * d * 2, 256);
+    p->ws_bytes = p->ws_parts_lse + align_up(states * 8, 256);
   }
   if (p->ws_bytes > ws_bytes)
     return fail(AIOS_ERR_WORKSPACE, "plan: workspace of %lld bytes is smaller than the %lld needed",
@@ -1180,6 +1273,290 @@ int aios_attnres_mix(const void* bank, int32_t bank_sources, int64_t num_tokens,
                      void* out, void* stream) {
   return aios_attnres_mix_ex(bank, bank_sources, num_tokens, hidden, partial, nullptr, nullptr,
                              weighted_query, eps, scores, out, stream);
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit KV cache
+
+// One layer's cache as the kernels address it: 32-bit byte offsets (a layer's
+// K or V codes below 4 GiB) and 24-bit page ids.
+static int kv8_layer(const char* what, void* k8, void* v8, void* scales, int64_t num_pages,
+                     int32_t hkv, int32_t d, aios::Kv8Layer* c) {
+  if (!k8 || !v8 || !scales) return fail(AIOS_ERR_INVALID, "%s: null pointer", what);
+  if (num_pages < 0 || hkv <= 0) return fail(AIOS_ERR_INVALID, "%s: bad cache sizes", what);
+  if (!aios::head_dim_supported(d))
+    return fail(AIOS_ERR_UNSUPPORTED, "%s: head_dim %d is not built", what, d);
+  if ((((uintptr_t)k8 | (uintptr_t)v8) & 15) != 0 || ((uintptr_t)scales & 3) != 0)
+    return fail(AIOS_ERR_INVALID, "%s: caches must be 16-byte and scales 4-byte aligned", what);
+  if (num_pages >= (1ll << 24) || (int64_t)hkv * d >= (1ll << 24))
+    return fail(AIOS_ERR_UNSUPPORTED, "%s: a pool of %lld pages of %lld codes exceeds the 2^24 - 1 "
+                "the kernels address", what, (long long)num_pages, (long long)hkv * d);
+  if (num_pages * (int64_t)hkv * d > 0xffff0000ll)
+    return fail(AIOS_ERR_UNSUPPORTED,
+                "%s: per-layer 8-bit cache of %lld bytes exceeds the 4 GiB the kernels address",
+                what, (long long)(num_pages * (int64_t)hkv * d));
+  *c = aios::Kv8Layer{static_cast<uint8_t*>(k8), static_cast<uint8_t*>(v8),
+                      static_cast<uint32_t*>(scales), num_pages, hkv * d};
+  return AIOS_OK;
+}
+
+int aios_kv8_append(void* k8, void* v8, void* scales, int64_t num_pages, int32_t num_kv_heads,
+                    int32_t head_dim, const int32_t* out_loc, const void* k, int64_t k_tok_stride,
+                    const void* v, int64_t v_tok_stride, int64_t n_tokens, void* stream) {
+  if (n_tokens < 0) return fail(AIOS_ERR_INVALID, "kv8_append: negative token count");
+  aios::Kv8Layer c;
+  int rc = kv8_layer("kv8_append", k8, v8, scales, num_pages, num_kv_heads, head_dim, &c);
+  if (rc) return rc;
+  if (n_tokens == 0) return AIOS_OK;
+  if (!out_loc || !k || !v) return fail(AIOS_ERR_INVALID, "kv8_append: null pointer");
+  if (k_tok_stride < c.tok_bytes || v_tok_stride < c.tok_bytes ||
+      ((k_tok_stride | v_tok_stride) & 1) != 0)
+    return fail(AIOS_ERR_INVALID, "kv8_append: K/V token strides must be >= Hkv*D and even");
+  if ((((uintptr_t)k | (uintptr_t)v) & 3) != 0)
+    return fail(AIOS_ERR_INVALID, "kv8_append: K/V rows must be 4-byte aligned");
+  if (n_tokens * num_kv_heads > (0x7fffffffll * 16))
+    return fail(AIOS_ERR_UNSUPPORTED, "kv8_append: too many rows");
+  return check_hip(aios::kv8_append(c, head_dim, out_loc, k, k_tok_stride, v, v_tok_stride,
+                                    n_tokens, static_cast<hipStream_t>(stream)),
+                   "kv8_append launch");
+}
+
+int aios_qk_norm_rope_append8(const void* qkv, int64_t qkv_stride, int64_t tokens,
+                              int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                              const void* q_weight, const void* k_weight, const float* cos_table,
+                              const float* sin_table, int64_t table_rows,
+                              const int32_t* positions, void* q_out, void* k8, void* v8,
+                              void* scales, int64_t num_pages, const int32_t* out_loc, float eps,
+                              void* stream) {
+  if (tokens < 0 || num_qo_heads <= 0 || num_kv_heads <= 0 || table_rows <= 0)
+    return fail(AIOS_ERR_INVALID, "qk_norm_rope_append8: bad sizes");
+  aios::Kv8Layer c;
+  int rc = kv8_layer("qk_norm_rope_append8", k8, v8, scales, num_pages, num_kv_heads, head_dim, &c);
+  if (rc) return rc;
+  if (qkv_stride < (int64_t)(num_qo_heads + 2 * num_kv_heads) * head_dim || qkv_stride % 2 != 0)
+    return fail(AIOS_ERR_INVALID, "qk_norm_rope_append8: qkv row stride too small");
+  if (tokens == 0) return AIOS_OK;
+  if (tokens > 0x7fffffffll) return fail(AIOS_ERR_UNSUPPORTED, "qk_norm_rope_append8: too many rows");
+  if (!qkv || !q_weight || !k_weight || !cos_table || !sin_table || !positions || !q_out || !out_loc)
+    return fail(AIOS_ERR_INVALID, "qk_norm_rope_append8: null pointer");
+  if ((((uintptr_t)qkv | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)q_out) & 3) != 0)
+    return fail(AIOS_ERR_INVALID, "qk_norm_rope_append8: rows must be 4-byte aligned");
+  return check_hip(aios::qk_norm_rope_append8(qkv, qkv_stride, tokens, num_qo_heads, num_kv_heads,
+                                              head_dim, q_weight, k_weight, cos_table, sin_table,
+                                              table_rows, positions, q_out, c, out_loc, eps,
+                                              static_cast<hipStream_t>(stream)),
+                   "qk_norm_rope_append8 launch");
+}
+
+int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                       const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                       const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k, void* out,
+                       void* workspace, int64_t workspace_bytes, float sm_scale, void* stream) {
+  int rc = check_plan(p, AIOS_PHASE_PREFILL8);
+  if (rc) return rc;
+  if (p->batch_size == 0 || p->total_q == 0) return AIOS_OK;
+  const int D = p->head_dim;
+  if (q_tok_stride < (int64_t)p->num_qo_heads * D || (q_tok_stride % 8) != 0)
+    return fail(AIOS_ERR_INVALID, "prefill8: q token stride %lld must be >= Hq*D and a multiple of 8",
+                (long long)q_tok_stride);
+  if (!q || !indices || !cu_q || !cu_k || !out)
+    return fail(AIOS_ERR_INVALID, "prefill8: null pointer");
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0)
+    return fail(AIOS_ERR_INVALID, "prefill8: q and out must be 16-byte aligned");
+  aios::Kv8Layer c;
+  rc = kv8_layer("prefill8", const_cast<void*>(k8), const_cast<void*>(v8),
+                 const_cast<void*>(scales), num_pages, p->num_kv_heads, D, &c);
+  if (rc) return rc;
+  aios::PrefillArgs a = {};
+  a.q = static_cast<const aios::bf16*>(q);
+  a.q_tok_stride = q_tok_stride;
+  a.indices = indices;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.num_qo_heads = p->num_qo_heads;
+  a.num_kv_heads = p->num_kv_heads;
+  a.group = p->group;
+  a.scale_log2 = sm_scale * aios::kLog2e;
+  a.q_tile = p->prefill_q_tile;
+  a.q_tiles = p->num_q_tiles;
+  a.batch = p->batch_size;
+  a.out = static_cast<aios::bf16*>(out);
+  if (p->num_parts > 1 && workspace && ((uintptr_t)workspace & 255) == 0 &&
+      p->ws_bytes <= workspace_bytes) {
+    char* ws = static_cast<char*>(workspace);
+    a.part_sub = p->prefix_chunk_len / 32;
+    a.n_parts = p->num_parts;
+    a.part_o = reinterpret_cast<float*>(ws + p->ws_parts_o);
+    a.part_ml = reinterpret_cast<float2*>(ws + p->ws_parts_lse);
+    a.part_rows = (p->max_q_len < a.q_tile ? p->max_q_len : a.q_tile) * a.group;
+    return check_hip(aios::launch_prefill8_split(D, a, c, static_cast<hipStream_t>(stream)),
+                     "prefill8 launch");
+  }
+  return check_hip(aios::launch_prefill8(D, a, c, static_cast<hipStream_t>(stream)),
+                   "prefill8 launch");
+}
+
+static int decode8_impl(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride, void* k8,
+                        void* v8, void* scales, int64_t num_pages, const int32_t* indices,
+                        const int32_t* cu_k, void* out, void* workspace, int64_t workspace_bytes,
+                        float sm_scale, void* stream, const NewKV* nk, const QkRopeIn* ro) {
+  int rc = check_plan(p, AIOS_PHASE_DECODE8);
+  if (rc) return rc;
+  if (p->batch_size == 0) return AIOS_OK;
+  const int D = p->head_dim;
+  if (q_tok_stride < (int64_t)p->num_qo_heads * D || (q_tok_stride % 8) != 0)
+    return fail(AIOS_ERR_INVALID, "decode8: q token stride %lld must be >= Hq*D and a multiple of 8",
+                (long long)q_tok_stride);
+  if (p->ws_bytes > workspace_bytes || (p->ws_bytes > 0 && !workspace))
+    return fail(AIOS_ERR_WORKSPACE, "decode8: workspace of %lld bytes is smaller than the %lld needed",
+                (long long)workspace_bytes, (long long)p->ws_bytes);
+  if (((uintptr_t)workspace & 255) != 0)
+    return fail(AIOS_ERR_INVALID, "decode8: workspace must be 256-byte aligned");
+  if (!q || !indices || !cu_k || !out) return fail(AIOS_ERR_INVALID, "decode8: null pointer");
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0)
+    return fail(AIOS_ERR_INVALID, "decode8: q and out must be 16-byte aligned");
+  aios::Decode8Args a = {};
+  if ((rc = kv8_layer("decode8", k8, v8, scales, num_pages, p->num_kv_heads, D, &a.kv))) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const int32_t mask = p->stage_mask == 0 ? 3 : p->stage_mask;
+  a.q = static_cast<const aios::bf16*>(q);
+  a.q_tok_stride = q_tok_stride;
+  a.indices = indices;
+  a.cu_k = cu_k;
+  a.batch = p->batch_size;
+  a.num_qo_heads = p->num_qo_heads;
+  a.num_kv_heads = p->num_kv_heads;
+  a.group = p->group;
+  a.scale_log2 = sm_scale * aios::kLog2e;
+  a.prefix_len = p->prefix_len;
+  a.chunk_len = p->prefix_chunk_len;
+  a.n_chunks = p->num_prefix_chunks;
+  a.m_rows = p->cascade_rows;
+  a.prefix_units = p->num_prefix_chunks * p->num_kv_heads;
+  a.prefix_wgs = a.prefix_units * (p->cascade_mgroups > 0 ? p->cascade_mgroups : 1);
+  a.split_len = p->suffix_split_len;
+  a.n_splits = p->num_suffix_splits;
+  a.suffix_items = p->batch_size * p->num_kv_heads * p->num_suffix_splits;
+  a.final_out = p->num_parts == 1 ? 1 : 0;
+  a.wave_parts = p->suffix_parts_per_item > 1 ? 1 : 0;
+  a.parts.o = reinterpret_cast<_Float16*>(ws + p->ws_parts_o);
+  a.parts.ls = reinterpret_cast<float2*>(ws + p->ws_parts_lse);
+  a.parts.n_parts = p->num_parts;
+  a.parts.n_chunks = p->num_prefix_chunks;
+  a.parts.rows = p->batch_size * p->group;
+  a.out = static_cast<aios::bf16*>(out);
+  if (nk) {
+    if (!nk->k || !nk->v || !nk->out_loc)
+      return fail(AIOS_ERR_INVALID, "append_decode8: null pointer");
+    if (nk->k_stride < a.kv.tok_bytes || nk->v_stride < a.kv.tok_bytes ||
+        ((nk->k_stride | nk->v_stride) & 1) != 0)
+      return fail(AIOS_ERR_INVALID, "append_decode8: K/V token strides must be >= Hkv*D and even");
+    if ((((uintptr_t)nk->k | (uintptr_t)nk->v) & 3) != 0)
+      return fail(AIOS_ERR_INVALID, "append_decode8: K/V rows must be 4-byte aligned");
+    if (p->min_kv_len < 1 || p->prefix_len >= p->min_kv_len)
+      return fail(AIOS_ERR_INVALID,
+                  "append_decode8: every row's new token must lie after the shared prefix");
+    a.k_new = static_cast<const aios::bf16*>(nk->k);
+    a.v_new = static_cast<const aios::bf16*>(nk->v);
+    a.k_new_stride = nk->k_stride;
+    a.v_new_stride = nk->v_stride;
+    a.out_loc = nk->out_loc;
+  }
+  if (ro) {
+    if (!ro->q_norm || !ro->k_norm || !ro->cos || !ro->sin || !ro->positions)
+      return fail(AIOS_ERR_INVALID, "append_decode_rope8: null pointer");
+    if (ro->rows < 1) return fail(AIOS_ERR_INVALID, "append_decode_rope8: empty rotation table");
+    if ((((uintptr_t)ro->q_norm | (uintptr_t)ro->k_norm | (uintptr_t)ro->cos |
+          (uintptr_t)ro->sin) & 15) != 0)
+      return fail(AIOS_ERR_INVALID,
+                  "append_decode_rope8: norm weights and tables must be 16-byte aligned");
+    a.q_norm = static_cast<const aios::bf16*>(ro->q_norm);
+    a.k_norm = static_cast<const aios::bf16*>(ro->k_norm);
+    a.rope_cos = static_cast<const aios::bf16*>(ro->cos);
+    a.rope_sin = static_cast<const aios::bf16*>(ro->sin);
+    a.rope_rows = ro->rows;
+    a.positions = ro->positions;
+    a.norm_eps = ro->eps;
+  }
+  if (mask & 1) {
+    rc = check_hip(aios::launch_decode8_main(D, a, s), "decode8 launch");
+    if (rc) return rc;
+  }
+  if (p->num_parts > 1 && (mask & 2))
+    return check_hip(aios::launch_decode8_combine(D, a, s), "decode8 combine launch");
+  return AIOS_OK;
+}
+
+int aios_attn_decode8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                      const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                      const int32_t* indices, const int32_t* cu_k, void* out, void* workspace,
+                      int64_t workspace_bytes, float sm_scale, void* stream) {
+  return decode8_impl(p, q, q_tok_stride, const_cast<void*>(k8), const_cast<void*>(v8),
+                      const_cast<void*>(scales), num_pages, indices, cu_k, out, workspace,
+                      workspace_bytes, sm_scale, stream, nullptr, nullptr);
+}
+
+int aios_attn_append_decode8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                             const void* k_new, int64_t k_tok_stride, const void* v_new,
+                             int64_t v_tok_stride, const int32_t* out_loc, void* k8, void* v8,
+                             void* scales, int64_t num_pages, const int32_t* indices,
+                             const int32_t* cu_k, void* out, void* workspace,
+                             int64_t workspace_bytes, float sm_scale, void* stream) {
+  const NewKV nk = {k_new, k_tok_stride, v_new, v_tok_stride, out_loc};
+  return decode8_impl(p, q, q_tok_stride, k8, v8, scales, num_pages, indices, cu_k, out, workspace,
+                      workspace_bytes, sm_scale, stream, &nk, nullptr);
+}
+
+int aios_attn_append_decode_rope8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                                  const void* k_new, int64_t k_tok_stride, const void* v_new,
+                                  int64_t v_tok_stride, const int32_t* out_loc, void* k8, void* v8,
+                                  void* scales, int64_t num_pages, const int32_t* indices,
+                                  const int32_t* cu_k, const void* q_norm, const void* k_norm,
+                                  const void* rope_cos, const void* rope_sin, int64_t rope_rows,
+                                  const int32_t* positions, float norm_eps, void* out,
+                                  void* workspace, int64_t workspace_bytes, float sm_scale,
+                                  void* stream) {
+  const NewKV nk = {k_new, k_tok_stride, v_new, v_tok_stride, out_loc};
+  const QkRopeIn ro = {q_norm, k_norm, rope_cos, rope_sin, rope_rows, positions, norm_eps};
+  return decode8_impl(p, q, q_tok_stride, k8, v8, scales, num_pages, indices, cu_k, out, workspace,
+                      workspace_bytes, sm_scale, stream, &nk, &ro);
+}
+
+// ---------------------------------------------------------------------------
+// scoring
+
+int64_t aios_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {
+  if (rows <= 0 || vocab <= 0 || top < 0 || top > aios::kLogprobMaxTop) return 0;
+  return aios::logprob_workspace(rows, aios::logprob_segments(rows, vocab, device_cus()), top);
+}
+
+int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab,
+                        int32_t elem_bytes, const int64_t* tokens, int32_t top, float* logprobs,
+                        float* entropies, int64_t* top_ids, float* top_logprobs, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (rows < 0 || vocab <= 0) return fail(AIOS_ERR_INVALID, "token_logprobs: bad sizes");
+  if (elem_bytes != 2 && elem_bytes != 4)
+    return fail(AIOS_ERR_UNSUPPORTED, "token_logprobs: logits must be bf16 or fp32");
+  if (row_stride < 0 || (row_stride > 0 && row_stride < vocab))
+    return fail(AIOS_ERR_INVALID, "token_logprobs: row stride smaller than the vocabulary");
+  if (top < 0 || top > vocab) return fail(AIOS_ERR_INVALID, "token_logprobs: top must be within 0..vocab");
+  if (top > aios::kLogprobMaxTop)
+    return fail(AIOS_ERR_UNSUPPORTED, "token_logprobs: at most %d alternatives", aios::kLogprobMaxTop);
+  if (rows == 0) return AIOS_OK;
+  if (!logits || !tokens || !logprobs || !entropies || (top > 0 && (!top_ids || !top_logprobs)))
+    return fail(AIOS_ERR_INVALID, "token_logprobs: null pointer");
+  if (((uintptr_t)logits & (uintptr_t)(elem_bytes - 1)) != 0)
+    return fail(AIOS_ERR_INVALID, "token_logprobs: misaligned logits");
+  if (rows > (1ll << 24)) return fail(AIOS_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  const aios::LogprobArgs a = {logits,   row_stride, rows,      vocab,   elem_bytes,  tokens,
+                               top,      logprobs,   entropies, top_ids, top_logprobs};
+  int32_t seg = aios::logprob_segments(rows, vocab, device_cus());
+  if (!workspace || ((uintptr_t)workspace & 15) != 0 ||
+      workspace_bytes < aios::logprob_workspace(rows, seg, top))
+    seg = 1;
+  return check_hip(aios::token_logprobs(a, seg, workspace, static_cast<hipStream_t>(stream)),
+                   "token_logprobs launch");
 }
 
 }  // extern "C"

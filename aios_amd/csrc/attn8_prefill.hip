@@ -1,0 +1,249 @@
+// Varlen causal prefill and extension over the 8-bit KV cache: the tiles,
+// order and KV split of attn_prefill.hip on the staging of engine8.hpp.
+#include "engine8.hpp"
+
+namespace aios {
+namespace {
+
+// bf16 output row from the lane's half of o.
+template <int D>
+__device__ __forceinline__ void store_row(const TileEngine32<D, true>& eng, float inv, bf16* row) {
+  bf16* po = row + 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+  for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint2 packed;
+      packed.x = pack_bf16x2(eng.o[nt][4 * j] * inv, eng.o[nt][4 * j + 1] * inv);
+      packed.y = pack_bf16x2(eng.o[nt][4 * j + 2] * inv, eng.o[nt][4 * j + 3] * inv);
+      *reinterpret_cast<uint2*>(po + nt * 32 + 8 * j) = packed;
+    }
+}
+
+__device__ __forceinline__ float inv_or_zero(float l) { return l > 0.f ? 1.f / l : l * 0.f; }
+
+template <int D>
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(PrefillArgs a, Kv8Layer kv) {
+  __shared__ __align__(16) uint8_t lds[Stage8<D>::LDS_BYTES];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int G = a.group;
+  const int flat = blockIdx.x;
+  const int h = flat % a.num_kv_heads;
+  const int rest = flat / a.num_kv_heads;
+  const int r = rest % a.batch;
+  const int qt = a.q_tiles - 1 - rest / a.batch;
+  const int q_start = a.cu_q[r];
+  const int q_len = a.cu_q[r + 1] - q_start;
+  if (qt * a.q_tile >= q_len) return;
+  const int kv_base = a.cu_k[r];
+  const int kv_len = a.cu_k[r + 1] - kv_base;
+  const int cached = kv_len - q_len;
+  const int q_hi = min(q_len, (qt + 1) * a.q_tile);
+
+  TileEngine32<D, true> eng;
+  const int m = wave * 32 + (lane & 31);
+  const int i = qt * a.q_tile + m / G;
+  const int g = m - (m / G) * G;
+  const bool ok = (m < a.q_tile * G) && (i < q_len);
+  const bf16* qr = a.q + (int64_t)(q_start + i) * a.q_tok_stride + (int64_t)(h * G + g) * D;
+  const int64_t out_off = ((int64_t)(q_start + i) * a.num_qo_heads + (h * G + g)) * D;
+  eng.limit = cached + i;
+  eng.min_limit = cached + qt * a.q_tile;
+  const int m0 = wave * 32;
+  const bool active = m0 < a.q_tile * G && qt * a.q_tile + m0 / G < q_len;
+  run_tile8<D, true>(eng, lds, kv, h, a.indices + kv_base, 0, min(kv_len, cached + q_hi),
+                     a.scale_log2, [&] { eng.load_q(qr, ok); }, active);
+  if (ok) store_row<D>(eng, inv_or_zero(eng.l_run), a.out + out_off);
+}
+
+// The parts of a tile of `rows` MFMA rows over kv positions (prefill_parts):
+// one, written directly, where it has more rows than the plan gave its parts
+// room for.
+__device__ __forceinline__ PrefillParts tile_parts8(const PrefillArgs& a, int rows, int kv) {
+  return prefill_parts(kv, a.part_sub, rows <= a.part_rows ? a.n_parts : 1);
+}
+
+template <int D>
+__device__ __forceinline__ int64_t part_o8(const PrefillArgs& a, int64_t part, int dg, int m) {
+  return ((part * (D / 8) + dg) * a.part_rows + m) * 8;
+}
+
+// One part of a tile's KV range per workgroup (prefill_split_kernel's scheme:
+// tiles of at most 64 rows share a part's sub-tiles over their wavefronts).
+template <int D>
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_split_kernel(PrefillArgs a, Kv8Layer kv) {
+  using S = Stage8<D>;
+  using T = typename S::T;
+  constexpr int kMl = 4 * 32 * 8;  // (m, l) of the four wavefronts' rows
+  __shared__ __align__(16) uint8_t lds[S::LDS_BYTES + kMl];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.group;
+  const int flat = blockIdx.x;
+  const int h = flat % a.num_kv_heads;
+  int rest = flat / a.num_kv_heads;
+  const int r = rest % a.batch;
+  rest /= a.batch;
+  const int qt = a.q_tiles - 1 - rest % a.q_tiles;
+  const int s = rest / a.q_tiles;
+  const int q_start = a.cu_q[r];
+  const int q_len = a.cu_q[r + 1] - q_start;
+  if (qt * a.q_tile >= q_len) return;
+  const int kv_base = a.cu_k[r];
+  const int kv_len = a.cu_k[r + 1] - kv_base;
+  const int cached = kv_len - q_len;
+  const int q_hi = min(q_len, (qt + 1) * a.q_tile);
+  const int kv_hi = min(kv_len, cached + q_hi);
+  const int rows = (q_hi - qt * a.q_tile) * G;
+  const PrefillParts pp = tile_parts8(a, rows, kv_hi);
+  if (s >= pp.n) return;
+  const int kv_begin = s * pp.per * kSubTok;
+  const int kv_end = min(kv_hi, kv_begin + pp.per * kSubTok);
+
+  const int nr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int rt = wave & (nr - 1);
+  const int share = nr == 4 ? 0 : nr == 2 ? wave >> 1 : wave;
+  const int m = rt * 32 + (lane & 31);
+  const int i = qt * a.q_tile + m / G;
+  const int g = m - (m / G) * G;
+  const bool ok = m < rows;
+  const int hl = lane >> 5;
+  const bf16* qr = a.q + (int64_t)(q_start + i) * a.q_tok_stride + (int64_t)(h * G + g) * D;
+
+  TileEngine32<D, true> eng;
+  eng.limit = cached + i;
+  eng.min_limit = cached + qt * a.q_tile;
+  const int64_t slot = ((int64_t)r * a.q_tiles + qt) * a.num_kv_heads + h;
+  const int64_t part = slot * a.n_parts + s;
+  bf16* out_row = a.out + ((int64_t)(q_start + i) * a.num_qo_heads + (h * G + g)) * D;
+
+  if (nr == 4) {
+    run_tile8<D, true>(eng, lds, kv, h, a.indices + kv_base, kv_begin, kv_end, a.scale_log2,
+                       [&] { eng.load_q(qr, ok); }, rt * 32 < rows);
+    if (!ok) return;
+    if (pp.n == 1) {
+      store_row<D>(eng, inv_or_zero(eng.l_run), out_row);
+      return;
+    }
+#pragma unroll
+    for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(a.part_o + part_o8<D>(a, part, nt * 4 + j, m) + 4 * hl) =
+            f32x4{eng.o[nt][4 * j], eng.o[nt][4 * j + 1], eng.o[nt][4 * j + 2],
+                  eng.o[nt][4 * j + 3]};
+    if (hl == 0) a.part_ml[part * a.part_rows + m] = make_float2(eng.m_run, eng.l_run);
+    return;
+  }
+
+  // Few rows: the wavefronts share the two sub-tiles of every step.  With one
+  // row tile the second pair of wavefronts takes the odd steps.
+  eng.reset();
+  const auto lo = eng.lane_offsets(lds);
+  S st(kv, h, a.indices + kv_base, kv_begin, kv_end);
+  const int n = st.steps();
+  if (n <= 2) {
+    // (the usual part: both steps staged, then one barrier)
+    typename S::Regs r0, r1;
+    typename S::Ids i0, i1;
+    st.ids(0, i0);
+    st.ids(1, i1);
+    st.load(0, i0, r0);
+    st.load(1, i1, r1);
+    eng.load_q(qr, ok);
+    st.store(lds, 0, r0);
+    st.store(lds, 1, r1);
+    lds_barrier();
+    const int n_sub = (kv_end - kv_begin + kSubTok - 1) / kSubTok;
+    for (int it = share; it < n_sub; it += 4 / nr)
+      eng.compute_at(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
+                     a.scale_log2);
+  } else {
+    // (more KV positions than the plan was built for)
+    st.stream(lds, [&] { eng.load_q(qr, ok); },
+              [&](uint32_t sb, int kv0) {
+                if (share == 0) eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
+              },
+              true);
+  }
+
+  static_assert(T::SUB_BYTES == 32 * D * 4, "a row tile's fp32 o fills one sub-tile");
+  lds_barrier();  // every wavefront is done with K/V
+  float* so = reinterpret_cast<float*>(lds + wave * T::SUB_BYTES);
+  float2* sml = reinterpret_cast<float2*>(lds + S::LDS_BYTES);  // [wave][32]
+#pragma unroll
+  for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4*>(so + ((nt * 4 + j) * 32 + (lane & 31)) * 8 + 4 * hl) =
+          f32x4{eng.o[nt][4 * j], eng.o[nt][4 * j + 1], eng.o[nt][4 * j + 2], eng.o[nt][4 * j + 3]};
+  if (hl == 0) sml[wave * 32 + (lane & 31)] = make_float2(eng.m_run, eng.ol[0]);
+  __syncthreads();
+  const int nrow = nr * 32;
+  for (int e = threadIdx.x; e < nrow * (D / 8); e += kEngineThreads) {
+    const int dg = e / nrow;
+    const int row = e - dg * nrow;
+    if (row >= rows) continue;
+    const int w0 = row >> 5;  // the row tile; its shares are wavefronts w0 + k * nr
+    float mx = kNegInf;
+    for (int w = w0; w < 4; w += nr) mx = vmax(mx, sml[w * 32 + (row & 31)].x);
+    const float mu = mx == kNegInf ? 0.f : mx;
+    f32x4 acc0 = f32x4{0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
+    float l = 0.f;
+    for (int w = w0; w < 4; w += nr) {
+      const float2 ml = sml[w * 32 + (row & 31)];
+      const float f = fast_exp2(ml.x - mu);
+      l += ml.y * f;
+      const f32x4* po = reinterpret_cast<const f32x4*>(lds + w * T::SUB_BYTES) +
+                        (dg * 32 + (row & 31)) * 2;
+      acc0 += po[0] * f;
+      acc1 += po[1] * f;
+    }
+    if (pp.n == 1) {
+      const float inv = inv_or_zero(l);
+      acc0 *= inv;
+      acc1 *= inv;
+      const int qi = q_start + qt * a.q_tile + row / G;
+      bf16* po = a.out + ((int64_t)qi * a.num_qo_heads + h * G + row % G) * D + dg * 8;
+      *reinterpret_cast<uint4*>(po) =
+          make_uint4(pack_bf16x2(acc0[0], acc0[1]), pack_bf16x2(acc0[2], acc0[3]),
+                     pack_bf16x2(acc1[0], acc1[1]), pack_bf16x2(acc1[2], acc1[3]));
+    } else {
+      f32x4* po = reinterpret_cast<f32x4*>(a.part_o + part_o8<D>(a, part, dg, row));
+      po[0] = acc0;
+      po[1] = acc1;
+      if (dg == 0) a.part_ml[part * a.part_rows + row] = make_float2(mx, l);
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+  const dim3 grid(a.q_tiles * a.num_kv_heads * a.batch), block(kEngineThreads);
+  if (grid.x == 0) return hipSuccess;
+  switch (D) {
+    case 64: hipLaunchKernelGGL(prefill8_kernel<64>, grid, block, 0, s, a, kv); break;
+    case 96: hipLaunchKernelGGL(prefill8_kernel<96>, grid, block, 0, s, a, kv); break;
+    case 128: hipLaunchKernelGGL(prefill8_kernel<128>, grid, block, 0, s, a, kv); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_prefill8_split(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+  const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
+  if (tiles == 0) return hipSuccess;
+  const dim3 grid(tiles * a.n_parts), block(kEngineThreads);
+  switch (D) {
+    case 64: hipLaunchKernelGGL(prefill8_split_kernel<64>, grid, block, 0, s, a, kv); break;
+    case 96: hipLaunchKernelGGL(prefill8_split_kernel<96>, grid, block, 0, s, a, kv); break;
+    case 128: hipLaunchKernelGGL(prefill8_split_kernel<128>, grid, block, 0, s, a, kv); break;
+    default: return hipErrorInvalidValue;
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? launch_prefill_combine(D, a, s) : e;
+}
+
+}  // namespace aios

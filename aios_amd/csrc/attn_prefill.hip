@@ -360,21 +360,35 @@ __global__ __launch_bounds__(NW * 64) void prefill_combine_kernel(PrefillArgs a,
 }
 
 template <int D>
-static hipError_t launch_split_d(const PrefillArgs& a, hipStream_t s) {
-  const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
-  if (tiles == 0) return hipSuccess;
-  hipLaunchKernelGGL(prefill_split_kernel<D>, dim3(tiles * a.n_parts), dim3(kEngineThreads), 0, s,
-                     a);
+static hipError_t launch_combine_d(const PrefillArgs& a, hipStream_t s) {
   if (a.n_parts > 1) {
     constexpr int RB = 64 / (D / 8);
     const int row_blocks = (a.part_rows + RB - 1) / RB;
-    const dim3 grid(tiles * row_blocks);
+    const dim3 grid(a.q_tiles * a.num_kv_heads * a.batch * row_blocks);
     if (a.n_parts <= 4)
       hipLaunchKernelGGL((prefill_combine_kernel<D, 1, 4>), grid, dim3(64), 0, s, a, row_blocks);
     else
       hipLaunchKernelGGL((prefill_combine_kernel<D, 4, 8>), grid, dim3(256), 0, s, a, row_blocks);
   }
   return hipGetLastError();
+}
+
+hipError_t launch_prefill_combine(int D, const PrefillArgs& a, hipStream_t s) {
+  switch (D) {
+    case 64: return launch_combine_d<64>(a, s);
+    case 96: return launch_combine_d<96>(a, s);
+    case 128: return launch_combine_d<128>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+template <int D>
+static hipError_t launch_split_d(const PrefillArgs& a, hipStream_t s) {
+  const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
+  if (tiles == 0) return hipSuccess;
+  hipLaunchKernelGGL(prefill_split_kernel<D>, dim3(tiles * a.n_parts), dim3(kEngineThreads), 0, s,
+                     a);
+  return launch_combine_d<D>(a, s);
 }
 
 hipError_t launch_prefill_split(int D, const PrefillArgs& a, hipStream_t s) {

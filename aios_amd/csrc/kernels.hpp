@@ -309,4 +309,119 @@ hipError_t launch_prefill_split(int D, const PrefillArgs& a, hipStream_t stream)
 bool head_dim_supported(int D);
 bool group_supported(int G);
 
+// ---------------------------------------------------------------------------
+// The 8-bit KV cache.  One layer: k, v [num_pages][hkv][D] e4m3 codes and
+// scales [hkv][num_pages] records, K's scale (bf16 bits) in the low half and
+// V's in the high half; a value of the cache is code * scale.
+struct Kv8Layer {
+  uint8_t* k;
+  uint8_t* v;
+  uint32_t* scales;
+  int64_t num_pages;
+  int32_t tok_bytes;  // hkv * D
+};
+
+// K / V rows (bf16, element token strides) quantised into pages out_loc[t];
+// entries outside the pool are skipped.
+hipError_t kv8_append(const Kv8Layer& c, int D, const int32_t* out_loc, const void* k,
+                      int64_t k_stride, const void* v, int64_t v_stride, int64_t n_tokens,
+                      hipStream_t stream);
+// qk_norm_rope_append with that cache.
+hipError_t qk_norm_rope_append8(const void* qkv, int64_t stride, int64_t tokens, int hq, int hkv,
+                                int D, const void* qw, const void* kw, const float* cos_t,
+                                const float* sin_t, int64_t table_rows, const int32_t* positions,
+                                void* q_out, const Kv8Layer& c, const int32_t* out_loc, float eps,
+                                hipStream_t stream);
+
+// Partial states of a decode batch over the 8-bit cache, as PartsArgs with o
+// as fp16 times a power of two of the row's own (the values then lie in
+// [-4, 4), where fp16 has 10 fraction bits: bf16 partial states alone would
+// add as much error as the final rounding) and ls = (lse, that power's
+// inverse).
+struct Parts8 {
+  _Float16* o;
+  float2* ls;
+  int32_t n_parts;
+  int32_t n_chunks;
+  int32_t rows;  // batch * G
+
+  __host__ __device__ int64_t o_index(int D, int h, int j, int m, int d) const {
+    return ((((int64_t)h * n_parts + j) * (D >> 4) + (d >> 4)) * rows + m) * 16 + (d & 15);
+  }
+  __host__ __device__ int64_t ls_index(int h, int j, int m) const {
+    return ((int64_t)h * n_parts + j) * rows + m;
+  }
+};
+
+struct Decode8Args {
+  const bf16* q;
+  int64_t q_tok_stride;
+  Kv8Layer kv;
+  const int32_t* indices;
+  const int32_t* cu_k;
+  int32_t batch;
+  int32_t num_qo_heads;
+  int32_t num_kv_heads;
+  int32_t group;
+  float scale_log2;
+  // shared prefix: chunks x kv-heads x groups of 128 query rows
+  int32_t prefix_len;
+  int32_t chunk_len;
+  int32_t n_chunks;
+  int32_t m_rows;
+  int32_t prefix_units;
+  int32_t prefix_wgs;
+  // the rows' own positions: (row, kv-head, split) items
+  int32_t split_len;
+  int32_t n_splits;
+  int32_t suffix_items;
+  int32_t final_out;   // 1: one part per (row, head): bf16 output directly
+  int32_t wave_parts;  // 1: each wavefront of an item writes its own part
+  Parts8 parts;
+  bf16* out;
+  const bf16* k_new;  // null: no fused append
+  const bf16* v_new;
+  int64_t k_new_stride;
+  int64_t v_new_stride;
+  const int32_t* out_loc;
+  const bf16* q_norm;  // null: q and k_new are final
+  const bf16* k_norm;
+  const bf16* rope_cos;
+  const bf16* rope_sin;
+  int64_t rope_rows;
+  const int32_t* positions;
+  float norm_eps;
+};
+hipError_t launch_decode8_main(int D, const Decode8Args& a, hipStream_t stream);
+hipError_t launch_decode8_combine(int D, const Decode8Args& a, hipStream_t stream);
+
+// Prefill over the 8-bit cache (the bf16 cache fields of p are not read).
+hipError_t launch_prefill8(int D, const PrefillArgs& p, const Kv8Layer& kv, hipStream_t stream);
+// The same with each tile's KV range split (p.part_sub > 0), merged by
+// launch_prefill_combine.
+hipError_t launch_prefill8_split(int D, const PrefillArgs& p, const Kv8Layer& kv,
+                                 hipStream_t stream);
+hipError_t launch_prefill_combine(int D, const PrefillArgs& a, hipStream_t stream);
+
+// Log probabilities of given tokens over rows of logits (logprobs.hip).
+struct LogprobArgs {
+  const void* logits;
+  int64_t row_stride;  // elements
+  int64_t rows;
+  int32_t vocab;
+  int32_t elem_bytes;  // 2: bf16, 4: fp32
+  const int64_t* tokens;
+  int32_t top;         // alternatives per row
+  float* logprobs;     // [rows]
+  float* entropies;    // [rows]
+  int64_t* top_ids;    // [rows][top]
+  float* top_logprobs; // [rows][top]
+};
+constexpr int kLogprobMaxTop = 32;
+// Segments that a row is split into, and the bytes of their states.
+int32_t logprob_segments(int64_t rows, int32_t vocab, int32_t cus);
+int64_t logprob_workspace(int64_t rows, int32_t segments, int32_t top);
+hipError_t token_logprobs(const LogprobArgs& a, int32_t segments, void* workspace,
+                          hipStream_t stream);
+
 }  // namespace aios

@@ -58,3 +58,47 @@ def store_cache(
         ),
         "aios_kv_append",
     )
+
+
+def store_cache8(
+    k8: torch.Tensor,
+    v8: torch.Tensor,
+    scales: torch.Tensor,
+    indices: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+) -> None:
+    """Quantise ``k[t]``/``v[t]`` (bfloat16) into page ``indices[t]`` of an
+    8-bit cache: k8, v8 float8_e4m3fn (num_slots, num_heads, head_dim) codes
+    and scales bfloat16 (num_heads, num_slots, 2), K's scale then V's, the
+    power of two that brings the row's largest magnitude to at most 448."""
+    if k8.ndim != 3 or v8.shape != k8.shape:
+        raise ValueError("KV cache must have shape (num_slots, num_heads, head_dim)")
+    slots, heads, dim = k8.shape
+    if k.shape[1:] != k8.shape[1:]:
+        raise ValueError("K/V input shape does not match the cache layout")
+    if indices.numel() != k.shape[0] or k.shape != v.shape:
+        raise ValueError("KV write indices and K/V tensors must have matching token counts")
+    if k8.dtype != torch.float8_e4m3fn or v8.dtype != torch.float8_e4m3fn:
+        raise ValueError("the 8-bit KV cache holds float8_e4m3fn codes")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("the 8-bit KV cache takes bfloat16 K/V rows")
+    if scales.dtype != torch.bfloat16 or scales.shape != (heads, slots, 2):
+        raise ValueError("scales must be bfloat16 (num_heads, num_slots, 2)")
+    if not (k8.is_contiguous() and v8.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("8-bit KV caches and their scales must be contiguous")
+    for name, t in (("k", k), ("v", v)):
+        if t.stride(2) != 1 or (t.stride(1) != dim and heads > 1):
+            raise ValueError(f"{name} must have contiguous (heads, head_dim) rows")
+    device = k8.get_device()
+    if any(t.get_device() != device for t in (v8, scales, indices, k, v)):
+        raise ValueError("the KV cache, its scales, the indices and K/V must be on one GPU")
+    if indices.dtype != torch.int32 or not indices.is_contiguous():
+        indices = indices.to(torch.int32).contiguous()
+    _lib.check(
+        _lib.lib().aios_kv8_append(
+            k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), slots, heads, dim,
+            indices.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0],
+            _lib.raw_stream(k8)),
+        "aios_kv8_append",
+    )

@@ -234,6 +234,37 @@ class HipOps:
         return q
 
     @staticmethod
+    def qk_norm_rope_append8(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                             cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                             num_qo_heads: int, eps: float, k8: torch.Tensor, v8: torch.Tensor,
+                             scales: torch.Tensor, out_loc: torch.Tensor) -> torch.Tensor:
+        """qk_norm_rope_append into the 8-bit cache: k8, v8 float8_e4m3fn
+        [slots, Hkv, D] and scales bfloat16 [Hkv, slots, 2]; returns q."""
+        slots, num_kv_heads, head_dim = k8.shape
+        HipOps._check_rope(qkv, cos, sin, positions, head_dim)
+        t = qkv.shape[0]
+        if qkv.shape[1] != (num_qo_heads + 2 * num_kv_heads) * head_dim:
+            raise ValueError("qkv rows must hold the q, k and v heads")
+        for c in (k8, v8):
+            if c.dtype != torch.float8_e4m3fn or c.shape != k8.shape or not c.is_contiguous():
+                raise ValueError("8-bit KV caches must be contiguous float8_e4m3fn tensors of one "
+                                 "shape")
+        if (scales.dtype != torch.bfloat16 or scales.shape != (num_kv_heads, slots, 2)
+                or not scales.is_contiguous()):
+            raise ValueError("scales must be contiguous bfloat16 (num_kv_heads, num_slots, 2)")
+        _check_gpu(k8, v8, scales, out_loc)
+        if out_loc.dtype != torch.int32 or out_loc.numel() != t or not out_loc.is_contiguous():
+            raise ValueError("out_loc must be contiguous int32 with one entry per token")
+        q = torch.empty(t, num_qo_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
+        _lib.check(_lib.lib().aios_qk_norm_rope_append8(
+            qkv.data_ptr(), qkv.stride(0), t, num_qo_heads, num_kv_heads, head_dim,
+            q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            positions.contiguous().data_ptr(), q.data_ptr(), k8.data_ptr(), v8.data_ptr(),
+            scales.data_ptr(), slots, out_loc.data_ptr(), eps, _stream(qkv)),
+            "aios_qk_norm_rope_append8")
+        return q
+
+    @staticmethod
     def attnres_mix(bank: torch.Tensor, partial: torch.Tensor | None,
                     weighted_query: torch.Tensor, eps: float) -> torch.Tensor:
         """Depth mix of bank [S, N, D] (+ partial as the last source)."""

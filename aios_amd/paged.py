@@ -26,19 +26,24 @@ def _host_i32(x) -> torch.Tensor:
 
 def plan(phase: str, cu_q, cu_k, num_qo_heads: int, num_kv_heads: int, head_dim: int, *,
          shared_prefix_len: int = 0, workspace_bytes: int = DEFAULT_WORKSPACE,
-         prefix_chunk_len: int = 0, suffix_split_len: int = 0) -> _lib.AttnPlan:
-    """Host-only schedule for one batch (aios_attn_plan)."""
+         prefix_chunk_len: int = 0, suffix_split_len: int = 0,
+         kv_bits: int = 16) -> _lib.AttnPlan:
+    """Host-only schedule for one batch over a cache of ``kv_bits`` (16:
+    bfloat16, aios_attn_plan; 8: the calls named ...8, aios_attn_plan8)."""
+    if kv_bits not in (8, 16):
+        raise ValueError("kv_bits must be 8 or 16")
     cu_q = _host_i32(cu_q)
     cu_k = _host_i32(cu_k)
     if cu_q.numel() != cu_k.numel() or cu_q.numel() < 1:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have batch_size + 1 entries")
     p = _lib.AttnPlan()
     code = _lib.PHASE_DECODE if phase == "decode" else _lib.PHASE_PREFILL
+    make = _lib.lib().aios_attn_plan8 if kv_bits == 8 else _lib.lib().aios_attn_plan
     _lib.check(
-        _lib.lib().aios_attn_plan(code, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1,
-                                  num_qo_heads, num_kv_heads, head_dim, 1, shared_prefix_len,
-                                  workspace_bytes, prefix_chunk_len, suffix_split_len, p),
-        "aios_attn_plan",
+        make(code, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, num_qo_heads, num_kv_heads,
+             head_dim, 1, shared_prefix_len, workspace_bytes, prefix_chunk_len, suffix_split_len,
+             p),
+        make.__name__,
     )
     return p
 
@@ -245,6 +250,170 @@ def prefill(p: _lib.AttnPlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
             k_cache.shape[0], indices.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
             ws.data_ptr() if ws is not None else None, p.ws_bytes, scale, _stream(q)),
         "aios_attn_prefill_ws",
+    )
+    return out
+
+
+def _check_kv8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+               scales: torch.Tensor) -> int:
+    """The 8-bit cache of one layer (aios_amd.kvcache.MHAKVCache8); returns
+    its number of pages."""
+    pages, hkv, d = k8.shape[0], p.num_kv_heads, p.head_dim
+    if k8.dtype != torch.float8_e4m3fn or v8.dtype != torch.float8_e4m3fn:
+        raise ValueError("the 8-bit KV cache holds float8_e4m3fn codes")
+    if k8.shape[-2:] != (hkv, d) or k8.numel() != pages * hkv * d or v8.shape != k8.shape:
+        raise ValueError("8-bit KV caches must be (num_pages, [1,] num_kv_heads, head_dim)")
+    if scales.dtype != torch.bfloat16 or scales.shape != (hkv, pages, 2):
+        raise ValueError("scales must be bfloat16 (num_kv_heads, num_pages, 2)")
+    if not (k8.is_contiguous() and v8.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("8-bit KV caches and their scales must be contiguous")
+    dev = q.get_device()
+    if not dev == k8.get_device() == v8.get_device() == scales.get_device():
+        raise ValueError("q, the KV caches and their scales must be on one GPU")
+    return pages
+
+
+def _check_decode8(p: _lib.AttnPlan, q: torch.Tensor, indices: torch.Tensor, cu_k: torch.Tensor,
+                   out: torch.Tensor | None, workspace: torch.Tensor | None) -> torch.Tensor:
+    if p.phase != _lib.PHASE_DECODE8:
+        raise ValueError("plan was not built for decode over the 8-bit cache (kv_bits=8)")
+    _check_q(q, p)
+    if q.shape[0] != p.batch_size:
+        raise ValueError("decode batch must contain one flat token per request")
+    _check_i32(indices, "indices", p.total_kv)
+    _check_i32(cu_k, "cu_k", p.batch_size + 1)
+    if p.ws_bytes and (workspace is None or workspace.nbytes < p.ws_bytes):
+        raise RuntimeError(f"decode needs a workspace of {p.ws_bytes} bytes")
+    if workspace is not None and not (workspace.is_cuda and workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous GPU tensor")
+    return _out_like(q, out)
+
+
+def _out_like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or \
+            out.device != q.device:
+        raise ValueError("out must be a contiguous bfloat16 GPU tensor shaped like q")
+    return out
+
+
+def _check_new8(k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, p: _lib.AttnPlan) -> None:
+    shape, d = (p.batch_size, p.num_kv_heads, p.head_dim), p.head_dim
+    for t in (k, v):
+        if t.dtype != torch.bfloat16 or not t.is_cuda:
+            raise ValueError("new K/V rows must be bfloat16 GPU tensors")
+        if t.shape != shape:
+            raise ValueError("K/V input shape does not match the cache layout")
+        if t.stride(2) != 1 or (t.stride(1) != d and shape[1] > 1):
+            raise ValueError("new K/V rows must have contiguous (heads, head_dim) rows")
+    _check_i32(out_loc, "out_loc", p.batch_size)
+
+
+def _ws8(workspace: torch.Tensor | None) -> tuple[int | None, int]:
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+
+
+def decode8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+            scales: torch.Tensor, indices: torch.Tensor, cu_k: torch.Tensor, *,
+            out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+            sm_scale: float | None = None) -> torch.Tensor:
+    """:func:`decode` over the 8-bit cache (k8, v8 float8_e4m3fn [pages, Hkv,
+    D], scales bfloat16 [Hkv, pages, 2]); the plan is one of ``kv_bits=8``."""
+    out = _check_decode8(p, q, indices, cu_k, out, workspace)
+    pages = _check_kv8(p, q, k8, v8, scales)
+    ws, ws_bytes = _ws8(workspace)
+    _lib.check(
+        _lib.lib().aios_attn_decode8(
+            p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
+            indices.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws, ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+        "aios_attn_decode8",
+    )
+    return out
+
+
+def append_decode8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                   out_loc: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, scales: torch.Tensor,
+                   indices: torch.Tensor, cu_k: torch.Tensor, *, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None,
+                   sm_scale: float | None = None) -> torch.Tensor:
+    """:func:`append_decode` over the 8-bit cache: the new rows are quantised
+    into page out_loc[b] and attended to as the cache holds them."""
+    out = _check_decode8(p, q, indices, cu_k, out, workspace)
+    pages = _check_kv8(p, q, k8, v8, scales)
+    _check_new8(k, v, out_loc, p)
+    ws, ws_bytes = _ws8(workspace)
+    _lib.check(
+        _lib.lib().aios_attn_append_decode8(
+            p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+            out_loc.data_ptr(), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
+            indices.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws, ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+        "aios_attn_append_decode8",
+    )
+    return out
+
+
+def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        out_loc: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+                        scales: torch.Tensor, indices: torch.Tensor, cu_k: torch.Tensor,
+                        q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor,
+                        sin: torch.Tensor, positions: torch.Tensor, eps: float, *,
+                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                        sm_scale: float | None = None) -> torch.Tensor:
+    """:func:`append_decode_rope` over the 8-bit cache."""
+    out = _check_decode8(p, q, indices, cu_k, out, workspace)
+    pages = _check_kv8(p, q, k8, v8, scales)
+    _check_new8(k, v, out_loc, p)
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w.dtype != torch.bfloat16 or w.numel() != p.head_dim or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bfloat16 [head_dim] tensor")
+    if (cos.dtype != torch.bfloat16 or sin.dtype != torch.bfloat16 or cos.shape != sin.shape
+            or cos.ndim != 2 or cos.shape[1] != p.head_dim or not cos.is_contiguous()
+            or not sin.is_contiguous()):
+        raise ValueError("cos/sin tables must be contiguous bfloat16 [positions, head_dim]")
+    dev = q.get_device()
+    if any(t.get_device() != dev for t in (q_norm, k_norm, cos, sin)):
+        raise ValueError("norm weights and rotary tables must be on q's GPU")
+    _check_i32(positions, "positions", p.batch_size)
+    ws, ws_bytes = _ws8(workspace)
+    _lib.check(
+        _lib.lib().aios_attn_append_decode_rope8(
+            p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+            out_loc.data_ptr(), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
+            indices.data_ptr(), cu_k.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+            cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), float(eps),
+            out.data_ptr(), ws, ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+        "aios_attn_append_decode_rope8",
+    )
+    return out
+
+
+def prefill8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+             scales: torch.Tensor, indices: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+             *, out: torch.Tensor | None = None, sm_scale: float | None = None) -> torch.Tensor:
+    """:func:`prefill` over the 8-bit cache (as :func:`decode8`)."""
+    if p.phase != _lib.PHASE_PREFILL8:
+        raise ValueError("plan was not built for prefill over the 8-bit cache (kv_bits=8)")
+    _check_q(q, p)
+    if q.shape[0] != p.total_q:
+        raise RuntimeError("prefill request lengths do not match flat Q tokens")
+    pages = _check_kv8(p, q, k8, v8, scales)
+    _check_i32(indices, "indices", p.total_kv)
+    _check_i32(cu_q, "cu_q", p.batch_size + 1)
+    _check_i32(cu_k, "cu_k", p.batch_size + 1)
+    out = _out_like(q, out)
+    # (a buffer of this call alone, as in prefill)
+    ws = torch.empty(p.ws_bytes, dtype=torch.uint8, device=q.device) if p.ws_bytes else None
+    _lib.check(
+        _lib.lib().aios_attn_prefill8(
+            p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
+            indices.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
+            None if ws is None else ws.data_ptr(), p.ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+        "aios_attn_prefill8",
     )
     return out
 

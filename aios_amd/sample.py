@@ -150,3 +150,49 @@ class Sampler:
 
     def sample(self, logits: torch.Tensor) -> torch.Tensor:
         return self.sample_with_logprobs(logits)[0]
+
+
+@dataclass(frozen=True)
+class TokenLogprobs:
+    """:func:`token_logprobs`'s answers for a batch of rows."""
+
+    logprobs: torch.Tensor      # float32 [rows]: ln p of the given tokens
+    entropies: torch.Tensor     # float32 [rows], in nats
+    top_ids: torch.Tensor       # int64 [rows, top], most likely first
+    top_logprobs: torch.Tensor  # float32 [rows, top]
+
+
+MAX_TOP_LOGPROBS = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens (int64 [rows]) under the rows of
+    ``logits`` (bfloat16 or float32 [rows, vocab]), each row's entropy and its
+    ``top`` most likely ids with their log probabilities (at most 32; equal
+    logits by ascending id), in one pass over the logits
+    (``aios_token_logprobs``).  A token outside the vocabulary has log
+    probability NaN, ids at -inf count as impossible, and a row without a
+    finite maximum gives NaN."""
+    _check_logits(logits)
+    rows, vocab = logits.shape
+    if tokens.dtype != torch.int64 or tokens.shape != (rows,) or \
+            tokens.get_device() != logits.get_device():
+        raise ValueError("tokens must be int64 [rows] on the logits' GPU")
+    if not 0 <= top <= min(vocab, MAX_TOP_LOGPROBS):
+        raise ValueError(f"top must be within 0..{min(vocab, MAX_TOP_LOGPROBS)}")
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    lib, dev = _lib.lib(), logits.device
+    lp = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    alt = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    # (the states of split rows: a buffer of this call alone, since calls may
+    # overlap on several streams)
+    ws_bytes = lib.aios_token_logprobs_workspace(rows, vocab, top)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    out = lp.data_ptr()
+    _lib.check(lib.aios_token_logprobs(
+        logits.data_ptr(), logits.stride(0), rows, vocab, logits.element_size(),
+        tokens.data_ptr(), top, out, out + 4 * rows, ids.data_ptr(), alt.data_ptr(),
+        None if ws is None else ws.data_ptr(), ws_bytes, _stream(logits)), "aios_token_logprobs")
+    return TokenLogprobs(lp[0], lp[1], ids, alt)

@@ -66,6 +66,9 @@ extern "C" {
 
 #define AIOS_PHASE_PREFILL 0
 #define AIOS_PHASE_DECODE 1
+/* (a plan's phase for the 8-bit cache: see aios_attn_plan8) */
+#define AIOS_PHASE_PREFILL8 2
+#define AIOS_PHASE_DECODE8 3
 
 /* Thread-local message for the last non-zero status of this thread. */
 const char* aios_last_error(void);
@@ -549,6 +552,106 @@ int aios_attnres_mix_ex(const void* bank, int32_t bank_sources, int64_t num_toke
                         int32_t hidden, const void* partial, const void* delta,
                         void* partial_out, const float* weighted_query, float eps, float* scores,
                         void* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit KV cache.  No counterpart in the reference.
+ *
+ * One layer is two arrays of codes, k8 and v8 [num_pages][Hkv][D] (e4m3, the
+ * OCP type with 448 as its largest value), and scales [Hkv][num_pages][2]
+ * (bf16: K's scale, then V's, of one head's row of one page); D is 64, 96 or
+ * 128.  A row's scale is the power of two 2^e with the smallest e >= -110
+ * for which max |x| <= 448 * 2^e, its codes are x / 2^e rounded to nearest
+ * even, and the value of the cache is code * scale (exact in bf16).  A row
+ * that holds a NaN or an infinity is given a NaN scale, its codes 0 there:
+ * every attention output that attends to the token is then NaN, and no other.
+ * The attention calls read scales as powers of two (or NaN): write them with
+ * the calls below.  Codes and scales: 16- and 4-byte aligned; num_pages below
+ * 2^24, a layer's codes (num_pages * Hkv * D bytes) below 4 GiB;
+ * AIOS_ERR_UNSUPPORTED otherwise.  Page ids outside [0, num_pages) read as
+ * all-zero rows, and out_loc entries outside it are not written.
+ */
+
+/* aios_kv_append into the 8-bit cache: K/V rows (bf16 [n_tokens][Hkv][D], even
+ * token strides in elements, 4-byte aligned) quantised into pages out_loc[t]
+ * (distinct, or outside the pool). */
+int aios_kv8_append(void* k8, void* v8, void* scales, int64_t num_pages, int32_t num_kv_heads,
+                    int32_t head_dim, const int32_t* out_loc, const void* k, int64_t k_tok_stride,
+                    const void* v, int64_t v_tok_stride, int64_t n_tokens, void* stream);
+
+/* aios_qk_norm_rope_append with the 8-bit cache: the same q_out, and the codes
+ * and scales of the same K and V rows. */
+int aios_qk_norm_rope_append8(const void* qkv, int64_t qkv_stride, int64_t tokens,
+                              int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                              const void* q_weight, const void* k_weight, const float* cos_table,
+                              const float* sin_table, int64_t table_rows,
+                              const int32_t* positions, void* q_out, void* k8, void* v8,
+                              void* scales, int64_t num_pages, const int32_t* out_loc, float eps,
+                              void* stream);
+
+/* aios_attn_plan for a batch over the 8-bit cache: the same arguments (phase
+ * AIOS_PHASE_PREFILL or AIOS_PHASE_DECODE); the plan's phase is
+ * AIOS_PHASE_PREFILL8 or AIOS_PHASE_DECODE8, which the calls below take and
+ * those of the bf16 cache refuse. */
+int aios_attn_plan8(int32_t phase, const int32_t* cu_q_host, const int32_t* cu_k_host,
+                    int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t page_size, int32_t shared_prefix_len,
+                    int64_t workspace_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
+                    aios_attn_plan_t* plan_out);
+
+/* aios_attn_prefill_ws over the 8-bit cache (workspace as there: without it
+ * every tile is one workgroup). */
+int aios_attn_prefill8(const aios_attn_plan_t* plan, const void* q, int64_t q_tok_stride,
+                       const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                       const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k, void* out,
+                       void* workspace, int64_t workspace_bytes, float sm_scale, void* stream);
+
+/* aios_attn_decode over the 8-bit cache. */
+int aios_attn_decode8(const aios_attn_plan_t* plan, const void* q, int64_t q_tok_stride,
+                      const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                      const int32_t* indices, const int32_t* cu_k, void* out, void* workspace,
+                      int64_t workspace_bytes, float sm_scale, void* stream);
+
+/* aios_attn_append_decode over the 8-bit cache: the new rows are quantised,
+ * written to page out_loc[b] and attended to as the cache holds them (the
+ * result of aios_kv8_append followed by aios_attn_decode8).  Token strides
+ * even, rows 4-byte aligned; other conditions as aios_attn_append_decode. */
+int aios_attn_append_decode8(const aios_attn_plan_t* plan, const void* q, int64_t q_tok_stride,
+                             const void* k_new, int64_t k_tok_stride, const void* v_new,
+                             int64_t v_tok_stride, const int32_t* out_loc, void* k8, void* v8,
+                             void* scales, int64_t num_pages, const int32_t* indices,
+                             const int32_t* cu_k, void* out, void* workspace,
+                             int64_t workspace_bytes, float sm_scale, void* stream);
+
+/* aios_attn_append_decode_rope over the 8-bit cache. */
+int aios_attn_append_decode_rope8(const aios_attn_plan_t* plan, const void* q,
+                                  int64_t q_tok_stride, const void* k_new, int64_t k_tok_stride,
+                                  const void* v_new, int64_t v_tok_stride, const int32_t* out_loc,
+                                  void* k8, void* v8, void* scales, int64_t num_pages,
+                                  const int32_t* indices, const int32_t* cu_k, const void* q_norm,
+                                  const void* k_norm, const void* rope_cos, const void* rope_sin,
+                                  int64_t rope_rows, const int32_t* positions, float norm_eps,
+                                  void* out, void* workspace, int64_t workspace_bytes,
+                                  float sm_scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Scoring: for every row of logits (elem_bytes 2: bf16, 4: fp32; rows
+ * row_stride elements apart, 0: one row for all; aligned to their element
+ * only), with p = softmax(row):
+ *   logprobs[r]  = ln p(tokens[r])  (NaN for an id outside [0, vocab))
+ *   entropies[r] = -sum p ln p      (ids at -inf add 0)
+ *   top_ids / top_logprobs [rows][top]: the `top` largest logits in
+ *     descending order, equal ones by ascending id (a NaN before all), and
+ *     their ln p; top from 0 (both pointers may be null) to min(vocab, 32).
+ * A row without a finite maximum (a NaN, +inf, or all -inf) gives NaN for all
+ * but top_ids.  All sums in fp32 or wider.  Long rows are split over
+ * workgroups when workspace, 16-byte aligned, holds the
+ * aios_token_logprobs_workspace(...) bytes (0: none used).
+ */
+int64_t aios_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top);
+int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab,
+                        int32_t elem_bytes, const int64_t* tokens, int32_t top, float* logprobs,
+                        float* entropies, int64_t* top_ids, float* top_logprobs, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
