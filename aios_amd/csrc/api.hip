@@ -1528,7 +1528,7 @@ int aios_attn_append_decode_rope8(const aios_attn_plan_t* p, const void* q, int6
 
 int64_t aios_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {
   if (rows <= 0 || vocab <= 0 || top < 0 || top > aios::kLogprobMaxTop) return 0;
-  return aios::logprob_workspace(rows, aios::logprob_segments(rows, vocab, device_cus()), top);
+  return aios::logprob_workspace(rows, vocab, aios::logprob_segments(rows, vocab, device_cus()), top);
 }
 
 int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int32_t vocab,
@@ -1548,12 +1548,13 @@ int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, in
     return fail(AIOS_ERR_INVALID, "token_logprobs: null pointer");
   if (((uintptr_t)logits & (uintptr_t)(elem_bytes - 1)) != 0)
     return fail(AIOS_ERR_INVALID, "token_logprobs: misaligned logits");
-  if (rows > (1ll << 24)) return fail(AIOS_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  if (rows > (1ll << 24) || vocab > (1 << 30))
+    return fail(AIOS_ERR_UNSUPPORTED, "token_logprobs: more than 2^24 rows or 2^30 ids");
   const aios::LogprobArgs a = {logits,   row_stride, rows,      vocab,   elem_bytes,  tokens,
                                top,      logprobs,   entropies, top_ids, top_logprobs};
   int32_t seg = aios::logprob_segments(rows, vocab, device_cus());
   if (!workspace || ((uintptr_t)workspace & 15) != 0 ||
-      workspace_bytes < aios::logprob_workspace(rows, seg, top))
+      workspace_bytes < aios::logprob_workspace(rows, vocab, seg, top))
     seg = 1;
   return check_hip(aios::token_logprobs(a, seg, workspace, static_cast<hipStream_t>(stream)),
                    "token_logprobs launch");

@@ -418,9 +418,9 @@ struct LogprobArgs {
   float* top_logprobs; // [rows][top]
 };
 constexpr int kLogprobMaxTop = 32;
-// Segments that a row is split into, and the bytes of their states.
+// Segments that a row is split into, and the bytes of their states (0: one).
 int32_t logprob_segments(int64_t rows, int32_t vocab, int32_t cus);
-int64_t logprob_workspace(int64_t rows, int32_t segments, int32_t top);
+int64_t logprob_workspace(int64_t rows, int32_t vocab, int32_t segments, int32_t top);
 hipError_t token_logprobs(const LogprobArgs& a, int32_t segments, void* workspace,
                           hipStream_t stream);
 

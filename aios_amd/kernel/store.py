@@ -72,33 +72,39 @@ def store_cache8(
     8-bit cache: k8, v8 float8_e4m3fn (num_slots, num_heads, head_dim) codes
     and scales bfloat16 (num_heads, num_slots, 2), K's scale then V's, the
     power of two that brings the row's largest magnitude to at most 448."""
-    if k8.ndim != 3 or v8.shape != k8.shape:
+    shape = k8.shape
+    if len(shape) != 3 or v8.shape != shape:
         raise ValueError("KV cache must have shape (num_slots, num_heads, head_dim)")
-    slots, heads, dim = k8.shape
-    if k.shape[1:] != k8.shape[1:]:
+    slots, heads, dim = shape
+    new = k.shape
+    if new[1:] != shape[1:]:
         raise ValueError("K/V input shape does not match the cache layout")
-    if indices.numel() != k.shape[0] or k.shape != v.shape:
+    tokens = new[0]
+    if indices.numel() != tokens or v.shape != new:
         raise ValueError("KV write indices and K/V tensors must have matching token counts")
-    if k8.dtype != torch.float8_e4m3fn or v8.dtype != torch.float8_e4m3fn:
+    if k8.dtype is not torch.float8_e4m3fn or v8.dtype is not torch.float8_e4m3fn:
         raise ValueError("the 8-bit KV cache holds float8_e4m3fn codes")
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    bf16 = torch.bfloat16
+    if k.dtype is not bf16 or v.dtype is not bf16:
         raise ValueError("the 8-bit KV cache takes bfloat16 K/V rows")
-    if scales.dtype != torch.bfloat16 or scales.shape != (heads, slots, 2):
+    if scales.dtype is not bf16 or scales.shape != (heads, slots, 2):
         raise ValueError("scales must be bfloat16 (num_heads, num_slots, 2)")
     if not (k8.is_contiguous() and v8.is_contiguous() and scales.is_contiguous()):
         raise ValueError("8-bit KV caches and their scales must be contiguous")
-    for name, t in (("k", k), ("v", v)):
-        if t.stride(2) != 1 or (t.stride(1) != dim and heads > 1):
+    k_stride, v_stride = k.stride(), v.stride()
+    for name, stride in (("k", k_stride), ("v", v_stride)):
+        if stride[2] != 1 or (stride[1] != dim and heads > 1):
             raise ValueError(f"{name} must have contiguous (heads, head_dim) rows")
-    device = k8.get_device()
-    if any(t.get_device() != device for t in (v8, scales, indices, k, v)):
+    dev = k8.get_device()
+    if not (dev == v8.get_device() == scales.get_device() == indices.get_device()
+            == k.get_device() == v.get_device()):
         raise ValueError("the KV cache, its scales, the indices and K/V must be on one GPU")
     if indices.dtype != torch.int32 or not indices.is_contiguous():
         indices = indices.to(torch.int32).contiguous()
     _lib.check(
         _lib.lib().aios_kv8_append(
             k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), slots, heads, dim,
-            indices.data_ptr(), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), k.shape[0],
+            indices.data_ptr(), k.data_ptr(), k_stride[0], v.data_ptr(), v_stride[0], tokens,
             _lib.raw_stream(k8)),
         "aios_kv8_append",
     )

@@ -254,64 +254,92 @@ def prefill(p: _lib.AttnPlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     return out
 
 
-def _check_kv8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+_BF16, _I32, _FP8 = torch.bfloat16, torch.int32, torch.float8_e4m3fn
+
+
+def _check_kv8(p: _lib.AttnPlan, dev: int, k8: torch.Tensor, v8: torch.Tensor,
                scales: torch.Tensor) -> int:
-    """The 8-bit cache of one layer (aios_amd.kvcache.MHAKVCache8); returns
-    its number of pages."""
-    pages, hkv, d = k8.shape[0], p.num_kv_heads, p.head_dim
-    if k8.dtype != torch.float8_e4m3fn or v8.dtype != torch.float8_e4m3fn:
+    """The 8-bit cache of one layer (aios_amd.kvcache.MHAKVCache8) on GPU
+    ``dev``; returns its number of pages."""
+    shape, hkv, d = k8.shape, p.num_kv_heads, p.head_dim
+    pages = shape[0]
+    if k8.dtype is not _FP8 or v8.dtype is not _FP8:
         raise ValueError("the 8-bit KV cache holds float8_e4m3fn codes")
-    if k8.shape[-2:] != (hkv, d) or k8.numel() != pages * hkv * d or v8.shape != k8.shape:
+    if (shape != (pages, hkv, d) and shape != (pages, 1, hkv, d)) or v8.shape != shape:
         raise ValueError("8-bit KV caches must be (num_pages, [1,] num_kv_heads, head_dim)")
-    if scales.dtype != torch.bfloat16 or scales.shape != (hkv, pages, 2):
+    if scales.dtype is not _BF16 or scales.shape != (hkv, pages, 2):
         raise ValueError("scales must be bfloat16 (num_kv_heads, num_pages, 2)")
     if not (k8.is_contiguous() and v8.is_contiguous() and scales.is_contiguous()):
         raise ValueError("8-bit KV caches and their scales must be contiguous")
-    dev = q.get_device()
     if not dev == k8.get_device() == v8.get_device() == scales.get_device():
         raise ValueError("q, the KV caches and their scales must be on one GPU")
     return pages
 
 
+def _check_q8(p: _lib.AttnPlan, q: torch.Tensor, tokens: int) -> int:
+    """q [tokens, Hq, D] (the plan's check_q); returns its GPU."""
+    d = p.head_dim
+    dev, shape, stride = q.get_device(), q.shape, q.stride()
+    if dev < 0 or q.dtype is not _BF16 or shape != (shape[0], p.num_qo_heads, d) or \
+            stride[2] != 1 or stride[1] != d:
+        _check_q(q, p)
+    if shape[0] != tokens:
+        if p.phase == _lib.PHASE_DECODE8:
+            raise ValueError("decode batch must contain one flat token per request")
+        raise RuntimeError("prefill request lengths do not match flat Q tokens")
+    return dev
+
+
+def _check_lists8(dev: int, *lists: tuple[torch.Tensor, str, int]) -> None:
+    """int32 lists (tensor, name, entries needed) on GPU ``dev``."""
+    for t, name, n in lists:
+        if t.dtype is not _I32 or not t.is_contiguous() or t.numel() < n or t.get_device() != dev:
+            raise ValueError(f"{name} must be a contiguous int32 tensor of >= {n} entries on q's "
+                             "GPU")
+
+
 def _check_decode8(p: _lib.AttnPlan, q: torch.Tensor, indices: torch.Tensor, cu_k: torch.Tensor,
-                   out: torch.Tensor | None, workspace: torch.Tensor | None) -> torch.Tensor:
+                   k8: torch.Tensor, v8: torch.Tensor, scales: torch.Tensor,
+                   out: torch.Tensor | None, workspace: torch.Tensor | None):
+    """(out, pages, workspace address and bytes)"""
     if p.phase != _lib.PHASE_DECODE8:
         raise ValueError("plan was not built for decode over the 8-bit cache (kv_bits=8)")
-    _check_q(q, p)
-    if q.shape[0] != p.batch_size:
-        raise ValueError("decode batch must contain one flat token per request")
-    _check_i32(indices, "indices", p.total_kv)
-    _check_i32(cu_k, "cu_k", p.batch_size + 1)
-    if p.ws_bytes and (workspace is None or workspace.nbytes < p.ws_bytes):
-        raise RuntimeError(f"decode needs a workspace of {p.ws_bytes} bytes")
-    if workspace is not None and not (workspace.is_cuda and workspace.is_contiguous()):
-        raise ValueError("workspace must be a contiguous GPU tensor")
-    return _out_like(q, out)
+    b = p.batch_size
+    dev = _check_q8(p, q, b)
+    _check_lists8(dev, (indices, "indices", p.total_kv), (cu_k, "cu_k", b + 1))
+    pages = _check_kv8(p, dev, k8, v8, scales)
+    need, ws, ws_bytes = p.ws_bytes, None, 0
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.nbytes
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous tensor on q's GPU")
+    if ws_bytes < need:
+        raise RuntimeError(f"decode needs a workspace of {need} bytes")
+    return _out_like(q, out), pages, ws, ws_bytes
 
 
 def _out_like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return (torch.empty_like(q) if q.is_contiguous()
+                else torch.empty(q.shape, dtype=q.dtype, device=q.device))
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or \
             out.device != q.device:
         raise ValueError("out must be a contiguous bfloat16 GPU tensor shaped like q")
     return out
 
 
-def _check_new8(k: torch.Tensor, v: torch.Tensor, out_loc: torch.Tensor, p: _lib.AttnPlan) -> None:
-    shape, d = (p.batch_size, p.num_kv_heads, p.head_dim), p.head_dim
+def _check_new8(p: _lib.AttnPlan, dev: int, k: torch.Tensor, v: torch.Tensor,
+                out_loc: torch.Tensor) -> None:
+    b, hkv, d = shape = p.batch_size, p.num_kv_heads, p.head_dim
     for t in (k, v):
-        if t.dtype != torch.bfloat16 or not t.is_cuda:
-            raise ValueError("new K/V rows must be bfloat16 GPU tensors")
+        if t.dtype is not _BF16 or t.get_device() != dev:
+            raise ValueError("new K/V rows must be bfloat16 tensors on q's GPU")
         if t.shape != shape:
             raise ValueError("K/V input shape does not match the cache layout")
-        if t.stride(2) != 1 or (t.stride(1) != d and shape[1] > 1):
+        stride = t.stride()
+        if stride[2] != 1 or (stride[1] != d and hkv > 1):
             raise ValueError("new K/V rows must have contiguous (heads, head_dim) rows")
-    _check_i32(out_loc, "out_loc", p.batch_size)
-
-
-def _ws8(workspace: torch.Tensor | None) -> tuple[int | None, int]:
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    _check_lists8(dev, (out_loc, "out_loc", b))
 
 
 def decode8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
@@ -320,9 +348,7 @@ def decode8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tenso
             sm_scale: float | None = None) -> torch.Tensor:
     """:func:`decode` over the 8-bit cache (k8, v8 float8_e4m3fn [pages, Hkv,
     D], scales bfloat16 [Hkv, pages, 2]); the plan is one of ``kv_bits=8``."""
-    out = _check_decode8(p, q, indices, cu_k, out, workspace)
-    pages = _check_kv8(p, q, k8, v8, scales)
-    ws, ws_bytes = _ws8(workspace)
+    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
     _lib.check(
         _lib.lib().aios_attn_decode8(
             p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
@@ -340,10 +366,8 @@ def append_decode8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: torch.
                    sm_scale: float | None = None) -> torch.Tensor:
     """:func:`append_decode` over the 8-bit cache: the new rows are quantised
     into page out_loc[b] and attended to as the cache holds them."""
-    out = _check_decode8(p, q, indices, cu_k, out, workspace)
-    pages = _check_kv8(p, q, k8, v8, scales)
-    _check_new8(k, v, out_loc, p)
-    ws, ws_bytes = _ws8(workspace)
+    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
+    _check_new8(p, q.get_device(), k, v, out_loc)
     _lib.check(
         _lib.lib().aios_attn_append_decode8(
             p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
@@ -363,9 +387,8 @@ def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: t
                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                         sm_scale: float | None = None) -> torch.Tensor:
     """:func:`append_decode_rope` over the 8-bit cache."""
-    out = _check_decode8(p, q, indices, cu_k, out, workspace)
-    pages = _check_kv8(p, q, k8, v8, scales)
-    _check_new8(k, v, out_loc, p)
+    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
+    _check_new8(p, q.get_device(), k, v, out_loc)
     for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w.dtype != torch.bfloat16 or w.numel() != p.head_dim or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous bfloat16 [head_dim] tensor")
@@ -376,8 +399,7 @@ def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: t
     dev = q.get_device()
     if any(t.get_device() != dev for t in (q_norm, k_norm, cos, sin)):
         raise ValueError("norm weights and rotary tables must be on q's GPU")
-    _check_i32(positions, "positions", p.batch_size)
-    ws, ws_bytes = _ws8(workspace)
+    _check_lists8(dev, (positions, "positions", p.batch_size))
     _lib.check(
         _lib.lib().aios_attn_append_decode_rope8(
             p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
@@ -397,13 +419,10 @@ def prefill8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
     """:func:`prefill` over the 8-bit cache (as :func:`decode8`)."""
     if p.phase != _lib.PHASE_PREFILL8:
         raise ValueError("plan was not built for prefill over the 8-bit cache (kv_bits=8)")
-    _check_q(q, p)
-    if q.shape[0] != p.total_q:
-        raise RuntimeError("prefill request lengths do not match flat Q tokens")
-    pages = _check_kv8(p, q, k8, v8, scales)
-    _check_i32(indices, "indices", p.total_kv)
-    _check_i32(cu_q, "cu_q", p.batch_size + 1)
-    _check_i32(cu_k, "cu_k", p.batch_size + 1)
+    dev = _check_q8(p, q, p.total_q)
+    pages = _check_kv8(p, dev, k8, v8, scales)
+    b = p.batch_size + 1
+    _check_lists8(dev, (indices, "indices", p.total_kv), (cu_q, "cu_q", b), (cu_k, "cu_k", b))
     out = _out_like(q, out)
     # (a buffer of this call alone, as in prefill)
     ws = torch.empty(p.ws_bytes, dtype=torch.uint8, device=q.device) if p.ws_bytes else None

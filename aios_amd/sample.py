@@ -19,6 +19,7 @@ from __future__ import annotations
 
 from collections.abc import Sequence
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -152,8 +153,7 @@ class Sampler:
         return self.sample_with_logprobs(logits)[0]
 
 
-@dataclass(frozen=True)
-class TokenLogprobs:
+class TokenLogprobs(NamedTuple):
     """:func:`token_logprobs`'s answers for a batch of rows."""
 
     logprobs: torch.Tensor      # float32 [rows]: ln p of the given tokens
@@ -183,16 +183,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     lib, dev = _lib.lib(), logits.device
-    lp = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
-    alt = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
+    ids = tokens.new_empty((rows, top))
+    alt = lp.new_empty((rows, top))
     # (the states of split rows: a buffer of this call alone, since calls may
     # overlap on several streams)
     ws_bytes = lib.aios_token_logprobs_workspace(rows, vocab, top)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    out = lp.data_ptr()
+    ws = ids.new_empty((ws_bytes + 7) // 8) if ws_bytes else None
     _lib.check(lib.aios_token_logprobs(
         logits.data_ptr(), logits.stride(0), rows, vocab, logits.element_size(),
-        tokens.data_ptr(), top, out, out + 4 * rows, ids.data_ptr(), alt.data_ptr(),
+        tokens.data_ptr(), top, lp.data_ptr(), ent.data_ptr(), ids.data_ptr(), alt.data_ptr(),
         None if ws is None else ws.data_ptr(), ws_bytes, _stream(logits)), "aios_token_logprobs")
-    return TokenLogprobs(lp[0], lp[1], ids, alt)
+    return TokenLogprobs(lp, ent, ids, alt)

@@ -23,21 +23,19 @@ TOL = 2.0 ** -17
 
 
 def _want(x, tokens, top):
-    """(log probabilities, entropies, ids, their log probabilities) of float64 rows."""
-    x = x.double().cpu().numpy()
-    with np.errstate(invalid="ignore", divide="ignore"):
-        m = x.max(-1, keepdims=True)
-        d = x - m
-        p = np.exp(d)
-        z = p.sum(-1, keepdims=True)
-        lp = d - np.log(z)
-        t = (p * np.where(p > 0, d, 0)).sum(-1)
-        ent = np.log(z[:, 0]) - t / z[:, 0]
-    ids = np.argsort(-x, axis=-1, kind="stable")[:, :top]  # (NaN-free rows)
-    tok = tokens.cpu().numpy()
-    ok = (tok >= 0) & (tok < x.shape[1])
-    got = np.where(ok, lp[np.arange(len(tok)), np.where(ok, tok, 0)], np.nan)
-    return got, ent, ids, np.take_along_axis(lp, ids, -1)
+    """(log probabilities, entropies, ids, their log probabilities) of the rows
+    (without a NaN) in float64."""
+    x = x.double()
+    d = x - x.amax(-1, keepdim=True)
+    p = d.exp()
+    z = p.sum(-1, keepdim=True)
+    lp = d - z.log()
+    ent = z[:, 0].log() - (p * torch.where(p > 0, d, 0.0)).sum(-1) / z[:, 0]
+    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top]
+    ok = (tokens >= 0) & (tokens < x.shape[1])
+    got = lp.gather(1, torch.where(ok, tokens, 0)[:, None])[:, 0]
+    got = torch.where(ok, got, float("nan"))
+    return [t.cpu().numpy() for t in (got, ent, ids, lp.gather(1, ids))]
 
 
 def _check(logits, tokens, top):
@@ -65,7 +63,7 @@ def _logits(rows, vocab, dtype, seed, spread=3.0):
 @pytest.mark.parametrize("rows,vocab,top", [
     (1, 1, 1), (3, 2, 2), (2, 7, 7), (5, 33, 32), (4, 511, 5), (3, 512, 1), (2, 513, 20),
     (9, 2048, 8), (5, 10007, 8), (24, 16384, 0), (1, 151936, 32), (7, 151936, 5), (3, 131071, 3),
-    (600, 6400, 2), (520, 2049, 32)])
+    (600, 6400, 2), (520, 2049, 32), (2, 300001, 6), (2, 1100003, 9), (513, 270001, 3)])
 def test_matches_float64(rows, vocab, top, dtype):
     _check(*_logits(rows, vocab, dtype, rows * vocab), top)
 
@@ -153,15 +151,23 @@ def test_strided_and_broadcast_rows():
     assert e.logprobs.shape == (0,) and e.top_ids.shape == (0, 6)
 
 
-def test_peaked_rows_keep_small_values():
-    """ln Z and T / Z of a row with one likely id are small: their absolute
-    error is that of Z's small terms and of one rounding next to 1."""
-    x = torch.full((1, 1000), -20.0, device=DEV)
-    x[0, 17] = 0.0
-    r = token_logprobs(x, torch.tensor([17], device=DEV), top=1)
-    small = 999 * math.exp(-20)
-    assert abs(r.logprobs.item() + math.log1p(small)) < 2.0 ** -23
-    assert abs(r.entropies.item() - (math.log1p(small) + 20 * small / (1 + small))) < 2.0 ** -22
+@pytest.mark.parametrize("rows,vocab", [(1, 1000), (2, 151936), (600, 9000)])
+def test_peaked_rows_keep_small_values(rows, vocab):
+    """ln Z = ln(1 + z) and T / Z of a row with one likely id are as exact as
+    the sum z of its small terms: relative 2^-18 (above), not 2^-24 of 1."""
+    x = torch.full((rows, vocab), -20.0, device=DEV)
+    x[:, 17] = 0.0
+    x[:, 20:900:7] = -23.5
+    tok = torch.full((rows,), 17, device=DEV)
+    r = token_logprobs(x, tok, top=1)
+    n = len(range(20, 900, 7))
+    z = n * math.exp(-23.5) + (vocab - 1 - n) * math.exp(-20)
+    t = -23.5 * n * math.exp(-23.5) - 20 * (vocab - 1 - n) * math.exp(-20)
+    lz = math.log1p(z)
+    for got, want in ((r.logprobs, -lz), (r.top_logprobs[:, 0], -lz),
+                      (r.entropies, lz - t / (1 + z))):
+        assert (got.double() - want).abs().max().item() <= 2.0 ** -18 * abs(want)
+    assert (r.top_ids == 17).all()
 
 
 def test_without_a_workspace_and_in_a_graph():
