@@ -384,6 +384,65 @@ int aios_attn_plan(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int3
   return AIOS_OK;
 }
 
+// Parts of all rows' own positions (behind the shared prefix), each row in
+// equal ones of at most `most`; longest: the longest part.
+static int64_t plan8_parts(const int32_t* cu_k, int32_t batch, int32_t prefix, int32_t most,
+                           int32_t* longest) {
+  int64_t n = 0;
+  *longest = 0;
+  for (int32_t b = 0; b < batch; ++b) {
+    const int32_t own = cu_k[b + 1] - cu_k[b] - prefix;
+    if (own <= 0) continue;
+    const int32_t parts = cdiv(own, most);
+    n += parts;
+    if (cdiv(own, parts) > *longest) *longest = cdiv(own, parts);
+  }
+  return n;
+}
+
+// How a decode over the 8-bit cache deals with the rows' own positions (at most
+// `longest`): 0 = one workgroup per (row, kv-head), else the most positions of
+// a part of a row.  Estimated in ns for passes of 128 positions of 128-dim rows,
+// with w workgroups under way (three share a unit): a pass takes 1,100 by
+// itself, 7.2 w up to about two workgroups per unit and 1,700 + 3.9 w from
+// there (4.6 and 5.4 TB/s); a workgroup has 3,000 of latency around its passes,
+// finding its part costs one
+// 600 more and the combine takes 2,400 and 20 a part.  Fitted to 16 rows of 32q/8kv x 128
+// over 8,192 positions (512 / 768 / 1,024 workgroups: 62 / 53 / 61 us), one row
+// of 16q/8kv over 16,001 (63 / 125 / 250 / 500 workgroups, with the combine: 21
+// / 15.6 / 14.6 / 15.5 us) and 64 rows of 500 (whole rows 15.4 us, halves 20.0).
+static int32_t plan8_split(const int32_t* cu_k, int32_t batch, int32_t prefix, int32_t longest,
+                           int32_t hkv, int32_t d, int32_t cus, int32_t most_parts,
+                           bool cascade) {
+  const int32_t pass = aios::kSuffixPass;
+  if (longest <= pass) return 0;
+  const int64_t slots = 3ll * cus;
+  auto time = [&](int64_t wgs, int64_t positions) {
+    auto round = [&](int64_t w) {
+      const int64_t bytes = 2 * d + 4;
+      const int64_t a = 72 * w * bytes / 2600, b = (17000 + 39 * w) * bytes / 2600;
+      const int64_t mem = a < b ? a : b;
+      return 3000 + positions * (mem > 1100 ? mem : 1100) / pass;
+    };
+    return wgs / slots * round(slots) + (wgs % slots ? round(wgs % slots) : 0);
+  };
+  int64_t best = time((int64_t)batch * hkv, longest) + (cascade ? 2400 : 0);
+  int32_t pick = 0;
+  for (int32_t k = 1; k * pass < longest; k += 1 + k / 16) {
+    const int32_t most = k * pass;
+    const int32_t parts = cdiv(longest, most);
+    if (parts > most_parts) continue;
+    int32_t len = 0;
+    const int64_t wgs = hkv * plan8_parts(cu_k, batch, prefix, most, &len);
+    const int64_t ns = time(wgs, len) + 3000 + 20 * parts;
+    if (ns < best) {
+      best = ns;
+      pick = most;
+    }
+  }
+  return pick;
+}
+
 int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
                     int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
                     int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
@@ -418,33 +477,26 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
     n_chunks = cdiv(P, chunk);
   }
   const int32_t max_suffix = p->max_kv_len - P;
-  const int32_t pass = aios::kSuffixPass;
-  int32_t split;
-  if (suffix_split_len > 0) {
-    split = suffix_split_len;
-  } else if (cascade) {
-    split = pass;
-  } else if (max_suffix <= 2 * pass) {
-    split = max_suffix > 0 ? max_suffix : 1;
-  } else {
-    // Rows of their own: about four items per compute unit.
-    const int64_t items = (int64_t)batch * hkv;
-    const int32_t want = (int32_t)((4ll * cus + items - 1) / items);
-    split = (int32_t)align_up(cdiv(max_suffix, want), pass);
+  // (at most three quarters of the parts a row may have are prefix chunks)
+  while (n_chunks > kMaxParts / 4 * 3 && max_suffix > aios::kSuffixPass) {
+    chunk = (int32_t)align_up((int64_t)chunk * 2, 32);
+    n_chunks = cdiv(P, chunk);
   }
-  int32_t n_splits = max_suffix > 0 ? cdiv(max_suffix, split) : 1;
-  while (n_chunks + n_splits > kMaxParts) {
-    if (n_splits > n_chunks) {
-      split *= 2;
-      n_splits = max_suffix > 0 ? cdiv(max_suffix, split) : 1;
-    } else {
-      chunk = (int32_t)align_up((int64_t)chunk * 2, 32);
-      n_chunks = cdiv(P, chunk);
-    }
+  while (n_chunks + aios::kSuffixWaves > kMaxParts) {
+    chunk = (int32_t)align_up((int64_t)chunk * 2, 32);
+    n_chunks = cdiv(P, chunk);
   }
-  const int32_t per_item =
-      (cascade && n_chunks + n_splits * aios::kSuffixWaves <= kMaxParts) ? aios::kSuffixWaves : 1;
-  const int32_t n_parts = n_chunks + n_splits * per_item;
+  int32_t split = suffix_split_len > 0
+                      ? (suffix_split_len < max_suffix ? suffix_split_len : 0)
+                      : plan8_split(cu_k, batch, P, max_suffix, hkv, d, cus, kMaxParts - n_chunks,
+                                    cascade);
+  while (split > 0 && cdiv(max_suffix, split) > kMaxParts - n_chunks) split *= 2;
+  // Whole rows beside the cascade leave one part per wavefront (the combine
+  // runs anyway), which saves the item's merge.
+  const int32_t per_item = split > 0 ? 0 : cascade ? aios::kSuffixWaves : 1;
+  const int32_t n_parts = n_chunks + (split > 0 ? cdiv(max_suffix, split) : per_item);
+  int32_t part_len = 0;
+  const int32_t n_splits = split > 0 ? (int32_t)plan8_parts(cu_k, batch, P, split, &part_len) : 1;
   p->suffix_parts_per_item = per_item;
   p->prefix_len = P;
   p->prefix_chunk_len = chunk;
@@ -453,7 +505,7 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
   p->cascade_mgroups = mgroups;
   p->suffix_split_len = split;
   p->num_suffix_splits = n_splits;
-  p->suffix_tpg = pass / 4;
+  p->suffix_tpg = aios::kSuffixPass / 4;
   p->num_parts = n_parts;
   if (n_parts > 1) {
     const int64_t states = (int64_t)batch * hkv * n_parts * G;
@@ -1435,9 +1487,10 @@ static int decode8_impl(const aios_attn_plan_t* p, const void* q, int64_t q_tok_
   a.m_rows = p->cascade_rows;
   a.prefix_units = p->num_prefix_chunks * p->num_kv_heads;
   a.prefix_wgs = a.prefix_units * (p->cascade_mgroups > 0 ? p->cascade_mgroups : 1);
+  a.split = p->suffix_parts_per_item == 0 ? 1 : 0;
   a.split_len = p->suffix_split_len;
   a.n_splits = p->num_suffix_splits;
-  a.suffix_items = p->batch_size * p->num_kv_heads * p->num_suffix_splits;
+  a.suffix_items = p->num_kv_heads * (a.split ? p->num_suffix_splits : p->batch_size);
   a.final_out = p->num_parts == 1 ? 1 : 0;
   a.wave_parts = p->suffix_parts_per_item > 1 ? 1 : 0;
   a.parts.o = reinterpret_cast<_Float16*>(ws + p->ws_parts_o);

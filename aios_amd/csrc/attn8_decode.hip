@@ -4,8 +4,10 @@
 //
 //   * prefix workgroups: the 128-row tile engine (engine8.hpp) over one chunk
 //     of the shared prefix;
-//   * row items: one (row, kv-head, split) of the row's own pages, its four
-//     wavefronts taking 32-position sub-tiles round-robin (RowEngine8 below).
+//   * row items: positions of the rows' own pages for one kv-head, the four
+//     wavefronts taking 32-position sub-tiles round-robin (RowEngine8 below):
+//     one row, whole, or one of the equal parts of a longer row (more of them
+//     the longer it is).
 #include "engine8.hpp"
 #include "rope_pairs.hpp"
 
@@ -132,11 +134,8 @@ struct RowEngine8 {
     if (lane < 32) reinterpret_cast<float*>(tile + V_BYTES)[lane] = vs;
   }
 
-  __device__ __forceinline__ void math(const uint8_t* tile, const Regs& r, int kv0, int end,
-                                       float scale_log2) {
-    const int lane = threadIdx.x & 63;
-    const int l16 = lane & 15, lg = lane >> 4;
-    f32x4 st[2];
+  // S^T of the sub-tile: st[tt] register i = row l16, position tt * 16 + lg * 4 + i.
+  __device__ __forceinline__ void scores(const Regs& r, f32x4 (&st)[2]) const {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
       float ks, vs;
@@ -154,6 +153,13 @@ struct RowEngine8 {
         st[tt] = mfma16x16x32(kv8_dequant8(w[0], w[1], ks), qf[2 * K16 + c], st[tt]);
       }
     }
+  }
+
+  // Softmax and O^T of the sub-tile whose V is in the wavefront's LDS tile.
+  __device__ __forceinline__ void update(const uint8_t* tile, const f32x4 (&st)[2], int kv0, int end,
+                                         float scale_log2) {
+    const int lane = threadIdx.x & 63;
+    const int l16 = lane & 15, lg = lane >> 4;
     // V^T: group lg reads the 8 positions of its lanes' scores, each row's 16
     // bytes by two lanes.
     const int rr = l16 >> 1;
@@ -311,8 +317,86 @@ struct Item8 {
   static constexpr int LDS_BYTES = NW * (WAVE_BYTES + STAGE_BYTES);
 };
 
+// A row's new token as the cache holds it: two values of K and of V per lane
+// (lanes below D / 2).
+template <int D>
+struct NewToken {
+  uint32_t code[2];  // K, V
+  uint32_t rec;
+  bool in_pool;      // the row's last page id is: the token is attended to
+
+  static __device__ __forceinline__ bool mine() { return (int)(threadIdx.x & 63) < D / 2; }
+
+  // kr, vr: the token's rows, 4-byte aligned, in memory or LDS
+  __device__ __forceinline__ void quantize(const bf16* kr, const bf16* vr) {
+    const int lane = threadIdx.x & 63;
+    uint32_t x[2] = {0u, 0u};
+    if (mine()) {
+      x[0] = reinterpret_cast<const uint32_t*>(kr)[lane];
+      x[1] = reinterpret_cast<const uint32_t*>(vr)[lane];
+    }
+    rec = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      bool bad = false;
+      uint32_t m = max(kv8_mag(x[w] & 0xffffu, bad), kv8_mag(x[w] >> 16, bad));
+      m = row16_max_u(m);
+      m = __float_as_uint(xrow_max(__uint_as_float(m)));
+      const bool row_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+      const int e = kv8_exp(m);
+      code[w] = kv8_codes2(lo_bf16(x[w]), hi_bf16(x[w]), kv8_pow2(-e));
+      rec |= kv8_scale_bits(e, row_bad) << (16 * w);
+    }
+  }
+  __device__ __forceinline__ void write(const Kv8Layer& kv, int h, int64_t slot) const {
+    const int lane = threadIdx.x & 63;
+    if (mine()) {
+      const int64_t off = slot * (int64_t)kv.tok_bytes + h * D + lane * 2;
+      *reinterpret_cast<uint16_t*>(kv.k + off) = (uint16_t)code[0];
+      *reinterpret_cast<uint16_t*>(kv.v + off) = (uint16_t)code[1];
+    }
+    if (lane == 0) kv.scales[(int64_t)h * kv.num_pages + slot] = rec;
+  }
+  // In place of position tl of a sub-tile's registers, by way of the token's
+  // V row of the wavefront's LDS tile (K's codes first, then V's).
+  template <class E>
+  __device__ __forceinline__ void put(uint8_t* tile, int tl, typename E::Regs& r) const {
+    const int lane = threadIdx.x & 63;
+    const int l16 = lane & 15, lg = lane >> 4;
+    uint8_t* row = tile + tl * D;
+    if (mine()) reinterpret_cast<uint16_t*>(row)[lane] = (uint16_t)code[0];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const bool at = l16 + 16 * tt == tl;
+      if (at) r.rec[tt] = rec;
+#pragma unroll
+      for (int c = 0; c < E::K16; ++c) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(row + c * 64 + lg * 16);
+        if (at) r.k16[tt][c] = w;
+      }
+#pragma unroll
+      for (int c = 0; c < E::K8; ++c) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(row + E::K16 * 64 + c * 32 + lg * 8);
+        if (at) r.k8[tt][c] = w;
+      }
+    }
+    if (mine()) reinterpret_cast<uint16_t*>(row)[lane] = (uint16_t)code[1];
+#pragma unroll
+    for (int j = 0; j < E::NV; ++j) {
+      const int ch = j * 64 + lane;
+      const int t = ch / E::CH;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(row + (ch - t * E::CH) * 16);
+      if (t == tl) r.v[j] = w;
+    }
+  }
+};
+
+// Positions [s_begin, s_end) of row b for kv-head h, as part `part` of the row
+// (or its output); kv_len positions with page ids idx.
 template <int D, int G, bool ROPE>
-__device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a, int item) {
+__device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a, int b, int h,
+                                             const int32_t* idx, int kv_len, int s_begin, int s_end,
+                                             int part) {
   using I = Item8<D, G>;
   using E = typename I::E;
   using RP = typename I::RP;
@@ -324,18 +408,8 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
   const int lg = lane >> 4;
   uint8_t* buf = lds + wave * I::WAVE_BYTES;
   uint8_t* stage = lds + NW * I::WAVE_BYTES + wave * I::STAGE_BYTES;
-  const int split = item % a.n_splits;
-  const int bh = item / a.n_splits;
-  const int h = bh % a.num_kv_heads;
-  const int b = bh / a.num_kv_heads;
-
-  const int base = a.cu_k[b];
-  const int kv_len = a.cu_k[b + 1] - base;
-  const int s_begin = a.prefix_len + split * a.split_len;
-  const int s_end = min(kv_len, s_begin + a.split_len);
   const bool append = a.out_loc != nullptr;
   const int t_new = append ? kv_len - 1 : -1;
-  const int32_t* idx = a.indices + base;
 
   E eng;
   eng.reset();
@@ -345,12 +419,15 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
   const bf16* vn = append ? a.v_new + (int64_t)b * a.v_new_stride + (int64_t)h * D : nullptr;
   const int kv0_first = s_begin + wave * kSubTok;
   if (kv0_first < s_end) {
-    typename E::Regs r0, r1;
-    typename E::Ids i0, i1;
+    typename E::Regs r;
+    typename E::Ids id;
     constexpr int STEP = NW * kSubTok;
-    E::ids(idx, kv0_first, s_end - 1, i0);
-    E::ids(idx, kv0_first + STEP, s_end - 1, i1);
-    E::load(hd, i0, kv0_first, s_end, t_new, r0);
+    // The wavefront whose sub-tile holds the new token.
+    const bool has_new = t_new >= s_begin && t_new < s_end &&
+                         ((t_new - s_begin) / kSubTok & (NW - 1)) == wave;
+    E::ids(idx, kv0_first, s_end - 1, id);
+    E::load(hd, id, kv0_first, s_end, t_new, r);
+    E::ids(idx, kv0_first + STEP, s_end - 1, id);
     if constexpr (ROPE) {
       const int64_t pos = (int64_t)a.positions[b];
       const int64_t rrow = min(max(pos, (int64_t)0), a.rope_rows - 1);
@@ -361,88 +438,33 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
     } else {
       eng.load_q(qrow0 + (int64_t)min(l16, G - 1) * D, l16 < G);
     }
-    // The sub-tile that holds the new token: its rows are quantised here (K
-    // rotated from the staging area), written to page out_loc[b] and, where
-    // the row's last page id is in the pool, put in the token's place.
-    auto take_new = [&](int kv0, typename E::Regs& r) {
-      const int tl = t_new - kv0;
+    // The new token's rows are quantised here (K rotated from the staging
+    // area) and written to page out_loc[b]; code and rec keep them for its
+    // sub-tile.  (Nothing in the loop below may load or store memory but the
+    // sub-tiles ahead: loads and stores complete in order, and behind a branch
+    // that may hold others the compiler waits for all of them.)
+    NewToken<D> nt;
+    if (has_new) {
+      const bf16* kr = ROPE ? reinterpret_cast<const bf16*>(stage) + G * D : kn;
       const int64_t slot = a.out_loc[b];
-      const bool slot_ok = slot >= 0 && slot < a.kv.num_pages;
-      const bool page_ok = (uint32_t)idx[t_new] < hd.n_pages;
-      constexpr int W = D / 2;  // words of a bf16 row, one per lane
-      const bool has = lane < W;
-      const uint32_t* kw = reinterpret_cast<const uint32_t*>(
-          ROPE ? reinterpret_cast<const bf16*>(stage) + G * D : kn);
-      uint32_t x[2] = {0u, 0u};
-      if (has) {
-        x[0] = kw[lane];
-        x[1] = reinterpret_cast<const uint32_t*>(vn)[lane];
-      }
-      uint32_t rec = 0;
-      uint32_t code[2];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        bool bad = false;
-        uint32_t m = max(kv8_mag(x[w] & 0xffffu, bad), kv8_mag(x[w] >> 16, bad));
-        m = row16_max_u(m);
-        m = __float_as_uint(xrow_max(__uint_as_float(m)));
-        const bool row_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-        const int e = kv8_exp(m);
-        code[w] = kv8_codes2(lo_bf16(x[w]), hi_bf16(x[w]), kv8_pow2(-e));
-        rec |= kv8_scale_bits(e, row_bad) << (16 * w);
-      }
-      // codes in the tile's V row of the token (K's first, read back by the
-      // lanes that hold the token, then V's)
-      uint8_t* row = buf + tl * D;
-      if (page_ok) {
-        if (has) reinterpret_cast<uint16_t*>(row)[lane] = (uint16_t)code[0];
-        const bool mine0 = tl < 16 && l16 == tl, mine1 = tl >= 16 && l16 == tl - 16;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          const bool mine = tt ? mine1 : mine0;
-          if (mine) r.rec[tt] = rec;
-#pragma unroll
-          for (int c = 0; c < E::K16; ++c) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(row + c * 64 + lg * 16);
-            if (mine) r.k16[tt][c] = w;
-          }
-#pragma unroll
-          for (int c = 0; c < E::K8; ++c) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(row + E::K16 * 64 + c * 32 + lg * 8);
-            if (mine) r.k8[tt][c] = w;
-          }
-        }
-        if (has) reinterpret_cast<uint16_t*>(row)[lane] = (uint16_t)code[1];
-#pragma unroll
-        for (int j = 0; j < E::NV; ++j) {
-          const int ch = j * 64 + lane;
-          const int t = ch / E::CH;
-          const u32x4 w = *reinterpret_cast<const u32x4*>(row + (ch - t * E::CH) * 16);
-          if (t == tl) r.v[j] = w;
-        }
-      }
-      if (slot_ok) {
-        const int64_t off = slot * (int64_t)a.kv.tok_bytes + h * D + lane * 2;
-        if (has) {
-          *reinterpret_cast<uint16_t*>(a.kv.k + off) = (uint16_t)code[0];
-          *reinterpret_cast<uint16_t*>(a.kv.v + off) = (uint16_t)code[1];
-        }
-        if (lane == 0) a.kv.scales[(int64_t)h * a.kv.num_pages + slot] = rec;
-      }
-    };
-    auto step = [&](int kv0, typename E::Regs& r, typename E::Regs& rn, typename E::Ids& i,
-                    typename E::Ids& in) {
-      if (kv0 + STEP < s_end) {
-        E::load(hd, in, kv0 + STEP, s_end, t_new, rn);
-        E::ids(idx, kv0 + 2 * STEP, s_end - 1, i);
-      }
-      if (kv0 <= t_new && t_new < kv0 + kSubTok && t_new < s_end) take_new(kv0, r);
+      nt.quantize(kr, vn);
+      nt.in_pool = (uint32_t)idx[t_new] < hd.n_pages;
+      if (slot >= 0 && slot < a.kv.num_pages) nt.write(a.kv, h, slot);
+    }
+    // One set of registers per sub-tile: K is used up by the scores and V by
+    // its LDS store, so the next sub-tile's loads go out ahead of the softmax
+    // and the O^T update, and three workgroups fit a unit.
+    for (int kv0 = kv0_first; kv0 < s_end; kv0 += STEP) {
+      if (has_new && nt.in_pool && kv0 <= t_new && t_new < kv0 + kSubTok)
+        nt.template put<E>(buf, t_new - kv0, r);
+      f32x4 st[2];
       E::store_v(buf, r);
-      eng.math(buf, r, kv0, s_end, a.scale_log2);
-    };
-    for (int kv0 = kv0_first; kv0 < s_end; kv0 += 2 * STEP) {
-      step(kv0, r0, r1, i0, i1);
-      if (kv0 + STEP < s_end) step(kv0 + STEP, r1, r0, i1, i0);
+      eng.scores(r, st);
+      // (past the item's end: zeros, without a memory access)
+      E::load(hd, id, kv0 + STEP, s_end, t_new, r);
+      E::ids(idx, kv0 + 2 * STEP, s_end - 1, id);
+      __builtin_amdgcn_sched_barrier(0);
+      eng.update(buf, st, kv0, s_end, a.scale_log2);
     }
   }
   eng.ls = xrow_sum(eng.ls);
@@ -489,7 +511,7 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
   };
 
   if (a.wave_parts) {
-    write_rows(eng.o, eng.ls, eng.m_run, buf, a.parts.n_chunks + split * NW + wave, false);
+    write_rows(eng.o, eng.ls, eng.m_run, buf, part + wave, false);
     return;
   }
 
@@ -533,7 +555,66 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
     for (int w = 1; w < NW; ++w)
       acc[dt] += reinterpret_cast<const f32x4*>(lds + w * I::WAVE_BYTES)[dt * 64 + lane] * f[w];
   }
-  write_rows(acc, l_tot, mx, buf, a.parts.n_chunks + split, a.final_out != 0);
+  write_rows(acc, l_tot, mx, buf, part, a.final_out != 0);
+}
+
+// A row's own positions in parts of at most `most` (split: how many, and the
+// length of each but the last).
+__device__ __forceinline__ int row_parts(int own, int most) { return (own + most - 1) / most; }
+__device__ __forceinline__ int row_part_len(int own, int parts) {
+  return ((own + parts - 1) / parts + kSubTok - 1) / kSubTok * kSubTok;
+}
+
+template <int D, int G, bool ROPE>
+__device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a, int item) {
+  int h, b, base, kv_len, s_begin, s_end, part = a.parts.n_chunks;
+  if (!a.split) {
+    h = item % a.num_kv_heads;
+    b = item / a.num_kv_heads;
+    base = a.cu_k[b];
+    kv_len = a.cu_k[b + 1] - base;
+    s_begin = a.prefix_len;
+    s_end = kv_len;
+  } else {
+    // Part w of head h's list of all rows' parts, found from the lengths: lane
+    // i counts the parts of row i.  (Parts side by side are one row's: heads
+    // side by side read one page's rows from eight XCDs at once, 5 to 10% less
+    // bandwidth.)
+    const int lane = threadIdx.x & 63;
+    h = item / a.n_splits;
+    int w = item - h * a.n_splits;
+    int own = 0, at = 0, n = 0, i = 0;
+    for (int b0 = 0;; b0 += 64) {
+      if (b0 >= a.batch) return;  // (fewer parts than the plan's longest rows have)
+      i = b0 + lane;
+      at = a.cu_k[min(i, a.batch)];
+      own = i < a.batch ? a.cu_k[min(i + 1, a.batch)] - at - a.prefix_len : 0;
+      n = row_parts(own, a.split_len);
+      int sum = n;
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) {
+        const int v = __shfl_up(sum, k);
+        if (lane >= k) sum += v;
+      }
+      const uint64_t past = __builtin_amdgcn_ballot_w64(sum > w);
+      if (past) {
+        const int src = __ffsll((unsigned long long)past) - 1;
+        b = b0 + src;
+        base = __builtin_amdgcn_readlane(at, src);
+        own = __builtin_amdgcn_readlane(own, src);
+        n = __builtin_amdgcn_readlane(n, src);
+        w -= __builtin_amdgcn_readlane(sum, src) - n;
+        break;
+      }
+      w -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    const int len = row_part_len(own, n);
+    kv_len = own + a.prefix_len;
+    s_begin = a.prefix_len + w * len;
+    s_end = min(kv_len, s_begin + len);
+    part += w;
+  }
+  decode8_rows<D, G, ROPE>(lds, a, b, h, a.indices + base, kv_len, s_begin, s_end, part);
 }
 
 template <int D, int G>
@@ -545,7 +626,7 @@ constexpr int decode8_lds(bool prefix) {
 // PREFIX: the launch has prefix workgroups (first: they carry most bytes);
 // without them the row items' smaller LDS lets more workgroups share a unit.
 template <int D, int G, bool ROPE, bool PREFIX>
-__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void decode8_main_kernel(
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(PREFIX ? 2 : 3, PREFIX ? 2 : 8))) void decode8_main_kernel(
     Decode8Args a) {
   __shared__ __align__(16) uint8_t lds[decode8_lds<D, G>(PREFIX)];
   const int wg = blockIdx.x;
@@ -580,7 +661,9 @@ __global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(Decode8A
   const int wave = tid >> 6;
   const int b = blockIdx.x / a.num_kv_heads;
   const int h = blockIdx.x - b * a.num_kv_heads;
-  const int np = a.parts.n_parts;
+  int np = a.parts.n_parts;
+  if (a.split)
+    np = a.parts.n_chunks + row_parts(a.cu_k[b + 1] - a.cu_k[b] - a.prefix_len, a.split_len);
   const int e = tid % E8;
   const int r = tid / E8;
   const bool active = r < R;

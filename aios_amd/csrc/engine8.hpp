@@ -117,10 +117,10 @@ struct Stage8 {
     const bool act = __builtin_amdgcn_readfirstlane((int)active) != 0;
     auto step = [&](int s, Regs& r, Ids& i, int slot) {
       store(lds, slot, r);
-      if (s + 2 < n) {
-        load(s + 2, i, r);
-        ids(s + 4, i);
-      }
+      // (unconditional, past the range without a memory access: behind a
+      // branch around loads the compiler waits for all that are in flight)
+      load(s + 2, i, r);
+      ids(s + 4, i);
       lds_barrier();  // the slot is written; every wavefront is done with the other one's readers
       if (act) {
         const int kv0 = begin + s * kStep8;
@@ -130,7 +130,8 @@ struct Stage8 {
     };
     for (int s = 0; s < n; s += 2) {
       step(s, r0, i0, 0);
-      if (s + 1 < n) step(s + 1, r1, i1, 1);
+      if (s + 1 >= n) break;
+      step(s + 1, r1, i1, 1);
     }
   }
 };

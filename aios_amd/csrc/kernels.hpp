@@ -371,7 +371,9 @@ struct Decode8Args {
   int32_t m_rows;
   int32_t prefix_units;
   int32_t prefix_wgs;
-  // the rows' own positions: (row, kv-head, split) items
+  // the rows' own positions: (row, kv-head) items, or (split) n_splits parts
+  // per kv-head, a row's own positions in equal parts of at most split_len
+  int32_t split;
   int32_t split_len;
   int32_t n_splits;
   int32_t suffix_items;
