@@ -161,11 +161,12 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
                      a.scale_log2);
   } else {
     // (more KV positions than the plan was built for)
-    st.stream(lds, [&] { eng.load_q(qr, ok); },
-              [&](uint32_t sb, int kv0) {
-                if (share == 0) eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
-              },
-              true);
+    st.template stream<1>(
+        lds, [&] { eng.load_q(qr, ok); },
+        [&](uint32_t sb, int kv0) {
+          if (share == 0) eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
+        },
+        true);
   }
 
   static_assert(T::SUB_BYTES == 32 * D * 4, "a row tile's fp32 o fills one sub-tile");

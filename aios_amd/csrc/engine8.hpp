@@ -100,27 +100,30 @@ struct Stage8 {
   }
 
   // Runs math(sb, kv0) on every sub-tile of the range (sb: its byte offset in
-  // lds); `qload()` issues the Q loads behind the first loads.
-  template <typename QLoad, typename Math>
+  // lds); `qload()` issues the Q loads behind the first loads.  AHEAD: steps in
+  // flight.  One (the prefill, whose math of a step outlasts a load) needs one
+  // set of registers, used up by the step's LDS store; two put both steps of a
+  // short range in flight at once.
+  template <int AHEAD, typename QLoad, typename Math>
   __device__ __forceinline__ void stream(uint8_t* lds, QLoad&& qload, Math&& math, bool active) {
     const int n = steps();
     if (n <= 0) return;
+    const bool act = __builtin_amdgcn_readfirstlane((int)active) != 0;
     Regs r0, r1;
     Ids i0, i1;
     ids(0, i0);
-    ids(1, i1);
+    if constexpr (AHEAD == 2) ids(1, i1);
     load(0, i0, r0);
     qload();
-    load(1, i1, r1);  // (past the range: zeros, without a memory access)
-    ids(2, i0);
-    ids(3, i1);
-    const bool act = __builtin_amdgcn_readfirstlane((int)active) != 0;
+    if constexpr (AHEAD == 2) load(1, i1, r1);  // (past the range: zeros, without a memory access)
+    ids(AHEAD, i0);
+    if constexpr (AHEAD == 2) ids(3, i1);
     auto step = [&](int s, Regs& r, Ids& i, int slot) {
       store(lds, slot, r);
       // (unconditional, past the range without a memory access: behind a
       // branch around loads the compiler waits for all that are in flight)
-      load(s + 2, i, r);
-      ids(s + 4, i);
+      load(s + AHEAD, i, r);
+      ids(s + 2 * AHEAD, i);
       lds_barrier();  // the slot is written; every wavefront is done with the other one's readers
       if (act) {
         const int kv0 = begin + s * kStep8;
@@ -128,10 +131,14 @@ struct Stage8 {
         if (kv0 + kSubTok < end) math((uint32_t)(slot * STEP_BYTES + T::SUB_BYTES), kv0 + kSubTok);
       }
     };
-    for (int s = 0; s < n; s += 2) {
-      step(s, r0, i0, 0);
-      if (s + 1 >= n) break;
-      step(s + 1, r1, i1, 1);
+    if constexpr (AHEAD == 1) {
+      for (int s = 0; s < n; ++s) step(s, r0, i0, s & 1);
+    } else {
+      for (int s = 0; s < n; s += 2) {
+        step(s, r0, i0, 0);
+        if (s + 1 >= n) break;
+        step(s + 1, r1, i1, 1);
+      }
     }
   }
 };
@@ -145,8 +152,9 @@ __device__ __forceinline__ void run_tile8(TileEngine32<D, CAUSAL>& eng, uint8_t*
   eng.reset();
   const auto lo = eng.lane_offsets(lds);
   Stage8<D> st(kv, h, idx, kv_begin, kv_end);
-  st.stream(lds, qload,
-            [&](uint32_t sb, int kv0) { eng.compute_at(lo, sb, kv0, kv_end, scale_log2); }, active);
+  st.template stream<CAUSAL ? 1 : 2>(
+      lds, qload,
+      [&](uint32_t sb, int kv0) { eng.compute_at(lo, sb, kv0, kv_end, scale_log2); }, active);
   if constexpr (CAUSAL) eng.l_run = eng.ol[0];
   else eng.l_run = xor32_sum(eng.ls);
 }
