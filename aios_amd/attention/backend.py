@@ -15,6 +15,11 @@ Public surface follows python/aios/attention/flashinfer.py:94-394:
   (aios_attn_append_decode).
 * ``metadata.get_last_indices(bs)`` = ``cu_seqlens_q[1:bs+1] - 1``.
 
+A pool in 8 bits (``MHAKVCache8``) is read by the kernels of that cache: its
+plans are those of aios_attn_plan8, made where the context's cache is such a
+pool (or ``kv_bits=8`` is given), and forward and forward_rope follow the
+pool they are given.
+
 There is one code path for every supported head dim (64, 96, 128), so the
 reference's torch-SDPA fallback for head_dim 96 (flashinfer.py:19-24,
 328-372) has no counterpart here.
@@ -36,8 +41,8 @@ from typing import TYPE_CHECKING
 import torch
 
 from aios_amd import _lib, paged
-from aios_amd.core import get_global_ctx, runs_as_built
-from aios_amd.kvcache import MHAKVCache
+from aios_amd.core import get_global_ctx, has_global_ctx, runs_as_built
+from aios_amd.kvcache import MHAKVCache, MHAKVCache8
 
 from .base import BaseAttentionBackend, BaseAttentionMetadata
 
@@ -159,6 +164,30 @@ def check_decode_preconditions(indices: torch.Tensor, cu_seqlens_k: torch.Tensor
 
 # What the one-launch append stands for, as this package defines it.
 _POOL = tuple((name, getattr(MHAKVCache, name)) for name in ("store_kv", "k_cache", "v_cache"))
+_POOL8 = tuple((name, getattr(MHAKVCache8, name))
+               for name in ("store_kv", "k_cache", "v_cache", "scales", "layer"))
+
+
+def _kv_bits(pool) -> int:
+    """8 for a pool of float8 codes with their scales (MHAKVCache8 or what
+    wraps one), else 16."""
+    return 8 if getattr(pool, "dtype", None) == torch.float8_e4m3fn and hasattr(pool, "layer") else 16
+
+
+def _make_plan(kv_bits: int):
+    """The planning call for a cache of kv_bits (8 or 16), and its name."""
+    if kv_bits == 8:
+        return _lib.lib().aios_attn_plan8, "aios_attn_plan8"
+    return _lib.lib().aios_attn_plan, "aios_attn_plan"
+
+
+def _context_kv_bits(kv_bits: int | None) -> int:
+    """kv_bits, or those of the context's cache."""
+    if kv_bits is None:
+        return _kv_bits(getattr(get_global_ctx(), "kv_cache", None)) if has_global_ctx() else 16
+    if kv_bits not in (8, 16):
+        raise ValueError("kv_bits must be 8 or 16")
+    return kv_bits
 
 
 class Mi355xAttentionBackend(BaseAttentionBackend):
@@ -245,8 +274,9 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
 
         shared = int(getattr(batch, "shared_prefix_len", 0)) if batch.is_decode else 0
         plan = _lib.AttnPlan()
+        make, name = _make_plan(_kv_bits(ctx.kv_cache))
         _lib.check(
-            _lib.lib().aios_attn_plan(
+            make(
                 _lib.PHASE_DECODE if batch.is_decode else _lib.PHASE_PREFILL,
                 cu_q.data_ptr(),
                 cu_k.data_ptr(),
@@ -261,7 +291,7 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
                 self.suffix_split_len,
                 plan,
             ),
-            "aios_attn_plan",
+            name,
         )
 
         indices = torch.empty(total_kv, dtype=torch.int32, device=device)
@@ -305,10 +335,12 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         return metadata
 
     def prepare_static_decode(self, row_ids: torch.Tensor, max_kv_len: int, shared_prefix_len: int,
-                              page_table: torch.Tensor) -> Mi355xStaticDecodeMetadata:
+                              page_table: torch.Tensor,
+                              kv_bits: int | None = None) -> Mi355xStaticDecodeMetadata:
         """Fixed-buffer decode metadata for graph-replayed steps (see
         :class:`Mi355xStaticDecodeMetadata`); ``shared_prefix_len`` may be any
-        length up to the prefix every row really shares."""
+        length up to the prefix every row really shares.  ``kv_bits``: of the
+        cache the steps read (default: the context's)."""
         bs = row_ids.numel()
         device = page_table.device
         if page_table.dtype != torch.int32 or max_kv_len > page_table.shape[1]:
@@ -316,12 +348,13 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         cu_q = torch.arange(bs + 1, dtype=torch.int32)
         cu_k = cu_q * max_kv_len
         plan = _lib.AttnPlan()
+        kv_bits = _context_kv_bits(kv_bits)
+        make, name = _make_plan(kv_bits)
         _lib.check(
-            _lib.lib().aios_attn_plan(_lib.PHASE_DECODE, cu_q.data_ptr(), cu_k.data_ptr(), bs,
-                                      self.num_heads, self.num_kv_heads, self.head_dim, 1,
-                                      shared_prefix_len, self.workspace_size,
-                                      self.prefix_chunk_len, self.suffix_split_len, plan),
-            "aios_attn_plan",
+            make(_lib.PHASE_DECODE, cu_q.data_ptr(), cu_k.data_ptr(), bs, self.num_heads,
+                 self.num_kv_heads, self.head_dim, 1, shared_prefix_len, self.workspace_size,
+                 self.prefix_chunk_len, self.suffix_split_len, plan),
+            name,
         )
         if plan.ws_bytes:
             self._get_workspace(device)
@@ -339,7 +372,7 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             page_size=1,
             pos_encoding_mode="NONE",
             seq_lens_cpu=torch.full((bs,), max_kv_len, dtype=torch.int32),
-            dtype=torch.bfloat16,
+            dtype=torch.float8_e4m3fn if kv_bits == 8 else torch.bfloat16,
             plan=plan,
             shared_prefix_len=shared_prefix_len,
             host_staging=cu_q,
@@ -350,10 +383,12 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         )
 
     def prepare_static_prefill(self, q_len: int, max_kv_len: int, page_table: torch.Tensor,
-                               row_id: int = 0) -> Mi355xStaticPrefillMetadata:
+                               row_id: int = 0,
+                               kv_bits: int | None = None) -> Mi355xStaticPrefillMetadata:
         """Fixed-buffer prefill metadata for graph-replayed prefills of
         ``q_len`` tokens against at most ``max_kv_len`` positions (see
-        :class:`Mi355xStaticPrefillMetadata`)."""
+        :class:`Mi355xStaticPrefillMetadata`); ``kv_bits`` as for
+        prepare_static_decode."""
         device = page_table.device
         if page_table.dtype != torch.int32 or max_kv_len > page_table.shape[1]:
             raise ValueError("max_kv_len exceeds the page-table row length")
@@ -362,12 +397,13 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         cu_q = torch.tensor([0, q_len], dtype=torch.int32)
         cu_k = torch.tensor([0, max_kv_len], dtype=torch.int32)
         plan = _lib.AttnPlan()
+        kv_bits = _context_kv_bits(kv_bits)
+        make, name = _make_plan(kv_bits)
         _lib.check(
-            _lib.lib().aios_attn_plan(_lib.PHASE_PREFILL, cu_q.data_ptr(), cu_k.data_ptr(), 1,
-                                      self.num_heads, self.num_kv_heads, self.head_dim, 1, 0,
-                                      self.workspace_size, self.prefix_chunk_len,
-                                      self.suffix_split_len, plan),
-            "aios_attn_plan",
+            make(_lib.PHASE_PREFILL, cu_q.data_ptr(), cu_k.data_ptr(), 1, self.num_heads,
+                 self.num_kv_heads, self.head_dim, 1, 0, self.workspace_size,
+                 self.prefix_chunk_len, self.suffix_split_len, plan),
+            name,
         )
         ramp = torch.arange(2, dtype=torch.int32, device=device)
         return Mi355xStaticPrefillMetadata(
@@ -383,7 +419,7 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             page_size=1,
             pos_encoding_mode="NONE",
             seq_lens_cpu=torch.tensor([max_kv_len], dtype=torch.int32),
-            dtype=torch.bfloat16,
+            dtype=torch.float8_e4m3fn if kv_bits == 8 else torch.bfloat16,
             plan=plan,
             shared_prefix_len=0,
             host_staging=cu_q,
@@ -458,6 +494,12 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             check_decode_preconditions(metadata.indices, metadata.cu_seqlens_k_gpu, out_loc,
                                        metadata.shared_prefix_len)
         ws = self._get_workspace(q.device) if plan.ws_bytes else None
+        if _kv_bits(paged_kv_cache) == 8:
+            out = paged.append_decode_rope8(plan, q, k, v, out_loc.contiguous(),
+                                            *paged_kv_cache.layer(layer_id), metadata.indices,
+                                            metadata.cu_seqlens_k_gpu, q_norm, k_norm, cos, sin,
+                                            positions, eps, workspace=ws, sm_scale=self.sm_scale)
+            return out.reshape(bsz, -1)
         k_cache, v_cache = self._layer_caches(paged_kv_cache, layer_id)
         out = paged.append_decode_rope(plan, q, k, v, out_loc.contiguous(),
                                        k_cache.view(-1, self.num_kv_heads, self.head_dim),
@@ -492,6 +534,8 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         if q.shape[0] != metadata.plan.total_q:
             raise RuntimeError("prefill request lengths do not match flat Q tokens")
         paged_kv_cache.store_kv(k, v, batch.out_loc.view(-1), layer_id)
+        if _kv_bits(paged_kv_cache) == 8:
+            return self.prefill8_appended(q, *paged_kv_cache.layer(layer_id), batch)
         return self.prefill_appended(q, *self.layer_kv(paged_kv_cache, layer_id), batch)
 
     def append_rope_applies(self, qkv: torch.Tensor, paged_kv_cache, batch: Batch) -> bool:
@@ -504,11 +548,33 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             return False
         if not (runs_as_built(self, _FORWARD) and runs_as_built(paged_kv_cache, _POOL)):
             return False  # (a caller's own forward or store_kv sees every call)
+        return paged_kv_cache.dtype == torch.bfloat16 and self._append_rows(qkv, paged_kv_cache,
+                                                                            batch)
+
+    def append_rope8_applies(self, qkv: torch.Tensor, paged_kv_cache, batch: Batch) -> bool:
+        """append_rope_applies for a pool in 8 bits (then prefill8_appended on
+        its layer runs the rest)."""
+        if not batch.is_prefill or not isinstance(batch.attn_metadata, Mi355xAttentionMetadata):
+            return False
+        if not (runs_as_built(self, _FORWARD) and runs_as_built(paged_kv_cache, _POOL8)):
+            return False
+        return self._append_rows(qkv, paged_kv_cache, batch)
+
+    def _append_rows(self, qkv: torch.Tensor, paged_kv_cache, batch: Batch) -> bool:
         loc = batch.out_loc
         return (paged_kv_cache.row_shape == (self.num_kv_heads, self.head_dim)
-                and paged_kv_cache.dtype == torch.bfloat16 and qkv.dtype == torch.bfloat16
+                and qkv.dtype == torch.bfloat16
                 and loc.dtype == torch.int32 and loc.is_contiguous() and loc.is_cuda
                 and loc.numel() == qkv.shape[0] == batch.attn_metadata.plan.total_q)
+
+    def prefill8_appended(self, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+                          scales: torch.Tensor, batch: Batch) -> torch.Tensor:
+        """prefill_appended over one layer of a pool in 8 bits."""
+        metadata = batch.attn_metadata
+        out = paged.prefill8(metadata.plan, q, k8, v8, scales, metadata.indices,
+                             metadata.cu_seqlens_q_gpu, metadata.cu_seqlens_k_gpu,
+                             sm_scale=self.sm_scale)
+        return out.reshape(q.size(0), -1)
 
     def layer_kv(self, paged_kv_cache, layer_id: int) -> tuple[torch.Tensor, torch.Tensor]:
         """One layer's K and V caches as [pages, Hkv, D]."""
@@ -549,6 +615,12 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
                 raise ValueError("K/V input shape does not match the cache layout")
             if out_loc.numel() != k.shape[0]:
                 raise ValueError("KV write indices and K/V tensors must have matching token counts")
+            if _kv_bits(paged_kv_cache) == 8:
+                out = paged.append_decode8(plan, q, k, v, out_loc.contiguous(),
+                                           *paged_kv_cache.layer(layer_id), metadata.indices,
+                                           metadata.cu_seqlens_k_gpu, workspace=ws,
+                                           sm_scale=self.sm_scale)
+                return out.reshape(bsz, -1)
             k_cache, v_cache = self._layer_caches(paged_kv_cache, layer_id)
             out = paged.append_decode(plan, q, k, v, out_loc.contiguous(),
                                       k_cache.view(-1, self.num_kv_heads, self.head_dim),
@@ -557,6 +629,10 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
                                       sm_scale=self.sm_scale)
             return out.reshape(bsz, -1)
         paged_kv_cache.store_kv(k, v, out_loc, layer_id)
+        if _kv_bits(paged_kv_cache) == 8:
+            out = paged.decode8(plan, q, *paged_kv_cache.layer(layer_id), metadata.indices,
+                                metadata.cu_seqlens_k_gpu, workspace=ws, sm_scale=self.sm_scale)
+            return out.reshape(bsz, -1)
         k_cache, v_cache = self._layer_caches(paged_kv_cache, layer_id)
         out = paged.decode(plan, q, k_cache.view(-1, self.num_kv_heads, self.head_dim),
                            v_cache.view(-1, self.num_kv_heads, self.head_dim), metadata.indices,

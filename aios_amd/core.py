@@ -146,6 +146,10 @@ def get_global_ctx() -> Context:
     return _GLOBAL_CTX
 
 
+def has_global_ctx() -> bool:
+    return _GLOBAL_CTX is not None
+
+
 def reset_global_ctx() -> None:
     """Drop the process-global context (tests and benches build several)."""
     global _GLOBAL_CTX

@@ -24,7 +24,8 @@ aios_stateless_uniforms).  Without it (the greedy configurations),
 candidate i starts from the i-th most likely first token and then decodes
 greedily (aios_greedy_select).  Either way each token's raw log-prob is
 kept and candidates are ranked by average raw log-prob (the reference's
-base score before text penalties, :1109-1115).  Text governance and
+base score before text penalties, :1109-1115).  ``CandidateGroupEngine.score``
+ranks continuations the caller brings by the same log-probs.  Text governance and
 refill rounds are not restated (no tokenizer ships with the synthetic
 models).
 """
@@ -42,8 +43,8 @@ from aios_amd import _lib
 from aios_amd.config import ModelConfig
 from aios_amd.core import (Batch, Context, Req, SamplingParams, captured, reset_global_ctx,
                            set_global_ctx)
-from aios_amd.sample import sample_step, stateless_uniforms
-from aios_amd.kvcache import MHAKVCache
+from aios_amd.sample import MAX_TOP_LOGPROBS, sample_step, stateless_uniforms, token_logprobs
+from aios_amd.kvcache import MHAKVCache, MHAKVCache8
 from aios_amd.paged import greedy_select
 from aios_amd.minimind_ime import build_causal_lm
 from aios_amd.scheduler import CacheManager
@@ -218,6 +219,23 @@ class CompletionResult:
     replayed_steps: int = 0
 
 
+@dataclass(frozen=True)
+class ScoredContinuation:
+    """The model's view of one given continuation: each token's raw log-prob
+    after the prefix and the tokens before it, the entropy of the distribution
+    it was drawn from, and that distribution's most likely tokens
+    ((token id, log-prob), most likely first)."""
+
+    token_ids: tuple[int, ...]
+    logprobs: tuple[float, ...]
+    entropies: tuple[float, ...]
+    alternatives: tuple[tuple[tuple[int, float], ...], ...] = ()
+
+    @property
+    def average_logprob(self) -> float:
+        return sum(self.logprobs) / len(self.logprobs)
+
+
 def select_top(candidates, k: int) -> tuple[Candidate, ...]:
     """Highest average log-prob first, distinct token sequences only."""
     seen = set()
@@ -234,20 +252,27 @@ def select_top(candidates, k: int) -> tuple[Candidate, ...]:
 
 class CandidateGroupRuntime:
     """Model + paged KV pool + page allocator + global context on one GPU
-    (the parts of python/aios/llm/llm.py:27-96 the IME path uses)."""
+    (the parts of python/aios/llm/llm.py:27-96 the IME path uses).
+    ``kv_bits=8`` keeps the pool in 8 bits (MHAKVCache8): half the bytes of a
+    page, and of what a decode step reads."""
 
     def __init__(self, config: ModelConfig, weights: dict, device="cuda", num_pages: int = 4096,
-                 max_attempts: int = 8, workspace_size: int = 8 << 20) -> None:
+                 max_attempts: int = 8, workspace_size: int = 8 << 20,
+                 kv_bits: int = 16) -> None:
         from aios_amd.attention import Mi355xAttentionBackend
 
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 8 or 16")
         self.config = config
         self.device = torch.device(device)
         self.num_pages = num_pages
         self.max_attempts = max_attempts
         backend = Mi355xAttentionBackend(config, workspace_size=workspace_size)
         self.model = build_causal_lm(config, weights, self.device, attn_backend=backend)
-        self.kv_cache = MHAKVCache(config.num_kv_heads, config.num_layers, config.head_dim,
-                                   num_pages, 1, torch.bfloat16, self.device)
+        pool, dtype = ((MHAKVCache8, torch.float8_e4m3fn) if kv_bits == 8
+                       else (MHAKVCache, torch.bfloat16))
+        self.kv_cache = pool(config.num_kv_heads, config.num_layers, config.head_dim, num_pages, 1,
+                             dtype, self.device)
         self.cache_manager = CacheManager(self.device, num_pages)
         reset_global_ctx()
         self.ctx = Context(page_size=1)
@@ -432,6 +457,85 @@ class CandidateGroupEngine:
         finally:
             if allocated:
                 self.rt.cache_manager._free(torch.cat(allocated))
+
+    # -- scoring -----------------------------------------------------------------
+    @torch.inference_mode()
+    def score(self, token_ids, continuations, top: int = 0) -> tuple[ScoredContinuation, ...]:
+        """Log-probs of the caller's ``continuations`` (token id sequences, at
+        least one token each) after the prefix ``token_ids``, with ``top``
+        alternatives for each token (aios_amd.sample.token_logprobs).  The
+        prefix is prepared as for :meth:`complete` (and kept for the next
+        call); the continuations extend it as one batch, max_attempts at a
+        time, whose pages are freed again."""
+        prefix = [int(t) for t in token_ids]
+        conts = [tuple(int(t) for t in c) for c in continuations]
+        rt = self.rt
+        if not prefix:
+            raise ValueError("prefix produced no input tokens")
+        if any(not c for c in conts):
+            raise ValueError("a continuation needs at least one token")
+        vocab = rt.model.w["embed"].shape[0]
+        if any(not 0 <= t < vocab for c in (prefix, *conts) for t in c):
+            raise ValueError("token id outside the vocabulary")
+        if not 0 <= top <= min(vocab, MAX_TOP_LOGPROBS):
+            raise ValueError(f"top must be within 0..{min(vocab, MAX_TOP_LOGPROBS)}")
+        longest = max((len(c) for c in conts), default=1)
+        if len(prefix) + longest - 1 > min(rt.config.max_position_embeddings, rt.max_context):
+            raise ValueError("prefix + continuation exceeds context limit")
+        groups = [conts[i : i + rt.max_attempts] for i in range(0, len(conts), rt.max_attempts)]
+        required = len(prefix) + max((sum(len(c) - 1 for c in g) for g in groups), default=0)
+        if required > rt.num_pages:
+            raise ValueError(
+                f"CandidateGroup KV budget is too small: need up to {required} pages, "
+                f"configured {rt.num_pages}")
+        with self._run_lock:
+            rt.ctx.page_table = rt.page_table
+            logits, _, _ = self._prepare_prefix(prefix, rt.page_table)
+            out: list[ScoredContinuation] = []
+            for g in groups:
+                out += self._score_group(logits, len(prefix), g, top)
+            return tuple(out)
+
+    def _score_group(self, prefix_logits, p: int, conts, top: int) -> list[ScoredContinuation]:
+        """The first tokens under the prefix's logits, the others under those
+        of one prefill over the rows that have any (a row's last token is not
+        fed: nothing follows it)."""
+        rt, dev = self.rt, self.rt.device
+        first = token_logprobs(prefix_logits[:1].expand(len(conts), -1),
+                               torch.tensor([c[0] for c in conts], device=dev), top)
+        long = [c for c in conts if len(c) > 1]
+        parts = [first]
+        if long:
+            fed = [len(c) - 1 for c in long]
+            pages = rt.cache_manager.allocate(sum(fed))
+            try:
+                for r, own in enumerate(pages.split(fed)):
+                    rt.page_table[r, p : p + fed[r]] = own
+                batch = Batch(reqs=[
+                    Req(input_ids=torch.empty(p + n, dtype=torch.long), cached_len=p, output_len=1,
+                        uid=r, sampling_params=SamplingParams(max_tokens=1), table_idx=r)
+                    for r, n in enumerate(fed)], phase="prefill")
+                batch.input_ids = torch.tensor([t for c in long for t in c[:-1]], device=dev)
+                batch.positions = torch.cat([torch.arange(p, p + n, dtype=torch.int32)
+                                             for n in fed]).to(dev)
+                batch.out_loc = pages
+                batch.return_all_logits = True
+                rt.model.attn_backend.prepare_metadata(batch)
+                with rt.ctx.forward_batch(batch):
+                    logits = rt.model.forward()
+                parts.append(token_logprobs(
+                    logits, torch.tensor([t for c in long for t in c[1:]], device=dev), top))
+            finally:
+                rt.cache_manager._free(pages)
+        lp, ent, ids, alt = (torch.cat(f).tolist() for f in zip(*parts))
+        out, at = [], len(conts)  # the other tokens follow the first ones
+        for i, c in enumerate(conts):
+            rows = [i, *range(at, at + len(c) - 1)]
+            at += len(c) - 1
+            out.append(ScoredContinuation(
+                c, tuple(lp[r] for r in rows), tuple(ent[r] for r in rows),
+                tuple(tuple(zip(ids[r], alt[r])) for r in rows) if top else ()))
+        return out
 
     # -- prefix ------------------------------------------------------------------
     def _prepare_prefix(self, token_ids, page_table):

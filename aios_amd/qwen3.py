@@ -129,7 +129,8 @@ class Qwen3ForCausalLM:
         q/k norm + RoPE and the backend call -> [T, Hq, D] (or [T, Hq*D]).
         An appending decode batch on the gfx950 ops takes the norm and
         rotation inside the decode launch (forward_rope); a prefill batch
-        writes K/V to their pages in the launch that rotates them."""
+        writes K/V to their pages in the launch that rotates them (either
+        cache)."""
         c = self.config
         lw = self.w["layers"][i]
         t = qkv.shape[0]
@@ -152,6 +153,14 @@ class Qwen3ForCausalLM:
                                              self.rotary.sin, positions, hq, c.rms_norm_eps,
                                              k_cache, v_cache, batch.out_loc.view(-1))
             out = be.prefill_appended(q, k_cache, v_cache, batch)
+        elif (getattr(self.ops, "rope_in_append", False) and runs_as_built(self.ops, _ROPE)
+                and issubclass(type(be), Mi355xAttentionBackend)
+                and be.append_rope8_applies(qkv, kv_cache, batch)):
+            layer = kv_cache.layer(i)
+            q = self.ops.qk_norm_rope_append8(qkv, lw["q_norm"], lw["k_norm"], self.rotary.cos,
+                                              self.rotary.sin, positions, hq, c.rms_norm_eps,
+                                              *layer, batch.out_loc.view(-1))
+            out = be.prefill8_appended(q, *layer, batch)
         else:
             v = qkv[:, self._q_size + self._kv_size:].view(t, hkv, d)
             q, k = self.ops.qk_norm_rope(qkv, lw["q_norm"], lw["k_norm"], self.rotary.cos,
