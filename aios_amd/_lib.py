@@ -123,6 +123,18 @@ def raw_stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def current_stream(t: torch.Tensor) -> int:
+    """raw_stream of a tensor on the current device.  A device's default stream
+    has handle 0, which a launch takes as the current device's: tensors of
+    another device are refused (enter ``torch.cuda.device`` first)."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"expected a GPU tensor, got one on {t.device}")
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on cuda:{index}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 

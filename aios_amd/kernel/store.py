@@ -71,7 +71,9 @@ def store_cache8(
     """Quantise ``k[t]``/``v[t]`` (bfloat16) into page ``indices[t]`` of an
     8-bit cache: k8, v8 float8_e4m3fn (num_slots, num_heads, head_dim) codes
     and scales bfloat16 (num_heads, num_slots, 2), K's scale then V's, the
-    power of two that brings the row's largest magnitude to at most 448."""
+    power of two that brings the row's largest magnitude to at most 448.
+    Indices outside the pool are not written; a page named twice holds some mix
+    of its rows."""
     shape = k8.shape
     if len(shape) != 3 or v8.shape != shape:
         raise ValueError("KV cache must have shape (num_slots, num_heads, head_dim)")
@@ -105,6 +107,6 @@ def store_cache8(
         _lib.lib().aios_kv8_append(
             k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), slots, heads, dim,
             indices.data_ptr(), k.data_ptr(), k_stride[0], v.data_ptr(), v_stride[0], tokens,
-            _lib.raw_stream(k8)),
+            _lib.current_stream(k8)),
         "aios_kv8_append",
     )

@@ -252,7 +252,15 @@ class HipOps:
         if (scales.dtype != torch.bfloat16 or scales.shape != (num_kv_heads, slots, 2)
                 or not scales.is_contiguous()):
             raise ValueError("scales must be contiguous bfloat16 (num_kv_heads, num_slots, 2)")
-        _check_gpu(k8, v8, scales, out_loc)
+        for w in (q_weight, k_weight):
+            if w.dtype != torch.bfloat16 or w.numel() != head_dim or not w.is_contiguous():
+                raise ValueError("norm weights must be contiguous bfloat16 [head_dim] tensors")
+        if qkv.dtype != torch.bfloat16 or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError("qkv must be bfloat16 and the cos/sin tables contiguous")
+        _check_gpu(k8, v8, scales, out_loc, q_weight, k_weight, cos, sin, positions)
+        if any(t.get_device() != qkv.get_device() for t in (
+                k8, v8, scales, out_loc, q_weight, k_weight, cos, sin, positions)):
+            raise ValueError("qkv, the KV caches and the tables must be on one GPU")
         if out_loc.dtype != torch.int32 or out_loc.numel() != t or not out_loc.is_contiguous():
             raise ValueError("out_loc must be contiguous int32 with one entry per token")
         q = torch.empty(t, num_qo_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
@@ -260,7 +268,7 @@ class HipOps:
             qkv.data_ptr(), qkv.stride(0), t, num_qo_heads, num_kv_heads, head_dim,
             q_weight.data_ptr(), k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
             positions.contiguous().data_ptr(), q.data_ptr(), k8.data_ptr(), v8.data_ptr(),
-            scales.data_ptr(), slots, out_loc.data_ptr(), eps, _stream(qkv)),
+            scales.data_ptr(), slots, out_loc.data_ptr(), eps, _lib.current_stream(qkv)),
             "aios_qk_norm_rope_append8")
         return q
 

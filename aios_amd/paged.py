@@ -353,7 +353,7 @@ def decode8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tenso
         _lib.lib().aios_attn_decode8(
             p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
             indices.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws, ws_bytes,
-            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
         "aios_attn_decode8",
     )
     return out
@@ -373,7 +373,7 @@ def append_decode8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: torch.
             p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
             out_loc.data_ptr(), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
             indices.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws, ws_bytes,
-            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
         "aios_attn_append_decode8",
     )
     return out
@@ -407,7 +407,7 @@ def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: t
             indices.data_ptr(), cu_k.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
             cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), float(eps),
             out.data_ptr(), ws, ws_bytes,
-            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
         "aios_attn_append_decode_rope8",
     )
     return out
@@ -431,7 +431,7 @@ def prefill8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
             p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
             indices.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
             None if ws is None else ws.data_ptr(), p.ws_bytes,
-            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _stream(q)),
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
         "aios_attn_prefill8",
     )
     return out

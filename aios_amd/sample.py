@@ -193,5 +193,5 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     _lib.check(lib.aios_token_logprobs(
         logits.data_ptr(), logits.stride(0), rows, vocab, logits.element_size(),
         tokens.data_ptr(), top, lp.data_ptr(), ent.data_ptr(), ids.data_ptr(), alt.data_ptr(),
-        None if ws is None else ws.data_ptr(), ws_bytes, _stream(logits)), "aios_token_logprobs")
+        None if ws is None else ws.data_ptr(), ws_bytes, _lib.current_stream(logits)), "aios_token_logprobs")
     return TokenLogprobs(lp, ent, ids, alt)
