@@ -402,31 +402,39 @@ static int64_t plan8_parts(const int32_t* cu_k, int32_t batch, int32_t prefix, i
 
 // How a decode over the 8-bit cache deals with the rows' own positions (at most
 // `longest`): 0 = one workgroup per (row, kv-head), else the most positions of
-// a part of a row.  Estimated in ns for passes of 128 positions of 128-dim rows,
-// with w workgroups under way (three share a unit): a pass takes 1,100 by
-// itself, 7.2 w up to about two workgroups per unit and 1,700 + 3.9 w from
-// there (4.6 and 5.4 TB/s); a workgroup has 3,000 of latency around its passes,
-// finding its part costs one
-// 600 more and the combine takes 2,400 and 20 a part.  Fitted to 16 rows of 32q/8kv x 128
-// over 8,192 positions (512 / 768 / 1,024 workgroups: 62 / 53 / 61 us), one row
-// of 16q/8kv over 16,001 (63 / 125 / 250 / 500 workgroups, with the combine: 21
-// / 15.6 / 14.6 / 15.5 us) and 64 rows of 500 (whole rows 15.4 us, halves 20.0).
+// a part of a row.  Estimated in ns, the larger of
+//   a workgroup's passes of 128 positions (520 / 630 / 750 at head sizes 64 /
+//     96 / 128) behind 5,600 of latency (3,900 for whole rows: no part to find
+//     and no state to write), a half longer for each further workgroup that a
+//     unit has, and a little for all the bytes, and
+//   the bytes at 5.2 TB/s, less where few workgroups ask for them, with 3 for
+//     each workgroup's start,
+// and the combine, 3,300 and 25 a part.  Measured, main launch + combine, parts
+// of 256 / 512 / 640 / 768 / 1,024 / 2,048: one row of 16q/8kv x 128 over 16,001
+// 16.8 / 15.3 / 15.2 / 15.6 / 16.9 / 22.5 us; four over 4,000 15.0 / 14.5 / 14.7
+// / 14.8 / 16.3 / 22.0; 16 of 32q/8kv over up to 8,192 66.6 / 58.1 / 57.4 / 58.1
+// / 57.5 / 60.2; 8 of 8q/2kv x 96 over 8,000 15.6 / 13.8 / 13.9 / 14.2 / 15.0 /
+// 19.9 (384, the parts on a unit and a third: 15.6); 64 of 32q/8kv over 500 22.0
+// in parts of 256, 15.6 as whole rows.
 static int32_t plan8_split(const int32_t* cu_k, int32_t batch, int32_t prefix, int32_t longest,
                            int32_t hkv, int32_t d, int32_t cus, int32_t most_parts,
                            bool cascade) {
   const int32_t pass = aios::kSuffixPass;
   if (longest <= pass) return 0;
-  const int64_t slots = 3ll * cus;
-  auto time = [&](int64_t wgs, int64_t positions) {
-    auto round = [&](int64_t w) {
-      const int64_t bytes = 2 * d + 4;
-      const int64_t a = 72 * w * bytes / 2600, b = (17000 + 39 * w) * bytes / 2600;
-      const int64_t mem = a < b ? a : b;
-      return 3000 + positions * (mem > 1100 ? mem : 1100) / pass;
-    };
-    return wgs / slots * round(slots) + (wgs % slots ? round(wgs % slots) : 0);
+  int64_t own = 0;  // positions of all rows
+  for (int32_t b = 0; b < batch; ++b) {
+    const int32_t n = cu_k[b + 1] - cu_k[b] - prefix;
+    own += n > 0 ? n : 0;
+  }
+  const int64_t row = 2 * d + 4, bytes = own * hkv * row;
+  auto time = [&](int64_t wgs, int64_t positions, int64_t latency) {
+    const int64_t alone = latency + cdiv(positions, pass) * (280 + row * 9 / 5) *
+                                    (1 + (wgs + cus - 1) / cus) / 2 + bytes / 24000;
+    const int64_t mem = bytes / 5200;
+    const int64_t all = 2500 + mem + mem * 40 / wgs + 3 * wgs;
+    return alone > all ? alone : all;
   };
-  int64_t best = time((int64_t)batch * hkv, longest) + (cascade ? 2400 : 0);
+  int64_t best = time((int64_t)batch * hkv, longest, 3900) + (cascade ? 3300 : 0);
   int32_t pick = 0;
   for (int32_t k = 1; k * pass < longest; k += 1 + k / 16) {
     const int32_t most = k * pass;
@@ -434,7 +442,7 @@ static int32_t plan8_split(const int32_t* cu_k, int32_t batch, int32_t prefix, i
     if (parts > most_parts) continue;
     int32_t len = 0;
     const int64_t wgs = hkv * plan8_parts(cu_k, batch, prefix, most, &len);
-    const int64_t ns = time(wgs, len) + 3000 + 20 * parts;
+    const int64_t ns = time(wgs, len, 5600) + 3300 + 25 * parts;
     if (ns < best) {
       best = ns;
       pick = most;
