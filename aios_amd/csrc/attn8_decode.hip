@@ -559,8 +559,10 @@ __device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a,
 }
 
 // A row's own positions in parts of at most `most` (split: how many, and the
-// length of each but the last).
-__device__ __forceinline__ int row_parts(int own, int most) { return (own + most - 1) / most; }
+// length of each but the last); a row longer than planned in longer ones.
+__device__ __forceinline__ int row_parts(int own, int most, int max_parts) {
+  return min((max(own, 0) + most - 1) / most, max_parts);
+}
 __device__ __forceinline__ int row_part_len(int own, int parts) {
   return ((own + parts - 1) / parts + kSubTok - 1) / kSubTok * kSubTok;
 }
@@ -589,7 +591,7 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
       i = b0 + lane;
       at = a.cu_k[min(i, a.batch)];
       own = i < a.batch ? a.cu_k[min(i + 1, a.batch)] - at - a.prefix_len : 0;
-      n = row_parts(own, a.split_len);
+      n = row_parts(own, a.split_len, a.parts.n_parts - a.parts.n_chunks);
       int sum = n;
 #pragma unroll
       for (int k = 1; k < 64; k <<= 1) {
@@ -623,12 +625,45 @@ constexpr int decode8_lds(bool prefix) {
   return prefix && a > b ? a : b;
 }
 
+// The fields that come before a workgroup's first memory access lead the kernel
+// arguments as scalars: with kernel-argument preloading they are in SGPRs at
+// wave start, where a by-value struct takes a memory round trip ahead of the
+// page ids.  The copies in Decode8Args are overridden with them.
+// n_parts_flags: parts of a row, of the prefix among them (8 bits each), then
+// the three flags.
+__host__ __device__ inline int32_t parts_flags(const Decode8Args& a) {
+  return a.parts.n_parts | a.parts.n_chunks << 8 | a.split << 16 | a.final_out << 17 |
+         a.wave_parts << 18;
+}
+
 // PREFIX: the launch has prefix workgroups (first: they carry most bytes);
 // without them the row items' smaller LDS lets more workgroups share a unit.
 template <int D, int G, bool ROPE, bool PREFIX>
 __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(PREFIX ? 2 : 3, PREFIX ? 2 : 8))) void decode8_main_kernel(
-    Decode8Args a) {
+    const int32_t* __restrict__ indices, const int32_t* __restrict__ cu_k,
+    const int32_t* __restrict__ out_loc, int32_t prefix_wgs, int32_t prefix_len, int32_t chunk_len,
+    int32_t prefix_units, int32_t num_kv_heads, int32_t n_parts_flags, int32_t split_len,
+    int32_t n_splits, int32_t batch, int32_t m_rows, Decode8Args args) {
   __shared__ __align__(16) uint8_t lds[decode8_lds<D, G>(PREFIX)];
+  Decode8Args a = args;
+  a.indices = indices;
+  a.cu_k = cu_k;
+  a.out_loc = out_loc;
+  a.prefix_wgs = prefix_wgs;
+  a.prefix_len = PREFIX ? prefix_len : 0;
+  a.chunk_len = chunk_len;
+  a.prefix_units = prefix_units;
+  a.num_kv_heads = num_kv_heads;
+  a.num_qo_heads = num_kv_heads * G;
+  a.parts.n_parts = n_parts_flags & 255;
+  a.parts.n_chunks = n_parts_flags >> 8 & 255;
+  a.split = n_parts_flags >> 16 & 1;
+  a.final_out = n_parts_flags >> 17 & 1;
+  a.wave_parts = n_parts_flags >> 18 & 1;
+  a.split_len = split_len;
+  a.n_splits = n_splits;
+  a.batch = batch;
+  a.m_rows = m_rows;
   const int wg = blockIdx.x;
   if constexpr (PREFIX) {
     if (wg < a.prefix_wgs) {
@@ -644,91 +679,127 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 // ---------------------------------------------------------------------------
 // combine: one workgroup per (row, kv-head); weight of part j for query row g
 // 2^(lse_j - m) / sum_i 2^(lse_i - m) times the inverse of the part's scale.
+// The states are asked for together with the weights' inputs (one memory round
+// trip instead of two): a thread's first kBatch parts, all of them for up to 32
+// parts of 4 heads x 128.
 constexpr int kComb8Threads = 256;
 constexpr int kComb8MaxParts = 64;
+constexpr int kComb8Batch = 8;
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) x = fmaxf(x, __shfl_xor(x, k));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) x += __shfl_xor(x, k);
+  return x;
+}
 
 template <int D, int G>
-__global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(Decode8Args a) {
+__global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(
+    const float2* __restrict__ states, const _Float16* __restrict__ po_base,
+    const int32_t* __restrict__ cu_k, bf16* __restrict__ out, int32_t n_parts_flags, int32_t rows,
+    int32_t num_kv_heads, int32_t prefix_len, int32_t split_len) {
   constexpr int E8 = G * D / 8;  // 8-dim elements per part
   static_assert(E8 <= kComb8Threads, "one element per thread per part");
   constexpr int R = kComb8Threads / E8;  // threads sharing one element
   constexpr int NW = kComb8Threads / 64;
   constexpr int WP = kComb8MaxParts + 1;
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
   __shared__ float w_s[G * WP];
   __shared__ f32x4 red[2][kComb8Threads];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
-  const int b = blockIdx.x / a.num_kv_heads;
-  const int h = blockIdx.x - b * a.num_kv_heads;
-  int np = a.parts.n_parts;
-  if (a.split)
-    np = a.parts.n_chunks + row_parts(a.cu_k[b + 1] - a.cu_k[b] - a.prefix_len, a.split_len);
+  const int b = blockIdx.x / num_kv_heads;
+  const int h = blockIdx.x - b * num_kv_heads;
+  Parts8 parts;
+  parts.n_parts = n_parts_flags & 255;
+  parts.n_chunks = n_parts_flags >> 8 & 255;
+  parts.rows = rows;
+  const bool split = n_parts_flags >> 16 & 1;
+  const int last = parts.n_parts - 1;
   const int e = tid % E8;
-  const int r = tid / E8;
-  const bool active = r < R;
-  const int q8 = e & 1;
+  const int r = min(tid / E8, R - 1);  // (threads past R * E8 repeat another one's work)
   const int g = (e >> 1) % G;
-  const int dt = e / (2 * G);
-  const int d = dt * 16 + q8 * 8;
-  const int64_t part_stride = (int64_t)(D / 16) * a.parts.rows * 16;
-  const _Float16* po = a.parts.o + a.parts.o_index(D, h, 0, b * G + g, d);
-  for (int gg = wave; gg < G; gg += NW) {
-    const float2 ls = lane < np ? a.parts.ls[a.parts.ls_index(h, lane, b * G + gg)]
-                                : make_float2(kNegInf, 0.f);
-    float mx = ls.x;
+  const int d = e / (2 * G) * 16 + (e & 1) * 8;
+  const int64_t part_stride = (int64_t)(D / 16) * rows * 16;
+  const _Float16* po = po_base + parts.o_index(D, h, 0, b * G + g, d);
+  constexpr int LG = (G + NW - 1) / NW;  // query rows per wavefront
+  float2 ls[LG];
 #pragma unroll
-    for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
-    const float mu = mx == kNegInf ? 0.f : mx;
-    const float w = fast_exp2(ls.x - mu);
-    float den = w;
+  for (int i = 0; i < LG; ++i)
+    ls[i] = states[parts.ls_index(h, min(lane, last), b * G + min(wave + i * NW, G - 1))];
+  f16x8 v[kComb8Batch];
 #pragma unroll
-    for (int k = 32; k > 0; k >>= 1) den += __shfl_xor(den, k);
-    w_s[gg * WP + lane] = (den > 0.f ? w / den : den * 0.f) * ls.y;
+  for (int i = 0; i < kComb8Batch; ++i)
+    v[i] = *reinterpret_cast<const f16x8*>(po + (int64_t)min(r + i * R, last) * part_stride);
+  int np = parts.n_parts;  // (parts behind them were not written)
+  if (split)
+    np = parts.n_chunks + row_parts(cu_k[b + 1] - cu_k[b] - prefix_len, split_len,
+                                    parts.n_parts - parts.n_chunks);
+#pragma unroll
+  for (int i = 0; i < LG; ++i) {
+    if (wave + i * NW >= G) break;
+    const float x = lane < np ? ls[i].x : kNegInf;
+    const float mx = wave_max(x);
+    const float w = fast_exp2(x - (mx == kNegInf ? 0.f : mx));
+    const float den = wave_sum(w);
+    w_s[(wave + i * NW) * WP + lane] = (den > 0.f ? w / den : den * 0.f) * (lane < np ? ls[i].y : 0.f);
   }
   __syncthreads();
   float acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  if (active) {
-#pragma unroll 8
-    for (int j = r; j < np; j += R) {
-      typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-      const f16x8 v = *reinterpret_cast<const f16x8*>(po + (int64_t)j * part_stride);
-      const float w = w_s[g * WP + j];
+  auto add = [&](const f16x8& x, int j) {
+    const float w = w_s[g * WP + j];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = fmaf((float)v[i], w, acc[i]);
-    }
-  }
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf((float)x[i], w, acc[i]);
+  };
+#pragma unroll
+  for (int i = 0; i < kComb8Batch; ++i)
+    if (r + i * R < np) add(v[i], r + i * R);
+  for (int j = r + kComb8Batch * R; j < np; j += R)
+    add(*reinterpret_cast<const f16x8*>(po + (int64_t)j * part_stride), j);
   f32x4 acc0 = f32x4{acc[0], acc[1], acc[2], acc[3]}, acc1 = f32x4{acc[4], acc[5], acc[6], acc[7]};
   if (R > 1) {
     red[0][tid] = acc0;
     red[1][tid] = acc1;
     __syncthreads();
-    if (r == 0)
+    if (tid < E8)
       for (int rr = 1; rr < R; ++rr) {
         acc0 += red[0][rr * E8 + e];
         acc1 += red[1][rr * E8 + e];
       }
   }
-  if (active && r == 0)
-    *reinterpret_cast<uint4*>(a.out + ((int64_t)b * a.num_qo_heads + h * G + g) * D + d) =
+  if (tid < E8)
+    *reinterpret_cast<uint4*>(out + ((int64_t)b * num_kv_heads * G + h * G + g) * D + d) =
         make_uint4(pack_bf16x2(acc0[0], acc0[1]), pack_bf16x2(acc0[2], acc0[3]),
                    pack_bf16x2(acc1[0], acc1[1]), pack_bf16x2(acc1[2], acc1[3]));
 }
 
+template <int D, int G, bool ROPE, bool PREFIX>
+void main_launch(const Decode8Args& a, hipStream_t s) {
+  hipLaunchKernelGGL((decode8_main_kernel<D, G, ROPE, PREFIX>),
+                     dim3(a.prefix_wgs + a.suffix_items), dim3(kEngineThreads), 0, s, a.indices,
+                     a.cu_k, a.out_loc, a.prefix_wgs, a.prefix_len, a.chunk_len, a.prefix_units,
+                     a.num_kv_heads, parts_flags(a), a.split_len, a.n_splits, a.batch, a.m_rows, a);
+}
+
 template <int D, int G>
 hipError_t main_dg(const Decode8Args& a, hipStream_t s) {
-  const dim3 grid(a.prefix_wgs + a.suffix_items), block(kEngineThreads);
-  if (grid.x == 0) return hipSuccess;
-  if (a.n_splits < 1) return hipErrorInvalidValue;
+  if (a.prefix_wgs + a.suffix_items == 0) return hipSuccess;
+  if (a.n_splits < 1 || a.parts.n_parts > kComb8MaxParts || a.num_qo_heads != a.num_kv_heads * G)
+    return hipErrorInvalidValue;
   const bool rope = a.q_norm != nullptr;
   if (a.prefix_wgs > 0) {
-    if (rope) hipLaunchKernelGGL((decode8_main_kernel<D, G, true, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((decode8_main_kernel<D, G, false, true>), grid, block, 0, s, a);
+    if (rope) main_launch<D, G, true, true>(a, s);
+    else main_launch<D, G, false, true>(a, s);
   } else {
-    if (rope) hipLaunchKernelGGL((decode8_main_kernel<D, G, true, false>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((decode8_main_kernel<D, G, false, false>), grid, block, 0, s, a);
+    if (rope) main_launch<D, G, true, false>(a, s);
+    else main_launch<D, G, false, false>(a, s);
   }
   return hipGetLastError();
 }
@@ -737,7 +808,10 @@ template <int D, int G>
 hipError_t combine_dg(const Decode8Args& a, hipStream_t s) {
   const dim3 grid(a.batch * a.num_kv_heads);
   if (grid.x == 0) return hipSuccess;
-  hipLaunchKernelGGL((decode8_combine_kernel<D, G>), grid, dim3(kComb8Threads), 0, s, a);
+  if (a.parts.n_parts > kComb8MaxParts) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((decode8_combine_kernel<D, G>), grid, dim3(kComb8Threads), 0, s, a.parts.ls,
+                     a.parts.o, a.cu_k, a.out, parts_flags(a), a.parts.rows, a.num_kv_heads,
+                     a.prefix_len, a.split_len);
   return hipGetLastError();
 }
 

@@ -90,7 +90,7 @@ def test_plans_cover_every_position():
                          ws=1 << 40)
         assert rc == 0
         own = lens - p.prefix_len
-        assert 1 <= p.num_parts <= 512
+        assert 1 <= p.num_parts <= 64  # a lane of the combine for each
         if p.prefix_len:
             assert p.prefix_len == shared
             assert p.num_prefix_chunks * p.prefix_chunk_len >= p.prefix_len
