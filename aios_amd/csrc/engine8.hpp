@@ -99,6 +99,37 @@ struct Stage8 {
     }
   }
 
+  // A range of at most two steps, in flight at once: runs pipe(ready), where
+  // ready(i) returns once sub-tile i (byte offset i * SUB_BYTES) is in LDS, to
+  // be called for every sub-tile in order.
+  template <typename QLoad, typename Pipe>
+  __device__ __forceinline__ void resident(uint8_t* lds, QLoad&& qload, Pipe&& pipe, bool active) {
+    const bool act = __builtin_amdgcn_readfirstlane((int)active) != 0;
+    const bool second = end - begin > kStep8;
+    Regs r0, r1;
+    Ids i0, i1;
+    ids(0, i0);
+    ids(1, i1);
+    qload();
+    load(0, i0, r0);
+    load(1, i1, r1);  // (past the range: zeros, without a memory access)
+    auto ready = [&](int sub) {
+      if (sub == 0) {
+        store(lds, 0, r0);
+        lds_barrier();
+      } else if (sub == 2) {
+        store(lds, 1, r1);
+        lds_barrier();
+      }
+    };
+    if (act) {
+      pipe(ready);
+    } else {
+      ready(0);
+      if (second) ready(2);
+    }
+  }
+
   // Runs math(sb, kv0) on every sub-tile of the range (sb: its byte offset in
   // lds); `qload()` issues the Q loads behind the first loads.  AHEAD: steps in
   // flight.  One (the prefill, whose math of a step outlasts a load) needs one
@@ -152,9 +183,31 @@ __device__ __forceinline__ void run_tile8(TileEngine32<D, CAUSAL>& eng, uint8_t*
   eng.reset();
   const auto lo = eng.lane_offsets(lds);
   Stage8<D> st(kv, h, idx, kv_begin, kv_end);
-  st.template stream<CAUSAL ? 1 : 2>(
-      lds, qload,
-      [&](uint32_t sb, int kv0) { eng.compute_at(lo, sb, kv0, kv_end, scale_log2); }, active);
+  auto stream = [&] {
+    st.template stream<CAUSAL ? 1 : 2>(
+        lds, qload,
+        [&](uint32_t sb, int kv0) { eng.compute_at(lo, sb, kv0, kv_end, scale_log2); }, active);
+  };
+  if constexpr (CAUSAL) {
+    stream();
+  } else {
+    // (a shared prefix's usual chunk: the engine's pipelined math)
+    auto pipe = [&](auto n) {
+      st.resident(
+          lds, qload,
+          [&](auto&& ready) {
+            eng.template pipe_n<decltype(n)::value>(lo, ready, kv_begin, kv_end, scale_log2);
+          },
+          active);
+    };
+    switch ((kv_end - kv_begin + kSubTok - 1) / kSubTok) {
+      case 1: pipe(std::integral_constant<int, 1>{}); break;
+      case 2: pipe(std::integral_constant<int, 2>{}); break;
+      case 3: pipe(std::integral_constant<int, 3>{}); break;
+      case 4: pipe(std::integral_constant<int, 4>{}); break;
+      default: stream();
+    }
+  }
   if constexpr (CAUSAL) eng.l_run = eng.ol[0];
   else eng.l_run = xor32_sum(eng.ls);
 }
