@@ -1408,6 +1408,13 @@ int aios_qk_norm_rope_append8(const void* qkv, int64_t qkv_stride, int64_t token
                    "qk_norm_rope_append8 launch");
 }
 
+// (a row's reference is its largest score times the scale)
+static int check_scale8(const char* what, float sm_scale) {
+  if (!(sm_scale > 0.f) || !__builtin_isfinite(sm_scale))
+    return fail(AIOS_ERR_INVALID, "%s: sm_scale must be positive and finite", what);
+  return AIOS_OK;
+}
+
 int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
                        const void* k8, const void* v8, const void* scales, int64_t num_pages,
                        const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k, void* out,
@@ -1421,6 +1428,7 @@ int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_s
                 (long long)q_tok_stride);
   if (!q || !indices || !cu_q || !cu_k || !out)
     return fail(AIOS_ERR_INVALID, "prefill8: null pointer");
+  if ((rc = check_scale8("prefill8", sm_scale))) return rc;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0)
     return fail(AIOS_ERR_INVALID, "prefill8: q and out must be 16-byte aligned");
   aios::Kv8Layer c;
@@ -1473,6 +1481,7 @@ static int decode8_impl(const aios_attn_plan_t* p, const void* q, int64_t q_tok_
   if (((uintptr_t)workspace & 255) != 0)
     return fail(AIOS_ERR_INVALID, "decode8: workspace must be 256-byte aligned");
   if (!q || !indices || !cu_k || !out) return fail(AIOS_ERR_INVALID, "decode8: null pointer");
+  if ((rc = check_scale8("decode8", sm_scale))) return rc;
   if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0)
     return fail(AIOS_ERR_INVALID, "decode8: q and out must be 16-byte aligned");
   aios::Decode8Args a = {};

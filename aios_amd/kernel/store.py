@@ -101,8 +101,12 @@ def store_cache8(
     if not (dev == v8.get_device() == scales.get_device() == indices.get_device()
             == k.get_device() == v.get_device()):
         raise ValueError("the KV cache, its scales, the indices and K/V must be on one GPU")
-    if indices.dtype != torch.int32 or not indices.is_contiguous():
-        indices = indices.to(torch.int32).contiguous()
+    if indices.dtype != torch.int32:
+        if indices.dtype.is_floating_point or indices.dtype == torch.bool:
+            raise ValueError("KV write indices must be integers")
+        indices = indices.clamp(-1, slots).to(torch.int32)  # (outside the pool stays outside)
+    if not indices.is_contiguous():
+        indices = indices.contiguous()
     _lib.check(
         _lib.lib().aios_kv8_append(
             k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), slots, heads, dim,

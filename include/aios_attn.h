@@ -568,12 +568,13 @@ int aios_attnres_mix_ex(const void* bank, int32_t bank_sources, int64_t num_toke
  * the calls below.  Codes and scales: 16- and 4-byte aligned; num_pages below
  * 2^24, a layer's codes (num_pages * Hkv * D bytes) below 4 GiB;
  * AIOS_ERR_UNSUPPORTED otherwise.  Page ids outside [0, num_pages) read as
- * all-zero rows, and out_loc entries outside it are not written.
+ * all-zero rows, and out_loc entries outside it are not written; a page that
+ * out_loc names twice is left with some mix of its rows.  sm_scale is positive
+ * and finite.
  */
 
 /* aios_kv_append into the 8-bit cache: K/V rows (bf16 [n_tokens][Hkv][D], even
- * token strides in elements, 4-byte aligned) quantised into pages out_loc[t]
- * (distinct, or outside the pool). */
+ * token strides in elements, 4-byte aligned) quantised into pages out_loc[t]. */
 int aios_kv8_append(void* k8, void* v8, void* scales, int64_t num_pages, int32_t num_kv_heads,
                     int32_t head_dim, const int32_t* out_loc, const void* k, int64_t k_tok_stride,
                     const void* v, int64_t v_tok_stride, int64_t n_tokens, void* stream);

@@ -118,6 +118,18 @@ def test_append_is_exact(tokens, hkv, d):
         assert torch.equal(_bits(scales[:, :, w]), _bits(ws))
 
 
+def test_append_with_64_bit_indices():
+    """Indices past 32 bits are outside the pool, not somewhere in it."""
+    g = torch.Generator().manual_seed(2)
+    k8, v8, scales = _pool(g, 8, 2, 64)
+    want = [x.clone() for x in (k8, v8, scales)]
+    k, v = _rows(g, 4, 2, 64).to(DEV), _rows(g, 4, 2, 64).to(DEV)
+    loc = torch.tensor([2 ** 32 + 3, 5, -2 ** 32 + 1, -1], device=DEV)
+    store_cache8(k8, v8, scales, loc, k, v)
+    store_cache8(*want, torch.tensor([-1, 5, 8, -1], dtype=torch.int32, device=DEV), k, v)
+    assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip((k8, v8, scales), want))
+
+
 @pytest.mark.parametrize("d", [64, 96, 128])
 def test_append_extreme_rows(d):
     """Zero rows, subnormals, the type's largest values, borders of the scale

@@ -149,22 +149,24 @@ def test_rope_append_refuses(kw):
     assert _rope_append(**kw) == _lib.AIOS_ERR_INVALID
 
 
-def _attn(p, q=ADDR, qs=None, k8=ADDR, v8=ADDR, s=ADDR, pages=64, idx=ADDR, cu_q=ADDR, cu_k=ADDR,
+def _attn(p, scale=0.1, q=ADDR, qs=None, k8=ADDR, v8=ADDR, s=ADDR, pages=64, idx=ADDR, cu_q=ADDR, cu_k=ADDR,
           out=ADDR, ws=ADDR, ws_bytes=1 << 40, new=None):
     lib, qs = _lib.lib(), p.num_qo_heads * p.head_dim if qs is None else qs
     if p.phase in (_lib.PHASE_PREFILL8, _lib.PHASE_PREFILL):
         return lib.aios_attn_prefill8(p, q, qs, k8, v8, s, pages, idx, cu_q, cu_k, out, ws, ws_bytes,
-                                      0.1, None)
+                                      scale, None)
     if new is None:
-        return lib.aios_attn_decode8(p, q, qs, k8, v8, s, pages, idx, cu_k, out, ws, ws_bytes, 0.1, None)
+        return lib.aios_attn_decode8(p, q, qs, k8, v8, s, pages, idx, cu_k, out, ws, ws_bytes, scale,
+                                     None)
     k, ks, v, vs, loc = new
     return lib.aios_attn_append_decode8(p, q, qs, k, ks, v, vs, loc, k8, v8, s, pages, idx, cu_k, out,
-                                        ws, ws_bytes, 0.1, None)
+                                        ws, ws_bytes, scale, None)
 
 
 BAD_ATTN = [dict(q=None), dict(k8=None), dict(v8=None), dict(s=None), dict(idx=None), dict(cu_k=None),
             dict(out=None), dict(qs=4088), dict(qs=4100), dict(q=ADDR + 8), dict(out=ADDR + 8),
-            dict(k8=ADDR + 8), dict(s=ADDR + 2), dict(pages=-1)]
+            dict(k8=ADDR + 8), dict(s=ADDR + 2), dict(pages=-1), dict(scale=0.0), dict(scale=-0.1),
+            dict(scale=float("nan")), dict(scale=float("inf"))]
 
 
 @pytest.mark.parametrize("kw", BAD_ATTN + [dict(ws=ADDR + 16), dict(ws=None), dict(ws_bytes=16)])
@@ -301,7 +303,8 @@ def test_store_launches(no_launch, kw):
     dict(scales=_gpu(2, 2, 8).transpose(1, 2)), dict(indices=_gpu(4, dtype=torch.int32)),
     dict(k=_gpu(3, 2, 64, dtype=torch.float16)), dict(v=_gpu(3, 2, 64, dtype=torch.float32)),
     dict(k=_gpu(3, 3, 64)), dict(v=_gpu(2, 2, 64)), dict(k=_gpu(3, 64, 2).transpose(1, 2)),
-    dict(k=_gpu(3, 4, 64)[:, ::2]), dict(k8=_gpu(8, 2, 128, dtype=FP8)[..., :64]),
+    dict(k=_gpu(3, 4, 64)[:, ::2]), dict(indices=_gpu(3, dtype=torch.float32)),
+    dict(indices=_gpu(3, dtype=torch.bool)), dict(k8=_gpu(8, 2, 128, dtype=FP8)[..., :64]),
     dict(scales=_gpu(2, 8, 2, on=1)), dict(indices=_gpu(3, dtype=torch.int32, on=1)),
     dict(k=torch.zeros(3, 2, 64, dtype=BF16))])
 def test_store_refuses(no_launch, kw):
