@@ -22,8 +22,38 @@ __device__ __forceinline__ void store_row(const TileEngine32<D, true>& eng, floa
 
 __device__ __forceinline__ float inv_or_zero(float l) { return l > 0.f ? 1.f / l : l * 0.f; }
 
+// Both kernels take the arguments that a workgroup needs before its first page
+// ids as leading scalars: preloaded into SGPRs, where a by-value struct takes a
+// memory round trip.  PrefillArgs' own copies are overridden with them.
+__device__ __forceinline__ PrefillArgs with_scalars(PrefillArgs a, const int32_t* cu_q,
+                                                    const int32_t* cu_k, const int32_t* indices,
+                                                    int32_t num_kv_heads, int32_t batch,
+                                                    int32_t q_tiles, int32_t q_tile, int32_t group,
+                                                    int32_t n_parts, int32_t part_sub,
+                                                    int32_t part_rows) {
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.indices = indices;
+  a.num_kv_heads = num_kv_heads;
+  a.num_qo_heads = num_kv_heads * group;
+  a.batch = batch;
+  a.q_tiles = q_tiles;
+  a.q_tile = q_tile;
+  a.group = group;
+  a.n_parts = n_parts;
+  a.part_sub = part_sub;
+  a.part_rows = part_rows;
+  return a;
+}
+
 template <int D>
-__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(PrefillArgs a, Kv8Layer kv) {
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
+    const int32_t* __restrict__ indices, int32_t num_kv_heads, int32_t batch, int32_t q_tiles,
+    int32_t q_tile, int32_t group, int32_t n_parts, int32_t part_sub, int32_t part_rows,
+    PrefillArgs args, Kv8Layer kv) {
+  const PrefillArgs a = with_scalars(args, cu_q, cu_k, indices, num_kv_heads, batch, q_tiles,
+                                     q_tile, group, n_parts, part_sub, part_rows);
   __shared__ __align__(16) uint8_t lds[Stage8<D>::LDS_BYTES];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
@@ -72,7 +102,13 @@ __device__ __forceinline__ int64_t part_o8(const PrefillArgs& a, int64_t part, i
 // One part of a tile's KV range per workgroup (prefill_split_kernel's scheme:
 // tiles of at most 64 rows share a part's sub-tiles over their wavefronts).
 template <int D>
-__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_split_kernel(PrefillArgs a, Kv8Layer kv) {
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_split_kernel(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
+    const int32_t* __restrict__ indices, int32_t num_kv_heads, int32_t batch, int32_t q_tiles,
+    int32_t q_tile, int32_t group, int32_t n_parts, int32_t part_sub, int32_t part_rows,
+    PrefillArgs args, Kv8Layer kv) {
+  const PrefillArgs a = with_scalars(args, cu_q, cu_k, indices, num_kv_heads, batch, q_tiles,
+                                     q_tile, group, n_parts, part_sub, part_rows);
   using S = Stage8<D>;
   using T = typename S::T;
   constexpr int kMl = 4 * 32 * 8;  // (m, l) of the four wavefronts' rows
@@ -219,32 +255,36 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
   }
 }
 
-}  // namespace
-
-hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
-  const dim3 grid(a.q_tiles * a.num_kv_heads * a.batch), block(kEngineThreads);
-  if (grid.x == 0) return hipSuccess;
-  switch (D) {
-    case 64: hipLaunchKernelGGL(prefill8_kernel<64>, grid, block, 0, s, a, kv); break;
-    case 96: hipLaunchKernelGGL(prefill8_kernel<96>, grid, block, 0, s, a, kv); break;
-    case 128: hipLaunchKernelGGL(prefill8_kernel<128>, grid, block, 0, s, a, kv); break;
-    default: return hipErrorInvalidValue;
-  }
+template <typename Kernel>
+hipError_t launch(Kernel kernel, int wgs, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+  if (wgs == 0) return hipSuccess;
+  hipLaunchKernelGGL(kernel, dim3(wgs), dim3(kEngineThreads), 0, s, a.cu_q, a.cu_k, a.indices,
+                     a.num_kv_heads, a.batch, a.q_tiles, a.q_tile, a.group, a.n_parts, a.part_sub,
+                     a.part_rows, a, kv);
   return hipGetLastError();
 }
 
-hipError_t launch_prefill8_split(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+}  // namespace
+
+hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
   const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
-  if (tiles == 0) return hipSuccess;
-  const dim3 grid(tiles * a.n_parts), block(kEngineThreads);
   switch (D) {
-    case 64: hipLaunchKernelGGL(prefill8_split_kernel<64>, grid, block, 0, s, a, kv); break;
-    case 96: hipLaunchKernelGGL(prefill8_split_kernel<96>, grid, block, 0, s, a, kv); break;
-    case 128: hipLaunchKernelGGL(prefill8_split_kernel<128>, grid, block, 0, s, a, kv); break;
+    case 64: return launch(prefill8_kernel<64>, tiles, a, kv, s);
+    case 96: return launch(prefill8_kernel<96>, tiles, a, kv, s);
+    case 128: return launch(prefill8_kernel<128>, tiles, a, kv, s);
     default: return hipErrorInvalidValue;
   }
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? launch_prefill_combine(D, a, s) : e;
+}
+
+hipError_t launch_prefill8_split(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+  const int wgs = a.q_tiles * a.num_kv_heads * a.batch * a.n_parts;
+  hipError_t e = hipErrorInvalidValue;
+  switch (D) {
+    case 64: e = launch(prefill8_split_kernel<64>, wgs, a, kv, s); break;
+    case 96: e = launch(prefill8_split_kernel<96>, wgs, a, kv, s); break;
+    case 128: e = launch(prefill8_split_kernel<128>, wgs, a, kv, s); break;
+  }
+  return e == hipSuccess && wgs > 0 ? launch_prefill_combine(D, a, s) : e;
 }
 
 }  // namespace aios
