@@ -264,7 +264,23 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 // part's loads of a wavefront are whole 128-byte lines; NW wavefronts share a
 // row block's parts, NB of them in flight per wavefront.
 template <int D, int NW, int NB>
-__global__ __launch_bounds__(NW * 64) void prefill_combine_kernel(PrefillArgs a, int32_t row_blocks) {
+__global__ __launch_bounds__(NW * 64) void prefill_combine_kernel(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, const float* part_o,
+    const float2* part_ml, int32_t num_kv_heads, int32_t batch, int32_t q_tiles, int32_t q_tile,
+    int32_t n_parts, int32_t part_sub, int32_t part_rows, int32_t row_blocks, PrefillArgs args) {
+  // (the leading scalars are preloaded: a by-value struct takes a memory round trip)
+  PrefillArgs a = args;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.part_o = const_cast<float*>(part_o);
+  a.part_ml = const_cast<float2*>(part_ml);
+  a.num_kv_heads = num_kv_heads;
+  a.batch = batch;
+  a.q_tiles = q_tiles;
+  a.q_tile = q_tile;
+  a.n_parts = n_parts;
+  a.part_sub = part_sub;
+  a.part_rows = part_rows;
   constexpr int DG = D / 8;
   constexpr int RB = 64 / DG;
   const int lane = threadIdx.x & 63;
@@ -359,25 +375,33 @@ __global__ __launch_bounds__(NW * 64) void prefill_combine_kernel(PrefillArgs a,
                  pack_bf16x2(acc1[0], acc1[1]), pack_bf16x2(acc1[2], acc1[3]));
 }
 
-template <int D>
+// MANY: tiles of more than 32 parts by eight wavefronts, which ask for 48 at once
+// instead of 32 (6 tokens of 32q/8kv x 128 on 4,093 in 33 parts of the 8-bit
+// cache: 14.6 -> 14.1 us; 100 tokens on 4,000 in 9 parts: 27.4 -> 29.4, so not
+// there).  Its order of additions is another one than four wavefronts'.
+template <int D, bool MANY>
 static hipError_t launch_combine_d(const PrefillArgs& a, hipStream_t s) {
   if (a.n_parts > 1) {
     constexpr int RB = 64 / (D / 8);
     const int row_blocks = (a.part_rows + RB - 1) / RB;
     const dim3 grid(a.q_tiles * a.num_kv_heads * a.batch * row_blocks);
-    if (a.n_parts <= 4)
-      hipLaunchKernelGGL((prefill_combine_kernel<D, 1, 4>), grid, dim3(64), 0, s, a, row_blocks);
-    else
-      hipLaunchKernelGGL((prefill_combine_kernel<D, 4, 8>), grid, dim3(256), 0, s, a, row_blocks);
+    auto run = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a.cu_q, a.cu_k, a.part_o, a.part_ml,
+                         a.num_kv_heads, a.batch, a.q_tiles, a.q_tile, a.n_parts, a.part_sub,
+                         a.part_rows, row_blocks, a);
+    };
+    if (a.n_parts <= 4) run(prefill_combine_kernel<D, 1, 4>, 64);
+    else if (!MANY || a.n_parts <= 32) run(prefill_combine_kernel<D, 4, 8>, 256);
+    else run(prefill_combine_kernel<D, 8, 6>, 512);
   }
   return hipGetLastError();
 }
 
 hipError_t launch_prefill_combine(int D, const PrefillArgs& a, hipStream_t s) {
   switch (D) {
-    case 64: return launch_combine_d<64>(a, s);
-    case 96: return launch_combine_d<96>(a, s);
-    case 128: return launch_combine_d<128>(a, s);
+    case 64: return launch_combine_d<64, true>(a, s);
+    case 96: return launch_combine_d<96, true>(a, s);
+    case 128: return launch_combine_d<128, true>(a, s);
     default: return hipErrorInvalidValue;
   }
 }
@@ -388,7 +412,7 @@ static hipError_t launch_split_d(const PrefillArgs& a, hipStream_t s) {
   if (tiles == 0) return hipSuccess;
   hipLaunchKernelGGL(prefill_split_kernel<D>, dim3(tiles * a.n_parts), dim3(kEngineThreads), 0, s,
                      a);
-  return launch_combine_d<D>(a, s);
+  return launch_combine_d<D, false>(a, s);
 }
 
 hipError_t launch_prefill_split(int D, const PrefillArgs& a, hipStream_t s) {
