@@ -451,6 +451,61 @@ static int32_t plan8_split(const int32_t* cu_k, int32_t batch, int32_t prefix, i
   return pick;
 }
 
+// The parts of a prefill over the 8-bit cache whose requests have at most 64
+// MFMA rows each (one tile): num_parts most parts of a tile, 0 for the kernel
+// whose wavefronts own a row tile each instead of sharing the sub-tiles.
+// Estimated in ns: a step of 64 positions takes 580 / 780 / 970 at head sizes 64
+// / 96 / 128 with one workgroup on a unit and 1.6 times that with two, behind
+// 7,000 of latency, or 8,000 and the states' bytes and combine; workgroups past
+// two on a unit wait for those and 5,000 more.  The other kernel takes 4,000, 18
+// a row and 540 / 630 / 720 for each sub-tile, a quarter more with two on a
+// unit, 3,200 for each further round.  Measured, 32q/8kv x 128, 8 tokens each, in
+// parts of 128 / 256 / 512 / 768 / 1,536 positions / whole / the other kernel: 8
+// requests on 4,091 45.8 / 33.8 / 30.7 / 26.4 / 31.7 / 66.9 / 98 us; 16 of them
+// 90.6 / 61.5 / 50.1 / 43.1 / 40.3 / 67.7 / 101.9; 64 on 1,000 90.3 / 58.4 / 44.5 /
+// 44.4 / 29.5 / 29.5 / 32.9; 64 on 120 whole 11.7, the other kernel 9.9; one of
+// 6 tokens on 4,093 14.1 / 13.7 / 16.7 / 19.3 / 29.8 / 68.4 / 99.
+static void plan8_few_rows(aios_attn_plan_t* p, const int32_t* cu_k, int32_t rows, int32_t cus,
+                           int64_t ws_bytes) {
+  const int32_t hkv = p->num_kv_heads, d = p->head_dim;
+  const int32_t longest = cdiv(p->max_kv_len, 32);
+  const int64_t slots = 2ll * cus;
+  // rounds of `slots` workgroups, each `one` long with one on a unit
+  auto rounds = [&](int64_t wgs, int64_t one, int64_t two, int64_t restart) {
+    const int64_t rest = wgs % slots;
+    return wgs / slots * two + (rest > cus ? two : rest > 0 ? one : 0) +
+           (cdiv((int32_t)(wgs < 0x7fffffff ? wgs : 0x7fffffff), (int32_t)slots) - 1) * restart;
+  };
+  const int64_t tiles = (int64_t)p->batch_size * hkv;
+  const int64_t sub = (int64_t)longest * (360 + 14 * d / 5);
+  int64_t best = 4000 + 18 * rows + rounds(tiles, sub, sub * 5 / 4, 3200);
+  for (int32_t k = 1;; k += 1 + k / 8) {
+    const int32_t part_sub = aios::kPrefillFewSub * k;
+    const int32_t n = cdiv(longest, part_sub);
+    if (n < 1) return;  // (no positions)
+    const int64_t parts = tiles * n;
+    const int64_t o_bytes = align_up(parts * rows * d * 4, 256);
+    const int64_t bytes = n > 1 ? o_bytes + align_up(parts * rows * 8, 256) : 0;
+    if (bytes <= ws_bytes && parts <= 0x3fffffff) {
+      int64_t wgs = 0;
+      for (int32_t b = 0; b < p->batch_size; ++b)
+        wgs += (int64_t)cdiv(cdiv(cu_k[b + 1] - cu_k[b], 32), part_sub) * hkv;
+      const int64_t steps = (cdiv(longest, n) + 1) / 2;
+      const int64_t one = steps * (190 + 61 * d / 10);
+      const int64_t ns = rounds(wgs, one, one * 8 / 5, 5000) +
+                         (n > 1 ? 8000 + wgs * rows * d / 650 + 60 * n : 7000);
+      if (ns < best) {
+        best = ns;
+        p->prefix_chunk_len = part_sub * 32;
+        p->num_parts = n;
+        p->ws_parts_lse = n > 1 ? o_bytes : 0;
+        p->ws_bytes = bytes;
+      }
+    }
+    if (n == 1) return;
+  }
+}
+
 int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
                     int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
                     int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
@@ -460,7 +515,10 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
   const int32_t cus = device_cus();
   p->phase = phase == AIOS_PHASE_PREFILL ? AIOS_PHASE_PREFILL8 : AIOS_PHASE_DECODE8;
   if (phase == AIOS_PHASE_PREFILL) {
-    plan_prefill_parts(p, cu_q, cu_k, cus, ws_bytes);
+    const int32_t rows = (p->max_q_len < p->prefill_q_tile ? p->max_q_len : p->prefill_q_tile) *
+                         p->group;
+    if (rows > 64) plan_prefill_parts(p, cu_q, cu_k, cus, ws_bytes);
+    else if (rows > 0) plan8_few_rows(p, cu_k, rows, cus, ws_bytes);
     return AIOS_OK;
   }
   if (shared_prefix < 0 || shared_prefix > p->min_kv_len)
@@ -1449,8 +1507,8 @@ int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_s
   a.q_tiles = p->num_q_tiles;
   a.batch = p->batch_size;
   a.out = static_cast<aios::bf16*>(out);
-  if (p->num_parts > 1 && workspace && ((uintptr_t)workspace & 255) == 0 &&
-      p->ws_bytes <= workspace_bytes) {
+  if (p->num_parts == 1 || (p->num_parts > 1 && workspace && ((uintptr_t)workspace & 255) == 0 &&
+                            p->ws_bytes <= workspace_bytes)) {
     char* ws = static_cast<char*>(workspace);
     a.part_sub = p->prefix_chunk_len / 32;
     a.n_parts = p->num_parts;

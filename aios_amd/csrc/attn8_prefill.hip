@@ -196,11 +196,12 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
       eng.compute_at(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
                      a.scale_log2);
   } else {
-    // (more KV positions than the plan was built for)
+    // (two sub-tiles a step, each for the wavefronts whose turn it is)
     st.template stream<1>(
         lds, [&] { eng.load_q(qr, ok); },
         [&](uint32_t sb, int kv0) {
-          if (share == 0) eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
+          if (((kv0 - kv_begin) / kSubTok & (4 / nr - 1)) == share)
+            eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
         },
         true);
   }

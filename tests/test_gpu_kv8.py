@@ -295,6 +295,11 @@ PREFILLS = [
     (8, 1, 64, [(17, 100)]), (6, 2, 96, [(45, 3)]), (6, 1, 128, [(23, 300)]),
     (32, 8, 128, [(6, 1501)]), (12, 4, 64, [(6, 1000), (1, 700)]), (16, 8, 128, [(17, 900)]),
     (32, 8, 128, [(100, 1700)]), (8, 2, 96, [(700, 0)]), (16, 8, 128, [(600, 65)]),
+    # few rows, parts of several steps: one row tile and two, ragged ends
+    (32, 8, 128, [(8 - i % 3, 1900 - 77 * i) for i in range(16)]),
+    (12, 4, 64, [(15, 3000), (21, 1203), (1, 64)]),
+    (8, 2, 96, [(10, 2500 - 131 * i) for i in range(9)]),
+    (16, 8, 128, [(9, 600 - i) for i in range(40)]),
 ]
 
 
@@ -320,7 +325,7 @@ def test_prefill_matches_oracle(hq, hkv, d, lens):
     _near(out, want, tol)
     # and without room for partial states
     p, whole = _run_prefill(cache, q, indices, cu_q, cu_k, hkv, workspace_bytes=0)
-    assert p.num_parts == 0 and p.ws_bytes == 0
+    assert p.num_parts <= 1 and p.ws_bytes == 0
     _near(whole, want, tol)
 
 
