@@ -327,10 +327,18 @@ __device__ __forceinline__ void lp_select(LpSelect<NT>& sh, const T* x, int voca
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t mine = 0;
   for (int i = tid; i < n_groups; i += NT) mine = max(mine, sh.group[i]);
-  // the largest value that at least `top` threads' maxima reach
+  // the largest value that at least `top` threads' maxima reach: by the largest
+  // remaining one at a time (about 100 cycles each), from 12 on by all
+  // comparisons
   uint32_t v;
-  if (top == 1) {
-    v = lp_wave_max_u(mine);
+  if (top < 12) {
+    uint32_t left = mine;
+    int reached = 0;
+    do {
+      v = lp_wave_max_u(left);
+      reached += __popcll(__builtin_amdgcn_ballot_w64(left == v));
+      if (left == v) left = 0;
+    } while (reached < top && v != 0);
   } else {
     int reach = 0;
 #pragma unroll 16
@@ -414,17 +422,23 @@ __device__ __forceinline__ void lp_select(LpSelect<NT>& sh, const T* x, int voca
   lp_rank_all<NT>(NW * top, top, [&](int e) { return sh.cand[e / top * kLpCap + e % top]; }, put);
 }
 
+// A row's token and its logit (NaN outside the vocabulary), asked for before the
+// row's sums: two dependent loads, 2 us of a short row behind them.
 template <typename T>
-__device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, const T* x, double m,
+__device__ __forceinline__ float lp_token(const LogprobArgs& a, int64_t row, const T* x) {
+  const int64_t tok = a.tokens[row];
+  const bool ok = tok >= 0 && tok < a.vocab;
+  const float v = (float)x[ok ? tok : 0];
+  return ok ? v : __builtin_nanf("");
+}
+
+__device__ __forceinline__ void lp_finish(const LogprobArgs& a, int64_t row, float x_tok, double m,
                                           double z, double t, double ones, double& ln_z) {
   // Z = z + ones.  (No finite maximum: every element -inf leaves 0; a NaN or
   // +inf leaves NaN.)
   ln_z = ones > 0.0 ? log1p(z + (ones - 1.0)) : z > 0.0 ? log(z) : __builtin_nan("");
   if (threadIdx.x == 0) {
-    const int64_t tok = a.tokens[row];
-    const bool ok = tok >= 0 && tok < a.vocab;
-    const double d = ok ? (double)(float)x[tok] - m : __builtin_nan("");
-    a.logprobs[row] = (float)(d - ln_z);
+    a.logprobs[row] = (float)((double)x_tok - m - ln_z);
     a.entropies[row] = (float)(ln_z - t / (z + ones));
   }
 }
@@ -458,6 +472,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a, int3
     __shared__ LpSelect<NT> sh;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const float x_tok = lp_token(a, row, x);
     const int r = lp_groups_per<NT>(a.vocab);
     const int wave = threadIdx.x >> 6;
     const int rounds = lp_rounds<NT>(a.vocab);
@@ -472,7 +487,7 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a, int3
       g = j % r == 0 ? key : max(g, key);
     });
     double ln_z;
-    lp_finish(a, row, x, (double)st.m, (double)st.z, (double)st.t, (double)st.one, ln_z);
+    lp_finish(a, row, x_tok, (double)st.m, (double)st.z, (double)st.t, (double)st.one, ln_z);
     if (a.top > 0)
       lp_select(sh, x, a.vocab, a.top, n_groups, r,
                 [&](int rank, uint64_t k) { lp_write_top(a, row, (double)st.m, ln_z, rank, k); });
@@ -490,7 +505,9 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprob_merge_kernel(LogprobA
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   const LpState st = lane < segs ? states[row * segs + lane] : LpState{kLpLowest, 0.f, 0.f, 0.f};
+  const float x_tok = lp_token(a, row, x);
   const int r = lp_groups_per<NT>(a.vocab);
   const int batches = (a.vocab + kLpBatch - 1) / kLpBatch;
   const int n_groups = (lp_rounds<NT>(a.vocab) + r - 1) / r * NT;
@@ -530,8 +547,7 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprob_merge_kernel(LogprobA
     one += __shfl_xor(one, k);
   }
   double ln_z;
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  lp_finish(a, row, x, (double)m, z, t, one, ln_z);
+  lp_finish(a, row, x_tok, (double)m, z, t, one, ln_z);
   if (a.top == 0) return;
   __syncthreads();
   lp_select(sh, x, a.vocab, a.top, n_groups, r,
