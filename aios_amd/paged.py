@@ -263,6 +263,13 @@ def _check_kv8(p: _lib.AttnPlan, dev: int, k8: torch.Tensor, v8: torch.Tensor,
     ``dev``; returns its number of pages."""
     shape, hkv, d = k8.shape, p.num_kv_heads, p.head_dim
     pages = shape[0]
+    # (one test for calls in order: these checks are a good part of a short
+    # step's time on the host)
+    if (k8.dtype is _FP8 is v8.dtype and scales.dtype is _BF16 and shape == (pages, hkv, d)
+            and v8.shape == shape and scales.shape == (hkv, pages, 2) and k8.is_contiguous()
+            and v8.is_contiguous() and scales.is_contiguous()
+            and dev == k8.get_device() == v8.get_device() == scales.get_device()):
+        return pages
     if k8.dtype is not _FP8 or v8.dtype is not _FP8:
         raise ValueError("the 8-bit KV cache holds float8_e4m3fn codes")
     if (shape != (pages, hkv, d) and shape != (pages, 1, hkv, d)) or v8.shape != shape:
@@ -279,9 +286,9 @@ def _check_kv8(p: _lib.AttnPlan, dev: int, k8: torch.Tensor, v8: torch.Tensor,
 def _check_q8(p: _lib.AttnPlan, q: torch.Tensor, tokens: int) -> int:
     """q [tokens, Hq, D] (the plan's check_q); returns its GPU."""
     d = p.head_dim
-    dev, shape, stride = q.get_device(), q.shape, q.stride()
+    dev, shape = q.get_device(), q.shape
     if dev < 0 or q.dtype is not _BF16 or shape != (shape[0], p.num_qo_heads, d) or \
-            stride[2] != 1 or stride[1] != d:
+            q.stride()[1:] != (d, 1):
         _check_q(q, p)
     if shape[0] != tokens:
         if p.phase == _lib.PHASE_DECODE8:
@@ -301,12 +308,15 @@ def _check_lists8(dev: int, *lists: tuple[torch.Tensor, str, int]) -> None:
 def _check_decode8(p: _lib.AttnPlan, q: torch.Tensor, indices: torch.Tensor, cu_k: torch.Tensor,
                    k8: torch.Tensor, v8: torch.Tensor, scales: torch.Tensor,
                    out: torch.Tensor | None, workspace: torch.Tensor | None):
-    """(out, pages, workspace address and bytes)"""
+    """(GPU, out, pages, workspace address and bytes)"""
     if p.phase != _lib.PHASE_DECODE8:
         raise ValueError("plan was not built for decode over the 8-bit cache (kv_bits=8)")
     b = p.batch_size
     dev = _check_q8(p, q, b)
-    _check_lists8(dev, (indices, "indices", p.total_kv), (cu_k, "cu_k", b + 1))
+    if not (indices.dtype is _I32 is cu_k.dtype and indices.is_contiguous()
+            and cu_k.is_contiguous() and indices.numel() >= p.total_kv and cu_k.numel() > b
+            and indices.get_device() == dev == cu_k.get_device()):
+        _check_lists8(dev, (indices, "indices", p.total_kv), (cu_k, "cu_k", b + 1))
     pages = _check_kv8(p, dev, k8, v8, scales)
     need, ws, ws_bytes = p.ws_bytes, None, 0
     if workspace is not None:
@@ -315,7 +325,7 @@ def _check_decode8(p: _lib.AttnPlan, q: torch.Tensor, indices: torch.Tensor, cu_
             raise ValueError("workspace must be a contiguous tensor on q's GPU")
     if ws_bytes < need:
         raise RuntimeError(f"decode needs a workspace of {need} bytes")
-    return _out_like(q, out), pages, ws, ws_bytes
+    return dev, _out_like(q, out), pages, ws, ws_bytes
 
 
 def _out_like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
@@ -331,6 +341,11 @@ def _out_like(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
 def _check_new8(p: _lib.AttnPlan, dev: int, k: torch.Tensor, v: torch.Tensor,
                 out_loc: torch.Tensor) -> None:
     b, hkv, d = shape = p.batch_size, p.num_kv_heads, p.head_dim
+    if (k.dtype is _BF16 is v.dtype and k.shape == shape == v.shape
+            and k.stride()[1:] == (d, 1) == v.stride()[1:] and out_loc.dtype is _I32
+            and out_loc.is_contiguous() and out_loc.numel() >= b
+            and k.get_device() == dev == v.get_device() == out_loc.get_device()):
+        return
     for t in (k, v):
         if t.dtype is not _BF16 or t.get_device() != dev:
             raise ValueError("new K/V rows must be bfloat16 tensors on q's GPU")
@@ -348,7 +363,8 @@ def decode8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tenso
             sm_scale: float | None = None) -> torch.Tensor:
     """:func:`decode` over the 8-bit cache (k8, v8 float8_e4m3fn [pages, Hkv,
     D], scales bfloat16 [Hkv, pages, 2]); the plan is one of ``kv_bits=8``."""
-    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
+    _, out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out,
+                                                 workspace)
     _lib.check(
         _lib.lib().aios_attn_decode8(
             p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
@@ -366,8 +382,9 @@ def append_decode8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: torch.
                    sm_scale: float | None = None) -> torch.Tensor:
     """:func:`append_decode` over the 8-bit cache: the new rows are quantised
     into page out_loc[b] and attended to as the cache holds them."""
-    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
-    _check_new8(p, q.get_device(), k, v, out_loc)
+    dev, out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out,
+                                                   workspace)
+    _check_new8(p, dev, k, v, out_loc)
     _lib.check(
         _lib.lib().aios_attn_append_decode8(
             p, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
@@ -387,8 +404,9 @@ def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: t
                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                         sm_scale: float | None = None) -> torch.Tensor:
     """:func:`append_decode_rope` over the 8-bit cache."""
-    out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out, workspace)
-    _check_new8(p, q.get_device(), k, v, out_loc)
+    dev, out, pages, ws, ws_bytes = _check_decode8(p, q, indices, cu_k, k8, v8, scales, out,
+                                                   workspace)
+    _check_new8(p, dev, k, v, out_loc)
     for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w.dtype != torch.bfloat16 or w.numel() != p.head_dim or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous bfloat16 [head_dim] tensor")
@@ -396,7 +414,6 @@ def append_decode_rope8(p: _lib.AttnPlan, q: torch.Tensor, k: torch.Tensor, v: t
             or cos.ndim != 2 or cos.shape[1] != p.head_dim or not cos.is_contiguous()
             or not sin.is_contiguous()):
         raise ValueError("cos/sin tables must be contiguous bfloat16 [positions, head_dim]")
-    dev = q.get_device()
     if any(t.get_device() != dev for t in (q_norm, k_norm, cos, sin)):
         raise ValueError("norm weights and rotary tables must be on q's GPU")
     _check_lists8(dev, (positions, "positions", p.batch_size))
@@ -422,7 +439,11 @@ def prefill8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
     dev = _check_q8(p, q, p.total_q)
     pages = _check_kv8(p, dev, k8, v8, scales)
     b = p.batch_size + 1
-    _check_lists8(dev, (indices, "indices", p.total_kv), (cu_q, "cu_q", b), (cu_k, "cu_k", b))
+    if not (indices.dtype is _I32 is cu_k.dtype and cu_q.dtype is _I32 and indices.is_contiguous()
+            and cu_q.is_contiguous() and cu_k.is_contiguous() and indices.numel() >= p.total_kv
+            and cu_q.numel() >= b and cu_k.numel() >= b
+            and dev == indices.get_device() == cu_q.get_device() == cu_k.get_device()):
+        _check_lists8(dev, (indices, "indices", p.total_kv), (cu_q, "cu_q", b), (cu_k, "cu_k", b))
     out = _out_like(q, out)
     # (a buffer of this call alone, as in prefill)
     ws = torch.empty(p.ws_bytes, dtype=torch.uint8, device=q.device) if p.ws_bytes else None

@@ -183,9 +183,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     lib, dev = _lib.lib(), logits.device
-    lp, ent = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
+    # (one allocation for the three: allocations are a good part of a short
+    # call's time on the host)
+    lp, ent, alt = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev).split_with_sizes(
+        (rows, rows, rows * top))
+    alt = alt.view(rows, top)
     ids = tokens.new_empty((rows, top))
-    alt = lp.new_empty((rows, top))
     # (the states of split rows: a buffer of this call alone, since calls may
     # overlap on several streams)
     ws_bytes = lib.aios_token_logprobs_workspace(rows, vocab, top)
@@ -193,5 +196,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     _lib.check(lib.aios_token_logprobs(
         logits.data_ptr(), logits.stride(0), rows, vocab, logits.element_size(),
         tokens.data_ptr(), top, lp.data_ptr(), ent.data_ptr(), ids.data_ptr(), alt.data_ptr(),
-        None if ws is None else ws.data_ptr(), ws_bytes, _lib.current_stream(logits)), "aios_token_logprobs")
+        None if ws is None else ws.data_ptr(), ws_bytes, _lib.current_stream(logits)),
+        "aios_token_logprobs")
     return TokenLogprobs(lp, ent, ids, alt)
