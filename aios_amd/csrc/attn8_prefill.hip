@@ -199,9 +199,9 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
     // (two sub-tiles a step, each for the wavefronts whose turn it is)
     st.template stream<1>(
         lds, [&] { eng.load_q(qr, ok); },
-        [&](uint32_t sb, int kv0) {
+        [&](auto sb, int kv0) {
           if (((kv0 - kv_begin) / kSubTok & (4 / nr - 1)) == share)
-            eng.compute_at(lo, sb, kv0, kv_end, a.scale_log2);
+            eng.template compute_at<decltype(sb)::value>(lo, 0, kv0, kv_end, a.scale_log2);
         },
         true);
   }

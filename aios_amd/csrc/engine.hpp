@@ -911,21 +911,25 @@ struct TileEngine32 {
                         std::make_integer_sequence<int, N>{});
   }
 
+  // SB: a part of the sub-tile's byte offset that is known at compile time (it
+  // goes into the reads' offset fields; sb then takes an addition per address).
+  template <uint32_t SB = 0>
   __device__ __forceinline__ void compute_at(const LaneOff& lo, uint32_t sb, int kv0, int kv_end,
                                              float scale_log2) {
     const int h = (threadIdx.x & 63) >> 5;
     bf16x8 kf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      kf[s] = *reinterpret_cast<AIOS_LDS const bf16x8*>((AIOS_LDS const uint8_t*)(uintptr_t)(lo.k[s] + sb));
+      kf[s] = *reinterpret_cast<AIOS_LDS const bf16x8*>(
+          (AIOS_LDS const uint8_t*)(uintptr_t)(lo.k[s] + sb + SB));
     bf16x4 va[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint32_t a = lo.v[nt] + sb;
-      va[nt][0] = lds_read_tr_at<0>(a);
-      va[nt][1] = lds_read_tr_at<8 * T::ROWB>(a);
-      va[nt][2] = lds_read_tr_at<16 * T::ROWB>(a);
-      va[nt][3] = lds_read_tr_at<24 * T::ROWB>(a);
+      va[nt][0] = lds_read_tr_at<SB>(a);
+      va[nt][1] = lds_read_tr_at<SB + 8 * T::ROWB>(a);
+      va[nt][2] = lds_read_tr_at<SB + 16 * T::ROWB>(a);
+      va[nt][3] = lds_read_tr_at<SB + 24 * T::ROWB>(a);
     }
     f32x16 st;
 #pragma unroll

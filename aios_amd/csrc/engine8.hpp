@@ -131,7 +131,7 @@ struct Stage8 {
   }
 
   // Runs math(sb, kv0) on every sub-tile of the range (sb: its byte offset in
-  // lds); `qload()` issues the Q loads behind the first loads.  AHEAD: steps in
+  // lds, a constant); `qload()` issues the Q loads behind the first loads.  AHEAD: steps in
   // flight.  One (the prefill, whose math of a step outlasts a load) needs one
   // set of registers, used up by the step's LDS store; two put both steps of a
   // short range in flight at once.
@@ -149,7 +149,8 @@ struct Stage8 {
     if constexpr (AHEAD == 2) load(1, i1, r1);  // (past the range: zeros, without a memory access)
     ids(AHEAD, i0);
     if constexpr (AHEAD == 2) ids(3, i1);
-    auto step = [&](int s, Regs& r, Ids& i, int slot) {
+    auto step = [&](int s, Regs& r, Ids& i, auto slot) {
+      constexpr uint32_t SB = decltype(slot)::value * STEP_BYTES;
       store(lds, slot, r);
       // (unconditional, past the range without a memory access: behind a
       // branch around loads the compiler waits for all that are in flight)
@@ -158,18 +159,17 @@ struct Stage8 {
       lds_barrier();  // the slot is written; every wavefront is done with the other one's readers
       if (act) {
         const int kv0 = begin + s * kStep8;
-        math((uint32_t)(slot * STEP_BYTES), kv0);
-        if (kv0 + kSubTok < end) math((uint32_t)(slot * STEP_BYTES + T::SUB_BYTES), kv0 + kSubTok);
+        math(std::integral_constant<uint32_t, SB>{}, kv0);
+        if (kv0 + kSubTok < end)
+          math(std::integral_constant<uint32_t, SB + T::SUB_BYTES>{}, kv0 + kSubTok);
       }
     };
-    if constexpr (AHEAD == 1) {
-      for (int s = 0; s < n; ++s) step(s, r0, i0, s & 1);
-    } else {
-      for (int s = 0; s < n; s += 2) {
-        step(s, r0, i0, 0);
-        if (s + 1 >= n) break;
-        step(s + 1, r1, i1, 1);
-      }
+    // (both slots written out: offsets in the LDS reads' offset fields)
+    for (int s = 0; s < n; s += 2) {
+      step(s, r0, i0, std::integral_constant<int, 0>{});
+      if (s + 1 >= n) break;
+      if constexpr (AHEAD == 1) step(s + 1, r0, i0, std::integral_constant<int, 1>{});
+      else step(s + 1, r1, i1, std::integral_constant<int, 1>{});
     }
   }
 };
@@ -186,7 +186,10 @@ __device__ __forceinline__ void run_tile8(TileEngine32<D, CAUSAL>& eng, uint8_t*
   auto stream = [&] {
     st.template stream<CAUSAL ? 1 : 2>(
         lds, qload,
-        [&](uint32_t sb, int kv0) { eng.compute_at(lo, sb, kv0, kv_end, scale_log2); }, active);
+        [&](auto sb, int kv0) {
+          eng.template compute_at<decltype(sb)::value>(lo, 0, kv0, kv_end, scale_log2);
+        },
+        active);
   };
   if constexpr (CAUSAL) {
     stream();
