@@ -567,6 +567,15 @@ __device__ __forceinline__ int row_part_len(int own, int parts) {
   return ((own + parts - 1) / parts + kSubTok - 1) / kSubTok * kSubTok;
 }
 
+// The by-value arguments behind an item's first loads, asked for with the row's
+// bounds: used only here, the compiler loads them behind the wait for those (a
+// memory round trip more ahead of the page ids and K/V).
+__device__ __forceinline__ void args_with_bounds(const Decode8Args& a) {
+  asm volatile("" ::"s"(a.kv.k), "s"(a.kv.v), "s"(a.kv.scales), "s"(a.kv.num_pages),
+               "s"(a.kv.tok_bytes), "s"(a.q), "s"(a.q_tok_stride), "s"(a.k_new), "s"(a.v_new),
+               "s"(a.k_new_stride), "s"(a.v_new_stride), "s"(a.scale_log2));
+}
+
 template <int D, int G, bool ROPE>
 __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a, int item) {
   int h, b, base, kv_len, s_begin, s_end, part = a.parts.n_chunks;
@@ -575,6 +584,7 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
     b = item / a.num_kv_heads;
     base = a.cu_k[b];
     kv_len = a.cu_k[b + 1] - base;
+    args_with_bounds(a);
     s_begin = a.prefix_len;
     s_end = kv_len;
   } else {
@@ -590,7 +600,9 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
       if (b0 >= a.batch) return;  // (fewer parts than the plan's longest rows have)
       i = b0 + lane;
       at = a.cu_k[min(i, a.batch)];
-      own = i < a.batch ? a.cu_k[min(i + 1, a.batch)] - at - a.prefix_len : 0;
+      own = a.cu_k[min(i + 1, a.batch)];
+      args_with_bounds(a);
+      own = i < a.batch ? own - at - a.prefix_len : 0;
       n = row_parts(own, a.split_len, a.parts.n_parts - a.parts.n_chunks);
       int sum = n;
 #pragma unroll
@@ -627,8 +639,8 @@ constexpr int decode8_lds(bool prefix) {
 
 // The fields that come before a workgroup's first memory access lead the kernel
 // arguments as scalars: with kernel-argument preloading they are in SGPRs at
-// wave start, where a by-value struct takes a memory round trip ahead of the
-// page ids.  The copies in Decode8Args are overridden with them.
+// wave start (14 dwords of them), where a by-value struct takes a memory round
+// trip ahead of the page ids.  The copies in Decode8Args are overridden with them.
 // n_parts_flags: parts of a row, of the prefix among them (8 bits each), then
 // the three flags.
 __host__ __device__ inline int32_t parts_flags(const Decode8Args& a) {
@@ -642,8 +654,8 @@ template <int D, int G, bool ROPE, bool PREFIX>
 __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(PREFIX ? 2 : 3, PREFIX ? 2 : 8))) void decode8_main_kernel(
     const int32_t* __restrict__ indices, const int32_t* __restrict__ cu_k,
     const int32_t* __restrict__ out_loc, int32_t prefix_wgs, int32_t prefix_len, int32_t chunk_len,
-    int32_t prefix_units, int32_t num_kv_heads, int32_t n_parts_flags, int32_t split_len,
-    int32_t n_splits, int32_t batch, int32_t m_rows, Decode8Args args) {
+    int32_t num_kv_heads, int32_t n_parts_flags, int32_t split_len, int32_t n_splits,
+    int32_t batch, Decode8Args args) {
   __shared__ __align__(16) uint8_t lds[decode8_lds<D, G>(PREFIX)];
   Decode8Args a = args;
   a.indices = indices;
@@ -652,18 +664,17 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
   a.prefix_wgs = prefix_wgs;
   a.prefix_len = PREFIX ? prefix_len : 0;
   a.chunk_len = chunk_len;
-  a.prefix_units = prefix_units;
   a.num_kv_heads = num_kv_heads;
   a.num_qo_heads = num_kv_heads * G;
   a.parts.n_parts = n_parts_flags & 255;
   a.parts.n_chunks = n_parts_flags >> 8 & 255;
+  a.prefix_units = a.parts.n_chunks * num_kv_heads;
   a.split = n_parts_flags >> 16 & 1;
   a.final_out = n_parts_flags >> 17 & 1;
   a.wave_parts = n_parts_flags >> 18 & 1;
   a.split_len = split_len;
   a.n_splits = n_splits;
   a.batch = batch;
-  a.m_rows = m_rows;
   const int wg = blockIdx.x;
   if constexpr (PREFIX) {
     if (wg < a.prefix_wgs) {
@@ -784,8 +795,8 @@ template <int D, int G, bool ROPE, bool PREFIX>
 void main_launch(const Decode8Args& a, hipStream_t s) {
   hipLaunchKernelGGL((decode8_main_kernel<D, G, ROPE, PREFIX>),
                      dim3(a.prefix_wgs + a.suffix_items), dim3(kEngineThreads), 0, s, a.indices,
-                     a.cu_k, a.out_loc, a.prefix_wgs, a.prefix_len, a.chunk_len, a.prefix_units,
-                     a.num_kv_heads, parts_flags(a), a.split_len, a.n_splits, a.batch, a.m_rows, a);
+                     a.cu_k, a.out_loc, a.prefix_wgs, a.prefix_len, a.chunk_len,
+                     a.num_kv_heads, parts_flags(a), a.split_len, a.n_splits, a.batch, a);
 }
 
 template <int D, int G>
