@@ -648,6 +648,12 @@ __host__ __device__ inline int32_t parts_flags(const Decode8Args& a) {
          a.wave_parts << 18;
 }
 
+// Bound: with few bytes the chain launch - row bounds - page ids - K/V - math -
+// states, with many the bandwidth of 128-byte rows.  32q/8kv x 128: 24 rows on a
+// shared 4,096 8.7 us; 16 rows of 5,191 to 8,192 on scattered pages 53 us, 4.3
+// TB/s (all 8,192 on pages in order: 57 us, 4.8 TB/s); one row of 16,001 of
+// 16q/8kv 10.7 us, 3.1 TB/s; 8 rows of 24 + 16 of 8q/2kv x 96 5.2 us.
+//
 // PREFIX: the launch has prefix workgroups (first: they carry most bytes);
 // without them the row items' smaller LDS lets more workgroups share a unit.
 template <int D, int G, bool ROPE, bool PREFIX>
@@ -692,7 +698,7 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 // 2^(lse_j - m) / sum_i 2^(lse_i - m) times the inverse of the part's scale.
 // The states are asked for together with the weights' inputs (one memory round
 // trip instead of two): a thread's first kBatch parts, all of them for up to 32
-// parts of 4 heads x 128.
+// parts of 4 heads x 128.  Bound: that trip and the launch, 2.8 to 3.5 us.
 constexpr int kComb8Threads = 256;
 constexpr int kComb8MaxParts = 64;
 constexpr int kComb8Batch = 8;

