@@ -533,7 +533,7 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
   if (cascade) {
     mgroups = cdiv(m_rows, 128);
     if (prefix_chunk_len > 0) {
-      chunk = (int32_t)align_up(prefix_chunk_len, 32);
+      chunk = (int32_t)align_up(prefix_chunk_len < P ? prefix_chunk_len : P, 32);
     } else {
       // About one prefix workgroup per compute unit, in whole staging steps.
       int32_t want = cdiv(cus, hkv * mgroups);

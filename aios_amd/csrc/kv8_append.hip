@@ -57,31 +57,29 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(
 // qk_norm_rope_append_kernel (model_ops.hip) with the 8-bit cache: a 16-lane
 // row of a wavefront per (token, head), E = D / 16 dims a lane; q heads are
 // normalised, rotated and stored as bf16, k heads the same and then quantised
-// from those bf16 values, v heads quantised as they come.
-template <int D, int GPW, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_append8_kernel(
+// from those bf16 values, v heads quantised as they come.  One wavefront per
+// token and four heads: with two of them in a workgroup, or eight heads a
+// wavefront, a prompt took as long or up to 20% more (1,024 tokens of 32q/8kv x
+// 128: 8.6 / 9.4 / 10.4 us; 4,096: 24.1 / 23.0 / 24.9, 3.8 TB/s).
+template <int D>
+__global__ __launch_bounds__(64) void qk_norm_rope_append8_kernel(
     const bf16* __restrict__ qkv, int64_t stride, int hq, int hkv, const bf16* __restrict__ qw,
     const bf16* __restrict__ kw, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, int64_t table_rows, const int32_t* __restrict__ positions,
-    bf16* __restrict__ q_out, Kv8Layer cache, const int32_t* __restrict__ out_loc, float eps,
-    int64_t tokens) {
+    bf16* __restrict__ q_out, Kv8Layer cache, const int32_t* __restrict__ out_loc, float eps) {
   constexpr int E = D / 16;
   constexpr int W = E / 2;
   const int lane = threadIdx.x & 63;
   const int l16 = lane & 15;
   const int heads = hq + 2 * hkv;
-  const int head0 = blockIdx.y * 4 * GPW + (lane >> 4);
-  const int64_t t = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
-  if (t >= tokens) return;
+  const int head = blockIdx.y * 4 + (lane >> 4);
+  const int64_t t = blockIdx.x;
   const int64_t pos = min(max((int64_t)positions[t], (int64_t)0), table_rows - 1);
   const int64_t slot = out_loc[t];
-  uint32_t x[GPW][W];
+  uint32_t x[W];
+  const bf16* src = qkv + t * stride + (int64_t)min(head, heads - 1) * D + l16 * E;
 #pragma unroll
-  for (int g = 0; g < GPW; ++g) {
-    const bf16* src = qkv + t * stride + (int64_t)min(head0 + 4 * g, heads - 1) * D + l16 * E;
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[g][i] = reinterpret_cast<const uint32_t*>(src)[i];
-  }
+  for (int i = 0; i < W; ++i) x[i] = reinterpret_cast<const uint32_t*>(src)[i];
   float c[E], s[E];
   const float* cr = cos_t + pos * D + l16 * E;
   const float* sr = sin_t + pos * D + l16 * E;
@@ -92,99 +90,88 @@ __global__ __launch_bounds__(WAVES * 64) void qk_norm_rope_append8_kernel(
   }
   const bool first_half = l16 < 8;
   const bool slot_ok = slot >= 0 && slot < cache.num_pages;
+  const bool is_q = head < hq;
+  const bool is_v = head >= hq + hkv;
+  const int hh = is_q ? head : is_v ? head - hq - hkv : head - hq;
+  uint32_t y[W];
 #pragma unroll
-  for (int g = 0; g < GPW; ++g) {
-    const int head = head0 + 4 * g;
-    const bool is_q = head < hq;
-    const bool is_v = head >= hq + hkv;
-    const int hh = is_q ? head : is_v ? head - hq - hkv : head - hq;
-    uint32_t y[W];
+  for (int i = 0; i < W; ++i) y[i] = x[i];
+  if (__ballot(!is_v) != 0) {  // (not four V heads)
+    const uint32_t* wp = reinterpret_cast<const uint32_t*>((is_q ? qw : kw) + l16 * E);
+    float v[E], wv[E];
 #pragma unroll
-    for (int i = 0; i < W; ++i) y[i] = x[g][i];
-    if (__ballot(!is_v) != 0) {  // (not four V heads)
-      const uint32_t* wp = reinterpret_cast<const uint32_t*>((is_q ? qw : kw) + l16 * E);
-      float v[E], wv[E];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const uint32_t b = wp[i];
-        v[2 * i] = lo_bf16(x[g][i]);
-        v[2 * i + 1] = hi_bf16(x[g][i]);
-        wv[2 * i] = lo_bf16(b);
-        wv[2 * i + 1] = hi_bf16(b);
-      }
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
-      const float inv = rsqrtf(row16_sum(ss) / (float)D + eps);
-      float xn[E], pn[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) xn[i] = round_bf16(v[i] * inv * wv[i]);
-#pragma unroll
-      for (int i = 0; i < E; ++i)  // lane l16 ^ 8
-        pn[i] = __int_as_float(
-            __builtin_amdgcn_update_dpp(0, __float_as_int(xn[i]), 0x128, 0xF, 0xF, false));
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float o[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int e = 2 * i + j;
-          const float rot = first_half ? -pn[e] : pn[e];
-          o[j] = round_bf16(round_bf16(xn[e] * c[e]) + round_bf16(rot * s[e]));
-        }
-        if (!is_v) y[i] = pack_bf16x2(o[0], o[1]);
-      }
+    for (int i = 0; i < W; ++i) {
+      const uint32_t b = wp[i];
+      v[2 * i] = lo_bf16(x[i]);
+      v[2 * i + 1] = hi_bf16(x[i]);
+      wv[2 * i] = lo_bf16(b);
+      wv[2 * i + 1] = hi_bf16(b);
     }
-    // (the row maxima below are taken by every lane: no lane has left yet)
-    bool bad = false;
-    uint32_t a = 0;
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i)
-      a = max(a, max(kv8_mag(y[i] & 0xffffu, bad), kv8_mag(y[i] >> 16, bad)));
-    a = row16_max_u(a);
-    const bool row_bad = row16_max_u(bad ? 1u : 0u) != 0;
-    if (head >= heads) continue;
-    if (is_q) {
-      uint32_t* dst = reinterpret_cast<uint32_t*>(q_out + (t * hq + hh) * D + l16 * E);
+    for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
+    const float inv = rsqrtf(row16_sum(ss) / (float)D + eps);
+    float xn[E], pn[E];
 #pragma unroll
-      for (int i = 0; i < W; ++i) dst[i] = y[i];
-      continue;
+    for (int i = 0; i < E; ++i) xn[i] = round_bf16(v[i] * inv * wv[i]);
+#pragma unroll
+    for (int i = 0; i < E; ++i)  // lane l16 ^ 8
+      pn[i] = __int_as_float(
+          __builtin_amdgcn_update_dpp(0, __float_as_int(xn[i]), 0x128, 0xF, 0xF, false));
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      float o[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int e = 2 * i + j;
+        const float rot = first_half ? -pn[e] : pn[e];
+        o[j] = round_bf16(round_bf16(xn[e] * c[e]) + round_bf16(rot * s[e]));
+      }
+      if (!is_v) y[i] = pack_bf16x2(o[0], o[1]);
     }
-    if (!slot_ok) continue;
-    const int e = kv8_exp(a);
-    const float inv = kv8_pow2(-e);
-    uint32_t q[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) q[i] = kv8_codes2(lo_bf16(y[i]), hi_bf16(y[i]), inv);
-    kv8_store_codes<E>((is_v ? cache.v : cache.k) + slot * cache.tok_bytes + hh * D + l16 * E, q);
-    if (l16 == 0)
-      reinterpret_cast<uint16_t*>(cache.scales + hh * cache.num_pages + slot)[is_v ? 1 : 0] =
-          (uint16_t)kv8_scale_bits(e, row_bad);
   }
+  // (the row maxima below are taken by every lane: no lane has left yet)
+  bool bad = false;
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    a = max(a, max(kv8_mag(y[i] & 0xffffu, bad), kv8_mag(y[i] >> 16, bad)));
+  a = row16_max_u(a);
+  const bool row_bad = row16_max_u(bad ? 1u : 0u) != 0;
+  if (head >= heads) return;
+  if (is_q) {
+    uint32_t* dst = reinterpret_cast<uint32_t*>(q_out + (t * hq + hh) * D + l16 * E);
+#pragma unroll
+    for (int i = 0; i < W; ++i) dst[i] = y[i];
+    return;
+  }
+  if (!slot_ok) return;
+  const int e = kv8_exp(a);
+  const float inv = kv8_pow2(-e);
+  uint32_t q[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) q[i] = kv8_codes2(lo_bf16(y[i]), hi_bf16(y[i]), inv);
+  kv8_store_codes<E>((is_v ? cache.v : cache.k) + slot * cache.tok_bytes + hh * D + l16 * E, q);
+  if (l16 == 0)
+    reinterpret_cast<uint16_t*>(cache.scales + hh * cache.num_pages + slot)[is_v ? 1 : 0] =
+        (uint16_t)kv8_scale_bits(e, row_bad);
 }
 
 }  // namespace
 
 namespace {
-// Launch shapes as qk_norm_rope_append's, by its count of four-head groups.
 template <int D>
 hipError_t rope_append8_d(const void* qkv, int64_t stride, int64_t tokens, int hq, int hkv,
                           const void* qw, const void* kw, const float* cos_t, const float* sin_t,
                           int64_t table_rows, const int32_t* positions, void* q_out,
                           const Kv8Layer& c, const int32_t* out_loc, float eps,
                           hipStream_t stream) {
-  const int heads = hq + 2 * hkv;
-  const int64_t units = tokens * ((heads + 3) / 4);
-  auto launch = [&](auto kernel, int sets, int waves) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + waves - 1) / waves), sets),
-                       dim3(waves * 64), 0, stream, static_cast<const bf16*>(qkv), stride, hq, hkv,
-                       static_cast<const bf16*>(qw), static_cast<const bf16*>(kw), cos_t, sin_t,
-                       table_rows, positions, static_cast<bf16*>(q_out), c, out_loc, eps, tokens);
-    return hipGetLastError();
-  };
-  if (units >= 4096) return launch(qk_norm_rope_append8_kernel<D, 2, 2>, (heads + 7) / 8, 2);
-  if (units >= 1536) return launch(qk_norm_rope_append8_kernel<D, 1, 2>, (heads + 3) / 4, 2);
-  return launch(qk_norm_rope_append8_kernel<D, 1, 1>, (heads + 3) / 4, 1);
+  hipLaunchKernelGGL(qk_norm_rope_append8_kernel<D>,
+                     dim3((unsigned)tokens, (unsigned)(hq + 2 * hkv + 3) / 4), dim3(64), 0, stream,
+                     static_cast<const bf16*>(qkv), stride, hq, hkv, static_cast<const bf16*>(qw),
+                     static_cast<const bf16*>(kw), cos_t, sin_t, table_rows, positions,
+                     static_cast<bf16*>(q_out), c, out_loc, eps);
+  return hipGetLastError();
 }
 }  // namespace
 

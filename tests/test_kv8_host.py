@@ -108,6 +108,40 @@ def test_plans_cover_every_position():
             assert p.ws_parts_lse >= states * d * 2 and p.ws_bytes >= p.ws_parts_lse + states * 8
 
 
+def test_plans_of_the_largest_parameters():
+    top = 2 ** 31 - 1
+    rc, p = _decode8([400] * 8, shared=400, chunk=top, split=top)
+    assert rc == 0 and p.num_prefix_chunks == 1 and p.prefix_chunk_len >= 400
+    rc, p = _decode8([top // 4] * 4, split=1, ws=1 << 50)
+    assert rc == 0 and p.num_parts <= 64 and p.suffix_split_len * 64 >= top // 4
+    rc, p = _plan8(_lib.PHASE_PREFILL, np.arange(5), np.arange(5) * (top // 4), ws=1 << 50)
+    assert rc == 0 and p.num_parts >= 1
+
+
+def test_prefill_plans_of_few_rows():
+    """Parts cover every tile; without room for states the KV range stays whole."""
+    rng = np.random.default_rng(7)
+    for _ in range(300):
+        batch = int(rng.integers(1, 80))
+        g, hkv, d = int(rng.choice([1, 2, 3, 4, 6, 8])), int(rng.integers(1, 17)), int(rng.choice([64, 96, 128]))
+        new = rng.integers(0, 64 // g + 1, batch)
+        kv = new + rng.integers(0, int(2 ** rng.uniform(0, 15)) + 1, batch)
+        cu_q, cu_k = np.cumsum([0, *new]), np.cumsum([0, *kv])
+        for room in (1 << 40, 0):
+            rc, p = _plan8(_lib.PHASE_PREFILL, cu_q, cu_k, hq=g * hkv, hkv=hkv, d=d, ws=room)
+            assert rc == 0
+            rows = min(int(new.max()), 128 // g) * g
+            if p.num_parts:
+                assert p.num_parts * p.prefix_chunk_len >= kv.max() and p.prefix_chunk_len % 32 == 0
+            if p.num_parts > 1:
+                parts = batch * hkv * p.num_q_tiles * p.num_parts
+                assert p.ws_parts_lse >= parts * rows * d * 4
+                assert p.ws_bytes >= p.ws_parts_lse + parts * rows * 8
+            else:
+                assert p.ws_bytes == 0
+            assert p.ws_bytes <= room
+
+
 # -- the C ABI refuses before it launches ---------------------------------------
 
 ADDR = 1 << 20  # an aligned address that no refused call reads
