@@ -1473,6 +1473,18 @@ static int check_scale8(const char* what, float sm_scale) {
   return AIOS_OK;
 }
 
+// Whether an unsplit prefill takes tiles of 256 MFMA rows: most units two of
+// them in turn, and at least 1,000 positions.  128 / 256 rows, 32q/8kv x 128: one
+// request of 2,048 tokens (256 wide workgroups) 61.7 / 69.3 us, of 3,500 (440) 130
+// / 118, of 4,096 (512) 175 / 155; four of 1,000 (512) 54.5 / 52.8; two of 2,048 on
+// 1,000 (512) 165 / 153; eight of 512 (512) 38.9 / 39.5; sixteen of 300 (640) 35.6
+// / 41.6.  16q/8kv, one of 6,000 (376) 180 / 191, of 8,192 (512) 337 / 295; 12q/4kv x
+// 64, one of 8,192 (388) 160 / 168, of 12,000 (568) 340 / 322.
+static bool prefill8_wide(const aios_attn_plan_t* p, int32_t cus) {
+  const int64_t tiles = (int64_t)((p->num_q_tiles + 1) / 2) * p->num_kv_heads * p->batch_size;
+  return p->max_kv_len >= 1000 && 10 * tiles >= 17ll * cus;
+}
+
 int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
                        const void* k8, const void* v8, const void* scales, int64_t num_pages,
                        const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k, void* out,
@@ -1518,7 +1530,8 @@ int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_s
     return check_hip(aios::launch_prefill8_split(D, a, c, static_cast<hipStream_t>(stream)),
                      "prefill8 launch");
   }
-  return check_hip(aios::launch_prefill8(D, a, c, static_cast<hipStream_t>(stream)),
+  return check_hip(aios::launch_prefill8(D, a, c, prefill8_wide(p, device_cus()),
+                                         static_cast<hipStream_t>(stream)),
                    "prefill8 launch");
 }
 

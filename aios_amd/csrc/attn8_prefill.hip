@@ -46,20 +46,22 @@ __device__ __forceinline__ PrefillArgs with_scalars(PrefillArgs a, const int32_t
   return a;
 }
 
-// One workgroup per (tile of 128 MFMA rows, kv-head), a row tile per wavefront.
-// Bound: the math, two wavefronts a SIMD; 4,096 tokens of 32q/8kv x 128 166 - 173
-// us, 795 - 830 TFLOP/s (150 - 160 us over the bf16 cache, whose K/V come to LDS
-// without passing through registers: a step of 64 positions takes 55 VALU
-// instructions a wavefront for loads, conversion and stores).
-template <int D>
-__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(
+// One workgroup of NT threads per (tile of NT / 2 MFMA rows, kv-head), a row tile
+// per wavefront.  Bound: the math, two wavefronts a SIMD, and the conversion,
+// which takes 55 VALU instructions a wavefront and step of 64 positions with four
+// wavefronts to share it and half of that with eight.  4,096 tokens of 32q/8kv x
+// 128 155 us, 887 TFLOP/s (bf16 cache, whose K/V come to LDS without passing
+// through registers: 150 - 158); with four wavefronts 175.  Eight share one
+// barrier and need longer ranges and more tiles to pay (prefill8_wide, api.hip).
+template <int D, int NT>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
     const int32_t* __restrict__ indices, int32_t num_kv_heads, int32_t batch, int32_t q_tiles,
     int32_t q_tile, int32_t group, int32_t n_parts, int32_t part_sub, int32_t part_rows,
     PrefillArgs args, Kv8Layer kv) {
   const PrefillArgs a = with_scalars(args, cu_q, cu_k, indices, num_kv_heads, batch, q_tiles,
                                      q_tile, group, n_parts, part_sub, part_rows);
-  __shared__ __align__(16) uint8_t lds[Stage8<D>::LDS_BYTES];
+  __shared__ __align__(16) uint8_t lds[Stage8<D, NT>::LDS_BYTES];
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int G = a.group;
@@ -84,11 +86,11 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
   const bf16* qr = a.q + (int64_t)(q_start + i) * a.q_tok_stride + (int64_t)(h * G + g) * D;
   const int64_t out_off = ((int64_t)(q_start + i) * a.num_qo_heads + (h * G + g)) * D;
   eng.limit = cached + i;
-  eng.min_limit = cached + qt * a.q_tile;
   const int m0 = wave * 32;
+  eng.min_limit = cached + qt * a.q_tile + m0 / G;  // (of the wavefront)
   const bool active = m0 < a.q_tile * G && qt * a.q_tile + m0 / G < q_len;
-  run_tile8<D, true>(eng, lds, kv, h, a.indices + kv_base, 0, min(kv_len, cached + q_hi),
-                     a.scale_log2, [&] { eng.load_q(qr, ok); }, active);
+  run_tile8<D, true, NT>(eng, lds, kv, h, a.indices + kv_base, 0, min(kv_len, cached + q_hi),
+                         a.scale_log2, [&] { eng.load_q(qr, ok); }, active);
   if (ok) store_row<D>(eng, inv_or_zero(eng.l_run), a.out + out_off);
 }
 
@@ -266,22 +268,35 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 }
 
 template <typename Kernel>
-hipError_t launch(Kernel kernel, int wgs, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
+hipError_t launch(Kernel kernel, int wgs, int threads, const PrefillArgs& a, const Kv8Layer& kv,
+                  hipStream_t s) {
   if (wgs == 0) return hipSuccess;
-  hipLaunchKernelGGL(kernel, dim3(wgs), dim3(kEngineThreads), 0, s, a.cu_q, a.cu_k, a.indices,
+  hipLaunchKernelGGL(kernel, dim3(wgs), dim3(threads), 0, s, a.cu_q, a.cu_k, a.indices,
                      a.num_kv_heads, a.batch, a.q_tiles, a.q_tile, a.group, a.n_parts, a.part_sub,
                      a.part_rows, a, kv);
   return hipGetLastError();
 }
 
+template <int D>
+hipError_t launch_whole(const PrefillArgs& args, const Kv8Layer& kv, bool wide, hipStream_t s) {
+  PrefillArgs a = args;
+  if (wide) {
+    a.q_tiles = (a.q_tiles + 1) / 2;
+    a.q_tile *= 2;
+  }
+  const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
+  return wide ? launch(prefill8_kernel<D, 512>, tiles, 512, a, kv, s)
+              : launch(prefill8_kernel<D, 256>, tiles, 256, a, kv, s);
+}
+
 }  // namespace
 
-hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
-  const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
+hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, bool wide,
+                           hipStream_t s) {
   switch (D) {
-    case 64: return launch(prefill8_kernel<64>, tiles, a, kv, s);
-    case 96: return launch(prefill8_kernel<96>, tiles, a, kv, s);
-    case 128: return launch(prefill8_kernel<128>, tiles, a, kv, s);
+    case 64: return launch_whole<64>(a, kv, wide, s);
+    case 96: return launch_whole<96>(a, kv, wide, s);
+    case 128: return launch_whole<128>(a, kv, wide, s);
     default: return hipErrorInvalidValue;
   }
 }
@@ -290,9 +305,9 @@ hipError_t launch_prefill8_split(int D, const PrefillArgs& a, const Kv8Layer& kv
   const int wgs = a.q_tiles * a.num_kv_heads * a.batch * a.n_parts;
   hipError_t e = hipErrorInvalidValue;
   switch (D) {
-    case 64: e = launch(prefill8_split_kernel<64>, wgs, a, kv, s); break;
-    case 96: e = launch(prefill8_split_kernel<96>, wgs, a, kv, s); break;
-    case 128: e = launch(prefill8_split_kernel<128>, wgs, a, kv, s); break;
+    case 64: e = launch(prefill8_split_kernel<64>, wgs, kEngineThreads, a, kv, s); break;
+    case 96: e = launch(prefill8_split_kernel<96>, wgs, kEngineThreads, a, kv, s); break;
+    case 128: e = launch(prefill8_split_kernel<128>, wgs, kEngineThreads, a, kv, s); break;
   }
   return e == hipSuccess && wgs > 0 ? launch_prefill_combine(D, a, s) : e;
 }

@@ -17,16 +17,17 @@ namespace aios {
 
 constexpr int kStep8 = 64;  // KV positions per step: two sub-tiles
 
-template <int D>
+// NT: threads of the workgroup.
+template <int D, int NT = kEngineThreads>
 struct Stage8 {
   using T = KVTile<D, true>;
   static constexpr int CH = D / 16;                    // 16-code chunks of a row
-  static constexpr int TPP = D == 64 ? 64 : 32;        // positions per pass of the threads
+  static constexpr int TPP = NT >= 64 * CH ? 64 : 32;  // positions per pass of the threads
   static constexpr int NTHR = TPP * CH;                // threads that load (192 of 256 at D = 96)
   static constexpr int NP = kStep8 / TPP;              // passes per step
   static constexpr int STEP_BYTES = 2 * T::SUB_BYTES;
   static constexpr int LDS_BYTES = 2 * STEP_BYTES;
-  static_assert(NTHR <= kEngineThreads, "one chunk per thread and pass");
+  static_assert(NTHR <= NT, "one chunk per thread and pass");
 
   struct Ids {
     int32_t id[NP];
@@ -175,14 +176,14 @@ struct Stage8 {
 };
 
 // TileEngine32 over range [kv_begin, kv_end) of the 8-bit cache.
-template <int D, bool CAUSAL, typename QLoad>
+template <int D, bool CAUSAL, int NT = kEngineThreads, typename QLoad>
 __device__ __forceinline__ void run_tile8(TileEngine32<D, CAUSAL>& eng, uint8_t* lds,
                                           const Kv8Layer& kv, int h, const int32_t* idx,
                                           int kv_begin, int kv_end, float scale_log2,
                                           QLoad&& qload, bool active) {
   eng.reset();
   const auto lo = eng.lane_offsets(lds);
-  Stage8<D> st(kv, h, idx, kv_begin, kv_end);
+  Stage8<D, NT> st(kv, h, idx, kv_begin, kv_end);
   auto stream = [&] {
     st.template stream<CAUSAL ? 1 : 2>(
         lds, qload,

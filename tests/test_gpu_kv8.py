@@ -329,6 +329,25 @@ def test_prefill_matches_oracle(hq, hkv, d, lens):
     _near(whole, want, tol)
 
 
+@pytest.mark.parametrize("hq,hkv,d,lens", [
+    (8, 8, 64, [(700 - 9 * i, 310 + 40 * i) for i in range(19)]),   # tiles of 256 tokens
+    (12, 2, 96, [(330 - 7 * i, 700) for i in range(28)]),           # of 42
+    (32, 8, 128, [(250 - i, 760 + i) for i in range(14)])])          # of 64
+def test_prefill_in_wide_tiles(hq, hkv, d, lens):
+    """Batches whose tiles hold 256 MFMA rows, the requests' ends inside them:
+    a sample of the rows against the oracle, every row against batches of one
+    request (whose tiles are the narrow ones)."""
+    g, cache, q, indices, cu_q, cu_k = _prefill_case(hq + d, hq, hkv, d, lens)
+    _, out = _run_prefill(cache, q, indices, cu_q, cu_k, hkv, workspace_bytes=0)
+    for r in range(len(lens)):
+        qs, ks = slice(int(cu_q[r]), int(cu_q[r + 1])), slice(int(cu_k[r]), int(cu_k[r + 1]))
+        one = (_cu([lens[r][0]]), _cu([sum(lens[r])]))
+        _, alone = _run_prefill(cache, q[qs], indices[ks], *one, hkv, workspace_bytes=0)
+        assert torch.equal(out[qs], alone)
+        if r in (0, len(lens) - 1):
+            _near(alone, *_oracle(q[qs], *_values(*cache), indices[ks], *one, weights=2))
+
+
 @pytest.mark.parametrize("prefix", [0, 320])
 def test_lengths_on_the_device(prefix):
     """A plan built for the longest rows serves shorter ones (a captured step's
