@@ -86,7 +86,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void
   const bf16* qr = a.q + (int64_t)(q_start + i) * a.q_tok_stride + (int64_t)(h * G + g) * D;
   const int64_t out_off = ((int64_t)(q_start + i) * a.num_qo_heads + (h * G + g)) * D;
   eng.limit = cached + i;
-  const int m0 = wave * 32;
+  const int m0 = __builtin_amdgcn_readfirstlane(wave * 32);
   eng.min_limit = cached + qt * a.q_tile + m0 / G;  // (of the wavefront)
   const bool active = m0 < a.q_tile * G && qt * a.q_tile + m0 / G < q_len;
   run_tile8<D, true, NT>(eng, lds, kv, h, a.indices + kv_base, 0, min(kv_len, cached + q_hi),
