@@ -1577,8 +1577,9 @@ static int decode8_impl(const aios_attn_plan_t* p, const void* q, int64_t q_tok_
   a.prefix_wgs = a.prefix_units * (p->cascade_mgroups > 0 ? p->cascade_mgroups : 1);
   a.split = p->suffix_parts_per_item == 0 ? 1 : 0;
   a.split_len = p->suffix_split_len;
-  a.n_splits = p->num_suffix_splits;
-  a.suffix_items = p->num_kv_heads * (a.split ? p->num_suffix_splits : p->batch_size);
+  // (a part for every row at least, also for those planned without a position)
+  a.n_splits = a.split && p->num_suffix_splits < p->batch_size ? p->batch_size : p->num_suffix_splits;
+  a.suffix_items = p->num_kv_heads * (a.split ? a.n_splits : p->batch_size);
   a.final_out = p->num_parts == 1 ? 1 : 0;
   a.wave_parts = p->suffix_parts_per_item > 1 ? 1 : 0;
   a.parts.o = reinterpret_cast<_Float16*>(ws + p->ws_parts_o);

@@ -392,11 +392,12 @@ struct NewToken {
 };
 
 // Positions [s_begin, s_end) of row b for kv-head h, as part `part` of the row
-// (or its output); kv_len positions with page ids idx.
+// (or its output); kv_len positions with page ids idx.  own_parts: of a split
+// row, the parts of its own positions (it goes to the combine with the state).
 template <int D, int G, bool ROPE>
 __device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a, int b, int h,
                                              const int32_t* idx, int kv_len, int s_begin, int s_end,
-                                             int part) {
+                                             int part, int own_parts) {
   using I = Item8<D, G>;
   using E = typename I::E;
   using RP = typename I::RP;
@@ -507,7 +508,8 @@ __device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a,
       }
     }
     if (!final && lg == 0 && l16 < G)
-      a.parts.ls[a.parts.ls_index(h, part, b * G + l16)] = make_float2(lse_of(l_tot, m), unscale);
+      a.parts.ls[a.parts.ls_index(h, part, b * G + l16)] =
+          make_float2(lse_of(l_tot, m), __uint_as_float(__float_as_uint(unscale) | (uint32_t)own_parts));
   };
 
   if (a.wave_parts) {
@@ -559,12 +561,36 @@ __device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a,
 }
 
 // A row's own positions in parts of at most `most` (split: how many, and the
-// length of each but the last); a row longer than planned in longer ones.
+// length of each but the last); a row of more parts than a row may have in
+// longer ones.
 __device__ __forceinline__ int row_parts(int own, int most, int max_parts) {
-  return min((max(own, 0) + most - 1) / most, max_parts);
+  return min((int)(((uint32_t)max(own, 0) + (uint32_t)most - 1u) / (uint32_t)most), max_parts);
+}
+// The next longer split of a batch whose rows have more parts than its list
+// (the lengths are the device's: rows may have outgrown the plan's); the last
+// one leaves every row whole, and the list has a part for every row.
+__device__ __forceinline__ int longer_split(int most) {
+  return most < (1 << 30) ? most * 2 : 0x7fffffff;
 }
 __device__ __forceinline__ int row_part_len(int own, int parts) {
   return ((own + parts - 1) / parts + kSubTok - 1) / kSubTok * kSubTok;
+}
+// The sum of the lanes' n up to each one.
+__device__ __forceinline__ int scan_add(int n) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const int v = __shfl_up(n, k);
+    if (lane >= k) n += v;
+  }
+  return n;
+}
+// The parts of all rows (uniform).
+__device__ __forceinline__ int parts_of_all(const Decode8Args& a, int most, int max_parts) {
+  int n = 0;
+  for (int i = threadIdx.x & 63; i < a.batch; i += 64)
+    n += row_parts(a.cu_k[i + 1] - a.cu_k[i] - a.prefix_len, most, max_parts);
+  return __builtin_amdgcn_readlane(scan_add(n), 63);
 }
 
 // The by-value arguments behind an item's first loads, asked for with the row's
@@ -578,7 +604,7 @@ __device__ __forceinline__ void args_with_bounds(const Decode8Args& a) {
 
 template <int D, int G, bool ROPE>
 __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a, int item) {
-  int h, b, base, kv_len, s_begin, s_end, part = a.parts.n_chunks;
+  int h, b, base, kv_len, s_begin, s_end, part = a.parts.n_chunks, own_parts = 0;
   if (!a.split) {
     h = item % a.num_kv_heads;
     b = item / a.num_kv_heads;
@@ -595,6 +621,11 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
     const int lane = threadIdx.x & 63;
     h = item / a.n_splits;
     int w = item - h * a.n_splits;
+    const int max_parts = a.parts.n_parts - a.parts.n_chunks;
+    int most = a.split_len;
+    // (the parts of more rows than lanes are counted ahead)
+    if (a.batch > 64)
+      while (parts_of_all(a, most, max_parts) > a.n_splits) most = longer_split(most);
     int own = 0, at = 0, n = 0, i = 0;
     for (int b0 = 0;; b0 += 64) {
       if (b0 >= a.batch) return;  // (fewer parts than the plan's longest rows have)
@@ -603,12 +634,14 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
       own = a.cu_k[min(i + 1, a.batch)];
       args_with_bounds(a);
       own = i < a.batch ? own - at - a.prefix_len : 0;
-      n = row_parts(own, a.split_len, a.parts.n_parts - a.parts.n_chunks);
-      int sum = n;
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const int v = __shfl_up(sum, k);
-        if (lane >= k) sum += v;
+      n = row_parts(own, most, max_parts);
+      int sum = scan_add(n);
+      if (a.batch <= 64 && __builtin_expect(__builtin_amdgcn_readlane(sum, 63) > a.n_splits, 0)) {
+        do {
+          most = longer_split(most);
+          n = row_parts(own, most, max_parts);
+          sum = scan_add(n);
+        } while (__builtin_amdgcn_readlane(sum, 63) > a.n_splits);
       }
       const uint64_t past = __builtin_amdgcn_ballot_w64(sum > w);
       if (past) {
@@ -622,13 +655,15 @@ __device__ __forceinline__ void decode8_item(uint8_t* lds, const Decode8Args& a,
       }
       w -= __builtin_amdgcn_readlane(sum, 63);
     }
+    own_parts = n;
     const int len = row_part_len(own, n);
     kv_len = own + a.prefix_len;
     s_begin = a.prefix_len + w * len;
     s_end = min(kv_len, s_begin + len);
     part += w;
   }
-  decode8_rows<D, G, ROPE>(lds, a, b, h, a.indices + base, kv_len, s_begin, s_end, part);
+  decode8_rows<D, G, ROPE>(lds, a, b, h, a.indices + base, kv_len, s_begin, s_end, part,
+                           own_parts);
 }
 
 template <int D, int G>
@@ -718,7 +753,7 @@ template <int D, int G>
 __global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(
     const float2* __restrict__ states, const _Float16* __restrict__ po_base,
     const int32_t* __restrict__ cu_k, bf16* __restrict__ out, int32_t n_parts_flags, int32_t rows,
-    int32_t num_kv_heads, int32_t prefix_len, int32_t split_len) {
+    int32_t num_kv_heads, int32_t prefix_len) {
   constexpr int E8 = G * D / 8;  // 8-dim elements per part
   static_assert(E8 <= kComb8Threads, "one element per thread per part");
   constexpr int R = kComb8Threads / E8;  // threads sharing one element
@@ -754,9 +789,11 @@ __global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(
   for (int i = 0; i < kComb8Batch; ++i)
     v[i] = *reinterpret_cast<const f16x8*>(po + (int64_t)min(r + i * R, last) * part_stride);
   int np = parts.n_parts;  // (parts behind them were not written)
-  if (split)
-    np = parts.n_chunks + row_parts(cu_k[b + 1] - cu_k[b] - prefix_len, split_len,
-                                    parts.n_parts - parts.n_chunks);
+  if (split) {
+    // (as the main launch counted them: see Parts8)
+    const int own = __builtin_amdgcn_readlane(__float_as_int(ls[0].y), parts.n_chunks) & 127;
+    np = parts.n_chunks + (cu_k[b + 1] - cu_k[b] > prefix_len ? own : 0);
+  }
 #pragma unroll
   for (int i = 0; i < LG; ++i) {
     if (wave + i * NW >= G) break;
@@ -764,7 +801,8 @@ __global__ __launch_bounds__(kComb8Threads) void decode8_combine_kernel(
     const float mx = wave_max(x);
     const float w = fast_exp2(x - (mx == kNegInf ? 0.f : mx));
     const float den = wave_sum(w);
-    w_s[(wave + i * NW) * WP + lane] = (den > 0.f ? w / den : den * 0.f) * (lane < np ? ls[i].y : 0.f);
+    const float unscale = __uint_as_float(__float_as_uint(ls[i].y) & 0xff800000u);
+    w_s[(wave + i * NW) * WP + lane] = (den > 0.f ? w / den : den * 0.f) * (lane < np ? unscale : 0.f);
   }
   __syncthreads();
   float acc[8];
@@ -828,7 +866,7 @@ hipError_t combine_dg(const Decode8Args& a, hipStream_t s) {
   if (a.parts.n_parts > kComb8MaxParts) return hipErrorInvalidValue;
   hipLaunchKernelGGL((decode8_combine_kernel<D, G>), grid, dim3(kComb8Threads), 0, s, a.parts.ls,
                      a.parts.o, a.cu_k, a.out, parts_flags(a), a.parts.rows, a.num_kv_heads,
-                     a.prefix_len, a.split_len);
+                     a.prefix_len);
   return hipGetLastError();
 }
 

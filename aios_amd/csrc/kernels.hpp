@@ -337,7 +337,8 @@ hipError_t qk_norm_rope_append8(const void* qkv, int64_t stride, int64_t tokens,
 // as fp16 times a power of two of the row's own (the values then lie in
 // [-4, 4), where fp16 has 10 fraction bits: bf16 partial states alone would
 // add as much error as the final rounding) and ls = (lse, that power's
-// inverse).
+// inverse; the seven low bits of a part of a split row hold how many parts
+// that row's own positions have).
 struct Parts8 {
   _Float16* o;
   float2* ls;
@@ -372,7 +373,8 @@ struct Decode8Args {
   int32_t prefix_units;
   int32_t prefix_wgs;
   // the rows' own positions: (row, kv-head) items, or (split) n_splits parts
-  // per kv-head, a row's own positions in equal parts of at most split_len
+  // per kv-head (at least one for every row), a row's own positions in equal
+  // parts of at most split_len
   int32_t split;
   int32_t split_len;
   int32_t n_splits;

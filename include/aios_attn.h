@@ -115,7 +115,8 @@ typedef struct aios_attn_plan {
   int32_t cascade_rows;      /* batch_size * group */
   int32_t cascade_mgroups;   /* 128-row groups of cascade_rows */
   int32_t suffix_split_len;  /* KV positions per suffix item */
-  int32_t num_suffix_splits; /* suffix items per (row, kv-head) */
+  int32_t num_suffix_splits; /* suffix items per (row, kv-head); of a split decode plan of
+                              * the 8-bit cache, of all rows together per kv-head */
   int32_t suffix_tpg;        /* KV positions a suffix wavefront gathers per pass */
   int32_t num_parts;         /* partial states per (row, kv-head); 1 = direct output */
   /* prefill */
@@ -592,7 +593,13 @@ int aios_qk_norm_rope_append8(const void* qkv, int64_t qkv_stride, int64_t token
 /* aios_attn_plan for a batch over the 8-bit cache: the same arguments (phase
  * AIOS_PHASE_PREFILL or AIOS_PHASE_DECODE); the plan's phase is
  * AIOS_PHASE_PREFILL8 or AIOS_PHASE_DECODE8, which the calls below take and
- * those of the bf16 cache refuse. */
+ * those of the bf16 cache refuse.  The KV lengths that cu_k holds on the device
+ * may differ from the planned ones, as in a captured step: a decode's rows may
+ * be shorter (down to the shared prefix) or longer than planned, also than the
+ * longest one, and a prefill's requests may have any KV length from their new
+ * tokens on and at most the planned longest number of those.  indices then
+ * holds what cu_k names.  Rows longer than planned are split into longer parts,
+ * not more of them, so a plan for the lengths themselves is faster. */
 int aios_attn_plan8(int32_t phase, const int32_t* cu_q_host, const int32_t* cu_k_host,
                     int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads,
                     int32_t head_dim, int32_t page_size, int32_t shared_prefix_len,
