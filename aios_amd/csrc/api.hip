@@ -506,6 +506,27 @@ static void plan8_few_rows(aios_attn_plan_t* p, const int32_t* cu_k, int32_t row
   }
 }
 
+// Whether an unsplit prefill takes tiles of 256 MFMA rows: most units two of
+// them in turn, and at least 1,000 positions.  128 / 256 rows, 32q/8kv x 128: one
+// request of 2,048 tokens (256 wide workgroups) 62.4 / 66.9 us, of 3,500 (440) 129
+// / 115, of 4,096 (512) 172 / 151; four of 1,000 (512) 54.5 / 52.8; two of 2,048 on
+// 1,000 (512) 165 / 153; eight of 512 (512) 38.9 / 39.5; sixteen of 300 (640) 35.6
+// / 41.6.  16q/8kv, one of 6,000 (376) 174 / 186, of 8,192 (512) 331 / 286; 12q/4kv x
+// 64, one of 8,192 (388) 160 / 168, of 12,000 (572) 327 / 306.
+// Requests of different lengths: which workgroups meet on a unit decides there as
+// much as the tile.  2,048 tokens with twelve of 200 (640) 71.4 / 67.3, 3,500 with
+// eight of 100 (568) 131 / 126, 1,500, 1,200, 900 and 700 (552) 90.1 / 97.4; fewer
+// than 436, 2,048 with three of 40 (280) 152 / 150, with seven of 100 (368) 157 /
+// 160, 1,024 with 30 of 20 (368) 34.1 / 37.8, 1,800 with one of 700 (320) 73.8 /
+// 67.6; 22 such batches, 9% faster to 12% slower, the same in the mean.
+static bool prefill8_wide(const aios_attn_plan_t* p, const int32_t* cu_q, int32_t cus) {
+  const int32_t q_tile = 2 * p->prefill_q_tile;
+  int64_t tiles = 0;  // (workgroups past a request's end leave at once: not counted)
+  for (int32_t b = 0; b < p->batch_size; ++b)
+    tiles += (int64_t)cdiv(cu_q[b + 1] - cu_q[b], q_tile) * p->num_kv_heads;
+  return p->max_kv_len >= 1000 && 10 * tiles >= 17ll * cus;
+}
+
 int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
                     int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int32_t shared_prefix,
                     int64_t ws_bytes, int32_t prefix_chunk_len, int32_t suffix_split_len,
@@ -519,6 +540,10 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
                          p->group;
     if (rows > 64) plan_prefill_parts(p, cu_q, cu_k, cus, ws_bytes);
     else if (rows > 0) plan8_few_rows(p, cu_k, rows, cus, ws_bytes);
+    if (p->num_parts == 0 && prefill8_wide(p, cu_q, cus)) {
+      p->prefill_q_tile *= 2;
+      p->num_q_tiles = cdiv(p->max_q_len, p->prefill_q_tile);
+    }
     return AIOS_OK;
   }
   if (shared_prefix < 0 || shared_prefix > p->min_kv_len)
@@ -1473,18 +1498,6 @@ static int check_scale8(const char* what, float sm_scale) {
   return AIOS_OK;
 }
 
-// Whether an unsplit prefill takes tiles of 256 MFMA rows: most units two of
-// them in turn, and at least 1,000 positions.  128 / 256 rows, 32q/8kv x 128: one
-// request of 2,048 tokens (256 wide workgroups) 61.7 / 69.3 us, of 3,500 (440) 130
-// / 118, of 4,096 (512) 175 / 155; four of 1,000 (512) 54.5 / 52.8; two of 2,048 on
-// 1,000 (512) 165 / 153; eight of 512 (512) 38.9 / 39.5; sixteen of 300 (640) 35.6
-// / 41.6.  16q/8kv, one of 6,000 (376) 180 / 191, of 8,192 (512) 337 / 295; 12q/4kv x
-// 64, one of 8,192 (388) 160 / 168, of 12,000 (568) 340 / 322.
-static bool prefill8_wide(const aios_attn_plan_t* p, int32_t cus) {
-  const int64_t tiles = (int64_t)((p->num_q_tiles + 1) / 2) * p->num_kv_heads * p->batch_size;
-  return p->max_kv_len >= 1000 && 10 * tiles >= 17ll * cus;
-}
-
 int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
                        const void* k8, const void* v8, const void* scales, int64_t num_pages,
                        const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k, void* out,
@@ -1530,8 +1543,7 @@ int aios_attn_prefill8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_s
     return check_hip(aios::launch_prefill8_split(D, a, c, static_cast<hipStream_t>(stream)),
                      "prefill8 launch");
   }
-  return check_hip(aios::launch_prefill8(D, a, c, prefill8_wide(p, device_cus()),
-                                         static_cast<hipStream_t>(stream)),
+  return check_hip(aios::launch_prefill8(D, a, c, static_cast<hipStream_t>(stream)),
                    "prefill8 launch");
 }
 

@@ -278,25 +278,21 @@ hipError_t launch(Kernel kernel, int wgs, int threads, const PrefillArgs& a, con
 }
 
 template <int D>
-hipError_t launch_whole(const PrefillArgs& args, const Kv8Layer& kv, bool wide, hipStream_t s) {
-  PrefillArgs a = args;
-  if (wide) {
-    a.q_tiles = (a.q_tiles + 1) / 2;
-    a.q_tile *= 2;
-  }
+hipError_t launch_whole(const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
   const int tiles = a.q_tiles * a.num_kv_heads * a.batch;
-  return wide ? launch(prefill8_kernel<D, 512>, tiles, 512, a, kv, s)
-              : launch(prefill8_kernel<D, 256>, tiles, 256, a, kv, s);
+  const int rows = a.q_tile * a.group;
+  if (rows > 256) return hipErrorInvalidValue;
+  return rows > 128 ? launch(prefill8_kernel<D, 512>, tiles, 512, a, kv, s)
+                    : launch(prefill8_kernel<D, 256>, tiles, 256, a, kv, s);
 }
 
 }  // namespace
 
-hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, bool wide,
-                           hipStream_t s) {
+hipError_t launch_prefill8(int D, const PrefillArgs& a, const Kv8Layer& kv, hipStream_t s) {
   switch (D) {
-    case 64: return launch_whole<64>(a, kv, wide, s);
-    case 96: return launch_whole<96>(a, kv, wide, s);
-    case 128: return launch_whole<128>(a, kv, wide, s);
+    case 64: return launch_whole<64>(a, kv, s);
+    case 96: return launch_whole<96>(a, kv, s);
+    case 128: return launch_whole<128>(a, kv, s);
     default: return hipErrorInvalidValue;
   }
 }

@@ -399,10 +399,9 @@ struct Decode8Args {
 hipError_t launch_decode8_main(int D, const Decode8Args& a, hipStream_t stream);
 hipError_t launch_decode8_combine(int D, const Decode8Args& a, hipStream_t stream);
 
-// Prefill over the 8-bit cache (the bf16 cache fields of p are not read); wide:
-// tiles of twice q_tile tokens by eight wavefronts (the same results).
-hipError_t launch_prefill8(int D, const PrefillArgs& p, const Kv8Layer& kv, bool wide,
-                           hipStream_t stream);
+// Prefill over the 8-bit cache (the bf16 cache fields of p are not read); tiles
+// of more than 128 MFMA rows by eight wavefronts (the same results).
+hipError_t launch_prefill8(int D, const PrefillArgs& p, const Kv8Layer& kv, hipStream_t stream);
 // The same with each tile's KV range split (p.part_sub > 0), merged by
 // launch_prefill_combine.
 hipError_t launch_prefill8_split(int D, const PrefillArgs& p, const Kv8Layer& kv,
