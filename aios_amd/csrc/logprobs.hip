@@ -518,23 +518,21 @@ __global__ __launch_bounds__(kLpMergeThreads) void logprob_merge_kernel(LogprobA
   const int n_groups = (lp_rounds<NT>(a.vocab) + r - 1) / r * NT;
   if (a.top > 0) {
     const uint32_t* in = keys + row * batches * 64;
-    constexpr int N = 10;  // loads in flight (151,936 ids: all of a thread's)
-    for (int g0 = tid; g0 < n_groups; g0 += N * NT) {
-      uint32_t key[N] = {};
-      for (int q = 0; q < r; ++q) {
-        uint32_t v[N];
+    constexpr int N = kLpMaxGroups / NT;  // groups of a thread, their loads in flight together
+    uint32_t key[N] = {};
+    for (int q = 0; q < r; ++q) {
+      uint32_t v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int64_t at = ((int64_t)(g0 / NT + k) * r + q) * NT + tid;  // batch * 64 + lane
-          v[k] = at < (int64_t)batches * 64 ? in[at] : 0u;
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) key[k] = max(key[k], v[k]);
+      for (int k = 0; k < N; ++k) {
+        const int64_t at = ((int64_t)k * r + q) * NT + tid;  // batch * 64 + lane
+        v[k] = at < (int64_t)batches * 64 ? in[at] : 0u;
       }
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (g0 + k * NT < n_groups) sh.group[g0 + k * NT] = key[k];
+      for (int k = 0; k < N; ++k) key[k] = max(key[k], v[k]);
     }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k * NT < n_groups) sh.group[k * NT + tid] = key[k];
   }
   const float m = lp_wave_max(st.m);
   const double d = fmax((double)st.m - (double)m, -800.0);
