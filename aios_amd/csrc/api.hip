@@ -560,7 +560,12 @@ int aios_attn_plan8(int32_t phase, const int32_t* cu_q, const int32_t* cu_k, int
     if (prefix_chunk_len > 0) {
       chunk = (int32_t)align_up(prefix_chunk_len < P ? prefix_chunk_len : P, 32);
     } else {
-      // About one prefix workgroup per compute unit, in whole staging steps.
+      // About one prefix workgroup per compute unit, in whole staging steps.  (No
+      // cost is weighed: just past a length whose chunks of 128 fill the units, a
+      // chunk is 192 on fewer of them and without the pipelined math.  24 rows of
+      // 32q/8kv x 128, chunks of 96 / 128 / 160 / 192: on 4,096 13.9 / 10.8 / 11.5 /
+      // 11.9 us, 128 taken; on 4,160 14.1 / 11.3 / 11.5 / 11.9, 192 taken; on 6,000
+      // - / 15.2 / 14.5 / 12.5, 192 taken.)
       int32_t want = cdiv(cus, hkv * mgroups);
       if (want < 1) want = 1;
       chunk = (int32_t)align_up(cdiv(P, want), 64);

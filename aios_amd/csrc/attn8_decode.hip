@@ -560,9 +560,9 @@ __device__ __forceinline__ void decode8_rows(uint8_t* lds, const Decode8Args& a,
   write_rows(acc, l_tot, mx, buf, part, a.final_out != 0);
 }
 
-// A row's own positions in parts of at most `most` (split: how many, and the
-// length of each but the last); a row of more parts than a row may have in
-// longer ones.
+// A row's own positions in equal parts of at most `most` (split: how many, and
+// the length of each but the last), longer ones where that would be more than
+// max_parts.
 __device__ __forceinline__ int row_parts(int own, int most, int max_parts) {
   return min((int)(((uint32_t)max(own, 0) + (uint32_t)most - 1u) / (uint32_t)most), max_parts);
 }
@@ -687,7 +687,9 @@ __host__ __device__ inline int32_t parts_flags(const Decode8Args& a) {
 // states, with many the bandwidth of 128-byte rows.  32q/8kv x 128: 24 rows on a
 // shared 4,096 8.7 us; 16 rows of 5,191 to 8,192 on scattered pages 53 us, 4.3
 // TB/s (all 8,192 on pages in order: 57 us, 4.8 TB/s); one row of 16,001 of
-// 16q/8kv 10.7 us, 3.1 TB/s; 8 rows of 24 + 16 of 8q/2kv x 96 5.2 us.
+// 16q/8kv 10.7 us, 3.1 TB/s; 8 rows of 24 + 16 of 8q/2kv x 96 5.2 us.  With the
+// norm and rotation inside (ROPE), both launches without / with: the 24 rows 12.3 /
+// 15.2 us, the 16 57.8 / 59.2, the one 13.9 / 14.9, the 8 5.2 / 5.8.
 //
 // PREFIX: the launch has prefix workgroups (first: they carry most bytes);
 // without them the row items' smaller LDS lets more workgroups share a unit.

@@ -50,9 +50,11 @@ __device__ __forceinline__ PrefillArgs with_scalars(PrefillArgs a, const int32_t
 // per wavefront.  Bound: the math, two wavefronts a SIMD, and the conversion,
 // which takes 55 VALU instructions a wavefront and step of 64 positions with four
 // wavefronts to share it and half of that with eight.  4,096 tokens of 32q/8kv x
-// 128 155 us, 887 TFLOP/s (bf16 cache, whose K/V come to LDS without passing
-// through registers: 150 - 158); with four wavefronts 175.  Eight share one
+// 128 150 - 153 us, 901 - 919 TFLOP/s (bf16 cache, whose K/V come to LDS without
+// passing through registers: 150 - 158); with four wavefronts 172.  Eight share one
 // barrier and need longer ranges and more tiles to pay (prefill8_wide, api.hip).
+// Fewer tiles than two a unit leave a SIMD one wavefront and nothing beside its
+// chain: seven requests of 301 to 204 tokens on 517, 12q/4kv x 64, 19.5 us.
 template <int D, int NT>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill8_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,

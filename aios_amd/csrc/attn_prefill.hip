@@ -376,9 +376,10 @@ __global__ __launch_bounds__(NW * 64) void prefill_combine_kernel(
 }
 
 // MANY: tiles of more than 32 parts by eight wavefronts, which ask for 48 at once
-// instead of 32 (6 tokens of 32q/8kv x 128 on 4,093 in 33 parts of the 8-bit
-// cache: 14.6 -> 14.1 us; 100 tokens on 4,000 in 9 parts: 27.4 -> 29.4, so not
-// there).  Its order of additions is another one than four wavefronts'.
+// instead of 32.  Over the 8-bit cache with four / eight, whole prefill: 7 tokens
+// of 8q/1kv x 64 on 9,000 (36 parts) 12.5 / 12.2 us, 6 of 12q/4kv x 64 on 12,000 (47)
+// 12.2 / 11.8, 3 of 16q/4kv x 128 on 15,000 (59) 16.1 / 16.0, 5 of 8q/2kv x 96 on
+// 20,000 (53) 16.5 / 16.6; 100 tokens on 4,000 in 9 parts 27.4 / 29.4, so not there.  Its order of additions is another one than four wavefronts'.
 template <int D, bool MANY>
 static hipError_t launch_combine_d(const PrefillArgs& a, hipStream_t s) {
   if (a.n_parts > 1) {

@@ -499,8 +499,8 @@ __global__ __launch_bounds__(kLpThreads) void logprob_kernel(LogprobArgs a, int3
 
 // One workgroup per row: lane s of every wavefront takes segment s's sums (in
 // 64 bits: exact references, one rounding at the end).  24 rows of 151,936 bf16
-// logits, both launches: 7.4 us, with 5 alternatives 13.4 (their chain: maxima,
-// limit, second read, ranks), with 20 19.4.
+// logits, both launches: 7.2 us, with 5 alternatives 13.2 (their chain: maxima,
+// limit, second read, ranks), with 20 18.7.
 template <typename T>
 __global__ __launch_bounds__(kLpMergeThreads) void logprob_merge_kernel(LogprobArgs a, int32_t segs,
                                                                         const LpState* states,
