@@ -23,6 +23,9 @@ PHASE_PREFILL = 0
 PHASE_DECODE = 1
 PHASE_PREFILL8 = 2  # a plan's phase for the 8-bit cache
 PHASE_DECODE8 = 3
+PHASE_TREE = 4  # a plan's phase for trees of drafts
+PHASE_TREE8 = 5
+TREE_MAX_NODES = 256
 PROLOGUE_NONE = 0
 PROLOGUE_ADD_RMSNORM = 1
 EPILOGUE_NONE = 0
@@ -71,6 +74,10 @@ EXPORTED_SYMBOLS = (
     "aios_attn_decode8",
     "aios_attn_append_decode8",
     "aios_attn_append_decode_rope8",
+    "aios_attn_plan_tree",
+    "aios_attn_tree",
+    "aios_attn_tree8",
+    "aios_tree_masks",
     "aios_token_logprobs_workspace",
     "aios_token_logprobs",
 )
@@ -259,6 +266,21 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp,
         _vp, _vp, _vp, _vp, _vp, _i64, _vp, _f32, _vp, _vp, _i64, _f32, _vp,
     ]
+    lib.aios_attn_plan_tree.restype = ctypes.c_int
+    lib.aios_attn_plan_tree.argtypes = [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i64,
+                                        ctypes.POINTER(AttnPlan)]
+    lib.aios_attn_tree.restype = ctypes.c_int
+    lib.aios_attn_tree.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp,
+        _i64, _f32, _vp,
+    ]
+    lib.aios_attn_tree8.restype = ctypes.c_int
+    lib.aios_attn_tree8.argtypes = [
+        ctypes.POINTER(AttnPlan), _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp,
+        _vp, _i64, _f32, _vp,
+    ]
+    lib.aios_tree_masks.restype = ctypes.c_int
+    lib.aios_tree_masks.argtypes = [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp]
     lib.aios_token_logprobs_workspace.restype = _i64
     lib.aios_token_logprobs_workspace.argtypes = [_i64, _i32, _i32]
     lib.aios_token_logprobs.restype = ctypes.c_int

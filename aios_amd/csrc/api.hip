@@ -1683,6 +1683,132 @@ int aios_attn_append_decode_rope8(const aios_attn_plan_t* p, const void* q, int6
 }
 
 // ---------------------------------------------------------------------------
+// trees of drafted tokens
+
+int aios_attn_plan_tree(const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t hq,
+                        int32_t hkv, int32_t d, int32_t page_size, int32_t kv_bits,
+                        int64_t ws_bytes, aios_attn_plan_t* p) {
+  int rc = plan_sizes(AIOS_PHASE_PREFILL, cu_q, cu_k, batch, hq, hkv, d, page_size, p);
+  if (rc) return rc;
+  if (kv_bits != 8 && kv_bits != 16)
+    return fail(AIOS_ERR_INVALID, "plan_tree: kv_bits must be 8 or 16");
+  if (p->max_q_len > aios::kTreeMaxNodes)
+    return fail(AIOS_ERR_UNSUPPORTED, "plan_tree: %d nodes exceed the %d of a request",
+                p->max_q_len, aios::kTreeMaxNodes);
+  p->phase = kv_bits == 8 ? AIOS_PHASE_TREE8 : AIOS_PHASE_TREE;
+  if (p->max_q_len == 0) return AIOS_OK;
+  // the fewest tiles of at most 128 MFMA rows, of equal size
+  p->prefill_q_tile = cdiv(p->max_q_len, p->num_q_tiles);
+  p->prefix_chunk_len = 32 * aios::kPrefillFewSub;
+  p->num_parts = 1;
+  return AIOS_OK;
+}
+
+// The checks and arguments common to both caches.
+static int tree_args(const char* what, const aios_attn_plan_t* p, const void* q,
+                     int64_t q_tok_stride, const int32_t* indices, const int32_t* cu_q,
+                     const int32_t* cu_k, const uint64_t* masks, int32_t mask_words, void* out,
+                     void* workspace, int64_t workspace_bytes, float sm_scale, aios::TreeArgs* t) {
+  if (q_tok_stride < (int64_t)p->num_qo_heads * p->head_dim || (q_tok_stride % 8) != 0)
+    return fail(AIOS_ERR_INVALID, "%s: q token stride %lld must be >= Hq*D and a multiple of 8",
+                what, (long long)q_tok_stride);
+  if (!q || !indices || !cu_q || !cu_k || !masks || !out)
+    return fail(AIOS_ERR_INVALID, "%s: null pointer", what);
+  if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0 || ((uintptr_t)masks & 7) != 0)
+    return fail(AIOS_ERR_INVALID, "%s: q and out must be 16-byte and masks 8-byte aligned", what);
+  if (mask_words < 1 || mask_words * 64 > aios::kTreeMaxNodes || mask_words * 64 < p->max_q_len)
+    return fail(AIOS_ERR_INVALID, "%s: %d mask words do not cover %d nodes (at most %d)", what,
+                mask_words, p->max_q_len, aios::kTreeMaxNodes);
+  const int rc = check_scale8(what, sm_scale);
+  if (rc) return rc;
+  aios::PrefillArgs& a = t->p;
+  a.q = static_cast<const aios::bf16*>(q);
+  a.q_tok_stride = q_tok_stride;
+  a.indices = indices;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.num_qo_heads = p->num_qo_heads;
+  a.num_kv_heads = p->num_kv_heads;
+  a.group = p->group;
+  a.scale_log2 = sm_scale * aios::kLog2e;
+  a.q_tile = p->prefill_q_tile;
+  a.q_tiles = p->num_q_tiles;
+  a.batch = p->batch_size;
+  a.out = static_cast<aios::bf16*>(out);
+  a.part_sub = p->prefix_chunk_len / 32;
+  a.n_parts = 1;
+  a.part_rows = a.q_tile * a.group;
+  if (p->num_parts > 1 && workspace && ((uintptr_t)workspace & 255) == 0 &&
+      p->ws_bytes <= workspace_bytes) {
+    char* ws = static_cast<char*>(workspace);
+    a.n_parts = p->num_parts;
+    a.part_o = reinterpret_cast<float*>(ws + p->ws_parts_o);
+    a.part_ml = reinterpret_cast<float2*>(ws + p->ws_parts_lse);
+  }
+  t->masks = reinterpret_cast<const uint32_t*>(masks);
+  t->words = 2 * mask_words;
+  return AIOS_OK;
+}
+
+int aios_attn_tree(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                   const void* k_cache, const void* v_cache, int64_t kv_num_pages,
+                   const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k,
+                   const uint64_t* masks, int32_t mask_words, void* out, void* workspace,
+                   int64_t workspace_bytes, float sm_scale, void* stream) {
+  int rc = check_plan(p, AIOS_PHASE_TREE);
+  if (rc) return rc;
+  if (p->batch_size == 0 || p->total_q == 0) return AIOS_OK;
+  aios::TreeArgs t = {};
+  rc = tree_args("tree", p, q, q_tok_stride, indices, cu_q, cu_k, masks, mask_words, out,
+                 workspace, workspace_bytes, sm_scale, &t);
+  if (rc) return rc;
+  if (!k_cache || !v_cache) return fail(AIOS_ERR_INVALID, "tree: null pointer");
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) != 0)
+    return fail(AIOS_ERR_INVALID, "tree: caches must be 16-byte aligned");
+  t.p.kv_tok_stride = (int64_t)p->num_kv_heads * p->head_dim;
+  if ((rc = check_cache(kv_num_pages, t.p.kv_tok_stride))) return rc;
+  t.p.k_cache = static_cast<const aios::bf16*>(k_cache);
+  t.p.v_cache = static_cast<const aios::bf16*>(v_cache);
+  t.p.num_pages = kv_num_pages;
+  return check_hip(aios::launch_tree(p->head_dim, 16, t, static_cast<hipStream_t>(stream)),
+                   "tree launch");
+}
+
+int aios_attn_tree8(const aios_attn_plan_t* p, const void* q, int64_t q_tok_stride,
+                    const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                    const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k,
+                    const uint64_t* masks, int32_t mask_words, void* out, void* workspace,
+                    int64_t workspace_bytes, float sm_scale, void* stream) {
+  int rc = check_plan(p, AIOS_PHASE_TREE8);
+  if (rc) return rc;
+  if (p->batch_size == 0 || p->total_q == 0) return AIOS_OK;
+  aios::TreeArgs t = {};
+  rc = tree_args("tree8", p, q, q_tok_stride, indices, cu_q, cu_k, masks, mask_words, out,
+                 workspace, workspace_bytes, sm_scale, &t);
+  if (rc) return rc;
+  rc = kv8_layer("tree8", const_cast<void*>(k8), const_cast<void*>(v8), const_cast<void*>(scales),
+                 num_pages, p->num_kv_heads, p->head_dim, &t.kv);
+  if (rc) return rc;
+  return check_hip(aios::launch_tree(p->head_dim, 8, t, static_cast<hipStream_t>(stream)),
+                   "tree8 launch");
+}
+
+int aios_tree_masks(const int32_t* parents, const int32_t* cu, int32_t batch, int64_t total,
+                    int32_t mask_words, uint64_t* masks, int32_t* depths, void* stream) {
+  if (batch < 0 || total < 0) return fail(AIOS_ERR_INVALID, "tree_masks: bad sizes");
+  if (mask_words < 1 || mask_words * 64 > aios::kTreeMaxNodes)
+    return fail(AIOS_ERR_INVALID, "tree_masks: 1 to %d mask words", aios::kTreeMaxNodes / 64);
+  if (batch == 0 || total == 0) return AIOS_OK;
+  if (!parents || !cu || !masks || !depths)
+    return fail(AIOS_ERR_INVALID, "tree_masks: null pointer");
+  if (((uintptr_t)masks & 7) != 0)
+    return fail(AIOS_ERR_INVALID, "tree_masks: masks must be 8-byte aligned");
+  return check_hip(aios::tree_masks(parents, cu, batch, total, 2 * mask_words, masks, depths,
+                                    static_cast<hipStream_t>(stream)),
+                   "tree_masks launch");
+}
+
+// ---------------------------------------------------------------------------
 // scoring
 
 int64_t aios_token_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {

@@ -1,0 +1,457 @@
+// Attention for trees of drafted tokens over the paged cache, bf16 or 8 bits.
+//
+// The last q_len positions of a request are its nodes (their K/V rows are in
+// their pages); node i sees every position before the nodes and those nodes
+// that bit n of its mask names:
+//   o_i = sum_j softmax_j(scale q_i k_j) v_j over j < cached and j = cached + n,
+// 0 where it sees nothing.  The tiles are those of the prefill: a workgroup
+// owns (request, kv-head, tile of nodes), 128 MFMA rows (node, query head of the
+// group), or one part of such a tile's KV range, merged by the prefill's combine.
+// Unlike a causal tile's, every tile's range is the whole request, and only the
+// sub-tiles that hold nodes are masked: a lane cuts the 32 bits of its row that
+// belong to the sub-tile out of the mask words, which the workgroup keeps in LDS.
+//
+// Values in masked places.  A score is replaced, not added to, so K may hold
+// anything there.  V meets a probability of 0 in the matrix product, and 0 times
+// an infinity or a NaN is NaN: a sub-tile with nodes whose V rows hold any is
+// multiplied without those elements, and the rows that do see them are given
+// them through products of what each row sees with where they are.
+// (8 bits: a row's values are finite, a NaN token makes its scores NaN.)
+#include "engine8.hpp"
+
+namespace aios {
+namespace {
+
+constexpr int kTreeMaxWords = kTreeMaxNodes / 32;  // 32-bit mask words of a node
+
+// TileEngine32 with the rows' masks.
+template <int D, int BITS>
+struct TreeEngine : TileEngine32<D, false> {
+  using Base = TileEngine32<D, false>;
+  using T = typename Base::T;
+  using LaneOff = typename Base::LaneOff;
+  using Base::NT;
+
+  int cached;     // positions before the nodes
+  uint32_t mask;  // LDS address of the lane's node's mask words
+  int words;
+
+  __device__ __forceinline__ uint32_t word(int i) const {
+    return *reinterpret_cast<AIOS_LDS const uint32_t*>((AIOS_LDS const uint8_t*)(uintptr_t)(mask + 4 * i));
+  }
+  // Which of the positions kv0 .. kv0 + 31 the lane's row sees.
+  __device__ __forceinline__ uint32_t window(int kv0, int kv_end) const {
+    const int o = kv0 - cached;  // (uniform; > -32)
+    uint32_t w;
+    if (o < 0) {
+      w = word(0) << -o | ((1u << -o) - 1);
+    } else {
+      const int i = o >> 5;
+      const uint32_t a = i < words ? word(i) : 0u;
+      const uint32_t b = i + 1 < words ? word(i + 1) : 0u;
+      w = __builtin_amdgcn_alignbit(b, a, o & 31);
+    }
+    const int n = kv_end - kv0;
+    return n < 32 ? w & ((1u << n) - 1) : w;
+  }
+
+  // The sub-tile at byte offset sb, positions kv0 ..
+  __device__ __forceinline__ void compute(const LaneOff& lo, uint32_t sb, int kv0, int kv_end,
+                                          float scale_log2) {
+    bf16x8 kf[Base::KS];
+    bf16x4 va[NT][4];
+    this->read_k_at(lo, sb, kf);
+    this->read_v_at(lo, sb, va);
+    f32x16 st = this->mma_s_at(kf);
+    const bool masked = kv0 + kSubTok > min(cached, kv_end);
+    uint32_t seen = 0;
+    if (masked) {
+      // bit 8 (r / 4) + r % 4 of `seen` is the lane's score r
+      seen = window(kv0, kv_end) >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        st[r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? st[r] : kNegInf;
+    }
+    bf16x8 pb0, pb1;
+    float al, psum;
+    const bool moved =
+        this->template softmax_at<false>(st, kv0, kv_end, scale_log2, pb0, pb1, al, psum);
+    if (__builtin_expect(moved, 0)) this->rescale(al);
+    this->ls += psum;
+    if constexpr (BITS == 16) {
+      if (masked) fix_values(va, seen);
+    }
+    this->mma_o_at(va, pb0, pb1);
+  }
+
+  // Takes the infinities and NaNs out of the V fragments and adds them to the o
+  // of the rows that see them.  Two bf16 a word, flags in their sign bits.
+  __device__ __forceinline__ void fix_values(bf16x4 (&va)[NT][4], uint32_t seen) {
+    constexpr uint32_t kMag = 0x7fff7fffu, kFlags = 0x80008000u;
+    uint32_t any = 0;  // (an exponent of ones: the addition carries into the sign bit)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      lds_wait_tied(va[nt][0], va[nt][1]);
+      lds_wait_tied(va[nt][2], va[nt][3]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint2 v = __builtin_bit_cast(uint2, va[nt][q]);
+        any |= ((v.x & kMag) + 0x00800080u) | ((v.y & kMag) + 0x00800080u);
+      }
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((any & kFlags) != 0) == 0, 1)) return;
+    // 1 where the row sees the token (B), times 1 where the value is one of a
+    // kind (A): more than 0 where the row sees one
+    auto ones = [](uint32_t f) { return (f >> 1) - (f >> 8); };  // flags -> bf16 ones
+    uint32_t see[8];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t b = seen >> (8 * (w >> 1) + 2 * (w & 1));
+      see[w] = ones((b & 1) << 15 | (b & 2) << 30);
+    }
+    const bf16x8 see0 = __builtin_bit_cast(bf16x8, make_uint4(see[0], see[1], see[2], see[3]));
+    const bf16x8 see1 = __builtin_bit_cast(bf16x8, make_uint4(see[4], see[5], see[6], see[7]));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t v[8], bad[8], nan[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint2 x = __builtin_bit_cast(uint2, va[nt][q]);
+        v[2 * q] = x.x;
+        v[2 * q + 1] = x.y;
+      }
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        bad[w] = ((v[w] & kMag) + 0x00800080u) & kFlags;
+        nan[w] = ((v[w] & kMag) + 0x007f007fu) & kFlags;
+      }
+      auto add = [&](auto&& flags, float special) {
+        f32x16 t;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[i] = 0.f;
+        uint32_t f[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) f[w] = ones(flags(w));
+        t = mfma32x32x16(__builtin_bit_cast(bf16x8, make_uint4(f[0], f[1], f[2], f[3])), see0, t);
+        t = mfma32x32x16(__builtin_bit_cast(bf16x8, make_uint4(f[4], f[5], f[6], f[7])), see1, t);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) this->o[nt][i] += t[i] > 0.f ? special : 0.f;
+      };
+      add([&](int w) { return bad[w] & ~nan[w] & ~v[w]; }, __builtin_inff());
+      add([&](int w) { return bad[w] & ~nan[w] & v[w]; }, -__builtin_inff());
+      add([&](int w) { return nan[w]; }, __builtin_nanf(""));
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v[w] &= ~((bad[w] << 1) - (bad[w] >> 15));
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        va[nt][q] = __builtin_bit_cast(bf16x4, make_uint2(v[2 * q], v[2 * q + 1]));
+    }
+  }
+};
+
+__device__ __forceinline__ float inv_or_zero(float l) { return l > 0.f ? 1.f / l : l * 0.f; }
+
+// Dims 8 dg .. 8 dg + 7 of row m in a part's o.
+template <int D>
+__device__ __forceinline__ int64_t part_o(const PrefillArgs& a, int64_t part, int dg, int m) {
+  return ((part * (D / 8) + dg) * a.part_rows + m) * 8;
+}
+
+// One part of a tile's KV range per workgroup (n_parts 1: the whole range).
+template <int D, int BITS>
+__global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void tree_kernel(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
+    const int32_t* __restrict__ indices, int32_t num_kv_heads, int32_t batch, int32_t q_tiles,
+    int32_t q_tile, int32_t group, int32_t n_parts, int32_t part_sub, int32_t part_rows,
+    TreeArgs args) {
+  // (the leading scalars are preloaded: a by-value struct takes a memory round trip)
+  PrefillArgs a = args.p;
+  a.num_kv_heads = num_kv_heads;
+  a.num_qo_heads = num_kv_heads * group;
+  a.q_tiles = q_tiles;
+  a.n_parts = n_parts;
+  a.part_rows = part_rows;
+  const int G = group;
+  using E = TreeEngine<D, BITS>;
+  using T = typename E::T;
+  using S = Stage8<D>;
+  constexpr int kTiles = BITS == 16 ? T::LDS_BYTES : S::LDS_BYTES;
+  __shared__ __align__(16) uint8_t lds[kTiles];
+  __shared__ uint32_t smask[128 * kTreeMaxWords];
+  __shared__ float2 sml[4 * 32];  // (m, l) of the four wavefronts' rows
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Consecutive workgroups: kv-heads, then requests, tiles, parts (the order of
+  // prefill_split_kernel, and its reasons).
+  const int flat = blockIdx.x;
+  const int h = flat % num_kv_heads;
+  int rest = flat / num_kv_heads;
+  const int r = rest % batch;
+  rest /= batch;
+  const int qt = rest % q_tiles;
+  const int s = rest / q_tiles;
+  const int q_start = cu_q[r];
+  const int q_len = cu_q[r + 1] - q_start;
+  if (qt * q_tile >= q_len) return;
+  const int kv_base = cu_k[r];
+  const int kv_len = cu_k[r + 1] - kv_base;
+  const int rows = min(q_tile, q_len - qt * q_tile) * G;
+  const PrefillParts pp = prefill_parts(kv_len, part_sub, rows <= part_rows ? n_parts : 1);
+  if (s >= pp.n) return;
+  const int kv_begin = s * pp.per * kSubTok;
+  const int kv_end = min(kv_len, kv_begin + pp.per * kSubTok);
+
+  // Wavefront -> (row tile, share of the sub-tiles).
+  const int nr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int ng = 4 / nr;
+  const int rt = wave & (nr - 1);
+  const int share = nr == 4 ? 0 : nr == 2 ? wave >> 1 : wave;
+  const int m = rt * 32 + (lane & 31);
+  const int node = m / G;
+  const int i = qt * q_tile + node;
+  const int g = m - node * G;
+  const bool ok = m < rows;
+  const int hl = lane >> 5;
+  const bf16* qr = a.q + (int64_t)(q_start + i) * a.q_tok_stride + (int64_t)(h * G + g) * D;
+
+  E eng;
+  eng.cached = kv_len - q_len;
+  eng.words = args.words;
+  eng.mask = (uint32_t)(uintptr_t)(AIOS_LDS const uint32_t*)(smask + node * kTreeMaxWords);
+  eng.reset();
+  const auto lo = eng.lane_offsets(lds);
+
+  // The tile's mask words, where the range holds nodes: asked for now, in LDS
+  // from the first barrier behind qload on.
+  constexpr int kMaskLoads = 128 * kTreeMaxWords / kEngineThreads;
+  const bool tail = kv_end > eng.cached;
+  uint32_t mw[kMaskLoads];
+  if (tail) {
+#pragma unroll
+    for (int j = 0; j < kMaskLoads; ++j) {
+      const int e = j * kEngineThreads + tid, n = e / kTreeMaxWords, w = e % kTreeMaxWords;
+      mw[j] = n * G < rows && w < args.words
+                  ? args.masks[(int64_t)(q_start + qt * q_tile + n) * args.words + w]
+                  : 0u;
+    }
+  }
+  auto qload = [&] {
+    eng.load_q(qr, ok);
+    if (tail) {
+#pragma unroll
+      for (int j = 0; j < kMaskLoads; ++j) smask[j * kEngineThreads + tid] = mw[j];
+    }
+  };
+  const int32_t* idx = indices + kv_base;
+  const int n_sub = (kv_end - kv_begin + kSubTok - 1) / kSubTok;
+  if constexpr (BITS == 16) {
+    stream_kv<T, 0, true>(
+        lds, reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * D * 2,
+        reinterpret_cast<const uint8_t*>(a.v_cache) + (int64_t)h * D * 2, a.kv_tok_stride * 2,
+        a.num_pages, idx, kv_begin, kv_end, qload,
+        [&](uint32_t sb, int kv0) {
+          if (share == 0) eng.compute(lo, sb, kv0, kv_end, a.scale_log2);
+        },
+        rt * 32 < rows,
+        [&](auto&& wait_sub, int) {
+          if (ng > 1) {
+            wait_sub(kRing - 1);
+            for (int it = share; it < n_sub; it += ng)
+              eng.compute(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
+                          a.scale_log2);
+            return;
+          }
+#pragma unroll
+          for (int it = 0; it < kRing; ++it) {
+            if (it >= n_sub) break;
+            wait_sub(it);
+            eng.compute(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
+                        a.scale_log2);
+          }
+        });
+  } else {
+    S st(args.kv, h, idx, kv_begin, kv_end);
+    if (ng > 1 && st.steps() <= 2) {
+      typename S::Regs r0, r1;
+      typename S::Ids i0, i1;
+      st.ids(0, i0);
+      st.ids(1, i1);
+      st.load(0, i0, r0);
+      st.load(1, i1, r1);
+      qload();
+      st.store(lds, 0, r0);
+      st.store(lds, 1, r1);
+      lds_barrier();
+      for (int it = share; it < n_sub; it += ng)
+        eng.compute(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
+                    a.scale_log2);
+    } else {
+      st.template stream<1>(
+          lds, qload,
+          [&](auto sb, int kv0) {
+            if (((kv0 - kv_begin) / kSubTok & (ng - 1)) == share)
+              eng.compute(lo, decltype(sb)::value, kv0, kv_end, a.scale_log2);
+          },
+          rt * 32 < rows);
+    }
+  }
+  eng.l_run = xor32_sum(eng.ls);
+
+  const int64_t part = (((int64_t)r * q_tiles + qt) * num_kv_heads + h) * n_parts + s;
+  if (ng == 1) {
+    if (!ok) return;
+    if (pp.n == 1) {
+      const float inv = inv_or_zero(eng.l_run);
+      bf16* po = a.out + ((int64_t)(q_start + i) * a.num_qo_heads + (h * G + g)) * D + 4 * hl;
+#pragma unroll
+      for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint2 packed;
+          packed.x = pack_bf16x2(eng.o[nt][4 * j] * inv, eng.o[nt][4 * j + 1] * inv);
+          packed.y = pack_bf16x2(eng.o[nt][4 * j + 2] * inv, eng.o[nt][4 * j + 3] * inv);
+          *reinterpret_cast<uint2*>(po + nt * 32 + 8 * j) = packed;
+        }
+      return;
+    }
+#pragma unroll
+    for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(a.part_o + part_o<D>(a, part, nt * 4 + j, m) + 4 * hl) =
+            f32x4{eng.o[nt][4 * j], eng.o[nt][4 * j + 1], eng.o[nt][4 * j + 2],
+                  eng.o[nt][4 * j + 3]};
+    if (hl == 0) a.part_ml[part * a.part_rows + m] = make_float2(eng.m_run, eng.l_run);
+    return;
+  }
+
+  // Few rows: the wavefronts of a row tile merge their states.
+  static_assert(T::SUB_BYTES == 32 * D * 4, "a row tile's fp32 o fills one sub-tile");
+  static_assert(kTiles >= 4 * T::SUB_BYTES, "four wavefronts' o in the tiles' LDS");
+  lds_barrier();  // every wavefront is done with K/V
+  float* so = reinterpret_cast<float*>(lds + wave * T::SUB_BYTES);
+#pragma unroll
+  for (int nt = 0; nt < D / 32; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<f32x4*>(so + ((nt * 4 + j) * 32 + (lane & 31)) * 8 + 4 * hl) =
+          f32x4{eng.o[nt][4 * j], eng.o[nt][4 * j + 1], eng.o[nt][4 * j + 2], eng.o[nt][4 * j + 3]};
+  if (hl == 0) sml[wave * 32 + (lane & 31)] = make_float2(eng.m_run, eng.l_run);
+  __syncthreads();
+  const int nrow = nr * 32;
+  for (int e = tid; e < nrow * (D / 8); e += kEngineThreads) {
+    const int dg = e / nrow;
+    const int row = e - dg * nrow;
+    if (row >= rows) continue;
+    const int w0 = row >> 5;  // the row tile; its shares are wavefronts w0 + k * nr
+    float mx = kNegInf;
+    for (int w = w0; w < 4; w += nr) mx = vmax(mx, sml[w * 32 + (row & 31)].x);
+    const float mu = mx == kNegInf ? 0.f : mx;
+    f32x4 acc0 = f32x4{0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
+    float l = 0.f;
+    for (int w = w0; w < 4; w += nr) {
+      const float2 ml = sml[w * 32 + (row & 31)];
+      const float f = fast_exp2(ml.x - mu);
+      l += ml.y * f;
+      const f32x4* po = reinterpret_cast<const f32x4*>(lds + w * T::SUB_BYTES) +
+                        (dg * 32 + (row & 31)) * 2;
+      acc0 += po[0] * f;
+      acc1 += po[1] * f;
+    }
+    if (pp.n == 1) {
+      const float inv = inv_or_zero(l);
+      acc0 *= inv;
+      acc1 *= inv;
+      const int qi = q_start + qt * q_tile + row / G;
+      bf16* po = a.out + ((int64_t)qi * a.num_qo_heads + h * G + row % G) * D + dg * 8;
+      *reinterpret_cast<uint4*>(po) =
+          make_uint4(pack_bf16x2(acc0[0], acc0[1]), pack_bf16x2(acc0[2], acc0[3]),
+                     pack_bf16x2(acc1[0], acc1[1]), pack_bf16x2(acc1[2], acc1[3]));
+    } else {
+      f32x4* po = reinterpret_cast<f32x4*>(a.part_o + part_o<D>(a, part, dg, row));
+      po[0] = acc0;
+      po[1] = acc1;
+      if (dg == 0) a.part_ml[part * a.part_rows + row] = make_float2(mx, l);
+    }
+  }
+}
+
+template <int D, int BITS>
+hipError_t launch_d(const TreeArgs& t, hipStream_t s) {
+  const PrefillArgs& a = t.p;
+  const int wgs = a.q_tiles * a.num_kv_heads * a.batch * a.n_parts;
+  if (wgs == 0) return hipSuccess;
+  hipLaunchKernelGGL((tree_kernel<D, BITS>), dim3(wgs), dim3(kEngineThreads), 0, s, a.cu_q, a.cu_k,
+                     a.indices, a.num_kv_heads, a.batch, a.q_tiles, a.q_tile, a.group, a.n_parts,
+                     a.part_sub, a.part_rows, t);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? launch_tree_combine(D, a, s) : e;
+}
+
+// Masks and depths of every request's nodes from their parents.  One workgroup
+// per request, a node per thread: with a[i] the ancestor 2^k levels up and m[i]
+// the set of the first 2^k nodes on the way up, m[i] |= m[a[i]] and a[i] =
+// a[a[i]] double k, so a chain of 256 takes eight rounds.
+__global__ __launch_bounds__(kTreeMaxNodes) void tree_masks_kernel(const int32_t* parents,
+                                                                   const int32_t* cu, int64_t total,
+                                                                   int32_t words, uint32_t* masks,
+                                                                   int32_t* depths) {
+  __shared__ uint32_t sm[kTreeMaxWords][kTreeMaxNodes];
+  __shared__ int32_t sa[kTreeMaxNodes], sd[kTreeMaxNodes];
+  const int i = threadIdx.x;
+  const int64_t first = cu[blockIdx.x];
+  const int64_t n = cu[blockIdx.x + 1] - first;
+  const bool live = i < n && first >= 0 && first + i < total;
+  uint32_t m[kTreeMaxWords];
+#pragma unroll
+  for (int w = 0; w < kTreeMaxWords; ++w) m[w] = w == i >> 5 ? 1u << (i & 31) : 0u;
+  int a = live ? parents[first + i] : -1;
+  a = a >= 0 && a < i ? a : -1;  // (an earlier node, or none)
+  int d = a >= 0 ? 1 : 0;
+  while (__syncthreads_or(a >= 0)) {
+#pragma unroll
+    for (int w = 0; w < kTreeMaxWords; ++w) sm[w][i] = m[w];
+    sa[i] = a;
+    sd[i] = d;
+    __syncthreads();
+    if (a >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeMaxWords; ++w) m[w] |= sm[w][a];
+      d += sd[a];
+      a = sa[a];
+    }
+  }
+  if (live) {
+#pragma unroll
+    for (int w = 0; w < kTreeMaxWords; ++w)
+      if (w < words) masks[(first + i) * words + w] = m[w];
+    depths[first + i] = d;
+  }
+  // (nodes past the most a request may have see nothing)
+  if (first >= 0)
+    for (int64_t j = first + kTreeMaxNodes + i; j < first + n && j < total; j += kTreeMaxNodes) {
+      for (int w = 0; w < words; ++w) masks[j * words + w] = 0;
+      depths[j] = 0;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_tree(int D, int bits, const TreeArgs& a, hipStream_t s) {
+  switch (D) {
+    case 64: return bits == 16 ? launch_d<64, 16>(a, s) : launch_d<64, 8>(a, s);
+    case 96: return bits == 16 ? launch_d<96, 16>(a, s) : launch_d<96, 8>(a, s);
+    case 128: return bits == 16 ? launch_d<128, 16>(a, s) : launch_d<128, 8>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t tree_masks(const int32_t* parents, const int32_t* cu, int32_t batch, int64_t total,
+                      int32_t words, void* masks, int32_t* depths, hipStream_t s) {
+  hipLaunchKernelGGL(tree_masks_kernel, dim3(batch), dim3(kTreeMaxNodes), 0, s, parents, cu, total,
+                     words, static_cast<uint32_t*>(masks), depths);
+  return hipGetLastError();
+}
+
+}  // namespace aios

@@ -29,7 +29,10 @@ def plan(phase: str, cu_q, cu_k, num_qo_heads: int, num_kv_heads: int, head_dim:
          prefix_chunk_len: int = 0, suffix_split_len: int = 0,
          kv_bits: int = 16) -> _lib.AttnPlan:
     """Host-only schedule for one batch over a cache of ``kv_bits`` (16:
-    bfloat16, aios_attn_plan; 8: the calls named ...8, aios_attn_plan8)."""
+    bfloat16, aios_attn_plan; 8: the calls named ...8, aios_attn_plan8).
+    ``phase``: "decode", "prefill", or "tree" for :func:`tree_attention`
+    (aios_attn_plan_tree, which takes no shared prefix and no lengths of
+    parts)."""
     if kv_bits not in (8, 16):
         raise ValueError("kv_bits must be 8 or 16")
     cu_q = _host_i32(cu_q)
@@ -37,6 +40,16 @@ def plan(phase: str, cu_q, cu_k, num_qo_heads: int, num_kv_heads: int, head_dim:
     if cu_q.numel() != cu_k.numel() or cu_q.numel() < 1:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have batch_size + 1 entries")
     p = _lib.AttnPlan()
+    if phase == "tree":
+        if shared_prefix_len or prefix_chunk_len or suffix_split_len:
+            raise ValueError("a plan for trees takes no shared prefix and no lengths of parts")
+        _lib.check(
+            _lib.lib().aios_attn_plan_tree(cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1,
+                                           num_qo_heads, num_kv_heads, head_dim, 1, kv_bits,
+                                           workspace_bytes, p),
+            "aios_attn_plan_tree",
+        )
+        return p
     code = _lib.PHASE_DECODE if phase == "decode" else _lib.PHASE_PREFILL
     make = _lib.lib().aios_attn_plan8 if kv_bits == 8 else _lib.lib().aios_attn_plan
     _lib.check(
@@ -456,6 +469,103 @@ def prefill8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
         "aios_attn_prefill8",
     )
     return out
+
+
+def _check_tree(p: _lib.AttnPlan, q: torch.Tensor, indices: torch.Tensor, cu_q: torch.Tensor,
+                cu_k: torch.Tensor, masks: torch.Tensor) -> int:
+    """The arguments that both caches' calls share; returns q's GPU."""
+    dev = _check_q8(p, q, p.total_q)
+    b = p.batch_size + 1
+    # (one test for calls in order, as for the 8-bit cache)
+    if not (indices.dtype is _I32 is cu_k.dtype and cu_q.dtype is _I32 and indices.is_contiguous()
+            and cu_q.is_contiguous() and cu_k.is_contiguous() and indices.numel() >= p.total_kv
+            and cu_q.numel() >= b and cu_k.numel() >= b
+            and dev == indices.get_device() == cu_q.get_device() == cu_k.get_device()):
+        _check_lists8(dev, (indices, "indices", p.total_kv), (cu_q, "cu_q", b), (cu_k, "cu_k", b))
+    if masks.dtype is not torch.int64 or masks.ndim != 2 or masks.shape[0] != p.total_q or \
+            not masks.is_contiguous() or masks.get_device() != dev:
+        raise ValueError("masks must be a contiguous int64 [nodes, words] tensor on q's GPU")
+    return dev
+
+
+def tree_attention(p: _lib.AttnPlan, q: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, indices: torch.Tensor, cu_q: torch.Tensor,
+                   cu_k: torch.Tensor, masks: torch.Tensor, *, out: torch.Tensor | None = None,
+                   sm_scale: float | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens of one layer (aios_attn_tree; the
+    plan is one of ``phase`` "tree"): [nodes, Hq, D] bf16.  The last positions
+    of every request are its nodes; node i attends to all positions before them
+    and to the nodes named by ``masks`` (int64 [nodes, words]: bit j % 64 of word
+    j / 64 for node j of its request, see :func:`tree_masks`).  A node that sees
+    nothing gives zeros."""
+    if p.phase != _lib.PHASE_TREE:
+        raise ValueError("plan was not built for trees over the bfloat16 cache")
+    dev = _check_tree(p, q, indices, cu_q, cu_k, masks)
+    _check_cache(k_cache, p)
+    _check_cache(v_cache, p)
+    if not dev == k_cache.get_device() == v_cache.get_device() or \
+            k_cache.shape != v_cache.shape:
+        raise ValueError("the KV caches must be on q's GPU and of one shape")
+    out = _out_like(q, out)
+    # (a buffer of this call alone, as in prefill)
+    ws = torch.empty(p.ws_bytes, dtype=torch.uint8, device=q.device) if p.ws_bytes else None
+    _lib.check(
+        _lib.lib().aios_attn_tree(
+            p, q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.shape[0], indices.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+            masks.data_ptr(), masks.shape[1], out.data_ptr(),
+            None if ws is None else ws.data_ptr(), p.ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
+        "aios_attn_tree",
+    )
+    return out
+
+
+def tree_attention8(p: _lib.AttnPlan, q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
+                    scales: torch.Tensor, indices: torch.Tensor, cu_q: torch.Tensor,
+                    cu_k: torch.Tensor, masks: torch.Tensor, *, out: torch.Tensor | None = None,
+                    sm_scale: float | None = None) -> torch.Tensor:
+    """:func:`tree_attention` over the 8-bit cache (as :func:`decode8`)."""
+    if p.phase != _lib.PHASE_TREE8:
+        raise ValueError("plan was not built for trees over the 8-bit cache (kv_bits=8)")
+    dev = _check_tree(p, q, indices, cu_q, cu_k, masks)
+    pages = _check_kv8(p, dev, k8, v8, scales)
+    out = _out_like(q, out)
+    ws = torch.empty(p.ws_bytes, dtype=torch.uint8, device=q.device) if p.ws_bytes else None
+    _lib.check(
+        _lib.lib().aios_attn_tree8(
+            p, q.data_ptr(), q.stride(0), k8.data_ptr(), v8.data_ptr(), scales.data_ptr(), pages,
+            indices.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), masks.data_ptr(),
+            masks.shape[1], out.data_ptr(), None if ws is None else ws.data_ptr(), p.ws_bytes,
+            p.head_dim ** -0.5 if sm_scale is None else sm_scale, _lib.current_stream(q)),
+        "aios_attn_tree8",
+    )
+    return out
+
+
+def tree_masks(parents: torch.Tensor, cu: torch.Tensor,
+               max_nodes: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(masks int64 [nodes, words], depths int32 [nodes]) of trees whose node i
+    continues node ``parents[i]`` of its request (int32, counted within the
+    request; -1: none), request r's nodes being ``cu[r] .. cu[r + 1]``, at most
+    ``max_nodes`` each (aios_tree_masks).  A node sees itself and its
+    ancestors."""
+    if not 1 <= max_nodes <= _lib.TREE_MAX_NODES:
+        raise ValueError(f"max_nodes must be within 1..{_lib.TREE_MAX_NODES}")
+    if parents.dtype is not _I32 or parents.ndim != 1 or not parents.is_contiguous() \
+            or not parents.is_cuda:
+        raise ValueError("parents must be a contiguous int32 [nodes] GPU tensor")
+    _check_lists8(parents.get_device(), (cu, "cu", 1))
+    n, words = parents.numel(), -(-max_nodes // 64)
+    masks = torch.empty((n, words), dtype=torch.int64, device=parents.device)
+    depths = torch.empty_like(parents)
+    _lib.check(
+        _lib.lib().aios_tree_masks(parents.data_ptr(), cu.data_ptr(), cu.numel() - 1, n, words,
+                                   masks.data_ptr(), depths.data_ptr(),
+                                   _lib.current_stream(parents)),
+        "aios_tree_masks",
+    )
+    return masks, depths
 
 
 def build_indices(page_table: torch.Tensor, row_ids: torch.Tensor, cu_k: torch.Tensor,

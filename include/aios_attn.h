@@ -642,6 +642,70 @@ int aios_attn_append_decode_rope8(const aios_attn_plan_t* plan, const void* q,
                                   float sm_scale, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Trees of drafted tokens.  No counterpart in the reference.
+ *
+ * The last q_len positions of a request are its nodes: the token that is
+ * already decided (node 0) and the drafts behind it, each a continuation of an
+ * earlier node, with their K/V rows in the request's last q_len pages.  A mask
+ * per node names the nodes that it sees: masks [total_q][mask_words] 64-bit
+ * words, bit j % 64 of word j / 64 for node j of the same request (bits past
+ * the request's nodes are ignored; a node past the words is seen by none).
+ */
+#define AIOS_TREE_MAX_NODES 256 /* nodes of a request */
+#define AIOS_PHASE_TREE 4       /* a plan's phase (see aios_attn_plan_tree) */
+#define AIOS_PHASE_TREE8 5
+
+/*
+ * The schedule of a batch of trees over a cache of kv_bits (16: bfloat16, for
+ * aios_attn_tree; 8: for aios_attn_tree8); the other arguments as for
+ * aios_attn_plan.  Requests of more than AIOS_TREE_MAX_NODES nodes return
+ * AIOS_ERR_UNSUPPORTED.  The lengths on the device may differ from the planned
+ * ones: any KV length from the request's nodes on, and at most the planned
+ * largest number of nodes; indices then holds what cu_k names.
+ */
+int aios_attn_plan_tree(const int32_t* cu_q_host, const int32_t* cu_k_host, int32_t batch_size,
+                        int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t page_size, int32_t kv_bits, int64_t workspace_bytes,
+                        aios_attn_plan_t* plan_out);
+
+/*
+ * Attention of the nodes (arguments as for aios_attn_prefill_ws): node i of
+ * request r attends to every position before the request's nodes and to the
+ * nodes that masks names, in any pattern; a node that sees nothing gives
+ * zeros.  What K and V hold at positions that a node does not see, infinities
+ * and NaNs included, does not reach its output.  mask_words * 64 covers the
+ * plan's largest number of nodes (at most 4 words); masks 8-byte aligned;
+ * sm_scale positive and finite.  Used with the workspace when it is given,
+ * 256-byte aligned, and holds plan->ws_bytes; otherwise every tile is one
+ * workgroup.
+ */
+int aios_attn_tree(const aios_attn_plan_t* plan, const void* q, int64_t q_tok_stride,
+                   const void* k_cache, const void* v_cache, int64_t kv_num_pages,
+                   const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k,
+                   const uint64_t* masks, int32_t mask_words, void* out, void* workspace,
+                   int64_t workspace_bytes, float sm_scale, void* stream);
+
+/* aios_attn_tree over the 8-bit cache. */
+int aios_attn_tree8(const aios_attn_plan_t* plan, const void* q, int64_t q_tok_stride,
+                    const void* k8, const void* v8, const void* scales, int64_t num_pages,
+                    const int32_t* indices, const int32_t* cu_q, const int32_t* cu_k,
+                    const uint64_t* masks, int32_t mask_words, void* out, void* workspace,
+                    int64_t workspace_bytes, float sm_scale, void* stream);
+
+/*
+ * Masks and depths of a batch of trees from their parents: request r owns
+ * nodes [cu[r], cu[r+1]) of total_nodes, parents[cu[r] + i] is the parent of
+ * its node i, counted within the request.  A node sees itself and its
+ * ancestors; depths is the number of those (the node's position is that of
+ * node 0 plus its depth).  A parent that is not an earlier node (-1: none) leaves
+ * a node without ancestors.  A node past AIOS_TREE_MAX_NODES of its request sees
+ * nothing, at depth 0; ancestors past mask_words (1 to 4) words are left out.
+ */
+int aios_tree_masks(const int32_t* parents, const int32_t* cu, int32_t batch_size,
+                    int64_t total_nodes, int32_t mask_words, uint64_t* masks, int32_t* depths,
+                    void* stream);
+
+/* ------------------------------------------------------------------------
  * Scoring: for every row of logits (elem_bytes 2: bf16, 4: fp32; rows
  * row_stride elements apart, 0: one row for all; aligned to their element
  * only), with p = softmax(row):
