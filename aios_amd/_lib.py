@@ -80,6 +80,8 @@ EXPORTED_SYMBOLS = (
     "aios_tree_masks",
     "aios_token_logprobs_workspace",
     "aios_token_logprobs",
+    "aios_verify_workspace",
+    "aios_verify_drafts",
 )
 
 
@@ -286,6 +288,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.aios_token_logprobs.restype = ctypes.c_int
     lib.aios_token_logprobs.argtypes = [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
                                         _vp, _i64, _vp]
+    lib.aios_verify_workspace.restype = _i64
+    lib.aios_verify_workspace.argtypes = [_i32, _i64, _i32, _i32]
+    lib.aios_verify_drafts.restype = ctypes.c_int
+    lib.aios_verify_drafts.argtypes = [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _i64,
+                                       _vp, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
     lib.aios_attnres_mix.restype = ctypes.c_int
     lib.aios_attnres_mix.argtypes = [_vp, _i32, _i64, _i32, _vp, _vp, _f32, _vp, _vp, _vp]
     lib.aios_attnres_mix_ex.restype = ctypes.c_int

@@ -1845,4 +1845,69 @@ int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, in
                    "token_logprobs launch");
 }
 
+// ---------------------------------------------------------------------------
+// verification of drafted tokens
+
+int64_t aios_verify_workspace(int32_t batch, int64_t total, int32_t vocab, int32_t drawn) {
+  if (batch <= 0 || total < 0 || total > (1ll << 24) || vocab <= 0) return 0;
+  return aios::verify_workspace(batch, total, vocab, drawn != 0);
+}
+
+int aios_verify_drafts(const void* logits, int64_t row_stride, const void* draft,
+                       int64_t draft_stride, int32_t vocab, int32_t elem_bytes,
+                       const int64_t* tokens, const int32_t* parents, const int32_t* cu,
+                       int32_t batch, int64_t total, const float* uniforms, float temperature,
+                       float draft_temperature, uint8_t* accepted, int32_t* counts, int32_t* last,
+                       int64_t* next_tokens, float* logprobs, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+  if (batch < 0 || total < 0 || vocab <= 0)
+    return fail(AIOS_ERR_INVALID, "verify_drafts: bad sizes");
+  if (elem_bytes != 2 && elem_bytes != 4)
+    return fail(AIOS_ERR_UNSUPPORTED, "verify_drafts: logits must be bf16 or fp32");
+  const bool greedy = temperature == 0.f;
+  auto warm = [](float t) { return t >= 1e-4f && t <= 1e4f; };
+  if (!greedy && (!warm(temperature) || (draft && !warm(draft_temperature))))
+    return fail(AIOS_ERR_INVALID, "verify_drafts: temperatures must be within 1e-4 .. 1e4 (or 0 "
+                "for the most likely tokens)");
+  if (row_stride < 0 || (row_stride > 0 && row_stride < vocab) ||
+      (draft && (draft_stride < 0 || (draft_stride > 0 && draft_stride < vocab))))
+    return fail(AIOS_ERR_INVALID, "verify_drafts: row stride smaller than the vocabulary");
+  if (batch == 0) return AIOS_OK;
+  if (total > (1ll << 24) || vocab > (1 << 30))
+    return fail(AIOS_ERR_UNSUPPORTED, "verify_drafts: more than 2^24 nodes or 2^30 ids");
+  if (greedy) draft = nullptr;
+  if (!aios::verify_fits(batch, total, vocab, draft != nullptr))
+    return fail(AIOS_ERR_UNSUPPORTED, "verify_drafts: too many nodes for one call");
+  if (!cu || !counts || !last || !next_tokens ||
+      (total > 0 && (!logits || !tokens || !parents || (!uniforms && !greedy) || !accepted || !logprobs)))
+    return fail(AIOS_ERR_INVALID, "verify_drafts: null pointer");
+  if ((((uintptr_t)logits | (uintptr_t)draft) & (uintptr_t)(elem_bytes - 1)) != 0)
+    return fail(AIOS_ERR_INVALID, "verify_drafts: misaligned logits");
+  if (!workspace || ((uintptr_t)workspace & 15) != 0 ||
+      workspace_bytes < aios::verify_workspace(batch, total, vocab, draft != nullptr))
+    return fail(AIOS_ERR_WORKSPACE, "verify_drafts: needs a workspace of %lld bytes, 16-byte aligned",
+                (long long)aios::verify_workspace(batch, total, vocab, draft != nullptr));
+  aios::VerifyArgs a = {};
+  a.logits = logits;
+  a.stride = row_stride;
+  a.draft = draft;
+  a.draft_stride = draft_stride;
+  a.vocab = vocab;
+  a.elem_bytes = elem_bytes;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.cu = cu;
+  a.batch = batch;
+  a.total = total;
+  a.uniforms = uniforms;
+  a.accepted = accepted;
+  a.counts = counts;
+  a.last = last;
+  a.next_tokens = next_tokens;
+  a.logprobs = logprobs;
+  return check_hip(aios::verify_drafts(a, temperature, draft_temperature, workspace,
+                                       static_cast<hipStream_t>(stream)),
+                   "verify_drafts launch");
+}
+
 }  // extern "C"

@@ -446,4 +446,35 @@ int64_t logprob_workspace(int64_t rows, int32_t vocab, int32_t segments, int32_t
 hipError_t token_logprobs(const LogprobArgs& a, int32_t segments, void* workspace,
                           hipStream_t stream);
 
+// Verification of drafted tokens (verify.hip).
+struct VerifyArgs {
+  const void* logits;  // [total][vocab], rows stride elements apart
+  int64_t stride;
+  const void* draft;   // the distributions that children were drawn from (may be null)
+  int64_t draft_stride;
+  int32_t vocab;
+  int32_t elem_bytes;  // of both: 2 bf16, 4 fp32
+  const int64_t* tokens;   // [total]
+  const int32_t* parents;  // [total], within the request
+  const int32_t* cu;       // [batch + 1]
+  int32_t batch;
+  int64_t total;
+  const float* uniforms;   // [total]
+  uint8_t* accepted;       // [total] bool
+  int32_t* counts;         // [batch]
+  int32_t* last;           // [batch]
+  int64_t* next_tokens;    // [batch]
+  float* logprobs;         // [total]
+  // (set by verify_drafts) 1 / T and log2(e) / T in two floats; how rows are split
+  double inv_t, inv_dt;
+  float thi, tlo, dhi, dlo;
+  int32_t segments, seg_len, walk_wgs;
+};
+constexpr int kVerifyMaxNodes = 256;  // of a request
+int64_t verify_workspace(int32_t batch, int64_t total, int32_t vocab, bool drawn);
+bool verify_fits(int32_t batch, int64_t total, int32_t vocab, bool drawn);
+// temperature 0: the most likely token alone (draft is not read)
+hipError_t verify_drafts(VerifyArgs a, double temperature, double draft_temperature,
+                         void* workspace, hipStream_t stream);
+
 }  // namespace aios

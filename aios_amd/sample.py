@@ -10,6 +10,7 @@ temperature / top-k / top-p on a sampling copy with forbidden ids at -inf,
 the token chosen by the candidate's uniform, and the raw log-probability of
 the unmodified distribution.  ``sample_step`` is the same launch with the
 step index read on the device, for graph-replayed decode loops.
+``verify_drafts`` is the acceptance rule of speculative decoding.
 
 Ties in the top-k order go to the lower token id.  Without ``uniforms`` the
 uniforms are drawn with ``torch.rand`` (the reference uses
@@ -199,3 +200,87 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         None if ws is None else ws.data_ptr(), ws_bytes, _lib.current_stream(logits)),
         "aios_token_logprobs")
     return TokenLogprobs(lp, ent, ids, alt)
+
+
+class VerifiedDrafts(NamedTuple):
+    """:func:`verify_drafts`'s answers for a batch of requests with nodes."""
+
+    accepted: torch.Tensor     # bool [nodes]: node 0 of a request and the accepted ones behind it
+    counts: torch.Tensor       # int32 [requests]: accepted drafts
+    last: torch.Tensor         # int32 [requests]: the last accepted node, counted in the request
+    next_tokens: torch.Tensor  # int64 [requests]: the token added behind it
+    logprobs: torch.Tensor     # float32 [nodes]: ln p of a node's token; node 0: of the added one
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
+                  cu: torch.Tensor, uniforms: torch.Tensor | None = None, *,
+                  draft_logits: torch.Tensor | None = None, temperature: float = 1.0,
+                  draft_temperature: float | None = None) -> VerifiedDrafts:
+    """Which drafted tokens the target accepts, and the token it adds, from
+    given random numbers (``aios_verify_drafts``): the tokens that come out are
+    distributed as the target's own at ``temperature``.
+
+    Request r's nodes are ``cu[r] .. cu[r + 1]`` (int32 [requests + 1], at most
+    256 each): node 0 is decided, node i drafts ``tokens[i]`` (int64 [nodes])
+    behind node ``parents[i]`` (int32 [nodes], counted within the request; -1:
+    a node that is never accepted).  ``logits`` row i (bfloat16 or float32
+    [nodes, vocab]) is the target's behind node i.  ``draft_logits`` row i, of
+    the same shape and type, is what the children of node i were drawn from at
+    ``draft_temperature`` (default: ``temperature``), one after another in their
+    order; without it the drafts count as certain (phrases of a list).
+    ``uniforms`` (float32 [nodes], in [0, 1)) decides on each draft, node 0's on
+    the added token.
+
+    Children are tried in ascending order, with p = softmax(logits /
+    temperature) and q the draft's: x is accepted if u q(x) < p(x), else p
+    becomes max(p - q, 0), normalised (certain drafts: p without x).  The added
+    token is drawn, in the order of the ids, from what p has become behind the
+    last accepted node.  ``temperature`` 0 accepts and adds the most likely
+    tokens (the lowest id of equal ones) and reads no uniforms and no draft
+    logits.  Log-probs are those of the unscaled logits, as the sampler's."""
+    _check_logits(logits)
+    n, vocab = logits.shape
+    dev = logits.get_device()
+    greedy = temperature == 0
+    if greedy:
+        draft_logits = None
+    for t, name, dtype in ((tokens, "tokens", torch.int64), (parents, "parents", torch.int32)):
+        if t.dtype is not dtype or t.shape != (n,) or t.get_device() != dev or \
+                not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} [nodes] tensor on the "
+                             "logits' GPU")
+    if cu.dtype is not torch.int32 or cu.ndim != 1 or cu.numel() < 1 or cu.get_device() != dev or \
+            not cu.is_contiguous():
+        raise ValueError("cu must be a contiguous int32 [requests + 1] tensor on the logits' GPU")
+    if not greedy and (uniforms is None or uniforms.dtype is not torch.float32
+                       or uniforms.shape != (n,) or uniforms.get_device() != dev
+                       or not uniforms.is_contiguous()):
+        raise ValueError("uniforms must be a contiguous float32 [nodes] tensor on the logits' GPU")
+    if draft_logits is not None:
+        _check_logits(draft_logits)
+        if draft_logits.shape != logits.shape or draft_logits.dtype is not logits.dtype or \
+                draft_logits.get_device() != dev:
+            raise ValueError("draft_logits must be of the logits' shape and type, on their GPU")
+    if draft_temperature is None:
+        draft_temperature = temperature
+    b = cu.numel() - 1
+    lib, device = _lib.lib(), logits.device
+    accepted = torch.empty(n, dtype=torch.bool, device=device)
+    counts, last = torch.empty(2 * b, dtype=torch.int32, device=device).split_with_sizes((b, b))
+    nxt = tokens.new_empty(b)
+    lp = torch.empty(n, dtype=torch.float32, device=device)
+    # (a buffer of this call alone, since calls may overlap on several streams)
+    ws_bytes = lib.aios_verify_workspace(b, n, vocab, draft_logits is not None)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    stride = logits.stride(0) if n > 1 else vocab  # (a single row's is not looked at)
+    draft, draft_stride = None, 0
+    if draft_logits is not None:
+        draft = draft_logits.data_ptr()
+        draft_stride = draft_logits.stride(0) if n > 1 else vocab
+    _lib.check(lib.aios_verify_drafts(
+        logits.data_ptr(), stride, draft, draft_stride, vocab, logits.element_size(),
+        tokens.data_ptr(), parents.data_ptr(), cu.data_ptr(), b, n,
+        None if greedy else uniforms.data_ptr(), temperature, draft_temperature,
+        accepted.data_ptr(), counts.data_ptr(), last.data_ptr(), nxt.data_ptr(), lp.data_ptr(),
+        ws.data_ptr(), ws_bytes, _lib.current_stream(logits)), "aios_verify_drafts")
+    return VerifiedDrafts(accepted, counts, last, nxt, lp)

@@ -725,6 +725,54 @@ int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, in
                         float* entropies, int64_t* top_ids, float* top_logprobs, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens.  No counterpart in the reference.
+ *
+ * Request r of a batch owns nodes [cu[r], cu[r+1]) of total_nodes, at most
+ * AIOS_VERIFY_MAX_NODES (further ones are never accepted): node 0 is decided,
+ * node i > 0 drafts tokens[i] behind node parents[i] (counted within the
+ * request; a node whose parent is not an earlier one of its request, such as -1,
+ * is never accepted).  logits row i is the target's behind node i, draft_logits
+ * row i the one that the children of node i were drawn from, one after another
+ * (NULL: drafts that no distribution drew; rows of nodes without children are
+ * not read; elem_bytes, 2 bf16 or 4 fp32, of both; rows aligned to their
+ * element only).  With p = softmax(logits / temperature), q = softmax(
+ * draft_logits / draft_temperature), from node 0 on:
+ *   the children are tried in ascending order: child i with token x is accepted
+ *   if uniforms[i] * q(x) < p(x); otherwise p becomes max(p - q, 0), normalised
+ *   (without draft_logits q is 1 at x: x is removed from p); behind an accepted
+ *   child its own children are tried;
+ *   the added token is the first id whose cumulative p, in ascending order,
+ *   exceeds uniforms[node 0]; where max(p - q, 0) has no mass left, of p as it
+ *   was at first.  (A draft whose number is not below 1 is not accepted; for the
+ *   added token such a number is the last possible id.)
+ * temperature 0: the most likely token (the lowest id of equal ones) is the only
+ * one accepted, and the one added; draft_logits and uniforms are not read (both
+ * may be NULL).  Otherwise both temperatures are within 1e-4 .. 1e4.
+ *   accepted[i]    1 for node 0 and the accepted nodes behind it, else 0
+ *   counts[r]      accepted drafts; last[r]: the last accepted node
+ *   next_tokens[r] the added token
+ *   logprobs[i]    ln softmax(logits of the parent)[tokens[i]] (at temperature
+ *                  1), accepted or not; of node 0: that of the added token
+ * Tokens outside the vocabulary are never accepted, their log-probability is
+ * NaN, as is that of a node without a parent.  Behind a node whose logits have
+ * no finite maximum nothing is accepted and the added token is -1 (NaN); with
+ * such draft_logits nothing is accepted and the added token is drawn from p.
+ * A request without nodes has count 0 and -1 twice; nodes of no request are
+ * not accepted, NaN.  Sums and tests in 64 bits.  workspace: 16-byte aligned,
+ * aios_verify_workspace(...) bytes (drawn: whether draft_logits are given).
+ */
+#define AIOS_VERIFY_MAX_NODES 256
+int64_t aios_verify_workspace(int32_t batch_size, int64_t total_nodes, int32_t vocab,
+                              int32_t drawn);
+int aios_verify_drafts(const void* logits, int64_t row_stride, const void* draft_logits,
+                       int64_t draft_stride, int32_t vocab, int32_t elem_bytes,
+                       const int64_t* tokens, const int32_t* parents, const int32_t* cu,
+                       int32_t batch_size, int64_t total_nodes, const float* uniforms,
+                       float temperature, float draft_temperature, uint8_t* accepted,
+                       int32_t* counts, int32_t* last, int64_t* next_tokens, float* logprobs,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
