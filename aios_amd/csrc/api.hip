@@ -1685,6 +1685,63 @@ int aios_attn_append_decode_rope8(const aios_attn_plan_t* p, const void* q, int6
 // ---------------------------------------------------------------------------
 // trees of drafted tokens
 
+// How many parts the KV ranges of a batch of trees are split into (num_parts 1:
+// none).  Estimated in ns, fitted to 6,700 batches of 1 to 32 requests of 1 to 256
+// nodes behind up to 16,000 positions at head sizes 64, 96 and 128 (12q/4kv, 8q/2kv,
+// 16q/8kv, 32q/8kv), each in up to 20 numbers of parts: a workgroup's start, its
+// sub-tiles (slower with two workgroups on a unit, and past two in further
+// rounds), and for parts the combine, each part and the states' bytes.  The
+// number taken is within 1.5% of the batch's best in the mean, 21% at the 99th
+// percentile.  Parts of 1 / 2 / 4 / 8 / 16 / 32: 16 requests of 33 to 4 nodes on
+// 1,500, 12q/4kv x 64 33 / 22 / 15.9 / 15.7 / 20.0 us; one of 40 on 16,001, 32q/8kv
+// x 128, bf16 494 / 256 / 132 / 71 / 42 / 31, 8 bits 354 / 186 / 98 / 55 / 34 /
+// 28.5; four of 200 to 143 on 8,192 (bf16) 265 / 151 / 155 / 171 / 180.
+struct TreeCost {
+  int32_t base, base_rows;  // a workgroup, and for 128 MFMA rows of it
+  int32_t sub, sub_d;       // a sub-tile, and for 128 dims of it
+  int32_t two;              // a sub-tile with two workgroups on a unit, percent
+  int32_t round;            // a further round of workgroups
+  int32_t join, part, state;  // combine, a part of it, 10^5 elements of states
+};
+static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int32_t* cu_k,
+                            bool bits8, int32_t cus, int64_t ws_bytes) {
+  const int32_t q_tile = p->prefill_q_tile, hkv = p->num_kv_heads, d = p->head_dim;
+  const int32_t rows = q_tile * p->group;
+  const TreeCost few16 = {5600, 0, 60, 730, 163, 4400, 2430, 50, 142};
+  const TreeCost few8 = {6400, 0, 106, 382, 145, 3000, 2430, 57, 164};
+  const TreeCost full16 = {3700, 2940, 385, 537, 133, 900, 1550, 49, 118};
+  const TreeCost full8 = {4240, 2700, 268, 451, 140, 0, 1450, 42, 115};
+  const TreeCost c = rows <= 64 ? (bits8 ? few8 : few16) : (bits8 ? full8 : full16);
+  const int32_t longest = cdiv(p->max_kv_len, 32);
+  const int64_t slots = (int64_t)p->batch_size * p->num_q_tiles * hkv;
+  int64_t best = -1;
+  for (int32_t want = 1; want <= longest; want += 1 + want / 8) {
+    const int32_t per = cdiv(longest, want), n = cdiv(longest, per);
+    const int64_t parts = slots * n;
+    const int64_t o_bytes = align_up(parts * rows * d * 2, 256);
+    const int64_t bytes = n > 1 ? o_bytes + align_up(parts * rows * 8, 256) : 0;
+    if (bytes > ws_bytes || parts > 0x3fffffff) break;
+    int64_t wgs = 0;
+    for (int32_t b = 0; b < p->batch_size; ++b) {
+      const int32_t nodes = cu_q[b + 1] - cu_q[b], kv = cu_k[b + 1] - cu_k[b];
+      if (nodes > 0) wgs += (int64_t)cdiv(nodes, q_tile) * hkv * cdiv(cdiv(kv, 32), per);
+    }
+    const int64_t one = per * (c.sub + (int64_t)c.sub_d * d / 128), two = one * c.two / 100;
+    const int64_t full = wgs / (2 * cus), rest = wgs % (2 * cus);
+    const int64_t rounds = full + (rest > 0);
+    int64_t ns = c.base + (int64_t)c.base_rows * rows / 128 + full * two +
+                 (rest > cus ? two : rest > 0 ? one : 0) + (rounds > 1 ? (rounds - 1) * c.round : 0);
+    if (n > 1) ns += c.join + (int64_t)c.part * n + wgs * rows * d * c.state / 100000;
+    if (best < 0 || ns < best) {
+      best = ns;
+      p->prefix_chunk_len = per * 32;
+      p->num_parts = n;
+      p->ws_parts_lse = n > 1 ? o_bytes : 0;
+      p->ws_bytes = bytes;
+    }
+  }
+}
+
 int aios_attn_plan_tree(const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t hq,
                         int32_t hkv, int32_t d, int32_t page_size, int32_t kv_bits,
                         int64_t ws_bytes, aios_attn_plan_t* p) {
@@ -1699,8 +1756,9 @@ int aios_attn_plan_tree(const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
   if (p->max_q_len == 0) return AIOS_OK;
   // the fewest tiles of at most 128 MFMA rows, of equal size
   p->prefill_q_tile = cdiv(p->max_q_len, p->num_q_tiles);
-  p->prefix_chunk_len = 32 * aios::kPrefillFewSub;
+  p->prefix_chunk_len = 32;
   p->num_parts = 1;
+  plan_tree_parts(p, cu_q, cu_k, kv_bits == 8, device_cus(), ws_bytes);
   return AIOS_OK;
 }
 
@@ -1742,7 +1800,7 @@ static int tree_args(const char* what, const aios_attn_plan_t* p, const void* q,
       p->ws_bytes <= workspace_bytes) {
     char* ws = static_cast<char*>(workspace);
     a.n_parts = p->num_parts;
-    a.part_o = reinterpret_cast<float*>(ws + p->ws_parts_o);
+    t->part_o = reinterpret_cast<_Float16*>(ws + p->ws_parts_o);
     a.part_ml = reinterpret_cast<float2*>(ws + p->ws_parts_lse);
   }
   t->masks = reinterpret_cast<const uint32_t*>(masks);

@@ -206,12 +206,14 @@ __device__ __forceinline__ bf16x8 qk_rope8(const float (&xn)[8], const float (&p
 // wait_sub(i) (every thread's loads of sub-tile i have landed: a wait and a
 // workgroup barrier) before it reads sub-tile i, for i = 0, 1, ... in order;
 // longer ranges, and ONCE = false, stream through the ring kLookahead
-// sub-tiles ahead with `math`.
+// sub-tiles ahead with `math`, or (PAIRS) two sub-tiles at a time: one wait and
+// one barrier for both, the next two requested behind it.
 struct NoPipe {
   template <typename W>
   __device__ void operator()(W&&, int) const {}
 };
-template <class T, int CPOL, bool ONCE, typename QLoad, typename Math, typename Pipe = NoPipe>
+template <class T, int CPOL, bool ONCE, bool PAIRS = false, typename QLoad, typename Math,
+          typename Pipe = NoPipe>
 __device__ __forceinline__ void stream_kv(uint8_t* lds, const uint8_t* kc, const uint8_t* vc,
                                           int64_t tok_bytes, int64_t num_pages, const int32_t* idx,
                                           int kv_begin, int kv_end, QLoad&& qload, Math&& math,
@@ -341,6 +343,37 @@ __device__ __forceinline__ void stream_kv(uint8_t* lds, const uint8_t* kc, const
       wait_vmcnt<0>();  // the zero-row loads past the range have landed too
       return;
     }
+  }
+
+  if constexpr (PAIRS) {
+    static_assert(kRing == 4, "two pairs of sub-tiles");
+    issue(0);
+    issue(1);  // (past the range: zero rows, as below)
+    auto loop = [&](auto with_math) {
+      for (int it = 0; it < n_sub; it += 2) {
+        wait_vmcnt<0>();
+        lds_barrier();  // the pair is in LDS; every wave is done with the one before
+        if (it + 2 < n_sub) {
+          if (kv_begin + (it + 2) * kSubTok >= win + kIdWindow) {
+            win += kIdWindow;
+            stage_ids();
+            lds_barrier();
+          }
+          issue(it + 2);
+          issue(it + 3);
+        }
+        if constexpr (decltype(with_math)::value) {
+          const uint32_t sb = (uint32_t)((it & 2) * T::SUB_BYTES);
+          math(sb, kv_begin + it * kSubTok);
+          if (it + 1 < n_sub) math(sb + T::SUB_BYTES, kv_begin + (it + 1) * kSubTok);
+        }
+      }
+    };
+    if (__builtin_amdgcn_readfirstlane((int)active))
+      loop(std::true_type{});
+    else
+      loop(std::false_type{});
+    return;
   }
 
   // The lookahead sub-tiles are issued unconditionally (those past the

@@ -410,17 +410,20 @@ hipError_t launch_prefill_combine(int D, const PrefillArgs& a, hipStream_t strea
 
 // Attention for trees of drafted tokens (attn_tree.hip): p as for the prefill
 // with parts of part_sub sub-tiles, n_parts 1 for tiles of one workgroup; p's
-// bf16 caches or kv (bits 16 or 8).  masks [nodes][words] 32-bit words.
+// bf16 caches or kv (bits 16 or 8).  masks [nodes][words] 32-bit words.  The
+// partial states (p.part_o is not used):
+//   part_o  [slots][n_parts][D / 8][part_rows][8] fp16, o times a power of two
+//   part_ml [slots][n_parts][part_rows] (p.part_ml): (m, l), m the row's reference
+//           plus that power's exponent and l the row sum in the same units
 struct TreeArgs {
   PrefillArgs p;
   Kv8Layer kv;
   const uint32_t* masks;
   int32_t words;
+  _Float16* part_o;
 };
 constexpr int kTreeMaxNodes = 256;  // of a request
 hipError_t launch_tree(int D, int bits, const TreeArgs& a, hipStream_t stream);
-// launch_prefill_combine for tiles whose KV range is their whole request's.
-hipError_t launch_tree_combine(int D, const PrefillArgs& a, hipStream_t stream);
 // Masks [total][words] (32-bit words) and depths [total] of every request's nodes.
 hipError_t tree_masks(const int32_t* parents, const int32_t* cu, int32_t batch, int64_t total,
                       int32_t words, void* masks, int32_t* depths, hipStream_t stream);
