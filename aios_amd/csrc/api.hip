@@ -1707,10 +1707,10 @@ static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int3
                             bool bits8, int32_t cus, int64_t ws_bytes) {
   const int32_t q_tile = p->prefill_q_tile, hkv = p->num_kv_heads, d = p->head_dim;
   const int32_t rows = q_tile * p->group;
-  const TreeCost few16 = {5600, 0, 60, 730, 163, 4400, 2430, 50, 142};
-  const TreeCost few8 = {6400, 0, 106, 382, 145, 3000, 2430, 57, 164};
-  const TreeCost full16 = {3700, 2940, 385, 537, 133, 900, 1550, 49, 118};
-  const TreeCost full8 = {4240, 2700, 268, 451, 140, 0, 1450, 42, 115};
+  const TreeCost few16 = {5500, 0, 60, 750, 160, 4500, 2360, 50, 140};
+  const TreeCost few8 = {6400, 0, 106, 387, 145, 2900, 2400, 57, 166};
+  const TreeCost full16 = {3500, 3100, 397, 575, 129, 2500, 1600, 49, 107};
+  const TreeCost full8 = {4100, 3200, 267, 450, 140, 0, 1445, 40, 105};
   const TreeCost c = rows <= 64 ? (bits8 ? few8 : few16) : (bits8 ? full8 : full16);
   const int32_t longest = cdiv(p->max_kv_len, 32);
   const int64_t slots = (int64_t)p->batch_size * p->num_q_tiles * hkv;
@@ -1941,10 +1941,10 @@ int aios_verify_drafts(const void* logits, int64_t row_stride, const void* draft
     return fail(AIOS_ERR_INVALID, "verify_drafts: null pointer");
   if ((((uintptr_t)logits | (uintptr_t)draft) & (uintptr_t)(elem_bytes - 1)) != 0)
     return fail(AIOS_ERR_INVALID, "verify_drafts: misaligned logits");
-  if (!workspace || ((uintptr_t)workspace & 15) != 0 ||
-      workspace_bytes < aios::verify_workspace(batch, total, vocab, draft != nullptr))
+  const int64_t need = aios::verify_workspace(batch, total, vocab, draft != nullptr);
+  if (!workspace || ((uintptr_t)workspace & 15) != 0 || workspace_bytes < need)
     return fail(AIOS_ERR_WORKSPACE, "verify_drafts: needs a workspace of %lld bytes, 16-byte aligned",
-                (long long)aios::verify_workspace(batch, total, vocab, draft != nullptr));
+                (long long)need);
   aios::VerifyArgs a = {};
   a.logits = logits;
   a.stride = row_stride;

@@ -470,7 +470,7 @@ struct VerifyArgs {
   float* logprobs;         // [total]
   // (set by verify_drafts) 1 / T and log2(e) / T in two floats; how rows are split
   double inv_t, inv_dt;
-  float thi, tlo, dhi, dlo;
+  float thi, tlo, tleast, dhi, dlo, dleast;
   int32_t segments, seg_len, walk_wgs;
 };
 constexpr int kVerifyMaxNodes = 256;  // of a request

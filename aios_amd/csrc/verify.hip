@@ -24,12 +24,14 @@
 // Every node's outcome (the accepted child, or none) is independent of the way
 // that leads to it, so the passes over the vocabulary run for all nodes at once:
 //   stats  maximum and sums of the rows of nodes with children, by segments
-//   join   those sums together, the first tests; F(1) where the first child of
-//          several is rejected, by segments
-//   walk   the other tests, the path, and the added token's weights by batches of
-//          2048 ids (a leaf's row is read here only)
+//   join   those sums together, the children's p and q; F(1) where the first child
+//          of several is rejected, by segments
+//   walk   the tests, the path, and the added token's weights by batches of 2048
+//          ids (a leaf's row is read here only)
 //   pick   the added token
 // Bound: the rows, read once from HBM (those of F(1) and of the last node again).
+// Rows of at most 16 batches take what follows the stats in one launch
+// (verify_rest_kernel).
 #include "logits.hpp"
 
 namespace aios {
@@ -40,30 +42,33 @@ constexpr int kVThreads = 256;
 static_assert(kVNodes <= kVThreads, "a node per thread");
 constexpr int kVSpan = kVThreads / 64 * kLpBatch;  // logits of a workgroup's round
 constexpr int kVMaxSegments = 64;                  // one per lane where they are joined
+constexpr int kVManyWgs = 4096;                    // more than this: longer segments
+constexpr int kVRestThreads = 1024;
 constexpr double kLn2 = 0.69314718055994530942;
 
-// Sums of one segment of a row relative to its maximum m: s of exp((x - m) / T),
-// s1 of exp(x - m); best: the first id at the maximum.
+// Sums of (a part of) a row relative to a reference m: s of exp((x - m) / T), s1 of
+// exp(x - m); best: the first id at the maximum (temperature 0: m is that maximum).
 struct VPart {
   double s, s1;
   float m;
   int32_t best;
 };
-// A node: its rows' sums, relative to the maxima m (target) and mq (draft).
-constexpr int kVNone = -1;    // next: no child is accepted
-constexpr int kVOpen = -2;    // the first one is rejected, F(1) decides on the second
-constexpr int kVMore = -3;    // (walk) F(lambda) is needed for the next
-constexpr int kVSummed = 1;   // flags: m, s, s1 are set (the node has children)
-constexpr int kVBad = 2;      // the target's row has no finite maximum
+constexpr int kVNone = -1;  // no child is accepted
+constexpr int kVMore = -2;  // F(lambda) is needed for the next child
+constexpr int kVSummed = 1;  // flags: the rows' sums are set (the node has children)
+constexpr int kVBad = 2;     // the target's row has no finite maximum
 constexpr int kVBadDraft = 4;
 struct VNode {
-  double s, s1, sq;
+  double s, ls1, sq;  // (ls1 = ln s1)
   float m, mq;
-  int32_t next, flags, best, pad;
+  int32_t flags, best;
+};
+struct VKid {  // a draft under its parent's distributions
+  double p, q;
 };
 // The last accepted node's row, as the pick needs it.
 struct VLast {
-  double s1;        // of the row (not of a leaf's)
+  double ls1;       // ln s1 of the row (not of a leaf's)
   float m, mq, khi, klo;
   int32_t node;     // -1: nothing to pick
   int32_t flags;    // kVSummed: m is set
@@ -75,30 +80,49 @@ struct VBatch {
   int32_t best;
 };
 
-struct VScale {  // log2(e) / T in two floats
-  float hi, lo;
+struct VScale {  // log2(e) / T in two floats, and the d at which exp(d / T) is taken as 0
+  float hi, lo, least;
 };
 
-// exp(d / T), d <= 0: the product's rounding error is added back.
+// exp(d / T), d at most a little above 0: the product's rounding error is added back.
 __device__ __forceinline__ float vexp(float d, VScale c) {
+  d = fmaxf(d, c.least);
   const float t = d * c.hi;
   const float r = fmaf(d, c.lo, fmaf(d, c.hi, -t));
   const float e = fast_exp2(t);
-  return t > -150.f ? fmaf(e, r * (float)kLn2, e) : 0.f;
+  return fmaf(e, r * (float)kLn2, e);
 }
 __device__ __forceinline__ double vexp64(double d, double inv_t) {
   return d * inv_t > -1000.0 ? exp(d * inv_t) : 0.0;
 }
 
-__device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) x += __shfl_xor(x, i);
+// Sums over the wavefront: DPP within rows of 16 lanes, lane swaps across.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp64(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane64(double x, int lane) {  // (lane uniform)
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Inclusive sums in the order of the lanes.
+__device__ __forceinline__ double wave_scan64(double x) {
+  x += dpp64<0x111>(x);       // row_shr 1, 2, 4, 8
+  x += dpp64<0x112>(x);
+  x += dpp64<0x114>(x);
+  x += dpp64<0x118>(x);
+  x += dpp64<0x142, 0xA>(x);  // the last lane of rows 0 and 2 to rows 1 and 3
+  x += dpp64<0x143, 0xC>(x);  // lane 31 to the upper half
   return x;
 }
+__device__ __forceinline__ double wave_sum64(double x) { return lane64(wave_scan64(x), 63); }
 __device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) x = min(x, __shfl_xor(x, i));
-  return x;
+  return (int)~lp_wave_max_u(~((uint32_t)x ^ 0x80000000u)) ^ (int)0x80000000u;
 }
 __device__ __forceinline__ bool finite_max(float m) { return m > kNegInf && m < __builtin_inff(); }
 
@@ -119,19 +143,194 @@ __device__ __forceinline__ int locate(const VerifyArgs& a, int64_t node, int64_t
 // A draft's random number; one that is not below 1 accepts nothing.
 __device__ __forceinline__ double number(float u) { return u < 1.f ? u : __builtin_inf(); }
 
+__host__ __device__ __forceinline__ int batches_of(int vocab) {
+  return (int)(((int64_t)vocab + kLpBatch - 1) / kLpBatch);
+}
+
 template <typename T>
 __device__ __forceinline__ const T* row_of(const void* x, int64_t stride, int64_t node) {
   return static_cast<const T*>(x) + node * stride;
 }
 
-// -- stats ---------------------------------------------------------------------
+// -- sums of rows ----------------------------------------------------------------
+
+// 16 logits a lane, as loaded: the lane's two groups of 8 lie 512 apart.
+constexpr int kVChunk = 64 * 16;
+struct RawBf16 {
+  uint4 v[2];
+};
+struct RawF32 {
+  float4 v[4];
+};
+__device__ __forceinline__ void raw_load(const bf16* x, int i, RawBf16& r) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    r.v[g] = __builtin_bit_cast(uint4, *reinterpret_cast<const u16x8*>(x + i + g * 512));
+}
+__device__ __forceinline__ void raw_load(const float* x, int i, RawF32& r) {
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    r.v[g] = __builtin_bit_cast(
+        float4, *reinterpret_cast<const f32x4u*>(x + i + (g >> 1) * 512 + (g & 1) * 4));
+}
+__device__ __forceinline__ void raw_values(const RawBf16& r, float (&f)[16]) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const uint32_t w[4] = {r.v[g].x, r.v[g].y, r.v[g].z, r.v[g].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[8 * g + 2 * k] = lo_bf16(w[k]);
+      f[8 * g + 2 * k + 1] = hi_bf16(w[k]);
+    }
+  }
+}
+__device__ __forceinline__ void raw_values(const RawF32& r, float (&f)[16]) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    f[4 * g] = r.v[g].x;
+    f[4 * g + 1] = r.v[g].y;
+    f[4 * g + 2] = r.v[g].z;
+    f[4 * g + 3] = r.v[g].w;
+  }
+}
+template <typename T>
+struct RawOf;
+template <>
+struct RawOf<bf16> { using type = RawBf16; };
+template <>
+struct RawOf<float> { using type = RawF32; };
+
+// Sums of one row's logits [begin, end), a wavefront's chunks from the wave-th on
+// in steps of `waves`, relative to a reference m that need not be the maximum: the
+// largest of the first chunk, moved where a logit is more than kVSlack above it
+// (the raw exponentials' exponents are rounded: a large term's has to be small).
+// Seven VALU
+// instructions and an exponential a logit, next to which the bytes take about as
+// long: 58 registers, so that eight wavefronts a SIMD overlap the two.
+constexpr float kVSlack = 1.f;
+// RAW: with s1; else (temperature 1, the draft's rows) s1 = s.
+template <typename T, bool RAW>
+__device__ __forceinline__ VPart row_sums(const T* x, int begin, int end, int wave, int waves,
+                                          VScale c, double inv_t) {
+  const int lane = threadIdx.x & 63;
+  VPart p = {0, 0, kNegInf, 0x7fffffff};
+  const float slack = inv_t < 1.0 ? kVSlack : kVSlack * (float)(1.0 / inv_t);
+  typename RawOf<T>::type raw;
+  float f[16];
+  auto fetch = [&](int b0) {
+    if (b0 + kVChunk <= end) raw_load(x, b0 + lane * 8, raw);
+  };
+  int b0 = begin + wave * kVChunk;
+  fetch(b0);
+  for (; b0 < end; b0 += waves * kVChunk) {
+    if (b0 + kVChunk <= end) {
+      raw_values(raw, f);
+      fetch(b0 + waves * kVChunk);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int i = b0 + (k >> 3) * 512 + lane * 8 + (k & 7);
+        f[k] = i < end ? (float)x[i] : kNegInf;
+      }
+    }
+    float mx = f[0];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) mx = vmax(mx, f[k]);
+    if (__builtin_amdgcn_ballot_w64(!(mx <= p.m + slack)) != 0) {  // (also a NaN)
+      const float m = vmax(p.m, lp_wave_max(mx));
+      if (p.m > kNegInf) {
+        p.s *= vexp64((double)p.m - m, inv_t);
+        if constexpr (RAW) p.s1 *= vexp64((double)p.m - m, 1.0);
+      }
+      p.m = m;
+    }
+    const float mu = p.m == kNegInf ? 0.f : p.m;
+    float us = 0.f, ur = 0.f, us1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float d = fmaxf(f[k] - mu, c.least);
+      const float t = d * c.hi;
+      const float r = fmaf(d, c.lo, fmaf(d, c.hi, -t));
+      const float e = fast_exp2(t);
+      us += e;
+      ur = fmaf(e, r, ur);
+      if constexpr (RAW) us1 += fast_exp2((f[k] - mu) * kLog2e);
+    }
+    p.s += (double)fmaf(ur, (float)kLn2, us);
+    if constexpr (RAW) p.s1 += us1;
+  }
+  p.s = wave_sum64(p.s);
+  p.s1 = RAW ? wave_sum64(p.s1) : p.s;
+  return p;
+}
+
+// The same for the most likely token: m is the maximum, best its first id, s = s1
+// the sum of exp(x - m).
+template <typename T>
+__device__ __forceinline__ VPart row_best(const T* x, int begin, int end, int wave, int waves) {
+  const int lane = threadIdx.x & 63;
+  VPart p = {0, 0, kNegInf, 0x7fffffff};
+  typename RawOf<T>::type raw;
+  float f[16];
+  auto fetch = [&](int b0) {
+    if (b0 + kVChunk <= end) raw_load(x, b0 + lane * 8, raw);
+  };
+  int b0 = begin + wave * kVChunk;
+  fetch(b0);
+  for (; b0 < end; b0 += waves * kVChunk) {
+    if (b0 + kVChunk <= end) {
+      raw_values(raw, f);
+      fetch(b0 + waves * kVChunk);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int i = b0 + (k >> 3) * 512 + lane * 8 + (k & 7);
+        f[k] = i < end ? (float)x[i] : kNegInf;
+      }
+    }
+    float mx = f[0];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) mx = vmax(mx, f[k]);
+    if (__builtin_amdgcn_ballot_w64(!(mx <= p.m)) != 0) {
+      const float m = vmax(p.m, lp_wave_max(mx));
+      if (p.m > kNegInf) p.s *= vexp64((double)p.m - m, 1.0);
+      p.m = m;
+      p.best = 0x7fffffff;
+    }
+    const float mu = p.m == kNegInf ? 0.f : p.m;
+    float us = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      us += fast_exp2((f[k] - mu) * kLog2e);
+      if (f[k] == p.m) p.best = min(p.best, b0 + (k >> 3) * 512 + lane * 8 + (k & 7));
+    }
+    p.s += us;
+  }
+  p.s1 = p.s = wave_sum64(p.s);
+  p.best = wave_min(p.best);
+  return p;
+}
+
+// A row's sums from n <= 64 parts, by one wavefront (every lane has them).
+__device__ __forceinline__ VPart join(const VPart* parts, int n, double inv_t) {
+  const int lane = threadIdx.x & 63;
+  VPart p = {0, 0, kNegInf, 0x7fffffff};
+  if (lane < n) p = parts[lane];
+  VPart r;
+  r.m = lp_wave_max(p.m);
+  const double d = (double)p.m - (r.m == kNegInf ? 0.f : r.m);
+  r.s = wave_sum64(p.s * vexp64(d, inv_t));
+  r.s1 = wave_sum64(p.s1 * vexp64(d, 1.0));
+  r.best = wave_min(p.m == r.m ? p.best : 0x7fffffff);
+  return r;
+}
 
 // One workgroup per (node, segment) and row kind (the target's, then the drafts').
 template <typename T, bool GREEDY>
 __global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a, VPart* parts) {
-  __shared__ double ss[4], ss1[4];
-  __shared__ float sm[4];
-  __shared__ int sb[4];
+  __shared__ VPart sp[4];
   const int seg = blockIdx.x % a.segments;
   const int64_t rest = blockIdx.x / a.segments;
   const int which = rest >= a.total;
@@ -142,88 +341,20 @@ __global__ __launch_bounds__(kVThreads) void verify_stats_kernel(VerifyArgs a, V
   const int i = (int)(node - first), tid = threadIdx.x;
   if (!__syncthreads_or(tid > i && tid < n && a.parents[first + tid] == i)) return;
   const T* x = which ? row_of<T>(a.draft, a.draft_stride, node) : row_of<T>(a.logits, a.stride, node);
-  const VScale c = which ? VScale{a.dhi, a.dlo} : VScale{a.thi, a.tlo};
-  const double inv_t = which ? a.inv_dt : a.inv_t;
-  const bool same = which || a.inv_t == 1.0;  // (no second sum)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const double inv_t = which ? a.inv_dt : a.inv_t;
   const int begin = seg * a.seg_len, end = min(a.vocab, begin + a.seg_len);
-  float m = kNegInf;
-  double s = 0, s1 = 0;
-  int best = 0x7fffffff;
-  for (int b0 = begin + wave * kLpBatch; b0 < end; b0 += kVSpan) {
-    float f[kLpUnroll][8];
-    lp_load_batch(x, b0, end, f);
-    float bm = kNegInf;
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u)
-      bm = vmax(bm, vmax(vmax(vmax(f[u][0], f[u][1]), vmax(f[u][2], f[u][3])),
-                         vmax(vmax(f[u][4], f[u][5]), vmax(f[u][6], f[u][7]))));
-    const float m_new = vmax(m, lp_wave_max(bm));
-    if (m_new != m) {  // (uniform; also for a NaN)
-      s *= vexp64((double)m - m_new, inv_t);
-      if constexpr (!GREEDY) s1 *= vexp64((double)m - m_new, 1.0);
-      m = m_new;
-      best = 0x7fffffff;
-    }
-    const float mu = m == kNegInf ? 0.f : m;
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      float us = 0.f, us1 = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = f[u][e] - mu;
-        if constexpr (GREEDY) {
-          us += fast_exp2(d * kLog2e);
-          if (f[u][e] == m)
-            best = min(best, b0 + u * 512 + (tid & 63) * 8 + e);
-        } else {
-          us += vexp(d, c);
-          if (!same) us1 += fast_exp2(d * kLog2e);
-        }
-      }
-      s += us;
-      s1 += us1;
-    }
-  }
-  s = wave_sum64(s);
-  if constexpr (GREEDY) best = wave_min(best);
-  else if (!same) s1 = wave_sum64(s1);
-  if ((tid & 63) == 0) {
-    ss[wave] = s;
-    ss1[wave] = s1;
-    sm[wave] = m;
-    sb[wave] = best;
-  }
+  const VScale c = which ? VScale{a.dhi, a.dlo, a.dleast} : VScale{a.thi, a.tlo, a.tleast};
+  VPart p;
+  if constexpr (GREEDY) p = row_best<T>(x, begin, end, wave, 4);
+  else if (which || a.inv_t == 1.0) p = row_sums<T, false>(x, begin, end, wave, 4, c, inv_t);
+  else p = row_sums<T, true>(x, begin, end, wave, 4, c, inv_t);
+  if ((tid & 63) == 0) sp[wave] = p;
   __syncthreads();
-  if (tid == 0) {
-    VPart p;
-    p.m = vmax(vmax(sm[0], sm[1]), vmax(sm[2], sm[3]));
-    p.s = p.s1 = 0;
-    p.best = 0x7fffffff;
-    const float mu = p.m == kNegInf ? 0.f : p.m;
-    for (int w = 0; w < 4; ++w) {
-      const double d = (double)sm[w] - mu;
-      p.s += ss[w] * vexp64(d, GREEDY ? 1.0 : inv_t);
-      p.s1 += ss1[w] * vexp64(d, 1.0);
-      if (sm[w] == p.m) p.best = min(p.best, sb[w]);
-    }
-    if (GREEDY || same) p.s1 = p.s;
-    parts[(node * (a.draft ? 2 : 1) + which) * a.segments + seg] = p;
+  if (wave == 0) {
+    const VPart r = join(sp, 4, GREEDY ? 1.0 : inv_t);
+    if (tid == 0) parts[(node * (a.draft ? 2 : 1) + which) * a.segments + seg] = r;
   }
-}
-
-// A row's sums from its segments, by one wavefront (every lane has them).
-__device__ __forceinline__ VPart join(const VPart* parts, int n, double inv_t) {
-  const int lane = threadIdx.x & 63;
-  VPart p = {0, 0, kNegInf, 0x7fffffff};
-  if (lane < n) p = parts[lane];
-  VPart r;
-  r.m = lp_wave_max(p.m);
-  const float mu = r.m == kNegInf ? 0.f : r.m;
-  r.s = wave_sum64(p.s * vexp64((double)p.m - mu, inv_t));
-  r.s1 = wave_sum64(p.s1 * vexp64((double)p.m - mu, 1.0));
-  r.best = wave_min(p.m == r.m ? p.best : 0x7fffffff);
-  return r;
 }
 
 // -- weights of a batch ----------------------------------------------------------
@@ -237,13 +368,21 @@ struct VRow {
   bool own_max;  // m is not known: each batch takes its own
 };
 
-// Weights and p of the lane's logits of batch b0; returns the batch's reference.
-// skip(id): removed ids' weights are 0.
-template <typename T, bool DRAWN>
-__device__ __forceinline__ float batch_weights(const VerifyArgs& a, const VRow& r, int b0,
-                                               const int64_t* gone, int n_gone,
+// lambda S_p / S_q in two floats.
+__device__ __forceinline__ void split_k(double k, VRow& r) {
+  r.khi = (float)k;
+  r.klo = (float)(k - (double)r.khi);
+}
+
+// Weights of the lane's logits of batch b (those of the n_gone removed ids are
+// 0), p's and the raw exponentials' sums over the lane; returns the reference.
+// RAW: s1 is wanted where the row's maximum is not known.
+template <typename T, bool DRAWN, bool RAW = false>
+__device__ __forceinline__ float batch_weights(const VerifyArgs& a, const VRow& r, int b,
+                                               const int32_t* gone, int n_gone,
                                                float (&w)[kLpUnroll][8], double& p, double& s1) {
   float f[kLpUnroll][8];
+  const int b0 = b * kLpBatch;
   lp_load_batch(static_cast<const T*>(r.x), b0, a.vocab, f);
   float m = r.m;
   if (r.own_max) {
@@ -255,20 +394,27 @@ __device__ __forceinline__ float batch_weights(const VerifyArgs& a, const VRow& 
     m = lp_wave_max(m);
   }
   const float mu = m == kNegInf ? 0.f : m;
-  const VScale c = {a.thi, a.tlo}, cd = {a.dhi, a.dlo};
+  const VScale c = {a.thi, a.tlo, a.tleast}, cd = {a.dhi, a.dlo, a.dleast};
   p = s1 = 0;
 #pragma unroll
   for (int u = 0; u < kLpUnroll; ++u) {
-    float up = 0.f, us1 = 0.f;
+    float up = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = f[u][e] - mu;
-      w[u][e] = vexp(d, c);
+      w[u][e] = vexp(f[u][e] - mu, c);
       up += w[u][e];
-      if (r.own_max) us1 += fast_exp2(d * kLog2e);
     }
     p += up;
-    s1 += us1;
+  }
+  if (RAW && r.own_max) {
+    asm volatile("");  // (behind the branch: not for the other rows)
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) {
+      float us1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) us1 += fast_exp2((f[u][e] - mu) * kLog2e);
+      s1 += us1;
+    }
   }
   if constexpr (DRAWN) {
     if (r.khi != 0.f) {  // (uniform)
@@ -283,9 +429,9 @@ __device__ __forceinline__ float batch_weights(const VerifyArgs& a, const VRow& 
     }
   }
   for (int j = 0; j < n_gone; ++j) {
-    const int64_t off = gone[j] - b0;
+    const int off = gone[j] - b0;
     if (off < 0 || off >= kLpBatch) continue;  // (uniform)
-    const int at = (int)off - (threadIdx.x & 63) * 8;
+    const int at = off - (threadIdx.x & 63) * 8;
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u)
 #pragma unroll
@@ -295,23 +441,45 @@ __device__ __forceinline__ float batch_weights(const VerifyArgs& a, const VRow& 
   return m;
 }
 
-// lambda S_p / S_q in two floats.
-__device__ __forceinline__ void split_k(double k, float& hi, float& lo) {
-  hi = (float)k;
-  lo = (float)(k - (double)hi);
+// The batch's sums by one wavefront (every lane has them), its weights in w.
+template <typename T, bool DRAWN>
+__device__ __forceinline__ VBatch batch_sums(const VerifyArgs& a, const VRow& r, int b,
+                                             const int32_t* gone, int n_gone,
+                                             float (&w)[kLpUnroll][8]) {
+  VBatch out;
+  double p, s1, sum = 0;
+  out.m = batch_weights<T, DRAWN, true>(a, r, b, gone, n_gone, w, p, s1);
+#pragma unroll
+  for (int u = 0; u < kLpUnroll; ++u) {
+    float us = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) us += w[u][e];
+    sum += us;
+  }
+  out.w = wave_sum64(sum);
+  out.p = wave_sum64(p);
+  out.s1 = r.own_max ? wave_sum64(s1) : 0.0;
+  out.best = 0x7fffffff;
+  return out;
+}
+template <typename T>
+__device__ __forceinline__ VBatch greedy_sums(const VerifyArgs& a, const VRow& r, int b) {
+  const int b0 = b * kLpBatch;
+  const VPart p = row_best<T>(static_cast<const T*>(r.x), b0, min(a.vocab, b0 + kLpBatch), 0, 1);
+  return VBatch{0, 0, p.s, p.m, p.best};
 }
 
-// Sum of max(p - l q, 0) over [begin, end), in units of p's exponentials, by the
-// whole workgroup (every thread has it).
-template <typename T>
-__device__ __forceinline__ double residual_sum(const VerifyArgs& a, VRow r, int begin, int end,
-                                               double* sh) {
+// Sum of max(p - l q, 0) over batches [begin, end), in units of p's exponentials,
+// by a workgroup of NT threads (every thread has it).
+template <typename T, int NT>
+__device__ __forceinline__ double residual_sum(const VerifyArgs& a, const VRow& r, int begin,
+                                               int end, double* sh) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   double sum = 0;
-  for (int b0 = begin + wave * kLpBatch; b0 < end; b0 += kVSpan) {
+  for (int b = begin + wave; b < end; b += NT / 64) {
     float w[kLpUnroll][8];
     double p, s1;
-    batch_weights<T, true>(a, r, b0, nullptr, 0, w, p, s1);
+    batch_weights<T, true>(a, r, b, nullptr, 0, w, p, s1);
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
       float s = 0.f;
@@ -324,22 +492,52 @@ __device__ __forceinline__ double residual_sum(const VerifyArgs& a, VRow r, int 
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[wave] = sum;
   __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  double total = 0;
+  for (int w = 0; w < NT / 64; ++w) total += sh[w];
+  return total;
 }
 
 // -- join ------------------------------------------------------------------------
 
+// A draft's p and q under its parent, and its log-prob.
+template <typename T, bool DRAWN>
+__device__ __forceinline__ VKid draft_under(const VerifyArgs& a, int64_t parent, int64_t tok,
+                                            const VNode& v, float& lp) {
+  VKid k = {0, 0};
+  lp = __builtin_nanf("");
+  if (tok < 0 || tok >= a.vocab) return k;
+  const double d = (double)(float)row_of<T>(a.logits, a.stride, parent)[tok] - v.m;
+  if ((v.flags & kVBad) == 0) {
+    k.p = vexp64(d, a.inv_t) / v.s;
+    lp = (float)(d - v.ls1);
+  }
+  if constexpr (DRAWN) {
+    if ((v.flags & kVBadDraft) == 0)
+      k.q = vexp64((double)(float)row_of<T>(a.draft, a.draft_stride, parent)[tok] - v.mq, a.inv_dt) /
+            v.sq;
+  }
+  return k;
+}
+// Whether a row has a finite maximum: a NaN or an infinity makes its sum one, no
+// finite logit makes it 0.
+__device__ __forceinline__ bool usable(const VPart& p) {
+  return finite_max(p.m) && p.s > 0.0 && p.s < __builtin_inf();
+}
+template <bool DRAWN>
+__device__ __forceinline__ VNode node_of(const VPart& p, const VPart& q) {
+  return VNode{p.s, log(p.s1), q.s, p.m, q.m,
+               kVSummed | (usable(p) ? 0 : kVBad) | (DRAWN && !usable(q) ? kVBadDraft : 0),
+               p.best};
+}
+
 // One workgroup per node, or (drawn drafts) per (node, segment).
 template <typename T, bool DRAWN, bool GREEDY>
 __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, const VPart* parts,
-                                                                VNode* nodes, double* f1) {
+                                                                VNode* nodes, VKid* kids,
+                                                                double* f1) {
   __shared__ VPart sp[2];
   __shared__ double sh[4];
-  __shared__ double kp[kVNodes], kq[kVNodes];
-  __shared__ int64_t ktok[kVNodes];
-  __shared__ double ku[kVNodes];
-  __shared__ int kid[kVNodes];
-  __shared__ int s_next, s_wave[4];
+  __shared__ int s_wave[4], s_open;
   const int segs = DRAWN ? a.segments : 1;
   const int seg = blockIdx.x % segs;
   const int64_t node = blockIdx.x / segs;
@@ -361,490 +559,559 @@ __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, co
   if (lane == 0) s_wave[wave] = __popcll(who);
   if (i == 0 && seg == 0 && tid > 0 && tid < n && (par < 0 || par >= tid))
     a.logprobs[first + tid] = __builtin_nanf("");
+  const int64_t tok = is_kid ? a.tokens[first + tid] : -1;
   __syncthreads();
-  int base = 0, k = 0;
+  int before = 0, k = 0;  // children in the wavefronts before, and in all
   for (int w = 0; w < 4; ++w) {
-    if (w < wave) base += s_wave[w];
+    if (w < wave) before += s_wave[w];
     k += s_wave[w];
   }
   if (k == 0) {
-    if (tid == 0 && seg == 0) nodes[node] = VNode{0, 0, 0, 0.f, 0.f, kVNone, 0, 0, 0};
+    if (tid == 0 && seg == 0) nodes[node] = VNode{0, 0, 0, 0.f, 0.f, 0, 0};
     return;
   }
   const VPart* mine = parts + node * (DRAWN ? 2 : 1) * a.segments;
-  if (wave == 0) {
-    const VPart p = join(mine, a.segments, GREEDY ? 1.0 : a.inv_t);
-    if (lane == 0) sp[0] = p;
-  } else if (DRAWN && wave == 1) {
-    const VPart p = join(mine + a.segments, a.segments, a.inv_dt);
-    if (lane == 0) sp[1] = p;
+  if (wave < (DRAWN ? 2 : 1)) {
+    const VPart p = join(mine + wave * a.segments, a.segments,
+                         GREEDY ? 1.0 : wave ? a.inv_dt : a.inv_t);
+    if (lane == 0) sp[wave] = p;
   }
+  if (tid == 0) s_open = 0;
   __syncthreads();
-  const VPart p = sp[0], q = DRAWN ? sp[1] : VPart{};
-  const bool bad = !finite_max(p.m), bad_draft = DRAWN && !finite_max(q.m);
+  const VNode v = node_of<DRAWN>(sp[0], DRAWN ? sp[1] : VPart{});
   if (is_kid) {
-    const int j = base + __popcll(who & ((1ull << lane) - 1));
-    const int64_t tok = a.tokens[first + tid];
-    const bool in = tok >= 0 && tok < a.vocab;
-    const float x = in ? (float)row_of<T>(a.logits, a.stride, node)[tok] : kNegInf;
-    kid[j] = tid;
-    ktok[j] = tok;
-    ku[j] = GREEDY ? 0.0 : number(a.uniforms[first + tid]);
-    kp[j] = bad || !in ? 0.0 : vexp64((double)x - p.m, a.inv_t) / p.s;
-    if constexpr (DRAWN) {
-      const float y = in ? (float)row_of<T>(a.draft, a.draft_stride, node)[tok] : kNegInf;
-      kq[j] = bad_draft || !in ? 0.0 : vexp64((double)y - q.m, a.inv_dt) / q.s;
+    float lp;
+    const VKid d = draft_under<T, DRAWN>(a, node, tok, v, lp);
+    if (seg == 0) {
+      a.logprobs[first + tid] = lp;
+      kids[first + tid] = d;
     }
-    if (seg == 0)
-      a.logprobs[first + tid] =
-          bad || !in ? __builtin_nanf("") : (float)(((double)x - p.m) - log(p.s1));
+    const bool leads = before + __popcll(who & ((1ull << lane) - 1)) == 0;
+    if (DRAWN && leads && k > 1 && (v.flags & (kVBad | kVBadDraft)) == 0 &&
+        !(number(a.uniforms[first + tid]) * d.q < d.p))
+      s_open = 1;
   }
-  __syncthreads();
-  if (tid == 0) {
-    int next = kVNone;
-    if (bad || bad_draft) {
-    } else if (GREEDY) {
-      for (int j = 0; j < k && next < 0; ++j)
-        if (ktok[j] == p.best) next = kid[j];
-    } else if (DRAWN) {
-      if (ku[0] * kq[0] < kp[0]) next = kid[0];
-      else if (k > 1) next = kVOpen;
-    } else {
-      double left = 1.0;
-      for (int j = 0; j < k && next < 0; ++j) {
-        double pj = kp[j];
-        for (int l = 0; l < j; ++l)
-          if (ktok[l] == ktok[j]) pj = 0.0;
-        if (ku[j] * left < pj) next = kid[j];
-        left -= pj;
-      }
-    }
-    s_next = next;
-    if (seg == 0)
-      nodes[node] = VNode{p.s, p.s1, q.s, p.m, q.m, next,
-                          kVSummed | (bad ? kVBad : 0) | (bad_draft ? kVBadDraft : 0),
-                          p.best, 0};
-  }
+  if (tid == 0 && seg == 0) nodes[node] = v;
   if constexpr (DRAWN) {
     __syncthreads();
-    if (s_next != kVOpen) return;  // (uniform)
+    if (!s_open) return;  // (uniform)
     VRow r = {row_of<T>(a.logits, a.stride, node), row_of<T>(a.draft, a.draft_stride, node),
-              p.m, q.m, 0.f, 0.f, false};
-    split_k(p.s / q.s, r.khi, r.klo);
-    const int begin = seg * a.seg_len;
-    const double f = residual_sum<T>(a, r, begin, min(a.vocab, begin + a.seg_len), sh);
-    if (tid == 0) f1[node * a.segments + seg] = f / p.s;
+              v.m, v.mq, 0.f, 0.f, false};
+    split_k(v.s / v.sq, r);
+    const int begin = seg * (a.seg_len / kLpBatch);
+    const double f = residual_sum<T, kVThreads>(
+        a, r, begin, min(batches_of(a.vocab), begin + a.seg_len / kLpBatch), sh);
+    if (tid == 0) f1[node * a.segments + seg] = f / v.s;
   }
 }
 
 // -- walk ------------------------------------------------------------------------
 
-// Inclusive sums over the workgroup's threads, in their order.
-__device__ __forceinline__ double block_scan(double x, double* sh, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    const double y = __shfl_up(x, i);
-    if (lane >= i) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) sh[wave] = x;
-  __syncthreads();
-  double base = 0;
-  total = 0;
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) base += sh[w];
-    total += sh[w];
-  }
-  return base + x;
+// What the tests of one request need, a node per thread.
+struct VWalk {
+  int par[kVNodes], next[kVNodes], tries[kVNodes], tok[kVNodes];
+  double p[kVNodes], q[kVNodes], u[kVNodes], lam[kVNodes], mass[kVNodes];
+  VNode node[kVNodes];
+  uint8_t on_path[kVNodes];
+  int32_t gone[kVNodes];
+  int v, count, n_gone;
+  double sh[16];
+};
+
+// Thread t's node as a draft: its parent (-1: none), token (-1: outside the
+// vocabulary) and number.
+template <bool GREEDY>
+__device__ __forceinline__ void load_draft(const VerifyArgs& a, VWalk& w, int64_t first, int n) {
+  const int t = threadIdx.x;
+  if (t >= n) return;
+  const int par = a.parents[first + t];
+  w.par[t] = t > 0 && par >= 0 && par < t ? par : -1;
+  const int64_t tok = a.tokens[first + t];
+  w.tok[t] = tok >= 0 && tok < a.vocab ? (int)tok : -1;
+  w.u[t] = GREEDY ? 0.0 : number(a.uniforms[first + t]);
+  w.on_path[t] = 0;
 }
 
-// The added token of one request from its row's batches, by the whole workgroup.
-template <typename T, bool DRAWN, bool GREEDY>
-__device__ __forceinline__ void pick(const VerifyArgs& a, int req, const VLast& l, const VRow& r,
-                                     const VBatch* batches, const int64_t* gone, int n_gone,
-                                     int64_t first) {
-  __shared__ double sh[4];
-  __shared__ float shm[4];
-  __shared__ int si[4];
-  __shared__ double s_base;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nb = (a.vocab + kLpBatch - 1) / kLpBatch;
-  float m = l.m;
-  double s1 = l.s1;
-  if (r.own_max) {
-    m = kNegInf;
-    for (int b = tid; b < nb; b += kVThreads) m = vmax(m, batches[b].m);
-    m = lp_wave_max(m);
-    if (lane == 0) shm[wave] = m;
-    __syncthreads();
-    m = vmax(vmax(shm[0], shm[1]), vmax(shm[2], shm[3]));
-    if (!finite_max(m)) {  // (uniform)
-      if (tid == 0) {
-        a.next_tokens[req] = -1;
-        a.logprobs[first] = __builtin_nanf("");
-      }
-      return;
-    }
-    s1 = 0;
-    for (int b = tid; b < nb; b += kVThreads)
-      s1 += batches[b].s1 * vexp64((double)batches[b].m - m, 1.0);
-    double total;
-    block_scan(s1, sh, total);
-    s1 = total;
-  }
-  if constexpr (GREEDY) {
-    int best = 0x7fffffff;
-    for (int b = tid; b < nb; b += kVThreads)
-      if (batches[b].m == m) best = min(best, batches[b].best);
-    best = wave_min(best);
-    if (lane == 0) si[wave] = best;
-    __syncthreads();
-    if (tid == 0) {
-      a.next_tokens[req] = min(min(si[0], si[1]), min(si[2], si[3]));
-      a.logprobs[first] = (float)-log(s1);
-    }
-    return;
-  }
-  // weights of batch b in the row's units; without any mass left, p's own
-  auto scale = [&](int b) {
-    return r.own_max ? vexp64((double)batches[b].m - m, a.inv_t) : 1.0;
-  };
-  auto sum = [&](int b, bool residual) {
-    return b < nb ? (residual ? batches[b].w : batches[b].p) * scale(b) : 0.0;
-  };
-  bool residual = true;
-  double total = 0;
-  for (int t = 0; t < 2; ++t) {
-    total = 0;
-    for (int b0 = 0; b0 < nb; b0 += kVThreads) {
-      double part;
-      block_scan(sum(b0 + tid, residual), sh, part);
-      total += part;
-    }
-    if (total > 0) break;  // (uniform)
-    residual = false;
-  }
-  const double target = (double)a.uniforms[first] * total;
-  // the first batch past the target, or the last one with any weight
-  double base = 0;
-  int at = 0x7fffffff, last = -1;
-  for (int b0 = 0; b0 < nb; b0 += kVThreads) {
-    const double x = sum(b0 + tid, residual);
-    double part;
-    const double cum = base + block_scan(x, sh, part);
-    const int hit = wave_min(cum > target && x > 0 ? b0 + tid : 0x7fffffff);
-    const int any = -wave_min(x > 0 ? -(b0 + tid) : 0x7fffffff);
-    __syncthreads();
-    if (lane == 0) {
-      si[wave] = hit;
-      shm[wave] = __int_as_float(any);
-    }
-    __syncthreads();
-    at = min(min(si[0], si[1]), min(si[2], si[3]));
-    for (int w = 0; w < 4; ++w) last = max(last, __float_as_int(shm[w]));
-    if (at != 0x7fffffff) {
-      if (b0 + tid == at) s_base = cum - x;
-      break;  // (uniform)
-    }
-    base += part;
-  }
-  const bool found = at != 0x7fffffff;
-  if (!found) at = last;
-  __syncthreads();
-  if (wave != 0) return;
-  // inside the batch: eight logits a lane, 512 at a time
-  float w[kLpUnroll][8];
-  double p, unused;
-  VRow one = r;
-  if (!residual) one.khi = one.klo = 0.f;
-  const float bm = batch_weights<T, DRAWN>(a, one, at * kLpBatch, gone, residual ? n_gone : 0, w, p,
-                                           unused);
-  const double f = scale(at);
-  double run = found ? s_base : 0.0;
-  int got = 0x7fffffff, tail = -1;
-#pragma unroll
-  for (int u = 0; u < kLpUnroll; ++u) {
-    double s = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += w[u][e];
-    s *= f;
-    double inc = s;
-#pragma unroll
-    for (int i = 1; i < 64; i <<= 1) {
-      const double y = __shfl_up(inc, i);
-      if (lane >= i) inc += y;
-    }
-    double c = run + (inc - s);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int id = at * kLpBatch + u * 512 + lane * 8 + e;
-      c += w[u][e] * f;
-      if (w[u][e] > 0.f) {
-        tail = id;
-        if (found && c > target) got = min(got, id);
-      }
-    }
-    run += __shfl(inc, 63);
-  }
-  got = wave_min(got);
-  tail = -wave_min(-tail);
-  const int id = got != 0x7fffffff ? got : tail;
-  if (lane == 0) {
-    a.next_tokens[req] = id;
-    const float x = (float)static_cast<const T*>(r.x)[id];
-    a.logprobs[first] = (float)(((double)x - m) - log(s1));
-  }
-}
-
-// Tokens of a node's children, in gone (drafts without a distribution: all of
-// them are rejected where the token is added).  Returns their number.
-__device__ __forceinline__ int rejected(const VerifyArgs& a, int64_t first, int n, int v,
-                                        int64_t* gone, int* count) {
-  const int tid = threadIdx.x;
-  if (tid == 0) *count = 0;
-  __syncthreads();
-  if (tid > v && tid < n && a.parents[first + tid] == v)
-    gone[atomicAdd(count, 1)] = a.tokens[first + tid];
-  __syncthreads();
-  return *count;  // (their order does not matter)
-}
-
-// A workgroup per (request, round of batches): the path, found by every one of
-// them, and its share of the batches; with one a request also the added token.
-template <typename T, bool DRAWN, bool GREEDY>
-__global__ __launch_bounds__(kVThreads) void verify_walk_kernel(VerifyArgs a, const VNode* nodes,
-                                                                const double* f1, VLast* lasts,
-                                                                VBatch* batches) {
-  __shared__ int par[kVNodes], next[kVNodes], tries[kVNodes];
-  __shared__ double lam[kVNodes], mass[kVNodes];
-  __shared__ uint8_t on_path[kVNodes];
-  __shared__ int64_t gone[kVNodes];
-  __shared__ int s_v, s_count, s_gone;
-  __shared__ double sh[4];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wgs = a.walk_wgs;
-  const int c = blockIdx.x % wgs, req = blockIdx.x / wgs;
-  const int64_t first = a.cu[req];
-  const int64_t size = (int64_t)a.cu[req + 1] - first;
-  const int n = (int)(size < kVNodes ? size : kVNodes);
-  if (n <= 0 || first < 0 || first + n > a.total) {
-    if (c == 0 && tid == 0) {
-      a.counts[req] = 0;
-      a.last[req] = -1;
-      a.next_tokens[req] = -1;
-      lasts[req].node = -1;
-    }
-    return;
-  }
-  if (tid < n) {
-    const VNode& v = nodes[first + tid];
-    par[tid] = a.parents[first + tid];
-    next[tid] = v.next;
-    on_path[tid] = 0;
-    if constexpr (DRAWN) {
-      lam[tid] = 1.0;  // (behind one rejected child)
-      double f = 0;
-      if (v.next == kVOpen)
-        for (int s = 0; s < a.segments; ++s) f += f1[(first + tid) * a.segments + s];
-      mass[tid] = f;
-      tries[tid] = 1;
-    }
-  }
-  __syncthreads();
-  // Tests of node v's next child against what p has become (mass, lam): sets
-  // next[v] to the child, kVNone, or kVMore where F is needed again.
-  auto test = [&](int v) {
-    const VNode& nd = nodes[first + v];
-    int left = tries[v];
+// Tries node v's children in turn, from the first that has not been tried, until
+// one is accepted (next[v]), none is left, or F is needed (kVMore, with lam).
+// f1: F(1) where it is known, else NaN.
+template <bool DRAWN, bool GREEDY>
+__device__ __forceinline__ void try_children(VWalk& w, int v, int n, double f1) {
+  int skip = w.tries[v], next = kVNone;
+  double lam = w.lam[v], mass = w.mass[v];
+  if ((w.node[v].flags & (kVSummed | kVBad | kVBadDraft)) == kVSummed) {
     for (int i = v + 1; i < n; ++i) {
-      if (par[i] != v) continue;
-      if (left > 0) {
-        --left;
+      if (w.par[i] != v) continue;
+      if (skip > 0) {
+        --skip;
         continue;
       }
-      if (tries[v] < 0) {  // (the tested child was not the last one)
-        next[v] = kVMore;
-        tries[v] = -tries[v];
-        return;
+      if constexpr (GREEDY) {
+        if (w.tok[i] != w.node[v].best) continue;
+        next = i;
+        break;
+      } else {
+        if constexpr (DRAWN) {
+          if (mass != mass) {  // (behind a rejected one: its sum is not known)
+            next = kVMore;
+            break;
+          }
+        }
+        double p = w.p[i];
+        if constexpr (!DRAWN) {
+          for (int j = v + 1; j < i; ++j)  // (removed already)
+            if (w.par[j] == v && w.tok[j] == w.tok[i]) p = 0.0;
+        }
+        const double q = DRAWN ? w.q[i] : 1.0;
+        if (w.u[i] * mass * q < (DRAWN ? p - lam * q : p)) {
+          next = i;
+          break;
+        }
+        ++w.tries[v];
+        if constexpr (DRAWN) {
+          lam += mass;
+          mass = w.tries[v] == 1 ? f1 : __builtin_nan("");
+        } else {
+          mass -= p;
+        }
       }
-      const int64_t tok = a.tokens[first + i];
-      double p = 0, q = 0;
-      if (tok >= 0 && tok < a.vocab) {
-        p = vexp64((double)(float)row_of<T>(a.logits, a.stride, first + v)[tok] - nd.m, a.inv_t) /
-            nd.s;
-        q = vexp64((double)(float)row_of<T>(a.draft, a.draft_stride, first + v)[tok] - nd.mq,
-                   a.inv_dt) / nd.sq;
-      }
-      if (number(a.uniforms[first + i]) * mass[v] * q < p - lam[v] * q) {
-        next[v] = i;
-        return;
-      }
-      lam[v] += mass[v];
-      tries[v] = -(tries[v] + 1);
-      left = 0;
     }
-    next[v] = kVNone;
-  };
-  if constexpr (DRAWN) {
-    if (tid < n && next[tid] == kVOpen) test(tid);
-    __syncthreads();
   }
+  w.lam[v] = lam;
+  w.mass[v] = mass;
+  w.next[v] = next;
+}
+
+// The path from node 0, with F's sums by the whole workgroup of NT threads where
+// they are needed; then w.v, w.count, w.on_path.
+template <typename T, bool DRAWN, bool GREEDY, int NT>
+__device__ __forceinline__ void follow(const VerifyArgs& a, VWalk& w, int64_t first, int n) {
+  const int tid = threadIdx.x;
   if (tid == 0) {
-    s_v = 0;
-    s_count = 0;
-    on_path[0] = 1;
+    w.v = w.count = 0;
+    w.on_path[0] = 1;
   }
   __syncthreads();
   for (;;) {
     if (tid == 0) {
-      int v = s_v, k = s_count;
-      while (next[v] >= 0) {
-        v = next[v];
-        on_path[v] = 1;
+      int v = w.v, k = w.count;
+      while (w.next[v] >= 0) {
+        v = w.next[v];
+        w.on_path[v] = 1;
         ++k;
       }
-      s_v = v;
-      s_count = k;
+      w.v = v;
+      w.count = k;
     }
     __syncthreads();
-    const int v = s_v;
-    if (!DRAWN || next[v] != kVMore) break;  // (uniform)
+    const int v = w.v;
+    if (!DRAWN || w.next[v] != kVMore) return;  // (uniform)
     if constexpr (DRAWN) {
-      // a third child or later: F at its lambda, by this workgroup alone
-      const VNode& nd = nodes[first + v];
+      const VNode& nd = w.node[v];
       VRow r = {row_of<T>(a.logits, a.stride, first + v),
                 row_of<T>(a.draft, a.draft_stride, first + v), nd.m, nd.mq, 0.f, 0.f, false};
-      split_k(lam[v] * (nd.s / nd.sq), r.khi, r.klo);
-      const double f = residual_sum<T>(a, r, 0, a.vocab, sh) / nd.s;
+      split_k(w.lam[v] * (nd.s / nd.sq), r);
+      const double f = residual_sum<T, NT>(a, r, 0, batches_of(a.vocab), w.sh) / nd.s;
       if (tid == 0) {
-        mass[v] = f;
-        test(v);
+        w.mass[v] = f;
+        try_children<DRAWN, GREEDY>(w, v, n, 0.0);
       }
       __syncthreads();
     }
   }
-  const int v = s_v;
-  const VNode nd = nodes[first + v];
-  if (c == 0) {
-    if (tid < n) a.accepted[first + tid] = on_path[tid];
+}
+
+// Behind the walk: the path's outputs, and the added token's row.  False where
+// there is nothing to draw (the token is set).
+template <typename T, bool DRAWN, bool GREEDY>
+__device__ __forceinline__ bool last_row(const VerifyArgs& a, VWalk& w, int req, int64_t first,
+                                         int n, const VNode& nd, bool writes, VRow& r) {
+  const int tid = threadIdx.x, v = w.v;
+  if (writes) {
+    if (tid < n) a.accepted[first + tid] = w.on_path[tid];
     if (tid == 0) {
-      a.counts[req] = s_count;
+      a.counts[req] = w.count;
       a.last[req] = v;
     }
   }
-  const bool summed = (nd.flags & kVSummed) != 0;
-  if ((nd.flags & kVBad) != 0 || (GREEDY && summed)) {
-    if (c == 0 && tid == 0) {
-      const bool bad = (nd.flags & kVBad) != 0;
+  const bool summed = (nd.flags & kVSummed) != 0, bad = (nd.flags & kVBad) != 0;
+  if (bad || (GREEDY && summed)) {
+    if (writes && tid == 0) {
       a.next_tokens[req] = bad ? -1 : nd.best;
-      a.logprobs[first] = bad ? __builtin_nanf("") : (float)-log(nd.s1);
-      lasts[req].node = -1;
+      a.logprobs[first] = bad ? __builtin_nanf("") : (float)-nd.ls1;
     }
-    return;
+    return false;
   }
-  VLast l = {nd.s1, nd.m, nd.mq, 0.f, 0.f, v, nd.flags};
-  if (DRAWN && summed && (nd.flags & kVBadDraft) == 0)
-    split_k(lam[v] * (nd.s / nd.sq), l.khi, l.klo);
-  VRow r = {row_of<T>(a.logits, a.stride, first + v),
-            DRAWN ? row_of<T>(a.draft, a.draft_stride, first + v) : nullptr, l.m, l.mq, l.khi,
-            l.klo, !summed};
-  const int n_gone = !DRAWN && !GREEDY && summed ? rejected(a, first, n, v, gone, &s_gone) : 0;
-  const int nb = (a.vocab + kLpBatch - 1) / kLpBatch;
-  VBatch* mine = batches + (int64_t)req * nb;
-  for (int b = c * 4 + wave; b < nb; b += wgs * 4) {
-    float w[kLpUnroll][8];
-    VBatch out;
-    out.best = 0x7fffffff;
-    if constexpr (GREEDY) {
-      float f[kLpUnroll][8];
-      lp_load_batch(static_cast<const T*>(r.x), b * kLpBatch, a.vocab, f);
-      float m = kNegInf;
-#pragma unroll
-      for (int u = 0; u < kLpUnroll; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = vmax(m, f[u][e]);
-      m = lp_wave_max(m);
-      const float mu = m == kNegInf ? 0.f : m;
-      double s = 0;
-      int best = 0x7fffffff;
-#pragma unroll
-      for (int u = 0; u < kLpUnroll; ++u) {
-        float us = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          us += fast_exp2((f[u][e] - mu) * kLog2e);
-          if (f[u][e] == m) best = min(best, b * kLpBatch + u * 512 + lane * 8 + e);
-        }
-        s += us;
-      }
-      out.w = out.p = 0;
-      out.s1 = wave_sum64(s);
-      out.m = m;
-      out.best = wave_min(best);
-    } else {
-      double p, s1;
-      out.m = batch_weights<T, DRAWN>(a, r, b * kLpBatch, gone, n_gone, w, p, s1);
-      double sum = 0;
-#pragma unroll
-      for (int u = 0; u < kLpUnroll; ++u) {
-        float us = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) us += w[u][e];
-        sum += us;
-      }
-      out.w = wave_sum64(sum);
-      out.p = wave_sum64(p);
-      out.s1 = wave_sum64(s1);
-    }
-    if (lane == 0) mine[b] = out;
-  }
-  if (wgs > 1) {
-    if (c == 0 && tid == 0) lasts[req] = l;
-    return;
-  }
-  __threadfence_block();
+  r = VRow{row_of<T>(a.logits, a.stride, first + v),
+           DRAWN ? row_of<T>(a.draft, a.draft_stride, first + v) : nullptr, nd.m, nd.mq, 0.f, 0.f,
+           !summed};
+  if (DRAWN && summed && (nd.flags & kVBadDraft) == 0) split_k(w.lam[v] * (nd.s / nd.sq), r);
+  if (tid == 0) w.n_gone = 0;
   __syncthreads();
-  pick<T, DRAWN, GREEDY>(a, req, l, r, mine, gone, n_gone, first);
+  if (!DRAWN && !GREEDY && tid < n && w.par[tid] == v && w.tok[tid] >= 0)
+    w.gone[atomicAdd(&w.n_gone, 1)] = w.tok[tid];  // (their order does not matter)
+  __syncthreads();
+  return true;
 }
 
 // -- pick ------------------------------------------------------------------------
 
+__device__ __forceinline__ void add_token(const VerifyArgs& a, int req, int64_t first, int64_t id,
+                                          float lp) {
+  a.next_tokens[req] = id;
+  a.logprobs[first] = lp;
+}
+
+// Where a row's added token lies: its batch (of nb) and the weights before it.
+struct VPlace {
+  bool done;      // the token is set
+  bool residual;  // weights, not p, are drawn from
+  bool found;     // in batch `at` (else: the last weight of that batch)
+  int at;
+  double start, target, scale;  // scale: of batch `at` to the row's units
+  double ls1;
+  float m;
+};
+
+// By one wavefront, from the row's batches.
+template <bool GREEDY>
+__device__ __forceinline__ VPlace place(const VerifyArgs& a, int req, int64_t first, bool own_max,
+                                        float m, double ls1, const VBatch* batches) {
+  const int lane = threadIdx.x & 63;
+  const int nb = batches_of(a.vocab);
+  VPlace o = {};
+  o.done = true;
+  if (own_max) {
+    m = kNegInf;
+    for (int b = lane; b < nb; b += 64) m = vmax(m, batches[b].m);
+    m = lp_wave_max(m);
+    if (!finite_max(m)) {  // (uniform)
+      if (lane == 0) add_token(a, req, first, -1, __builtin_nanf(""));
+      return o;
+    }
+    double s1 = 0;
+    for (int b = lane; b < nb; b += 64)
+      s1 += batches[b].s1 * vexp64((double)batches[b].m - m, 1.0);
+    ls1 = log(wave_sum64(s1));
+  }
+  if constexpr (GREEDY) {
+    int best = 0x7fffffff;
+    for (int b = lane; b < nb; b += 64)
+      if (batches[b].m == m) best = min(best, batches[b].best);
+    best = wave_min(best);
+    if (lane == 0) add_token(a, req, first, best, (float)-ls1);
+    return o;
+  }
+  // weights in the row's units; without any mass left, p's own
+  auto scale = [&](int b) {
+    return own_max ? vexp64((double)batches[b].m - m, a.inv_t) : 1.0;
+  };
+  double total = 0, whole = 0;
+  for (int b = lane; b < nb; b += 64) {
+    const double f = scale(b);
+    total += batches[b].w * f;
+    whole += batches[b].p * f;
+  }
+  total = wave_sum64(total);
+  whole = wave_sum64(whole);
+  o.done = false;
+  o.residual = total > 0;
+  o.target = (double)a.uniforms[first] * (o.residual ? total : whole);
+  o.m = m;
+  o.ls1 = ls1;
+  // the first batch past the target, or the last one with any weight
+  double base = 0;
+  int last = 0;
+  for (int b0 = 0; b0 < nb; b0 += 64) {
+    const int b = b0 + lane;
+    const double x = b < nb ? (o.residual ? batches[b].w : batches[b].p) * scale(b) : 0.0;
+    const double cum = base + wave_scan64(x);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(cum > o.target && x > 0);
+    const uint64_t any = __builtin_amdgcn_ballot_w64(x > 0);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      last = b0 + l;
+      o.start = lane64(cum - x, l);
+      o.found = true;
+      break;
+    }
+    if (any) last = b0 + 63 - __clzll((long long)any);
+    base = lane64(cum, 63);
+  }
+  o.at = last;
+  o.scale = scale(o.at);
+  return o;
+}
+
+// The token inside the batch, from the wavefront's weights of U * 512 ids at id0:
+// the first id whose cumulative weight, from `start` on, exceeds the target, and
+// the last with any weight; moves `start` behind them.
+template <int U>
+__device__ __forceinline__ void seek(const float (&w)[U][8], int id0, const VPlace& o,
+                                     double& start, int& got, int& tail) {
+  const int lane = threadIdx.x & 63;
+  got = 0x7fffffff;
+  tail = -1;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    double s = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += w[u][e];
+    s *= o.scale;
+    const double inc = wave_scan64(s);
+    double c = start + (inc - s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int id = id0 + u * 512 + lane * 8 + e;
+      c += w[u][e] * o.scale;
+      if (w[u][e] > 0.f) {
+        tail = id;
+        if (o.found && c > o.target) got = min(got, id);
+      }
+    }
+    start += lane64(inc, 63);
+  }
+  got = wave_min(got);
+  tail = -wave_min(-tail);
+}
+
+template <typename T>
+__device__ __forceinline__ void add_drawn(const VerifyArgs& a, int req, int64_t first,
+                                          const VRow& r, const VPlace& o, int got, int tail) {
+  const int id = got != 0x7fffffff ? got : tail;
+  add_token(a, req, first, id,
+            (float)(((double)(float)static_cast<const T*>(r.x)[id] - o.m) - o.ls1));
+}
+
+// A request's nodes, or false (with its outputs set) if it has none.
+__device__ __forceinline__ bool request(const VerifyArgs& a, int req, bool writes, int64_t& first,
+                                        int& n) {
+  first = a.cu[req];
+  const int64_t size = (int64_t)a.cu[req + 1] - first;
+  n = (int)(size < kVNodes ? size : kVNodes);
+  if (n > 0 && first >= 0 && first + n <= a.total) return true;
+  if (writes && threadIdx.x == 0) {
+    a.counts[req] = 0;
+    a.last[req] = -1;
+    a.next_tokens[req] = -1;
+  }
+  return false;
+}
+
+// A workgroup per (request, round of batches): the path, found by every one of
+// them, and its share of the batches.
 template <typename T, bool DRAWN, bool GREEDY>
-__global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a, const VLast* lasts,
-                                                                const VBatch* batches) {
-  __shared__ int64_t gone[kVNodes];
-  __shared__ int s_gone;
-  const int req = blockIdx.x;
+__global__ __launch_bounds__(kVThreads) void verify_walk_kernel(VerifyArgs a, const VNode* nodes,
+                                                                const VKid* kids, const double* f1,
+                                                                VLast* lasts, VBatch* batches) {
+  __shared__ VWalk w;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wgs = a.walk_wgs;
+  const int c = blockIdx.x % wgs, req = blockIdx.x / wgs;
+  int64_t first;
+  int n;
+  if (!request(a, req, c == 0, first, n)) {
+    if (c == 0 && tid == 0) lasts[req].node = -1;
+    return;
+  }
+  double f = __builtin_nan("");
+  if (tid < n) {
+    const VNode v = w.node[tid] = nodes[first + tid];
+    if (tid > 0) {
+      w.p[tid] = kids[first + tid].p;  // (not set, and not used, without a parent)
+      w.q[tid] = kids[first + tid].q;
+    }
+    w.lam[tid] = 0.0;
+    w.mass[tid] = 1.0;
+    w.tries[tid] = 0;
+    if constexpr (DRAWN) {
+      f = 0.0;  // (set where the first of several children is rejected)
+      if (v.flags & kVSummed)
+        for (int s = 0; s < a.segments; ++s) f += f1[(first + tid) * a.segments + s];
+    }
+  }
+  load_draft<GREEDY>(a, w, first, n);
+  __syncthreads();
+  if (tid < n) try_children<DRAWN, GREEDY>(w, tid, n, f);
+  __syncthreads();
+  follow<T, DRAWN, GREEDY, kVThreads>(a, w, first, n);
+  const VNode& nd = w.node[w.v];
+  VRow r;
+  if (!last_row<T, DRAWN, GREEDY>(a, w, req, first, n, nd, c == 0, r)) {
+    if (c == 0 && tid == 0) lasts[req].node = -1;
+    return;
+  }
+  const int nb = batches_of(a.vocab);
+  VBatch* mine = batches + (int64_t)req * nb;
+  for (int b = c * 4 + wave; b < nb; b += wgs * 4) {
+    VBatch out;
+    float wt[kLpUnroll][8];
+    if constexpr (GREEDY) out = greedy_sums<T>(a, r, b);
+    else out = batch_sums<T, DRAWN>(a, r, b, w.gone, w.n_gone, wt);
+    if ((tid & 63) == 0) mine[b] = out;
+  }
+  if (c == 0 && tid == 0) lasts[req] = VLast{nd.ls1, r.m, r.mq, r.khi, r.klo, w.v, nd.flags};
+}
+
+// A workgroup per request, every wavefront of which finds the batch.
+template <typename T, bool DRAWN, bool GREEDY>
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a, const VLast* lasts,
+                                                         const VBatch* batches) {
+  __shared__ int32_t gone[kVNodes];
+  __shared__ int n_gone;
+  const int req = blockIdx.x, tid = threadIdx.x;
   const VLast l = lasts[req];
   if (l.node < 0) return;
   const int64_t first = a.cu[req];
-  const int64_t size = (int64_t)a.cu[req + 1] - first;
-  const int n = (int)(size < kVNodes ? size : kVNodes);
   const bool summed = (l.flags & kVSummed) != 0;
+  const VPlace o = place<GREEDY>(a, req, first, !summed, l.m, l.ls1,
+                                 batches + (int64_t)req * batches_of(a.vocab));
+  if (o.done) return;  // (uniform)
+  if (tid == 0) n_gone = 0;
+  __syncthreads();
+  if (!DRAWN && !GREEDY && summed) {
+    const int64_t size = (int64_t)a.cu[req + 1] - first;
+    const int n = (int)(size < kVNodes ? size : kVNodes);
+    for (int t = l.node + 1 + tid; t < n; t += 64) {
+      const int64_t tok = a.tokens[first + t];
+      if (a.parents[first + t] == l.node && tok >= 0 && tok < a.vocab)
+        gone[atomicAdd(&n_gone, 1)] = (int32_t)tok;
+    }
+    __syncthreads();
+  }
   VRow r = {row_of<T>(a.logits, a.stride, first + l.node),
-            DRAWN ? row_of<T>(a.draft, a.draft_stride, first + l.node) : nullptr, l.m, l.mq, l.khi,
-            l.klo, !summed};
-  const int n_gone = !DRAWN && !GREEDY && summed ? rejected(a, first, n, l.node, gone, &s_gone) : 0;
-  const int nb = (a.vocab + kLpBatch - 1) / kLpBatch;
-  pick<T, DRAWN, GREEDY>(a, req, l, r, batches + (int64_t)req * nb, gone, n_gone, first);
+            DRAWN ? row_of<T>(a.draft, a.draft_stride, first + l.node) : nullptr, l.m, l.mq,
+            l.khi, l.klo, !summed};
+  if (!o.residual) r.khi = r.klo = 0.f;
+  float w[kLpUnroll][8];
+  double p, s1, start = o.start;
+  batch_weights<T, DRAWN>(a, r, o.at, gone, o.residual ? n_gone : 0, w, p, s1);
+  int got, tail;
+  seek(w, o.at * kLpBatch, o, start, got, tail);
+  if (tid == 0) add_drawn<T>(a, req, first, r, o, got, tail);
 }
 
+// -- short rows --------------------------------------------------------------------
+
+// Behind the stats, a workgroup per request for everything else, where a row has
+// no more batches than the workgroup wavefronts: F's sums as the path needs them,
+// and the added token out of the registers that hold its batch's weights.
+template <typename T, bool DRAWN, bool GREEDY>
+__global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a,
+                                                                    const VPart* parts) {
+  constexpr int NW = kVRestThreads / 64;
+  __shared__ VWalk w;
+  __shared__ VBatch batches[NW];
+  __shared__ int16_t inner[kVNodes];
+  __shared__ int s_wave[NW];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int req = blockIdx.x;
+  int64_t first;
+  int n;
+  auto nobody = [&](int64_t begin, int64_t end) {  // nodes that no path can hold
+    if (end > a.total) end = a.total;
+    for (int64_t t = (begin > 0 ? begin : 0) + tid; t < end; t += kVRestThreads) {
+      a.accepted[t] = 0;
+      a.logprobs[t] = __builtin_nanf("");
+    }
+  };
+  if (req == 0) {
+    nobody(0, a.cu[0]);
+    nobody(a.cu[a.batch], a.total);
+  }
+  if (!request(a, req, true, first, n)) return;
+  nobody(first + kVNodes, a.cu[req + 1]);
+  load_draft<GREEDY>(a, w, first, n);
+  if (tid < n) w.node[tid].flags = 0;
+  __syncthreads();
+  if (tid > 0 && tid < n && w.par[tid] >= 0) w.node[w.par[tid]].flags = kVSummed;
+  __syncthreads();
+  // the nodes with children, and their sums
+  const bool in = tid < n && w.node[tid].flags != 0;
+  const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+  if (lane == 0) s_wave[wave] = __popcll(who);
+  __syncthreads();
+  int rank = __popcll(who & ((1ull << lane) - 1)), k = 0;
+  for (int x = 0; x < NW; ++x) {
+    if (x < wave) rank += s_wave[x];
+    k += s_wave[x];
+  }
+  if (in) inner[rank] = (int16_t)tid;
+  __syncthreads();
+  for (int e = wave; e < k; e += NW) {
+    const VPart* mine = parts + (first + inner[e]) * (DRAWN ? 2 : 1) * a.segments;
+    const VPart p = join(mine, a.segments, GREEDY ? 1.0 : a.inv_t);
+    VPart q = {};
+    if constexpr (DRAWN) q = join(mine + a.segments, a.segments, a.inv_dt);
+    const VNode v = node_of<DRAWN>(p, q);
+    if (lane == 0) w.node[inner[e]] = v;
+  }
+  __syncthreads();
+  if (tid < n) {
+    const int par = w.par[tid];
+    float lp = __builtin_nanf("");
+    VKid d = {0, 0};
+    if (par >= 0) d = draft_under<T, DRAWN>(a, first + par, w.tok[tid], w.node[par], lp);
+    if (tid > 0) a.logprobs[first + tid] = lp;
+    w.p[tid] = d.p;
+    w.q[tid] = d.q;
+    w.lam[tid] = 0.0;
+    w.mass[tid] = 1.0;
+    w.tries[tid] = 0;
+  }
+  __syncthreads();
+  if (tid < n) try_children<DRAWN, GREEDY>(w, tid, n, __builtin_nan(""));
+  __syncthreads();
+  follow<T, DRAWN, GREEDY, kVRestThreads>(a, w, first, n);
+  const VNode& nd = w.node[w.v];
+  VRow r;
+  if (!last_row<T, DRAWN, GREEDY>(a, w, req, first, n, nd, true, r)) return;
+  const int nb = batches_of(a.vocab);
+  float wt[kLpUnroll][8];
+  VBatch mine = {};
+  if (wave < nb) {
+    if constexpr (GREEDY) mine = greedy_sums<T>(a, r, wave);
+    else mine = batch_sums<T, DRAWN>(a, r, wave, w.gone, w.n_gone, wt);
+    if (lane == 0) batches[wave] = mine;
+  }
+  __syncthreads();
+  const VPlace o = place<GREEDY>(a, req, first, r.own_max, r.m, nd.ls1, batches);
+  if constexpr (!GREEDY) {
+    if (o.done || wave != o.at) return;
+    double p, s1, start = o.start;
+    if (!o.residual) {
+      r.khi = r.klo = 0.f;
+      batch_weights<T, DRAWN>(a, r, wave, nullptr, 0, wt, p, s1);
+    }
+    int got, tail;
+    seek(wt, wave * kLpBatch, o, start, got, tail);
+    if (lane == 0) add_drawn<T>(a, req, first, r, o, got, tail);
+  }
+}
+
+// -- host --------------------------------------------------------------------------
+
 struct Layout {
+  bool rest;  // short rows: one launch behind the stats
   int32_t segments, seg_len, walk_wgs;
-  int64_t parts, nodes, f1, lasts, batches, bytes;
+  int64_t parts, nodes, kids, f1, lasts, batches, bytes;
 };
 
 Layout layout(int32_t batch, int64_t total, int32_t vocab, bool drawn) {
-  Layout l;
-  const int32_t spans = (vocab + kVSpan - 1) / kVSpan;
-  const int32_t rounds = (spans + kVMaxSegments - 1) / kVMaxSegments;
-  l.seg_len = rounds * kVSpan;
-  l.segments = (vocab + l.seg_len - 1) / l.seg_len;
-  l.walk_wgs = l.segments;
-  const int64_t nb = (vocab + kLpBatch - 1) / kLpBatch;
+  Layout l = {};
+  const int64_t nb = batches_of(vocab);
+  l.rest = nb <= kVRestThreads / 64;
+  // segments of one round of a workgroup, of more where the nodes alone would
+  // make for many more workgroups than the units hold
+  const int32_t spans = (int32_t)((vocab + (int64_t)kVSpan - 1) / kVSpan);
+  int64_t rounds = total * (drawn ? 2 : 1) * spans / kVManyWgs;
+  const int32_t least = (spans + kVMaxSegments - 1) / kVMaxSegments;
+  rounds = rounds < least ? least : rounds > spans ? spans : rounds;
+  l.seg_len = (int32_t)rounds * kVSpan;
+  l.segments = (int32_t)((vocab + (int64_t)l.seg_len - 1) / l.seg_len);
+  l.walk_wgs = spans < kVMaxSegments ? spans : kVMaxSegments;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t p = at;
@@ -852,36 +1119,44 @@ Layout layout(int32_t batch, int64_t total, int32_t vocab, bool drawn) {
     return p;
   };
   l.parts = take(total * (drawn ? 2 : 1) * l.segments * (int64_t)sizeof(VPart));
-  l.nodes = take(total * (int64_t)sizeof(VNode));
-  l.f1 = take(drawn ? total * l.segments * 8 : 0);
-  l.lasts = take(batch * (int64_t)sizeof(VLast));
-  l.batches = take(batch * nb * (int64_t)sizeof(VBatch));
-  l.bytes = at;
+  if (!l.rest) {
+    l.nodes = take(total * (int64_t)sizeof(VNode));
+    l.kids = take(total * (int64_t)sizeof(VKid));
+    l.f1 = take(drawn ? total * l.segments * 8 : 0);
+    l.lasts = take(batch * (int64_t)sizeof(VLast));
+    l.batches = take(batch * nb * (int64_t)sizeof(VBatch));
+  }
+  l.bytes = at > 0 ? at : 16;
   return l;
 }
 
 template <typename T, bool DRAWN, bool GREEDY>
-hipError_t run(VerifyArgs a, const Layout& l, char* ws, hipStream_t s) {
+hipError_t run(const VerifyArgs& a, const Layout& l, char* ws, hipStream_t s) {
   VPart* parts = reinterpret_cast<VPart*>(ws + l.parts);
+  const dim3 block(kVThreads);
+  const int64_t rows = a.total * (DRAWN ? 2 : 1) * l.segments;
+  if (rows > 0)
+    hipLaunchKernelGGL((verify_stats_kernel<T, GREEDY>), dim3((uint32_t)rows), block, 0, s, a,
+                       parts);
+  if (l.rest) {
+    hipLaunchKernelGGL((verify_rest_kernel<T, DRAWN, GREEDY>), dim3((uint32_t)a.batch),
+                       dim3(kVRestThreads), 0, s, a, parts);
+    return hipGetLastError();
+  }
   VNode* nodes = reinterpret_cast<VNode*>(ws + l.nodes);
+  VKid* kids = reinterpret_cast<VKid*>(ws + l.kids);
   double* f1 = reinterpret_cast<double*>(ws + l.f1);
   VLast* lasts = reinterpret_cast<VLast*>(ws + l.lasts);
   VBatch* batches = reinterpret_cast<VBatch*>(ws + l.batches);
-  const dim3 block(kVThreads);
-  const int64_t rows = a.total * (DRAWN ? 2 : 1) * l.segments;
-  if (a.total > 0) {
-    hipLaunchKernelGGL((verify_stats_kernel<T, GREEDY>), dim3((uint32_t)rows), block, 0, s, a,
-                       parts);
+  if (rows > 0)
     hipLaunchKernelGGL((verify_join_kernel<T, DRAWN, GREEDY>),
                        dim3((uint32_t)(a.total * (DRAWN ? l.segments : 1))), block, 0, s, a, parts,
-                       nodes, f1);
-  }
+                       nodes, kids, f1);
   hipLaunchKernelGGL((verify_walk_kernel<T, DRAWN, GREEDY>),
-                     dim3((uint32_t)((int64_t)a.batch * l.walk_wgs)), block, 0, s, a, nodes, f1,
-                     lasts, batches);
-  if (l.walk_wgs > 1)
-    hipLaunchKernelGGL((verify_pick_kernel<T, DRAWN, GREEDY>), dim3((uint32_t)a.batch), block, 0, s,
-                       a, lasts, batches);
+                     dim3((uint32_t)((int64_t)a.batch * l.walk_wgs)), block, 0, s, a, nodes, kids,
+                     f1, lasts, batches);
+  hipLaunchKernelGGL((verify_pick_kernel<T, DRAWN, GREEDY>), dim3((uint32_t)a.batch), dim3(64), 0, s,
+                     a, lasts, batches);
   return hipGetLastError();
 }
 
@@ -907,14 +1182,15 @@ hipError_t verify_drafts(VerifyArgs a, double temperature, double draft_temperat
   const bool greedy = temperature == 0.0;
   if (greedy) a.draft = nullptr;
   const Layout l = layout(a.batch, a.total, a.vocab, a.draft != nullptr);
-  auto split = [](double t, double& inv, float& hi, float& lo) {
+  auto split = [](double t, double& inv, float& hi, float& lo, float& least) {
     inv = t > 0 ? 1.0 / t : 1.0;
     const double c = 1.4426950408889634074 * inv;
     hi = (float)c;
     lo = (float)(c - (double)hi);
+    least = (float)(-160.0 / c);  // (2^-160 is 0 in fp32)
   };
-  split(temperature, a.inv_t, a.thi, a.tlo);
-  split(draft_temperature, a.inv_dt, a.dhi, a.dlo);
+  split(temperature, a.inv_t, a.thi, a.tlo, a.tleast);
+  split(draft_temperature, a.inv_dt, a.dhi, a.dlo, a.dleast);
   a.segments = l.segments;
   a.seg_len = l.seg_len;
   a.walk_wgs = l.walk_wgs;

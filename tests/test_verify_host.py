@@ -65,18 +65,20 @@ def test_c_refusals():
         assert _call(**{name: None}) == INVALID, name
     assert _call(elem=1) == UNSUPPORTED and _call(total=(1 << 24) + 1) == UNSUPPORTED
     assert _call(vocab=(1 << 30) + 1, stride=1 << 31, dstride=1 << 31) == UNSUPPORTED
-    assert _call(total=1 << 24, vocab=1 << 30, stride=1 << 30, dstride=0) == UNSUPPORTED
+    assert _call(batch=(1 << 31) - 1, vocab=1 << 30, stride=1 << 30, dstride=0) == UNSUPPORTED
+    big = dict(vocab=151936, stride=151936, dstride=151936)
     for kw in ({"ws": None}, {"ws": 72}, {"ws_bytes": 100}):
-        assert _call(**kw) == _lib.AIOS_ERR_WORKSPACE, kw
+        assert _call(**big, **kw) == _lib.AIOS_ERR_WORKSPACE, kw
     assert _call(batch=0, logits=None, ws=None) == OK
 
 
 def test_workspace_sizes():
     f = _lib.lib().aios_verify_workspace
     assert f(0, 9, 100, 1) == 0 and f(2, -1, 100, 1) == 0 and f(2, 9, 0, 1) == 0
-    assert 0 < f(2, 9, 100, 0) < f(2, 9, 100, 1) < f(2, 90, 100, 1) < f(2, 90, 151936, 1)
-    need = f(2, 9, 100, 1)
-    assert _call(ws_bytes=need - 1) == _lib.AIOS_ERR_WORKSPACE
+    v = 151936
+    assert 0 < f(2, 9, 100, 0) < f(2, 9, 100, 1) < f(2, 9, v, 0) < f(2, 9, v, 1) < f(2, 90, v, 1) < f(4, 90, v, 1)
+    need = f(2, 9, v, 1)
+    assert _call(vocab=v, stride=v, dstride=v, ws_bytes=need - 1) == _lib.AIOS_ERR_WORKSPACE
 
 
 def test_python_refusals():
