@@ -27,7 +27,9 @@
 //   join   those sums together, the children's p and q; F(1) where the first child
 //          of several is rejected, by segments
 //   walk   the tests, the path, and the added token's weights by batches of 2048
-//          ids (a leaf's row is read here only)
+//          ids (a leaf's row is read here only); where the path needs F behind two
+//          or more rejected children that sum is this launch's work, and the next
+//          one goes on (drawn drafts have kVStages of these launches)
 //   pick   the added token
 // Bound: the rows, read once from HBM (those of F(1) and of the last node again).
 // Rows of at most 16 batches take what follows the stats in one launch
@@ -66,6 +68,12 @@ struct VNode {
 struct VKid {  // a draft under its parent's distributions
   double p, q;
 };
+// A sum of F that a walk's launch took: behind j rejected children of a node.
+struct VOpen {
+  int32_t node;  // -1: none was needed, the request's batches are done
+  int32_t j;
+};
+constexpr int kVStages = 3;  // launches of the walk over drawn drafts
 // The last accepted node's row, as the pick needs it.
 struct VLast {
   double ls1;       // ln s1 of the row (not of a leaf's)
@@ -469,14 +477,14 @@ __device__ __forceinline__ VBatch greedy_sums(const VerifyArgs& a, const VRow& r
   return VBatch{0, 0, p.s, p.m, p.best};
 }
 
-// Sum of max(p - l q, 0) over batches [begin, end), in units of p's exponentials,
-// by a workgroup of NT threads (every thread has it).
+// Sum of max(p - l q, 0) over the share-th of `shares` of batches [0, end), in units
+// of p's exponentials, by a workgroup of NT threads (every thread has it).
 template <typename T, int NT>
-__device__ __forceinline__ double residual_sum(const VerifyArgs& a, const VRow& r, int begin,
-                                               int end, double* sh) {
+__device__ __forceinline__ double residual_sum(const VerifyArgs& a, const VRow& r, int share,
+                                               int shares, int end, double* sh, int begin = 0) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   double sum = 0;
-  for (int b = begin + wave; b < end; b += NT / 64) {
+  for (int b = begin + share * (NT / 64) + wave; b < end; b += shares * (NT / 64)) {
     float w[kLpUnroll][8];
     double p, s1;
     batch_weights<T, true>(a, r, b, nullptr, 0, w, p, s1);
@@ -530,6 +538,49 @@ __device__ __forceinline__ VNode node_of(const VPart& p, const VPart& q) {
                p.best};
 }
 
+// The sum of a node's segments, asked for eight at a time.
+__device__ __forceinline__ double sum_parts(const double* f, int n) {
+  double sum = 0;
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    double v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = s0 + j < n ? f[s0 + j] : 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[j];
+  }
+  return sum;
+}
+
+// Segment seg of F(lambda) of one node, by the workgroup.
+template <typename T>
+__device__ __forceinline__ void segment_f(const VerifyArgs& a, int64_t node, int seg, const VNode& v,
+                                          double lambda, double* sh, double* f) {
+  VRow r = {row_of<T>(a.logits, a.stride, node), row_of<T>(a.draft, a.draft_stride, node),
+            v.m, v.mq, 0.f, 0.f, false};
+  split_k(lambda * (v.s / v.sq), r);
+  const int begin = seg * (a.seg_len / kLpBatch);
+  const double sum = residual_sum<T, kVThreads>(
+      a, r, 0, 1, min(batches_of(a.vocab), begin + a.seg_len / kLpBatch), sh, begin);
+  if (threadIdx.x == 0) f[node * a.segments + seg] = sum / v.s;
+}
+
+// The children of node i: whether the thread's node is one, how many come before
+// it, and the number of all (every thread of the workgroup calls it).
+__device__ __forceinline__ bool child_rank(bool is_kid, int* s_wave, int& rank, int& k) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t who = __builtin_amdgcn_ballot_w64(is_kid);
+  if (lane == 0) s_wave[wave] = __popcll(who);
+  __syncthreads();
+  rank = __popcll(who & ((1ull << lane) - 1));
+  k = 0;
+  for (int w = 0; w < kVThreads / 64; ++w) {
+    if (w < wave) rank += s_wave[w];
+    k += s_wave[w];
+  }
+  return is_kid;
+}
+
 // One workgroup per node, or (drawn drafts) per (node, segment).
 template <typename T, bool DRAWN, bool GREEDY>
 __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, const VPart* parts,
@@ -555,17 +606,11 @@ __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, co
   const int i = (int)(node - first);
   const int par = tid < n ? a.parents[first + tid] : -1;
   const bool is_kid = tid > i && tid < n && par == i;
-  const uint64_t who = __builtin_amdgcn_ballot_w64(is_kid);
-  if (lane == 0) s_wave[wave] = __popcll(who);
+  const int64_t tok = is_kid ? a.tokens[first + tid] : -1;
   if (i == 0 && seg == 0 && tid > 0 && tid < n && (par < 0 || par >= tid))
     a.logprobs[first + tid] = __builtin_nanf("");
-  const int64_t tok = is_kid ? a.tokens[first + tid] : -1;
-  __syncthreads();
-  int before = 0, k = 0;  // children in the wavefronts before, and in all
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += s_wave[w];
-    k += s_wave[w];
-  }
+  int rank, k;
+  child_rank(is_kid, s_wave, rank, k);
   if (k == 0) {
     if (tid == 0 && seg == 0) nodes[node] = VNode{0, 0, 0, 0.f, 0.f, 0, 0};
     return;
@@ -586,8 +631,7 @@ __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, co
       a.logprobs[first + tid] = lp;
       kids[first + tid] = d;
     }
-    const bool leads = before + __popcll(who & ((1ull << lane) - 1)) == 0;
-    if (DRAWN && leads && k > 1 && (v.flags & (kVBad | kVBadDraft)) == 0 &&
+    if (DRAWN && rank == 0 && k > 1 && (v.flags & (kVBad | kVBadDraft)) == 0 &&
         !(number(a.uniforms[first + tid]) * d.q < d.p))
       s_open = 1;
   }
@@ -595,13 +639,7 @@ __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, co
   if constexpr (DRAWN) {
     __syncthreads();
     if (!s_open) return;  // (uniform)
-    VRow r = {row_of<T>(a.logits, a.stride, node), row_of<T>(a.draft, a.draft_stride, node),
-              v.m, v.mq, 0.f, 0.f, false};
-    split_k(v.s / v.sq, r);
-    const int begin = seg * (a.seg_len / kLpBatch);
-    const double f = residual_sum<T, kVThreads>(
-        a, r, begin, min(batches_of(a.vocab), begin + a.seg_len / kLpBatch), sh);
-    if (tid == 0) f1[node * a.segments + seg] = f / v.s;
+    segment_f<T>(a, node, seg, v, 1.0, sh, f1);
   }
 }
 
@@ -612,6 +650,7 @@ struct VWalk {
   int par[kVNodes], next[kVNodes], tries[kVNodes], tok[kVNodes];
   double p[kVNodes], q[kVNodes], u[kVNodes], lam[kVNodes], mass[kVNodes];
   VNode node[kVNodes];
+  uint64_t kids[kVNodes][kVNodes / 64];  // bit t: node t is a child
   uint8_t on_path[kVNodes];
   int32_t gone[kVNodes];
   int v, count, n_gone;
@@ -632,60 +671,92 @@ __device__ __forceinline__ void load_draft(const VerifyArgs& a, VWalk& w, int64_
   w.on_path[t] = 0;
 }
 
+// Every node's children (behind load_draft and a barrier).  All parents pass by
+// every thread out of the wavefront's registers: looking for them in LDS, one
+// dependent read after the other, took longer than a launch.
+__device__ __forceinline__ void list_children(VWalk& w, int n) {
+  const int t = threadIdx.x, lane = t & 63;
+  if ((t & ~63) >= n) return;  // (uniform per wavefront)
+#pragma unroll
+  for (int g = 0; g < kVNodes / 64; ++g) {
+    uint64_t mask = 0;
+    if (g * 64 < n) {
+      const int par = g * 64 + lane < n ? w.par[g * 64 + lane] : -1;
+      const int m = min(n - g * 64, 64);
+      for (int j = 0; j < m; ++j)
+        mask |= (uint64_t)(__builtin_amdgcn_readlane(par, j) == t) << j;
+    }
+    if (t < n) w.kids[t][g] = mask;
+  }
+}
+// The next child of node v behind node i (-1: none).
+__device__ __forceinline__ int next_child(const VWalk& w, int v, int i) {
+  int g = (i + 1) >> 6;
+  if (g >= kVNodes / 64) return -1;
+  uint64_t m = w.kids[v][g] & (~0ull << ((i + 1) & 63));
+  while (m == 0) {
+    if (++g >= kVNodes / 64) return -1;
+    m = w.kids[v][g];
+  }
+  return g * 64 + __ffsll((unsigned long long)m) - 1;
+}
+
 // Tries node v's children in turn, from the first that has not been tried, until
 // one is accepted (next[v]), none is left, or F is needed (kVMore, with lam).
-// f1: F(1) where it is known, else NaN.
-template <bool DRAWN, bool GREEDY>
-__device__ __forceinline__ void try_children(VWalk& w, int v, int n, double f1) {
-  int skip = w.tries[v], next = kVNone;
+// sums(j): F behind j rejected children where it is known, else NaN.
+template <bool DRAWN, bool GREEDY, typename Sums>
+__device__ __forceinline__ void try_children(VWalk& w, int v, int n, Sums&& sums) {
+  int next = kVNone, tried = w.tries[v];
   double lam = w.lam[v], mass = w.mass[v];
   if ((w.node[v].flags & (kVSummed | kVBad | kVBadDraft)) == kVSummed) {
-    for (int i = v + 1; i < n; ++i) {
-      if (w.par[i] != v) continue;
-      if (skip > 0) {
-        --skip;
-        continue;
-      }
+    int i = next_child(w, v, v);
+    for (int k = 0; k < tried && i >= 0; ++k) i = next_child(w, v, i);
+    for (; i >= 0; i = next_child(w, v, i)) {
       if constexpr (GREEDY) {
         if (w.tok[i] != w.node[v].best) continue;
         next = i;
         break;
       } else {
         if constexpr (DRAWN) {
-          if (mass != mass) {  // (behind a rejected one: its sum is not known)
+          if (mass != mass) mass = sums(tried);
+          if (mass != mass) {
             next = kVMore;
             break;
           }
         }
         double p = w.p[i];
         if constexpr (!DRAWN) {
-          for (int j = v + 1; j < i; ++j)  // (removed already)
-            if (w.par[j] == v && w.tok[j] == w.tok[i]) p = 0.0;
+          for (int j = next_child(w, v, v); j < i; j = next_child(w, v, j))  // (removed already)
+            if (w.tok[j] == w.tok[i]) p = 0.0;
         }
         const double q = DRAWN ? w.q[i] : 1.0;
         if (w.u[i] * mass * q < (DRAWN ? p - lam * q : p)) {
           next = i;
           break;
         }
-        ++w.tries[v];
+        ++tried;
         if constexpr (DRAWN) {
           lam += mass;
-          mass = w.tries[v] == 1 ? f1 : __builtin_nan("");
+          mass = __builtin_nan("");  // (asked for where there is a next one)
         } else {
           mass -= p;
         }
       }
     }
   }
+  w.tries[v] = tried;
   w.lam[v] = lam;
   w.mass[v] = mass;
   w.next[v] = next;
 }
 
-// The path from node 0, with F's sums by the whole workgroup of NT threads where
-// they are needed; then w.v, w.count, w.on_path.
-template <typename T, bool DRAWN, bool GREEDY, int NT>
-__device__ __forceinline__ void follow(const VerifyArgs& a, VWalk& w, int64_t first, int n) {
+// The path from node 0: w.v, w.count, w.on_path.  Where it needs F behind j rejected
+// children of a node, known(v, j) gives it (NaN: not known); else put_off(v, j, row)
+// may take the sum elsewhere (the path ends there: false), or the whole workgroup
+// of NT threads takes it.
+template <typename T, bool DRAWN, bool GREEDY, int NT, typename Known, typename PutOff>
+__device__ __forceinline__ bool follow(const VerifyArgs& a, VWalk& w, int64_t first, int n,
+                                       Known&& known, PutOff&& put_off) {
   const int tid = threadIdx.x;
   if (tid == 0) {
     w.v = w.count = 0;
@@ -695,26 +766,34 @@ __device__ __forceinline__ void follow(const VerifyArgs& a, VWalk& w, int64_t fi
   for (;;) {
     if (tid == 0) {
       int v = w.v, k = w.count;
-      while (w.next[v] >= 0) {
-        v = w.next[v];
-        w.on_path[v] = 1;
-        ++k;
+      for (;;) {
+        while (w.next[v] >= 0) {
+          v = w.next[v];
+          w.on_path[v] = 1;
+          ++k;
+        }
+        if (!DRAWN || w.next[v] != kVMore) break;
+        const double f = known(v, w.tries[v]);
+        if (f != f) break;
+        w.mass[v] = f;
+        try_children<DRAWN, GREEDY>(w, v, n, [&](int j) { return known(v, j); });
       }
       w.v = v;
       w.count = k;
     }
     __syncthreads();
     const int v = w.v;
-    if (!DRAWN || w.next[v] != kVMore) return;  // (uniform)
+    if (!DRAWN || w.next[v] != kVMore) return true;  // (uniform)
     if constexpr (DRAWN) {
       const VNode& nd = w.node[v];
       VRow r = {row_of<T>(a.logits, a.stride, first + v),
                 row_of<T>(a.draft, a.draft_stride, first + v), nd.m, nd.mq, 0.f, 0.f, false};
       split_k(w.lam[v] * (nd.s / nd.sq), r);
-      const double f = residual_sum<T, NT>(a, r, 0, batches_of(a.vocab), w.sh) / nd.s;
+      if (put_off(v, w.tries[v], r)) return false;  // (uniform)
+      const double f = residual_sum<T, NT>(a, r, 0, 1, batches_of(a.vocab), w.sh) / nd.s;
       if (tid == 0) {
         w.mass[v] = f;
-        try_children<DRAWN, GREEDY>(w, v, n, 0.0);
+        try_children<DRAWN, GREEDY>(w, v, n, [](int) { return __builtin_nan(""); });
       }
       __syncthreads();
     }
@@ -899,25 +978,34 @@ __device__ __forceinline__ bool request(const VerifyArgs& a, int req, bool write
 }
 
 // A workgroup per (request, round of batches): the path, found by every one of
-// them, and its share of the batches.
+// them, and its share of the batches, or of the sum of F that the path needs next.
 template <typename T, bool DRAWN, bool GREEDY>
-__global__ __launch_bounds__(kVThreads) void verify_walk_kernel(VerifyArgs a, const VNode* nodes,
-                                                                const VKid* kids, const double* f1,
-                                                                VLast* lasts, VBatch* batches) {
+__global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
+    VerifyArgs a, int stage, const VNode* nodes, const VKid* kids, const double* f1, VOpen* open,
+    double* f2, VLast* lasts, VBatch* batches) {
   __shared__ VWalk w;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wgs = a.walk_wgs;
   const int c = blockIdx.x % wgs, req = blockIdx.x / wgs;
+  VOpen* mine_open = open + (int64_t)req * kVStages;
+  double* mine_f2 = f2 + (int64_t)req * kVStages * wgs;
+  if constexpr (DRAWN) {
+    if (stage > 0 && mine_open[stage - 1].node < 0) {
+      if (c == 0 && tid == 0) mine_open[stage].node = -1;
+      return;
+    }
+    // (what this launch leaves open is known to the next one)
+    if (c == 0 && tid == 0) mine_open[stage] = VOpen{-1, 0};
+  }
   int64_t first;
   int n;
   if (!request(a, req, c == 0, first, n)) {
     if (c == 0 && tid == 0) lasts[req].node = -1;
     return;
   }
-  double f = __builtin_nan("");
   if (tid < n) {
-    const VNode v = w.node[tid] = nodes[first + tid];
+    w.node[tid] = nodes[first + tid];
     if (tid > 0) {
       w.p[tid] = kids[first + tid].p;  // (not set, and not used, without a parent)
       w.q[tid] = kids[first + tid].q;
@@ -925,17 +1013,33 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(VerifyArgs a, co
     w.lam[tid] = 0.0;
     w.mass[tid] = 1.0;
     w.tries[tid] = 0;
-    if constexpr (DRAWN) {
-      f = 0.0;  // (set where the first of several children is rejected)
-      if (v.flags & kVSummed)
-        for (int s = 0; s < a.segments; ++s) f += f1[(first + tid) * a.segments + s];
-    }
   }
   load_draft<GREEDY>(a, w, first, n);
   __syncthreads();
-  if (tid < n) try_children<DRAWN, GREEDY>(w, tid, n, f);
+  list_children(w, n);
+  if (tid < n)
+    try_children<DRAWN, GREEDY>(w, tid, n, [&](int j) {
+      return j == 1 ? sum_parts(f1 + (first + tid) * a.segments, a.segments) : __builtin_nan("");
+    });
   __syncthreads();
-  follow<T, DRAWN, GREEDY, kVThreads>(a, w, first, n);
+  const bool ends = follow<T, DRAWN, GREEDY, kVThreads>(
+      a, w, first, n,
+      [&](int v, int j) {
+        for (int s = 0; s < stage; ++s)
+          if (mine_open[s].node == v && mine_open[s].j == j)
+            return sum_parts(mine_f2 + s * wgs, wgs) / w.node[v].s;
+        return __builtin_nan("");
+      },
+      [&](int v, int j, const VRow& r) {
+        if (stage + 1 >= kVStages) return false;
+        const double f = residual_sum<T, kVThreads>(a, r, c, wgs, batches_of(a.vocab), w.sh);
+        if (tid == 0) {
+          mine_f2[stage * wgs + c] = f;
+          if (c == 0) mine_open[stage] = VOpen{v, j};
+        }
+        return true;
+      });
+  if (!ends) return;
   const VNode& nd = w.node[w.v];
   VRow r;
   if (!last_row<T, DRAWN, GREEDY>(a, w, req, first, n, nd, c == 0, r)) {
@@ -954,7 +1058,7 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(VerifyArgs a, co
   if (c == 0 && tid == 0) lasts[req] = VLast{nd.ls1, r.m, r.mq, r.khi, r.klo, w.v, nd.flags};
 }
 
-// A workgroup per request, every wavefront of which finds the batch.
+// A wavefront per request.
 template <typename T, bool DRAWN, bool GREEDY>
 __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a, const VLast* lasts,
                                                          const VBatch* batches) {
@@ -1039,6 +1143,7 @@ __global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a
     k += s_wave[x];
   }
   if (in) inner[rank] = (int16_t)tid;
+  list_children(w, n);
   __syncthreads();
   for (int e = wave; e < k; e += NW) {
     const VPart* mine = parts + (first + inner[e]) * (DRAWN ? 2 : 1) * a.segments;
@@ -1062,9 +1167,11 @@ __global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a
     w.tries[tid] = 0;
   }
   __syncthreads();
-  if (tid < n) try_children<DRAWN, GREEDY>(w, tid, n, __builtin_nan(""));
+  if (tid < n) try_children<DRAWN, GREEDY>(w, tid, n, [](int) { return __builtin_nan(""); });
   __syncthreads();
-  follow<T, DRAWN, GREEDY, kVRestThreads>(a, w, first, n);
+  follow<T, DRAWN, GREEDY, kVRestThreads>(
+      a, w, first, n, [](int, int) { return __builtin_nan(""); },
+      [](int, int, const VRow&) { return false; });
   const VNode& nd = w.node[w.v];
   VRow r;
   if (!last_row<T, DRAWN, GREEDY>(a, w, req, first, n, nd, true, r)) return;
@@ -1096,7 +1203,7 @@ __global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a
 struct Layout {
   bool rest;  // short rows: one launch behind the stats
   int32_t segments, seg_len, walk_wgs;
-  int64_t parts, nodes, kids, f1, lasts, batches, bytes;
+  int64_t parts, nodes, kids, f1, open, f2, lasts, batches, bytes;
 };
 
 Layout layout(int32_t batch, int64_t total, int32_t vocab, bool drawn) {
@@ -1123,6 +1230,8 @@ Layout layout(int32_t batch, int64_t total, int32_t vocab, bool drawn) {
     l.nodes = take(total * (int64_t)sizeof(VNode));
     l.kids = take(total * (int64_t)sizeof(VKid));
     l.f1 = take(drawn ? total * l.segments * 8 : 0);
+    l.open = take(drawn ? (int64_t)batch * kVStages * (int64_t)sizeof(VOpen) : 0);
+    l.f2 = take(drawn ? (int64_t)batch * kVStages * l.walk_wgs * 8 : 0);
     l.lasts = take(batch * (int64_t)sizeof(VLast));
     l.batches = take(batch * nb * (int64_t)sizeof(VBatch));
   }
@@ -1146,15 +1255,18 @@ hipError_t run(const VerifyArgs& a, const Layout& l, char* ws, hipStream_t s) {
   VNode* nodes = reinterpret_cast<VNode*>(ws + l.nodes);
   VKid* kids = reinterpret_cast<VKid*>(ws + l.kids);
   double* f1 = reinterpret_cast<double*>(ws + l.f1);
+  VOpen* open = reinterpret_cast<VOpen*>(ws + l.open);
+  double* f2 = reinterpret_cast<double*>(ws + l.f2);
   VLast* lasts = reinterpret_cast<VLast*>(ws + l.lasts);
   VBatch* batches = reinterpret_cast<VBatch*>(ws + l.batches);
   if (rows > 0)
     hipLaunchKernelGGL((verify_join_kernel<T, DRAWN, GREEDY>),
                        dim3((uint32_t)(a.total * (DRAWN ? l.segments : 1))), block, 0, s, a, parts,
                        nodes, kids, f1);
-  hipLaunchKernelGGL((verify_walk_kernel<T, DRAWN, GREEDY>),
-                     dim3((uint32_t)((int64_t)a.batch * l.walk_wgs)), block, 0, s, a, nodes, kids,
-                     f1, lasts, batches);
+  for (int stage = 0; stage < (DRAWN ? kVStages : 1); ++stage)
+    hipLaunchKernelGGL((verify_walk_kernel<T, DRAWN, GREEDY>),
+                       dim3((uint32_t)((int64_t)a.batch * l.walk_wgs)), block, 0, s, a, stage,
+                       nodes, kids, f1, open, f2, lasts, batches);
   hipLaunchKernelGGL((verify_pick_kernel<T, DRAWN, GREEDY>), dim3((uint32_t)a.batch), dim3(64), 0, s,
                      a, lasts, batches);
   return hipGetLastError();
