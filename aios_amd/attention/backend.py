@@ -20,6 +20,10 @@ plans are those of aios_attn_plan8, made where the context's cache is such a
 pool (or ``kv_bits=8`` is given), and forward and forward_rope follow the
 pool they are given.
 
+A prefill batch with ``Batch.tree_parents`` is one of trees of drafted tokens:
+its plan is that of aios_attn_plan_tree, and the kernels of trees take the place
+of the prefill's behind the same append.
+
 There is one code path for every supported head dim (64, 96, 128), so the
 reference's torch-SDPA fallback for head_dim 96 (flashinfer.py:19-24,
 328-372) has no counterpart here.
@@ -72,6 +76,8 @@ class Mi355xAttentionMetadata(BaseAttentionMetadata):
     shared_prefix_len: int
     host_staging: torch.Tensor
     initialized: bool = True
+    # a prefill of trees of drafts: what each new token sees of its request's
+    tree_masks: torch.Tensor | None = None
 
     def get_last_indices(self, bs: int) -> torch.Tensor:
         return self.cu_seqlens_q_gpu[1 : 1 + bs].to(torch.long) - 1
@@ -273,26 +279,32 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         total_kv = int(cu_k[bs]) if bs else 0
 
         shared = int(getattr(batch, "shared_prefix_len", 0)) if batch.is_decode else 0
-        plan = _lib.AttnPlan()
-        make, name = _make_plan(_kv_bits(ctx.kv_cache))
-        _lib.check(
-            make(
-                _lib.PHASE_DECODE if batch.is_decode else _lib.PHASE_PREFILL,
-                cu_q.data_ptr(),
-                cu_k.data_ptr(),
-                bs,
-                self.num_heads,
-                self.num_kv_heads,
-                self.head_dim,
-                1,
-                shared,
-                self.workspace_size,
-                self.prefix_chunk_len,
-                self.suffix_split_len,
-                plan,
-            ),
-            name,
-        )
+        parents = getattr(batch, "tree_parents", None) if batch.is_prefill else None
+        masks = None
+        if parents is not None:
+            plan, masks = self._plan_trees(parents, seqlens_q, cu_q, cu_k, cu_q_gpu,
+                                           _kv_bits(ctx.kv_cache))
+        else:
+            plan = _lib.AttnPlan()
+            make, name = _make_plan(_kv_bits(ctx.kv_cache))
+            _lib.check(
+                make(
+                    _lib.PHASE_DECODE if batch.is_decode else _lib.PHASE_PREFILL,
+                    cu_q.data_ptr(),
+                    cu_k.data_ptr(),
+                    bs,
+                    self.num_heads,
+                    self.num_kv_heads,
+                    self.head_dim,
+                    1,
+                    shared,
+                    self.workspace_size,
+                    self.prefix_chunk_len,
+                    self.suffix_split_len,
+                    plan,
+                ),
+                name,
+            )
 
         indices = torch.empty(total_kv, dtype=torch.int32, device=device)
         if total_kv:
@@ -328,11 +340,26 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             plan=plan,
             shared_prefix_len=shared,
             host_staging=host,
+            tree_masks=masks,
         )
         if plan.ws_bytes and batch.is_decode:
             self._get_workspace(device)
         batch.attn_metadata = metadata
         return metadata
+
+    def _plan_trees(self, parents, lens, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                    cu_q_gpu: torch.Tensor, kv_bits: int):
+        """(plan, masks) of a prefill batch of trees (Batch.tree_parents)."""
+        if [len(p) for p in parents] != lens:
+            raise ValueError("tree_parents must name a parent for every new token of each request")
+        for p in parents:
+            if any(not -1 <= x < i for i, x in enumerate(p)):
+                raise ValueError("a node's parent is an earlier one of its request, or -1")
+        plan = paged.plan("tree", cu_q, cu_k, self.num_heads, self.num_kv_heads, self.head_dim,
+                          workspace_bytes=self.workspace_size, kv_bits=kv_bits)
+        flat = torch.tensor([x for p in parents for x in p], dtype=torch.int32)
+        masks, _ = paged.tree_masks(flat.to(cu_q_gpu.device), cu_q_gpu, max(1, plan.max_q_len))
+        return plan, masks
 
     def prepare_static_decode(self, row_ids: torch.Tensor, max_kv_len: int, shared_prefix_len: int,
                               page_table: torch.Tensor,
@@ -571,6 +598,11 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
                           scales: torch.Tensor, batch: Batch) -> torch.Tensor:
         """prefill_appended over one layer of a pool in 8 bits."""
         metadata = batch.attn_metadata
+        if metadata.tree_masks is not None:
+            out = paged.tree_attention8(metadata.plan, q, k8, v8, scales, metadata.indices,
+                                        metadata.cu_seqlens_q_gpu, metadata.cu_seqlens_k_gpu,
+                                        metadata.tree_masks, sm_scale=self.sm_scale)
+            return out.reshape(q.size(0), -1)
         out = paged.prefill8(metadata.plan, q, k8, v8, scales, metadata.indices,
                              metadata.cu_seqlens_q_gpu, metadata.cu_seqlens_k_gpu,
                              sm_scale=self.sm_scale)
@@ -587,6 +619,11 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         """The prefill of a batch whose K/V rows are in their pages of one
         layer's caches (layer_kv)."""
         metadata = batch.attn_metadata
+        if metadata.tree_masks is not None:
+            out = paged.tree_attention(metadata.plan, q, k_cache, v_cache, metadata.indices,
+                                       metadata.cu_seqlens_q_gpu, metadata.cu_seqlens_k_gpu,
+                                       metadata.tree_masks, sm_scale=self.sm_scale)
+            return out.reshape(q.size(0), -1)
         out = paged.prefill(metadata.plan, q, k_cache, v_cache, metadata.indices,
                             metadata.cu_seqlens_q_gpu, metadata.cu_seqlens_k_gpu,
                             sm_scale=self.sm_scale)

@@ -12,6 +12,10 @@ that guarantee what they state (the CandidateGroup engine here):
   is that row's last page, ``page_table[row, device_len - 1]`` (as in
   ime.py:1228-1229), so the backend may append the new K/V inside the decode
   launch instead of running ``store_kv`` first (flashinfer.py:389).
+
+A third, ``Batch.tree_parents``, makes a prefill batch one of trees of drafted
+tokens: each new token attends to the cached ones, itself and the new tokens it
+continues.
 """
 from __future__ import annotations
 
@@ -93,6 +97,10 @@ class Batch:
     # The rows' embeddings when the caller has gathered them already (a
     # captured CandidateGroup step does it with its step preparation).
     input_embeds: Optional[torch.Tensor] = None
+    # A prefill of trees of drafts: for every request the parent of each new
+    # token among its new tokens (an earlier one, or -1: it sees the cached
+    # tokens and itself).  The caller sets positions to cached_len + depth.
+    tree_parents: Optional[List[List[int]]] = None
 
     @property
     def is_prefill(self) -> bool:

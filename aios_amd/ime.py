@@ -25,7 +25,9 @@ candidate i starts from the i-th most likely first token and then decodes
 greedily (aios_greedy_select).  Either way each token's raw log-prob is
 kept and candidates are ranked by average raw log-prob (the reference's
 base score before text penalties, :1109-1115).  ``CandidateGroupEngine.score``
-ranks continuations the caller brings by the same log-probs.  Text governance and
+ranks continuations the caller brings by the same log-probs, and
+``complete_drafted`` decodes one candidate with drafted tokens that a caller
+proposes, several tokens a pass.  Text governance and
 refill rounds are not restated (no tokenizer ships with the synthetic
 models).
 """
@@ -43,7 +45,9 @@ from aios_amd import _lib
 from aios_amd.config import ModelConfig
 from aios_amd.core import (Batch, Context, Req, SamplingParams, captured, reset_global_ctx,
                            set_global_ctx)
-from aios_amd.sample import MAX_TOP_LOGPROBS, sample_step, stateless_uniforms, token_logprobs
+from aios_amd.drafts import DraftTree
+from aios_amd.sample import (MAX_TOP_LOGPROBS, sample_step, stateless_uniforms, token_logprobs,
+                             verify_drafts)
 from aios_amd.kvcache import MHAKVCache, MHAKVCache8
 from aios_amd.paged import greedy_select
 from aios_amd.minimind_ime import build_causal_lm
@@ -234,6 +238,20 @@ class ScoredContinuation:
     @property
     def average_logprob(self) -> float:
         return sum(self.logprobs) / len(self.logprobs)
+
+
+@dataclass(frozen=True)
+class DraftedCompletion:
+    """One candidate decoded with drafts: the candidate, the forward passes over
+    drafts that it took, and how many drafts were checked and accepted in
+    them."""
+
+    candidate: Candidate
+    passes: int
+    drafted: int
+    accepted: int
+    reused_prefix_tokens: int
+    cancelled: bool
 
 
 def select_top(candidates, k: int) -> tuple[Candidate, ...]:
@@ -536,6 +554,198 @@ class CandidateGroupEngine:
                 c, tuple(lp[r] for r in rows), tuple(ent[r] for r in rows),
                 tuple(tuple(zip(ids[r], alt[r])) for r in rows) if top else ()))
         return out
+
+    # -- drafts ------------------------------------------------------------------
+    @torch.inference_mode()
+    def complete_drafted(self, token_ids, drafter, config: CandidateGroupConfig | None = None,
+                         cancellation: CancellationToken | None = None) -> DraftedCompletion:
+        """One candidate behind the prefix ``token_ids``, with drafts: each
+        forward pass checks the tree that ``drafter(context, room)`` proposes
+        (aios_amd.drafts.DraftTree or None; ``context`` the tokens so far,
+        ``room`` how many more may come) and adds the accepted drafts and one
+        token of the model's own.
+
+        Drafts without logits are accepted where they are the token the
+        candidate would take itself: the most likely one (greedy), or the one
+        that its uniform stream draws; the tokens are then those of
+        :meth:`complete`'s candidate 0, but for the rounding of other launches.
+        Drafts with logits (drawn from them at the sampling temperature) go
+        through aios_amd.sample.verify_drafts, which keeps the candidate's
+        distribution; that needs sampling without top_k, top_p and min_new_tokens.  The drafter
+        runs while the engine is locked: it must not call the engine.  Of
+        ``config``, max_new_tokens, eos_token_id, sampling, seed, min_new_tokens
+        and blocked_token_ids count."""
+        config = config or CandidateGroupConfig()
+        cancellation = cancellation or self.new_generation()
+        config.validate()
+        prefix = [int(t) for t in token_ids]
+        rt = self.rt
+        if not prefix:
+            raise ValueError("prefix produced no input tokens")
+        vocab = rt.model.w["embed"].shape[0]
+        if any(not 0 <= t < vocab for t in prefix):
+            raise ValueError("token id outside the vocabulary")
+        if len(prefix) + config.max_new_tokens > min(rt.config.max_position_embeddings,
+                                                     rt.max_context):
+            raise ValueError("prefix + output exceeds context limit")
+        if len(prefix) + config.max_new_tokens > rt.num_pages:
+            raise ValueError(
+                f"CandidateGroup KV budget is too small: need up to "
+                f"{len(prefix) + config.max_new_tokens} pages, configured {rt.num_pages}")
+        with self._run_lock:
+            if cancellation.cancelled:
+                return DraftedCompletion(Candidate((), float("-inf"), "cancelled"), 0, 0, 0, 0, True)
+            rt.ctx.page_table = rt.page_table
+            logits, _, reused = self._prepare_prefix(prefix, rt.page_table)
+            return self._drafted(prefix, logits, reused, drafter, config, cancellation)
+
+    def _drafted(self, prefix, logits, reused: int, drafter, config, cancellation):
+        rt = self.rt
+        first = self._draft_picks(logits[:1], [0], config)
+        out, lps = [int(first[0])], [float(first[1])]
+        kept: list[torch.Tensor] = []  # the pages of the accepted tokens that were fed
+        passes = drafted = accepted = 0
+        cancelled = False
+        try:
+            while len(out) < config.max_new_tokens and out[-1] != config.eos_token_id:
+                if cancellation.cancelled:  # observed between passes
+                    cancelled = True
+                    break
+                context = prefix + out
+                room = config.max_new_tokens - len(out)
+                tree = self._trim(drafter(list(context), room), room, len(context), config)
+                ids, chosen, more, pages = self._draft_pass(context, tree, len(out), config)
+                kept.append(pages)
+                passes += 1
+                drafted += len(tree.tokens)
+                accepted += chosen
+                out += ids
+                lps += more
+        finally:
+            if kept:
+                rt.cache_manager._free(torch.cat(kept))
+        stop = "cancelled" if cancelled else "max_new_tokens"
+        if config.eos_token_id in out:
+            at = out.index(config.eos_token_id)
+            out, lps, stop = out[:at], lps[:at], "eos"
+        out, lps = out[: config.max_new_tokens], lps[: config.max_new_tokens]
+        avg = sum(lps) / len(lps) if lps else float("-inf")
+        return DraftedCompletion(Candidate(tuple(out), avg, stop), passes, drafted, accepted, reused,
+                                 cancelled)
+
+    def _trim(self, tree, room: int, length: int, config) -> DraftTree:
+        """The drafts that can be checked: not deeper than the tokens that may
+        still come, as many as the context and the free pages hold (drafts
+        behind a dropped one go with it; an index keeps its place in the
+        order)."""
+        rt = self.rt
+        if tree is None:
+            return DraftTree((), ())
+        tree.validate(rt.model.w["embed"].shape[0])
+        if tree.logits is not None:
+            sp = config.sampling
+            if sp is not None and not sp.is_greedy and (
+                    sp.top_k > 0 or sp.top_p < 1.0 or config.min_new_tokens > 0):
+                raise ValueError("drafts with logits need sampling without top_k, top_p and "
+                                 "min_new_tokens")
+        limit = min(rt.cache_manager.available_size, rt.page_table.shape[1] - length + 1) - 1
+        keep: dict[int, int] = {}
+        for i, (p, d) in enumerate(zip(tree.parents, tree.depths())):
+            if d < room and len(keep) < limit and (p < 0 or p in keep):
+                keep[i] = len(keep)
+        if len(keep) == len(tree.tokens):
+            return tree
+        rows = None
+        if tree.logits is not None:
+            # (a place behind which not all drafts are kept draws anew: the ones
+            # that are left are still the first of their draws)
+            rows = tree.logits[torch.tensor([0, *(i + 1 for i in keep)],
+                                            device=tree.logits.device)]
+        return DraftTree([tree.tokens[i] for i in keep],
+                         [keep[tree.parents[i]] if tree.parents[i] >= 0 else -1 for i in keep], rows)
+
+    def _draft_picks(self, logits: torch.Tensor, steps: list[int], config):
+        """(tokens, raw log-probs) that the candidate takes itself, row r at its
+        token index steps[r]."""
+        sp = config.sampling
+        if sp is None:
+            return greedy_select(logits)
+        dev = self.rt.device
+        col = torch.tensor(steps, device=dev)
+        uni = stateless_uniforms([config.seed], max(steps) + 1, dev)[0, col].unsqueeze(1)
+        blocked = config.blocked_ids()
+        by_row = None
+        if blocked and min(steps) < config.min_new_tokens:
+            ids = torch.tensor(blocked, dtype=torch.int64, device=dev)
+            early = col[:, None] < config.min_new_tokens
+            by_row = torch.where(early, ids[None], torch.full_like(ids, -1)[None]).contiguous()
+        return sample_step(logits, sp, uni.contiguous(),
+                           torch.zeros(1, dtype=torch.int64, device=dev), forbidden_by_row=by_row)
+
+    def _draft_pass(self, context, tree: DraftTree, n_out: int, config):
+        """Feeds the last token of the context and the drafts behind it; returns
+        (added tokens, accepted drafts, log-probs, the pages of the fed tokens
+        that stay)."""
+        rt, dev = self.rt, self.rt.device
+        cached = len(context) - 1
+        tokens = [context[-1], *(int(t) for t in tree.tokens)]
+        parents = [-1, *(p + 1 for p in tree.parents)]
+        depths = [0, *tree.depths()]
+        n = len(tokens)
+        pages = rt.cache_manager.allocate(n)
+        stays = [0]
+        try:
+            rt.page_table[0, cached : cached + n] = pages
+            req = Req(input_ids=torch.empty(cached + n, dtype=torch.long), cached_len=cached,
+                      output_len=1, uid=0, sampling_params=SamplingParams(max_tokens=1),
+                      table_idx=0)
+            batch = Batch(reqs=[req], phase="prefill")
+            batch.input_ids = torch.tensor(tokens, dtype=torch.long, device=dev)
+            batch.positions = torch.tensor([cached + d for d in depths], dtype=torch.int32,
+                                           device=dev)
+            batch.out_loc = pages
+            batch.return_all_logits = True
+            batch.tree_parents = [parents]
+            rt.model.attn_backend.prepare_metadata(batch)
+            with rt.ctx.forward_batch(batch):
+                logits = rt.model.forward()
+            sp = config.sampling
+            if sp is None or sp.is_greedy or tree.logits is None:
+                picks, raw = self._draft_picks(logits, [n_out + d for d in depths], config)
+                picks, raw = picks.tolist(), raw.tolist()
+                v, path, lps = 0, [], [raw[0]]
+                while True:
+                    v = next((i for i in range(v + 1, n) if parents[i] == v
+                              and tokens[i] == picks[v]), None)
+                    if v is None:
+                        break
+                    path.append(v)
+                    lps.append(raw[v])
+                added = [tokens[i] for i in path] + [picks[path[-1] if path else 0]]
+            else:
+                par = torch.tensor(parents, dtype=torch.int32, device=dev)
+                # (numbers of their own: not the stream that picks tokens)
+                uni = stateless_uniforms([config.seed + 7_919 * (n_out + 1)], n, dev)[0]
+                r = verify_drafts(logits, batch.input_ids, par,
+                                  torch.tensor([0, n], dtype=torch.int32, device=dev), uni,
+                                  draft_logits=tree.logits, temperature=sp.temperature)
+                took = r.accepted.tolist()
+                path = [i for i in range(1, n) if took[i]]
+                lp = r.logprobs.tolist()
+                lps = [lp[i] for i in path] + [lp[0]]
+                added = [tokens[i] for i in path] + [int(r.next_tokens[0])]
+            stays += path
+        except BaseException:
+            rt.cache_manager._free(pages)
+            raise
+        # a page holds one token, rotated to its depth: the accepted ones only
+        # change places in the table
+        keep = pages[torch.tensor(stays, device=dev)]
+        rt.page_table[0, cached : cached + len(stays)] = keep
+        gone = [i for i in range(n) if i not in set(stays)]
+        if gone:
+            rt.cache_manager._free(pages[torch.tensor(gone, device=dev)])
+        return added, len(path), lps, keep
 
     # -- prefix ------------------------------------------------------------------
     def _prepare_prefix(self, token_ids, page_table):

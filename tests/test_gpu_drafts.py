@@ -1,0 +1,257 @@
+"""A model over trees of drafts (append with rotation, tree attention, verification)
+and the engine that decodes with them, over both pools.
+
+Logits of every node are held to the float32 oracle on the tokens of its path, with
+the bf16 model's 0.125 (over the 8-bit pool on the K and V that the pool holds);
+log-probs and their averages to twice that.
+"""
+from __future__ import annotations
+
+from dataclasses import replace
+
+import pytest
+import torch
+
+from aios_amd.config import MINIMIND_ATTNRES_0P214B, MINIMIND_IME_0P1B, QWEN3_0P6B
+from aios_amd.core import Batch, Req, SamplingParams, reset_global_ctx
+from aios_amd.drafts import DraftTree, PhraseDrafter, draft_tree
+from aios_amd.ime import CandidateGroupConfig, CandidateGroupEngine, CandidateGroupRuntime
+from aios_amd.qwen3 import init_weights, weights_to
+from aios_amd.sample import sample_step, stateless_uniforms
+from oracle.model import OracleModel
+from tests.test_gpu_kv8 import _values
+from tests.test_gpu_kv8_engine import PoolOracle
+
+pytestmark = pytest.mark.gpu
+LOGIT_TOL = 0.125
+QWEN3 = replace(QWEN3_0P6B, num_layers=3, vocab_size=8192)
+IME = MINIMIND_IME_0P1B.with_layers(3)
+CONFIGS = pytest.mark.parametrize("config", [IME, QWEN3, MINIMIND_ATTNRES_0P214B],
+                                  ids=["minimind-ime-h64-g3", "qwen3-0.6b-h128-g2",
+                                       "minimind-attnres"])
+BITS = pytest.mark.parametrize("kv_bits", [16, 8])
+
+
+def teardown_function(_):
+    reset_global_ctx()
+    torch.cuda.empty_cache()
+
+
+def _engine(config, kv_bits, seed=3, num_pages=512):
+    w = init_weights(config, seed, "cpu")
+    rt = CandidateGroupRuntime(config, weights_to(w, "cuda"), "cuda", num_pages=num_pages,
+                               kv_bits=kv_bits)
+    return CandidateGroupEngine(rt), w
+
+
+def _ids(config, n, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(config.vocab_size, (n,), generator=g).tolist()
+
+
+def _oracle(config, w, rt, ids, pages):
+    """The oracle's logits behind the last of ids, whose K/V rows lie in pages."""
+    if rt.kv_cache.dtype == torch.bfloat16:
+        return OracleModel(config, w).logits(torch.tensor(ids)[None], 0)[0, -1]
+    om = PoolOracle(config, w)
+    om.kv = []
+    for i in range(config.num_layers):
+        k, v = _values(*rt.kv_cache.layer(i))
+        om.kv.append((torch.from_numpy(k[pages]).float(), torch.from_numpy(v[pages]).float()))
+    return om.logits(torch.tensor(ids)[None], 0)[0, -1]
+
+
+@CONFIGS
+@BITS
+def test_a_batch_of_trees_gives_every_path_s_logits(config, kv_bits):
+    eng, w = _engine(config, kv_bits)
+    rt = eng.rt
+    prefixes = [_ids(config, 41, 1), _ids(config, 7, 2)]
+    parents = [[-1, 0, 1, 0, 3, 3, -1], [-1, 0, 0]]
+    news = [_ids(config, len(p), 5 + i) for i, p in enumerate(parents)]
+    held = []
+    for r, ids in enumerate(prefixes):  # the prefixes, one after the other
+        pages = rt.cache_manager.allocate(len(ids))
+        rt.page_table[r, : len(ids)] = pages
+        b = Batch(reqs=[Req(input_ids=torch.empty(len(ids), dtype=torch.long), cached_len=0,
+                            output_len=1, uid=r, sampling_params=SamplingParams(), table_idx=r)],
+                  phase="prefill")
+        b.input_ids = torch.tensor(ids, device="cuda")
+        b.positions = torch.arange(len(ids), dtype=torch.int32, device="cuda")
+        b.out_loc = pages
+        with torch.inference_mode():
+            rt.model.attn_backend.prepare_metadata(b)
+            with rt.ctx.forward_batch(b):
+                rt.model.forward()
+        held.append(pages)
+    own = rt.cache_manager.allocate(10)
+    depths, paths = [], []
+    for p in parents:
+        for i, x in enumerate(p):
+            path = [i]
+            while p[path[0]] >= 0:
+                path.insert(0, p[path[0]])
+            paths.append(path)
+            depths.append(len(path) - 1)
+    cached = [41] * 7 + [7] * 3
+    rt.page_table[0, 41:48] = own[:7]
+    rt.page_table[1, 7:10] = own[7:]
+    b = Batch(reqs=[Req(input_ids=torch.empty(c + len(n), dtype=torch.long), cached_len=c,
+                        output_len=1, uid=i, sampling_params=SamplingParams(), table_idx=i)
+                    for i, (c, n) in enumerate(zip((41, 7), news))], phase="prefill")
+    b.input_ids = torch.tensor(sum(news, []), device="cuda")
+    b.positions = torch.tensor([c + d for c, d in zip(cached, depths)], dtype=torch.int32,
+                               device="cuda")
+    b.out_loc = own
+    b.return_all_logits = True
+    b.tree_parents = parents
+    with torch.inference_mode():
+        rt.model.attn_backend.prepare_metadata(b)
+        with rt.ctx.forward_batch(b):
+            logits = rt.model.forward()
+    assert logits.shape[0] == 10
+    for row, path in enumerate(paths):
+        r = 0 if row < 7 else 1
+        base = 0 if r == 0 else 7
+        ids = prefixes[r] + [news[r][i] for i in path]
+        pages = torch.cat((held[r], own[base + torch.tensor(path, device="cuda")])).long().cpu()
+        want = _oracle(config, w, rt, ids, pages)
+        assert (logits[row].float().cpu() - want).abs().max() <= LOGIT_TOL
+
+
+@CONFIGS
+@BITS
+def test_greedy_tokens_with_drafts(config, kv_bits):
+    eng, w = _engine(config, kv_bits)
+    rt = eng.rt
+    prefix = _ids(config, 33, 9)
+    cfg = CandidateGroupConfig(max_new_tokens=9)
+    plain = eng.complete_drafted(prefix, lambda context, room: None, cfg)
+    assert rt.cache_manager.available_size == rt.num_pages - len(prefix)
+    tokens = list(plain.candidate.token_ids)
+    assert len(tokens) == 9 and plain.passes == 8 and plain.drafted == 0
+    assert plain.candidate.stop_reason == "max_new_tokens"
+    # greedy under the oracle, up to both logits' errors, and its log-probs
+    ref = OracleModel(config, w).logits(torch.tensor(prefix + tokens[:-1])[None], 0)[0, 32:]
+    if kv_bits == 16:
+        gap = ref.max(-1).values - ref.gather(1, torch.tensor(tokens)[:, None])[:, 0]
+        assert gap.max().item() <= 2 * LOGIT_TOL
+        lp = ref.log_softmax(-1).gather(1, torch.tensor(tokens)[:, None]).mean().item()
+        assert abs(lp - plain.candidate.average_logprob) <= 2 * LOGIT_TOL
+    # the same tokens drafted, with others beside them: fewer passes
+    wrong = _ids(config, 8, 77)
+
+    def drafter(context, room):
+        at = len(context) - len(prefix)
+        assert room == 9 - at
+        return draft_tree([wrong[:3], tokens[at : at + 4] + wrong[:2], tokens[at : at + 1] + wrong])
+
+    r = eng.complete_drafted(prefix, drafter, cfg)
+    assert list(r.candidate.token_ids) == tokens and r.reused_prefix_tokens == len(prefix)
+    assert r.passes == 2 and r.accepted == 6 and r.drafted > 6  # 1 + (4 + 1) + (2 + 1)
+    assert abs(r.candidate.average_logprob - plain.candidate.average_logprob) <= 2 * LOGIT_TOL
+    assert rt.cache_manager.available_size == rt.num_pages - len(prefix)
+    r = eng.complete_drafted(prefix, PhraseDrafter([prefix[-3:] + tokens, wrong]), cfg)
+    assert list(r.candidate.token_ids) == tokens and r.passes == 1
+    # an end of sequence inside the accepted drafts
+    cut = next(i for i in range(1, 9) if tokens[i] not in tokens[:i])
+    r = eng.complete_drafted(prefix, drafter, replace(cfg, eos_token_id=tokens[cut]))
+    assert list(r.candidate.token_ids) == tokens[:cut] and r.candidate.stop_reason == "eos"
+    assert rt.cache_manager.available_size == rt.num_pages - len(prefix)
+
+
+@BITS
+def test_sampled_tokens_do_not_depend_on_the_drafts(kv_bits):
+    """Drafts without logits: the candidate's own draws, whatever is drafted.
+
+    The forward runs as ever, and then the logits of position p are row p of a
+    table, so that no launch's rounding enters: a draw depends on the order of the
+    probabilities, and random weights leave neighbours closer than a bf16 step, so
+    the tokens of two launches' own logits need not be the same."""
+    eng, _ = _engine(IME, kv_bits)
+    rt = eng.rt
+    prefix = _ids(IME, 20, 4)
+    cfg = CandidateGroupConfig(max_new_tokens=8, min_new_tokens=3, blocked_token_ids=(5, 9),
+                               sampling=SamplingParams(temperature=0.7, top_k=50, top_p=0.9))
+    table = 4 * torch.randn(28, IME.vocab_size, generator=torch.Generator().manual_seed(0))
+    table[:, [5, 9]] = 30.0  # what the ban keeps out, and would be drawn without it
+    table = table.to("cuda", torch.bfloat16)
+    forward = rt.model.forward
+
+    def with_table():
+        b = rt.ctx.batch
+        rows = forward().shape[0]
+        at = b.positions if rows == b.positions.numel() else b.positions[-1:]
+        return table[at.long()]
+
+    rt.model.forward = with_table
+    uni = stateless_uniforms([cfg.seed], 8, "cuda")
+    ban = torch.tensor(cfg.blocked_ids(), dtype=torch.int32, device="cuda")
+    want, lps = [], []
+    for t in range(8):
+        pick, lp = sample_step(table[19 + t :][:1], cfg.sampling, uni,
+                               torch.tensor(t, device="cuda"), ban, 3)
+        want.append(int(pick))
+        lps.append(float(lp))
+    assert not {5, 9} & set(want[:3]) and {5, 9} & set(want[3:])
+    for width in (0, 1, 2, 8):
+        r = eng.complete_drafted(prefix, lambda context, room: draft_tree(
+            [want[len(context) - 20 :][:width], _ids(IME, 3, len(context))]), cfg)
+        assert list(r.candidate.token_ids) == want
+        assert abs(r.candidate.average_logprob - sum(lps) / 8) < 1e-5
+        assert r.passes == {0: 7, 1: 4, 2: 3, 8: 1}[width]
+    assert rt.cache_manager.available_size == rt.num_pages - 20
+
+
+@BITS
+def test_drawn_drafts(kv_bits):
+    """A drafter with a distribution of its own: the log-probs are the model's, all
+    pages come back, and a draft drawn from the model's own logits is accepted."""
+    eng, w = _engine(QWEN3, kv_bits)
+    rt = eng.rt
+    prefix = _ids(QWEN3, 18, 6)
+    cfg = CandidateGroupConfig(max_new_tokens=7, sampling=SamplingParams(temperature=0.9))
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def drafter(context, room):
+        rows = torch.randn(5, 8192, generator=g, device="cuda").to(torch.bfloat16)
+        t = torch.multinomial(torch.softmax(rows[:3].float() / 0.9, -1), 2, replacement=True,
+                              generator=g)
+        # two behind the context, two behind the first of them
+        return DraftTree([int(t[0, 0]), int(t[0, 1]), int(t[1, 0]), int(t[1, 1])], [-1, -1, 0, 0],
+                         rows)
+
+    r = eng.complete_drafted(prefix, drafter, cfg)
+    assert len(r.candidate.token_ids) == 7 and rt.cache_manager.available_size == rt.num_pages - 18
+    ids = list(r.candidate.token_ids)
+    ref = OracleModel(QWEN3, w).logits(torch.tensor(prefix + ids[:-1])[None], 0)[0, 17:]
+    lp = ref.log_softmax(-1).gather(1, torch.tensor(ids)[:, None]).mean().item()
+    if kv_bits == 16:
+        assert abs(lp - r.candidate.average_logprob) <= 2 * LOGIT_TOL
+    with pytest.raises(ValueError, match="without top_k"):
+        eng.complete_drafted(prefix, drafter, replace(cfg, sampling=SamplingParams(0.9, top_k=5)))
+    assert rt.cache_manager.available_size == rt.num_pages - 18
+
+
+def test_a_drafter_that_fails_leaves_no_pages_behind():
+    eng, _ = _engine(IME, 16)
+    prefix = _ids(IME, 12, 8)
+
+    def drafter(context, room):
+        if len(context) > 14:
+            raise RuntimeError("drafter")
+        return None
+
+    with pytest.raises(RuntimeError, match="drafter"):
+        eng.complete_drafted(prefix, drafter)
+    assert eng.rt.cache_manager.available_size == eng.rt.num_pages - 12
+    token = eng.new_generation()
+
+    def cancels(context, room):
+        token.cancel()
+        return None
+
+    r = eng.complete_drafted(prefix, cancels, cancellation=token)
+    assert r.cancelled and len(r.candidate.token_ids) == 2
+    assert r.candidate.stop_reason == "cancelled"
+    assert eng.rt.cache_manager.available_size == eng.rt.num_pages - 12
