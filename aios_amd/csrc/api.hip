@@ -1732,7 +1732,7 @@ static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int3
     int64_t ns = c.base + (int64_t)c.base_rows * rows / 128 + full * two +
                  (rest > cus ? two : rest > 0 ? one : 0) + (rounds > 1 ? (rounds - 1) * c.round : 0);
     if (n > 1) ns += c.join + (int64_t)c.part * n + wgs * rows * d * c.state / 100000;
-    if (best < 0 || ns < best) {
+    if (best < 0 || ns < best - best / 32) {
       best = ns;
       p->prefix_chunk_len = per * 32;
       p->num_parts = n;
