@@ -615,6 +615,7 @@ __global__ __launch_bounds__(kVThreads) void verify_join_kernel(VerifyArgs a, co
     if (tid == 0 && seg == 0) nodes[node] = VNode{0, 0, 0, 0.f, 0.f, 0, 0};
     return;
   }
+  if (DRAWN && seg > 0 && k == 1) return;  // (no F is asked for)
   const VPart* mine = parts + node * (DRAWN ? 2 : 1) * a.segments;
   if (wave < (DRAWN ? 2 : 1)) {
     const VPart p = join(mine + wave * a.segments, a.segments,
