@@ -1686,31 +1686,36 @@ int aios_attn_append_decode_rope8(const aios_attn_plan_t* p, const void* q, int6
 // trees of drafted tokens
 
 // How many parts the KV ranges of a batch of trees are split into (num_parts 1:
-// none).  Estimated in ns, fitted to 6,700 batches of 1 to 32 requests of 1 to 256
-// nodes behind up to 16,000 positions at head sizes 64, 96 and 128 (12q/4kv, 8q/2kv,
-// 16q/8kv, 32q/8kv), each in up to 20 numbers of parts: a workgroup's start, its
-// sub-tiles (slower with two workgroups on a unit, and past two in further
-// rounds), and for parts the combine, each part and the states' bytes.  The
-// number taken is within 1.5% of the batch's best in the mean, 21% at the 99th
-// percentile.  Parts of 1 / 2 / 4 / 8 / 16 / 32: 16 requests of 33 to 4 nodes on
-// 1,500, 12q/4kv x 64 33 / 22 / 15.9 / 15.7 / 20.0 us; one of 40 on 16,001, 32q/8kv
-// x 128, bf16 494 / 256 / 132 / 71 / 42 / 31, 8 bits 354 / 186 / 98 / 55 / 34 /
-// 28.5; four of 200 to 143 on 8,192 (bf16) 265 / 151 / 155 / 171 / 180.
+// none).  Estimated in ns, fitted to 6,700 batches (19,700 of at most 64 MFMA rows a
+// tile) of 1 to 32 requests of 1 to 256 nodes behind up to 16,000 positions at head
+// sizes 64, 96 and 128 (12q/4kv, 8q/2kv, 16q/8kv, 32q/8kv), each in up to 20 numbers
+// of parts: a workgroup's start, its sub-tiles (slower with two workgroups on a unit,
+// and past two in further rounds), and for parts the combine, each part and the
+// states' bytes.  Two numbers' estimates within 1.6% are taken as equal, and the
+// fewer parts chosen.  The choice is within 1.7% of the batch's best in the mean and
+// 19% at the 99th percentile (tiles of at most 64 rows: 1% and 13%).  Parts of 1 / 2
+// / 4 / 8 / 16 / 32: 16 requests of 33 to 4 nodes on 1,500, 12q/4kv x 64 33 / 22 /
+// 15.9 / 15.7 / 20.0 us; one of 40 on 16,001, 32q/8kv x 128, bf16 494 / 256 / 132 /
+// 71 / 42 / 31, 8 bits 354 / 186 / 98 / 55 / 34 / 28.5; four of 200 to 143 on 8,192
+// (bf16) 265 / 151 / 155 / 171 / 180.
 struct TreeCost {
-  int32_t base, base_rows;  // a workgroup, and for 128 MFMA rows of it
-  int32_t sub, sub_d;       // a sub-tile, and for 128 dims of it
-  int32_t two;              // a sub-tile with two workgroups on a unit, percent
-  int32_t round;            // a further round of workgroups
+  struct Range {  // a workgroup's range of up to kTreeShareSub sub-tiles, or more
+    int32_t base, sub, sub_d;  // besides the sub-tiles, one of them, 128 dims of one
+    int32_t two;               // with two workgroups on a unit, percent
+  } range[2];
+  int32_t start, start_rows;  // a workgroup, and for 128 MFMA rows of it
+  int32_t round;              // a further round of workgroups
   int32_t join, part, state;  // combine, a part of it, 10^5 elements of states
 };
 static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int32_t* cu_k,
                             bool bits8, int32_t cus, int64_t ws_bytes) {
   const int32_t q_tile = p->prefill_q_tile, hkv = p->num_kv_heads, d = p->head_dim;
   const int32_t rows = q_tile * p->group;
-  const TreeCost few16 = {5500, 0, 60, 750, 160, 4500, 2360, 50, 140};
-  const TreeCost few8 = {6400, 0, 106, 387, 145, 2900, 2400, 57, 166};
-  const TreeCost full16 = {3500, 3100, 397, 575, 129, 2500, 1600, 49, 107};
-  const TreeCost full8 = {4100, 3200, 267, 450, 140, 0, 1445, 40, 105};
+  const TreeCost::Range all16 = {0, 397, 575, 129}, all8 = {0, 267, 450, 140};
+  const TreeCost few16 = {{{0, 158, 600, 154}, {0, 99, 718, 158}}, 4940, 0, 3850, 2460, 47, 124};
+  const TreeCost few8 = {{{0, 165, 532, 133}, {1670, 119, 367, 140}}, 4590, 0, 1570, 2520, 54, 122};
+  const TreeCost full16 = {{all16, all16}, 3500, 3100, 2500, 1600, 49, 107};
+  const TreeCost full8 = {{all8, all8}, 4100, 3200, 0, 1445, 40, 105};
   const TreeCost c = rows <= 64 ? (bits8 ? few8 : few16) : (bits8 ? full8 : full16);
   const int32_t longest = cdiv(p->max_kv_len, 32);
   const int64_t slots = (int64_t)p->batch_size * p->num_q_tiles * hkv;
@@ -1726,13 +1731,15 @@ static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int3
       const int32_t nodes = cu_q[b + 1] - cu_q[b], kv = cu_k[b + 1] - cu_k[b];
       if (nodes > 0) wgs += (int64_t)cdiv(nodes, q_tile) * hkv * cdiv(cdiv(kv, 32), per);
     }
-    const int64_t one = per * (c.sub + (int64_t)c.sub_d * d / 128), two = one * c.two / 100;
+    const TreeCost::Range& k = c.range[per > aios::kTreeShareSub];
+    const int64_t one = k.base + per * (k.sub + (int64_t)k.sub_d * d / 128);
+    const int64_t two = one * k.two / 100;
     const int64_t full = wgs / (2 * cus), rest = wgs % (2 * cus);
     const int64_t rounds = full + (rest > 0);
-    int64_t ns = c.base + (int64_t)c.base_rows * rows / 128 + full * two +
+    int64_t ns = c.start + (int64_t)c.start_rows * rows / 128 + full * two +
                  (rest > cus ? two : rest > 0 ? one : 0) + (rounds > 1 ? (rounds - 1) * c.round : 0);
     if (n > 1) ns += c.join + (int64_t)c.part * n + wgs * rows * d * c.state / 100000;
-    if (best < 0 || ns < best - best / 32) {
+    if (best < 0 || ns < best - best / 64) {
       best = ns;
       p->prefix_chunk_len = per * 32;
       p->num_parts = n;

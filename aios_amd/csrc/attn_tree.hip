@@ -180,6 +180,7 @@ __device__ __forceinline__ _Float16* part_o(const TreeArgs& t, int64_t part, int
 }
 
 // One part of a tile's KV range per workgroup (n_parts 1: the whole range).
+static_assert(kRing <= kTreeShareSub, "a range that fits the ring is not shared");
 template <int D, int BITS>
 __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void tree_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
@@ -225,7 +226,8 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
   const int kv_end = min(kv_len, kv_begin + pp.per * kSubTok);
 
   // Wavefront -> (row tile, share of the sub-tiles).
-  const int nr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int n_sub = (kv_end - kv_begin + kSubTok - 1) / kSubTok;
+  const int nr = n_sub <= kTreeShareSub || rows > 64 ? 4 : rows <= 32 ? 1 : 2;
   const int ng = 4 / nr;
   const int rt = wave & (nr - 1);
   const int share = nr == 4 ? 0 : nr == 2 ? wave >> 1 : wave;
@@ -255,7 +257,6 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
     for (int e = tid + kEngineThreads; e < n_mask; e += kEngineThreads) smask[e] = masks[e];
   };
   const int32_t* idx = indices + kv_base;
-  const int n_sub = (kv_end - kv_begin + kSubTok - 1) / kSubTok;
   if constexpr (BITS == 16) {
     stream_kv<T, 0, true, true>(
         lds, reinterpret_cast<const uint8_t*>(a.k_cache) + (int64_t)h * D * 2,
@@ -266,40 +267,23 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
             eng.compute(lo, sb, kv0, kv_end, a.scale_log2);
         },
         rt * 32 < rows,
-        [&](auto&& wait_sub, int) {
-          if (ng > 1) wait_sub(kRing - 1);
+        [&](auto&& wait_sub, int) {  // (at most kRing sub-tiles: none shares them)
 #pragma unroll 1
-          for (int it = share; it < n_sub; it += ng) {
-            if (ng == 1) wait_sub(it);
+          for (int it = 0; it < n_sub; ++it) {
+            wait_sub(it);
             eng.compute(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
                         a.scale_log2);
           }
         });
   } else {
     S st(args.kv, h, idx, kv_begin, kv_end);
-    if (ng > 1 && st.steps() <= 2) {
-      typename S::Regs r0, r1;
-      typename S::Ids i0, i1;
-      st.ids(0, i0);
-      st.ids(1, i1);
-      st.load(0, i0, r0);
-      st.load(1, i1, r1);
-      qload();
-      st.store(lds, 0, r0);
-      st.store(lds, 1, r1);
-      lds_barrier();
-      for (int it = share; it < n_sub; it += ng)
-        eng.compute(lo, (uint32_t)(it * T::SUB_BYTES), kv_begin + it * kSubTok, kv_end,
-                    a.scale_log2);
-    } else {
-      st.template stream<1>(
-          lds, qload,
-          [&](auto sb, int kv0) {
-            if (((kv0 - kv_begin) / kSubTok & (ng - 1)) == share)
-              eng.compute(lo, decltype(sb)::value, kv0, kv_end, a.scale_log2);
-          },
-          rt * 32 < rows);
-    }
+    st.template stream<1>(
+        lds, qload,
+        [&](auto sb, int kv0) {
+          if (((kv0 - kv_begin) / kSubTok & (ng - 1)) == share)
+            eng.compute(lo, decltype(sb)::value, kv0, kv_end, a.scale_log2);
+        },
+        rt * 32 < rows);
   }
   eng.l_run = xor32_sum(eng.ls);
 

@@ -423,6 +423,12 @@ struct TreeArgs {
   _Float16* part_o;
 };
 constexpr int kTreeMaxNodes = 256;  // of a request
+// With at most 64 rows two or four wavefronts can share a part's sub-tiles, which
+// costs merging their states: 1.5 - 3 us.  Parts of up to this many are faster
+// without, in us a launch (shared / not, 32 rows): 4 sub-tiles of 64 requests in 8
+// bits x 128 10.8 / 8.9, 8 16.0 / 13.7, 12 18.4 / 16.8, 32 30.0 / 32.4; bf16 x 64, one
+// request, 4 6.3 / 6.8, 8 8.3 / 8.6, 16 11.5 / 13.0.
+constexpr int kTreeShareSub = 8;
 hipError_t launch_tree(int D, int bits, const TreeArgs& a, hipStream_t stream);
 // Masks [total][words] (32-bit words) and depths [total] of every request's nodes.
 hipError_t tree_masks(const int32_t* parents, const int32_t* cu, int32_t batch, int64_t total,
