@@ -245,6 +245,9 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
 
     # -- interface -------------------------------------------------------------
     def prepare_metadata(self, batch: Batch) -> Mi355xAttentionMetadata:
+        parents = getattr(batch, "tree_parents", None)
+        if parents is not None and not batch.is_prefill:
+            raise ValueError("trees of drafts are a prefill batch")
         ctx = get_global_ctx()
         page_table = ctx.page_table
         assert page_table.is_cuda, "the MI355X backend requires a GPU page table"
@@ -279,7 +282,6 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
         total_kv = int(cu_k[bs]) if bs else 0
 
         shared = int(getattr(batch, "shared_prefix_len", 0)) if batch.is_decode else 0
-        parents = getattr(batch, "tree_parents", None) if batch.is_prefill else None
         masks = None
         if parents is not None:
             plan, masks = self._plan_trees(parents, seqlens_q, cu_q, cu_k, cu_q_gpu,

@@ -180,6 +180,14 @@ __device__ __forceinline__ _Float16* part_o(const TreeArgs& t, int64_t part, int
 }
 
 // One part of a tile's KV range per workgroup (n_parts 1: the whole range).
+// Bound, replayed from a graph with the combine: few rows by the chain of round trips
+// (lengths, page ids, K/V) and sub-tiles, 0.65 us each at 128 dims, which is why a
+// range is cut into parts of few: 8 nodes on 24 positions, 8q/2kv x 96, 5.6 us; 17 on
+// 4,093, 16q/8kv, 12.7 in 13 parts (main 9.1, combine 3.2), 145 in one; 40 on 16,001,
+// 32q/8kv, 8 bits 32, of them 26.6 here; eight chains of 6 on 2,500 in 8 bits 18.9.
+// Full tiles by the math chain of a sub-tile (products and softmax overlap only
+// between the two wavefronts of a SIMD): four requests of 200 - 165 nodes on 8,192,
+// 32q/8kv x 128, 160 - 178 us, 600 TFLOP/s of the unmasked products.
 static_assert(kRing <= kTreeShareSub, "a range that fits the ring is not shared");
 template <int D, int BITS>
 __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void tree_kernel(
@@ -394,6 +402,9 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 // Merges the parts of each row: out = sum_j 2^(m_j - m) o_j / sum_j 2^(m_j - m) l_j,
 // m = max_j m_j.  A wavefront takes RB rows, one (row, 8-dim group) per lane; NW
 // wavefronts share a row block's parts, NB of them in flight per wavefront.
+// Bound: two round trips (states, then the sums' exchange) and the states' bytes: 3.2
+// us for 13 parts of 34 rows, 5.1 for 28 parts of 80 (16 heads and tiles), 6.5 for 2
+// parts of 116 rows in 200 tiles (13 MB of states).
 template <int D, int NW, int NB>
 __global__ __launch_bounds__(NW * 64) void tree_combine_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
@@ -525,7 +536,8 @@ hipError_t launch_d(const TreeArgs& t, hipStream_t s) {
 // Masks and depths of every request's nodes from their parents.  One workgroup
 // per request, a node per thread: with a[i] the ancestor 2^k levels up and m[i]
 // the set of the first 2^k nodes on the way up, m[i] |= m[a[i]] and a[i] =
-// a[a[i]] double k, so a chain of 256 takes eight rounds.
+// a[a[i]] double k, so a chain of 256 takes eight rounds.  Bound: a launch and those
+// rounds' barriers; 4.1 us for four trees of 200.
 __global__ __launch_bounds__(kTreeMaxNodes) void tree_masks_kernel(const int32_t* parents,
                                                                    const int32_t* cu, int64_t total,
                                                                    int32_t words, uint32_t* masks,

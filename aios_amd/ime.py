@@ -607,7 +607,7 @@ class CandidateGroupEngine:
         passes = drafted = accepted = 0
         cancelled = False
         try:
-            while len(out) < config.max_new_tokens and out[-1] != config.eos_token_id:
+            while len(out) < config.max_new_tokens and config.eos_token_id not in out:
                 if cancellation.cancelled:  # observed between passes
                     cancelled = True
                     break

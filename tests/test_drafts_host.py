@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from aios_amd.attention.backend import Mi355xAttentionBackend
-from aios_amd.core import SamplingParams
+from aios_amd.core import Batch, Req, SamplingParams, reset_global_ctx, set_global_ctx
 from aios_amd.drafts import DraftTree, PhraseDrafter, draft_tree
 from aios_amd.ime import CandidateGroupConfig, CandidateGroupEngine
 from aios_amd.scheduler import CacheManager
@@ -120,3 +120,17 @@ def test_backend_refuses_parents_that_are_no_tree():
                            ([[-1, 1, 0]], "earlier one"), ([[-1, 0, -2]], "earlier one")):
         with pytest.raises(ValueError, match=match):
             be._plan_trees(parents, [3], cu, cu, cu, 16)
+
+
+def test_backend_refuses_a_decode_batch_of_trees():
+    be = Mi355xAttentionBackend(SimpleNamespace(num_qo_heads=4, num_kv_heads=2, head_dim=64))
+    ctx = SimpleNamespace(page_table=torch.zeros(1, 8, dtype=torch.int32), kv_cache=None)
+    b = Batch(reqs=[Req(input_ids=torch.empty(4, dtype=torch.long), cached_len=3, output_len=1,
+                        uid=0, sampling_params=SamplingParams(), table_idx=0)], phase="decode")
+    b.tree_parents = [[-1]]
+    set_global_ctx(ctx)
+    try:
+        with pytest.raises(ValueError, match="prefill batch"):
+            be.prepare_metadata(b)
+    finally:
+        reset_global_ctx()

@@ -157,6 +157,7 @@ def test_greedy_tokens_with_drafts(config, kv_bits):
     cut = next(i for i in range(1, 9) if tokens[i] not in tokens[:i])
     r = eng.complete_drafted(prefix, drafter, replace(cfg, eos_token_id=tokens[cut]))
     assert list(r.candidate.token_ids) == tokens[:cut] and r.candidate.stop_reason == "eos"
+    assert r.passes == (0 if cut == 0 else 1 if cut <= 5 else 2)  # (none behind the end)
     assert rt.cache_manager.available_size == rt.num_pages - len(prefix)
 
 
@@ -255,3 +256,21 @@ def test_a_drafter_that_fails_leaves_no_pages_behind():
     assert r.cancelled and len(r.candidate.token_ids) == 2
     assert r.candidate.stop_reason == "cancelled"
     assert eng.rt.cache_manager.available_size == eng.rt.num_pages - 12
+
+
+@BITS
+def test_groups_before_and_behind_a_drafted_completion(kv_bits):
+    """The same captured steps give the same candidates; their pages and table rows
+    are as they were."""
+    eng, _ = _engine(IME, kv_bits)
+    prefix = _ids(IME, 24, 12)
+    cfg = CandidateGroupConfig(max_new_tokens=6)
+    before = eng.complete(prefix, cfg)
+    scores = eng.score(prefix, [[1, 2, 3], [4]])
+    r = eng.complete_drafted(prefix, PhraseDrafter([prefix[-2:] + [7, 8, 9], [3, 4]]), cfg)
+    assert len(r.candidate.token_ids) == 6 and r.reused_prefix_tokens == 24
+    behind = eng.complete(prefix, cfg)
+    assert [c.token_ids for c in behind.raw_candidates] == [c.token_ids for c in
+                                                            before.raw_candidates]
+    assert [s.logprobs for s in eng.score(prefix, [[1, 2, 3], [4]])] == [s.logprobs for s in scores]
+    assert eng.rt.cache_manager.available_size == eng.rt.num_pages - 24
