@@ -663,6 +663,8 @@ struct VWalk {
   int32_t gone[kVNodes];
   int v, count, n_gone;
   double sh[16];
+  VOpen open[kVStages];  // the sums of F of earlier launches
+  double f[kVStages];
 };
 
 // Thread t's node as a draft: its parent (-1: none), token (-1: outside the
@@ -677,25 +679,17 @@ __device__ __forceinline__ void load_draft(const VerifyArgs& a, VWalk& w, int64_
   w.tok[t] = tok >= 0 && tok < a.vocab ? (int)tok : -1;
   w.u[t] = GREEDY ? 0.0 : number(a.uniforms[first + t]);
   w.on_path[t] = 0;
+#pragma unroll
+  for (int g = 0; g < kVNodes / 64; ++g) w.kids[t][g] = 0;
 }
 
-// Every node's children (behind load_draft and a barrier).  All parents pass by
-// every thread out of the wavefront's registers: looking for them in LDS, one
-// dependent read after the other, took longer than a launch.
+// Every node's children (between two barriers behind load_draft): bits set in LDS, in
+// whatever order.  0.2 us; 64 parents passing by every thread out of the wavefront's
+// registers took 2.9.
 __device__ __forceinline__ void list_children(VWalk& w, int n) {
-  const int t = threadIdx.x, lane = t & 63;
-  if ((t & ~63) >= n) return;  // (uniform per wavefront)
-#pragma unroll
-  for (int g = 0; g < kVNodes / 64; ++g) {
-    uint64_t mask = 0;
-    if (g * 64 < n) {
-      const int par = g * 64 + lane < n ? w.par[g * 64 + lane] : -1;
-      const int m = min(n - g * 64, 64);
-      for (int j = 0; j < m; ++j)
-        mask |= (uint64_t)(__builtin_amdgcn_readlane(par, j) == t) << j;
-    }
-    if (t < n) w.kids[t][g] = mask;
-  }
+  const int t = threadIdx.x;
+  if (t < n && w.par[t] >= 0)
+    atomicOr(reinterpret_cast<unsigned long long*>(&w.kids[w.par[t]][t >> 6]), 1ull << (t & 63));
 }
 // The next child of node v behind node i (-1: none).
 __device__ __forceinline__ int next_child(const VWalk& w, int v, int i) {
@@ -889,44 +883,47 @@ __device__ __forceinline__ VPlace place(const VerifyArgs& a, int req, int64_t fi
     if (lane == 0) add_token(a, req, first, best, (float)-ls1);
     return o;
   }
-  // weights in the row's units; without any mass left, p's own
+  // weights in the row's units; without any mass left, p's own.  A lane takes
+  // consecutive batches, so that one pass and one scan find its lane.
   auto scale = [&](int b) {
     return own_max ? vexp64((double)batches[b].m - m, a.inv_t) : 1.0;
   };
-  double total = 0, whole = 0;
-  for (int b = lane; b < nb; b += 64) {
+  const int each = (nb + 63) / 64, from = min(lane * each, nb), to = min(from + each, nb);
+  double lw = 0, lp = 0;
+  for (int b = from; b < to; ++b) {
     const double f = scale(b);
-    total += batches[b].w * f;
-    whole += batches[b].p * f;
+    lw += batches[b].w * f;
+    lp += batches[b].p * f;
   }
-  total = wave_sum64(total);
-  whole = wave_sum64(whole);
+  double cum = wave_scan64(lw);
+  const double total = lane64(cum, 63);
   o.done = false;
   o.residual = total > 0;
-  o.target = (double)a.uniforms[first] * (o.residual ? total : whole);
+  if (!o.residual) {  // (uniform)
+    lw = lp;
+    cum = wave_scan64(lp);
+  }
+  o.target = (double)a.uniforms[first] * lane64(cum, 63);
   o.m = m;
   o.ls1 = ls1;
   // the first batch past the target, or the last one with any weight
-  double base = 0;
-  int last = 0;
-  for (int b0 = 0; b0 < nb; b0 += 64) {
-    const int b = b0 + lane;
-    const double x = b < nb ? (o.residual ? batches[b].w : batches[b].p) * scale(b) : 0.0;
-    const double cum = base + wave_scan64(x);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(cum > o.target && x > 0);
-    const uint64_t any = __builtin_amdgcn_ballot_w64(x > 0);
-    if (hit) {
-      const int l = __ffsll((unsigned long long)hit) - 1;
-      last = b0 + l;
-      o.start = lane64(cum - x, l);
-      o.found = true;
-      break;
+  const uint64_t hit = __builtin_amdgcn_ballot_w64(cum > o.target && lw > 0);
+  const uint64_t any = __builtin_amdgcn_ballot_w64(lw > 0);
+  o.found = hit != 0;
+  const int l = hit   ? __ffsll((unsigned long long)hit) - 1
+                : any ? 63 - __clzll((long long)any)
+                      : 0;
+  double base = l > 0 ? lane64(cum, l - 1) : 0.0;
+  for (int b = l * each; b < min(l * each + each, nb); ++b) {  // (uniform)
+    const double f = scale(b), x = (o.residual ? batches[b].w : batches[b].p) * f;
+    if (x > 0) {
+      o.at = b;
+      o.start = base;
+      o.scale = f;
+      if (o.found && base + x > o.target) break;
     }
-    if (any) last = b0 + 63 - __clzll((long long)any);
-    base = lane64(cum, 63);
+    base += x;
   }
-  o.at = last;
-  o.scale = scale(o.at);
   return o;
 }
 
@@ -1023,9 +1020,19 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
     w.mass[tid] = 1.0;
     w.tries[tid] = 0;
   }
+  if (DRAWN && wave < stage) {  // (one lane per workgroup's share)
+    static_assert(kVMaxSegments <= 64 && kVStages <= kVThreads / 64, "");
+    const int lane = tid & 63;
+    const double f = wave_sum64(lane < wgs ? mine_f2[wave * wgs + lane] : 0.0);
+    if (lane == 0) {
+      w.f[wave] = f;
+      w.open[wave] = mine_open[wave];
+    }
+  }
   load_draft<GREEDY>(a, w, first, n);
   __syncthreads();
   list_children(w, n);
+  __syncthreads();
   if (tid < n)
     try_children<DRAWN, GREEDY>(w, tid, n, [&](int j) {
       return j == 1 ? sum_parts(f1 + (first + tid) * a.segments, a.segments) : __builtin_nan("");
@@ -1035,8 +1042,7 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
       a, w, first, n,
       [&](int v, int j) {
         for (int s = 0; s < stage; ++s)
-          if (mine_open[s].node == v && mine_open[s].j == j)
-            return sum_parts(mine_f2 + s * wgs, wgs) / w.node[v].s;
+          if (w.open[s].node == v && w.open[s].j == j) return w.f[s] / w.node[v].s;
         return __builtin_nan("");
       },
       [&](int v, int j, const VRow& r) {
