@@ -860,6 +860,7 @@ __device__ __forceinline__ VPlace place(const VerifyArgs& a, int req, int64_t fi
                                         float m, double ls1, const VBatch* batches) {
   const int lane = threadIdx.x & 63;
   const int nb = batches_of(a.vocab);
+  const double u = GREEDY ? 0.0 : (double)a.uniforms[first];  // (on its way with the batches)
   VPlace o = {};
   o.done = true;
   if (own_max) {
@@ -903,7 +904,7 @@ __device__ __forceinline__ VPlace place(const VerifyArgs& a, int req, int64_t fi
     lw = lp;
     cum = wave_scan64(lp);
   }
-  o.target = (double)a.uniforms[first] * lane64(cum, 63);
+  o.target = u * lane64(cum, 63);
   o.m = m;
   o.ls1 = ls1;
   // the first batch past the target, or the last one with any weight
@@ -967,11 +968,11 @@ __device__ __forceinline__ void add_drawn(const VerifyArgs& a, int req, int64_t 
             (float)(((double)(float)static_cast<const T*>(r.x)[id] - o.m) - o.ls1));
 }
 
-// A request's nodes, or false (with its outputs set) if it has none.
-__device__ __forceinline__ bool request(const VerifyArgs& a, int req, bool writes, int64_t& first,
-                                        int& n) {
-  first = a.cu[req];
-  const int64_t size = (int64_t)a.cu[req + 1] - first;
+// A request's nodes (begin .. end), or false (with its outputs set) if it has none.
+__device__ __forceinline__ bool request(const VerifyArgs& a, int req, int begin, int end,
+                                        bool writes, int64_t& first, int& n) {
+  first = begin;
+  const int64_t size = (int64_t)end - first;
   n = (int)(size < kVNodes ? size : kVNodes);
   if (n > 0 && first >= 0 && first + n <= a.total) return true;
   if (writes && threadIdx.x == 0) {
@@ -984,7 +985,8 @@ __device__ __forceinline__ bool request(const VerifyArgs& a, int req, bool write
 
 // A workgroup per (request, round of batches): the path, found by every one of
 // them, and its share of the batches, or of the sum of F that the path needs next.
-// Bound: 4 - 5 us of dependent steps; 1 us a launch that has nothing left to do.
+// Bound: dependent steps, 1.6 us for lengths and nodes, 1.4 for the tests, 0.6 - 2 for
+// the path, 1.9 - 2.5 for a batch; 1 us a launch that has nothing left to do.
 template <typename T, bool DRAWN, bool GREEDY>
 __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
     VerifyArgs a, int stage, const VNode* nodes, const VKid* kids, const double* f1, VOpen* open,
@@ -996,6 +998,7 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
   const int c = blockIdx.x % wgs, req = blockIdx.x / wgs;
   VOpen* mine_open = open + (int64_t)req * kVStages;
   double* mine_f2 = f2 + (int64_t)req * kVStages * wgs;
+  const int begin = a.cu[req], end = a.cu[req + 1];  // (on their way with `open`)
   if constexpr (DRAWN) {
     if (stage > 0 && mine_open[stage - 1].node < 0) {
       if (c == 0 && tid == 0) mine_open[stage].node = -1;
@@ -1006,7 +1009,7 @@ __global__ __launch_bounds__(kVThreads) void verify_walk_kernel(
   }
   int64_t first;
   int n;
-  if (!request(a, req, c == 0, first, n)) {
+  if (!request(a, req, begin, end, c == 0, first, n)) {
     if (c == 0 && tid == 0) lasts[req].node = -1;
     return;
   }
@@ -1117,9 +1120,9 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a, const VLa
 // Behind the stats, a workgroup per request for everything else, where a row has
 // no more batches than the workgroup wavefronts: F's sums as the path needs them,
 // and the added token out of the registers that hold its batch's weights.  Bound: that
-// chain, 11.5 - 13 us for 1 to 24 requests (in thousands of cycles: lengths 1.7,
-// children 2.4, sums 4, p and q 1.8, tests and path 2.5 - 4, weights 5.5 - 7, the
-// batch 1.6 - 5, the token 3); five launches took 24 us of the host, two take 19.
+// chain, 10.5 - 12 us for 1 to 24 requests: lengths, sums, p and q, tests and path,
+// weights, batch and token, none above 3; five launches took 24 us of the host, two
+// take 19.
 template <typename T, bool DRAWN, bool GREEDY>
 __global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a,
                                                                     const VPart* parts) {
@@ -1144,7 +1147,7 @@ __global__ __launch_bounds__(kVRestThreads) void verify_rest_kernel(VerifyArgs a
     nobody(0, a.cu[0]);
     nobody(a.cu[a.batch], a.total);
   }
-  if (!request(a, req, true, first, n)) return;
+  if (!request(a, req, a.cu[req], a.cu[req + 1], true, first, n)) return;
   nobody(first + kVNodes, a.cu[req + 1]);
   load_draft<GREEDY>(a, w, first, n);
   if (tid < n) w.node[tid].flags = 0;
