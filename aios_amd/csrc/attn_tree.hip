@@ -183,8 +183,8 @@ __device__ __forceinline__ _Float16* part_o(const TreeArgs& t, int64_t part, int
 // Bound, replayed from a graph with the combine: few rows by the chain of round trips
 // (lengths, page ids, K/V) and sub-tiles, 0.65 us each at 128 dims, which is why a
 // range is cut into parts of few: 8 nodes on 24 positions, 8q/2kv x 96, 5.6 us; 17 on
-// 4,093, 16q/8kv, 12.7 in 13 parts (main 9.1, combine 3.2), 145 in one; 40 on 16,001,
-// 32q/8kv, 8 bits 32, of them 26.6 here; eight chains of 6 on 2,500 in 8 bits 18.9.
+// 4,093, 16q/8kv, 12.6 in 26 parts (main 8.2, combine 3.3), 145 in one; 40 on 16,001,
+// 32q/8kv, 8 bits 32, of them 25 here; eight chains of 6 on 2,500 in 8 bits 18.9.
 // Full tiles by the math chain of a sub-tile (products and softmax overlap only
 // between the two wavefronts of a SIMD): four requests of 200 - 165 nodes on 8,192,
 // 32q/8kv x 128, 160 - 178 us, 600 TFLOP/s of the unmasked products.
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kEngineThreads) __attribute__((amdgpu_waves_per_eu(
 // m = max_j m_j.  A wavefront takes RB rows, one (row, 8-dim group) per lane; NW
 // wavefronts share a row block's parts, NB of them in flight per wavefront.
 // Bound: two round trips (states, then the sums' exchange) and the states' bytes: 3.2
-// us for 13 parts of 34 rows, 5.1 for 28 parts of 80 (16 heads and tiles), 6.5 for 2
+// us for 26 parts of 34 rows, 5.3 for 32 parts of 80 (16 heads and tiles), 6.4 for 2
 // parts of 116 rows in 200 tiles (13 MB of states).
 template <int D, int NW, int NB>
 __global__ __launch_bounds__(NW * 64) void tree_combine_kernel(

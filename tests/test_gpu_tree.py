@@ -370,3 +370,41 @@ def test_masks_leave_rows_past_the_last_request():
     assert masks[:4].flatten().tolist() == [1, 2, 4, 8]
     assert masks[4:].flatten().tolist() == [1, 2, 4, 8, 16, 32]
     assert (depths == 0).all()
+
+
+@BITS
+@pytest.mark.parametrize("parts", [False, True])
+@pytest.mark.parametrize("nodes,cached,hq,hkv,d", [
+    ([6, 1], [3100, 2600], 8, 2, 96), ([16], [4030], 8, 4, 64), ([17, 9], [0, 3900], 16, 8, 128),
+    ([31], [2500], 16, 8, 128), ([9], [247], 8, 8, 128), ([9], [279], 8, 8, 128),
+])
+def test_few_rows_with_long_parts(bits, parts, nodes, cached, hq, hkv, d):
+    """At most 64 rows and more than eight sub-tiles a part, which its wavefronts share:
+    without a workspace, and where the device's lengths are six times the planned."""
+    c = Case(nodes, cached, hq, hkv, d, bits, seed=sum(cached) + d)
+    short = _cu([n + x // 6 for n, x in zip(nodes, cached)])
+    plan = paged.plan("tree", c.cu_q, short if parts else c.cu_k, hq, hkv, d, kv_bits=bits,
+                      **({} if parts else {"workspace_bytes": 0}))
+    if not parts:
+        assert plan.num_parts == 1
+    plan.total_kv = int(c.cu_k[-1])  # (what the indices are checked for)
+    cache, k, v = c.cache()
+    c.check(c.call(cache, plan=plan), k, v)
+
+
+@BITS
+def test_values_nobody_sees_in_a_shared_part(bits):
+    c = Case([12, 3], [610, 290], 8, 4, 64, bits, seed=77)
+    g = torch.Generator().manual_seed(3)
+    c.seen = [sorted({i} | set(torch.randint(12, (2,), generator=g).tolist())) for i in range(12)]
+    c.seen = [[j for j in s if j != 5] for s in c.seen] + [[0], [], [0, 2]]
+    if bits == 16:
+        c.v[c.indices[610 + 5].long()] = float("nan")  # node 5 is seen by none
+        c.v[c.indices[-2].long()] = float("-inf")      # nor is node 1 of the second
+    plan = paged.plan("tree", c.cu_q, c.cu_k, 8, 4, 64, kv_bits=bits, workspace_bytes=0)
+    cache, k, v = c.cache()
+    out = c.call(cache, plan=plan)
+    if bits == 16:
+        k, v = k.copy(), np.where(np.isfinite(v), v, 0.0)
+    c.check(out, k, v)
+    assert torch.isfinite(out).all()
