@@ -502,9 +502,10 @@ def tree_attention(p: _lib.AttnPlan, q: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError("plan was not built for trees over the bfloat16 cache")
     dev = _check_tree(p, q, indices, cu_q, cu_k, masks)
     _check_cache(k_cache, p)
-    _check_cache(v_cache, p)
-    if not dev == k_cache.get_device() == v_cache.get_device() or \
-            k_cache.shape != v_cache.shape:
+    # (one test for calls in order, as for the lists)
+    if not (v_cache.dtype is _BF16 and v_cache.shape == k_cache.shape and v_cache.is_contiguous()
+            and dev == k_cache.get_device() == v_cache.get_device()):
+        _check_cache(v_cache, p)
         raise ValueError("the KV caches must be on q's GPU and of one shape")
     out = _out_like(q, out)
     # (a buffer of this call alone, as in prefill)
