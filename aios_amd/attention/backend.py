@@ -139,6 +139,29 @@ class Mi355xStaticPrefillMetadata(Mi355xAttentionMetadata):
         )
 
 
+@dataclass
+class Mi355xStaticTreeMetadata(Mi355xStaticPrefillMetadata):
+    """The same for one request's tree of at most ``plan.max_q_len`` nodes
+    (Batch.tree_parents): refresh(kv_len, nodes, parents) takes the number of
+    nodes and their parents (int32, one per planned node; those behind the
+    tree's do not count) from the device as well.  Rows behind the tree's nodes
+    are left as they are."""
+
+    _depths: torch.Tensor | None = None
+
+    def refresh(self, kv_len: torch.Tensor, nodes: torch.Tensor, parents: torch.Tensor) -> None:
+        super().refresh(kv_len)
+        torch.mul(self._ramp, nodes, out=self.cu_seqlens_q_gpu)
+        masks = self.tree_masks
+        _lib.check(
+            _lib.lib().aios_tree_masks(
+                parents.data_ptr(), self.cu_seqlens_q_gpu.data_ptr(), 1, masks.shape[0],
+                masks.shape[1], masks.data_ptr(), self._depths.data_ptr(),
+                torch.cuda.current_stream(masks.device).cuda_stream),
+            "aios_tree_masks",
+        )
+
+
 def check_decode_preconditions(indices: torch.Tensor, cu_seqlens_k: torch.Tensor,
                                out_loc: torch.Tensor | None, shared_prefix_len: int) -> None:
     """Raise ``ValueError`` unless the decode batch keeps the caller
@@ -413,11 +436,13 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
 
     def prepare_static_prefill(self, q_len: int, max_kv_len: int, page_table: torch.Tensor,
                                row_id: int = 0,
-                               kv_bits: int | None = None) -> Mi355xStaticPrefillMetadata:
+                               kv_bits: int | None = None,
+                               trees: bool = False) -> Mi355xStaticPrefillMetadata:
         """Fixed-buffer prefill metadata for graph-replayed prefills of
         ``q_len`` tokens against at most ``max_kv_len`` positions (see
         :class:`Mi355xStaticPrefillMetadata`); ``kv_bits`` as for
-        prepare_static_decode."""
+        prepare_static_decode.  ``trees``: of a tree of at most ``q_len`` nodes
+        (:class:`Mi355xStaticTreeMetadata`)."""
         device = page_table.device
         if page_table.dtype != torch.int32 or max_kv_len > page_table.shape[1]:
             raise ValueError("max_kv_len exceeds the page-table row length")
@@ -425,17 +450,26 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             raise ValueError("q_len must be within 1..max_kv_len")
         cu_q = torch.tensor([0, q_len], dtype=torch.int32)
         cu_k = torch.tensor([0, max_kv_len], dtype=torch.int32)
-        plan = _lib.AttnPlan()
         kv_bits = _context_kv_bits(kv_bits)
-        make, name = _make_plan(kv_bits)
-        _lib.check(
-            make(_lib.PHASE_PREFILL, cu_q.data_ptr(), cu_k.data_ptr(), 1, self.num_heads,
-                 self.num_kv_heads, self.head_dim, 1, 0, self.workspace_size,
-                 self.prefix_chunk_len, self.suffix_split_len, plan),
-            name,
-        )
+        if trees:
+            plan = paged.plan("tree", cu_q, cu_k, self.num_heads, self.num_kv_heads,
+                              self.head_dim, workspace_bytes=self.workspace_size, kv_bits=kv_bits)
+            words = -(-q_len // 64)
+            kind, extra = Mi355xStaticTreeMetadata, {
+                "tree_masks": torch.zeros((q_len, words), dtype=torch.int64, device=device),
+                "_depths": torch.zeros(q_len, dtype=torch.int32, device=device)}
+        else:
+            plan = _lib.AttnPlan()
+            make, name = _make_plan(kv_bits)
+            _lib.check(
+                make(_lib.PHASE_PREFILL, cu_q.data_ptr(), cu_k.data_ptr(), 1, self.num_heads,
+                     self.num_kv_heads, self.head_dim, 1, 0, self.workspace_size,
+                     self.prefix_chunk_len, self.suffix_split_len, plan),
+                name,
+            )
+            kind, extra = Mi355xStaticPrefillMetadata, {}
         ramp = torch.arange(2, dtype=torch.int32, device=device)
-        return Mi355xStaticPrefillMetadata(
+        return kind(
             cu_seqlens_q_cpu=cu_q,
             cu_seqlens_k_cpu=cu_k,
             cu_seqlens_q_gpu=cu_q.to(device),
@@ -456,6 +490,7 @@ class Mi355xAttentionBackend(BaseAttentionBackend):
             page_table=page_table,
             max_kv_len=max_kv_len,
             _ramp=ramp,
+            **extra,
         )
 
     def forward(

@@ -338,6 +338,7 @@ class CandidateGroupEngine:
         self.use_graphs = use_graphs
         self._graphs: OrderedDict[tuple, _DecodeGraph] = OrderedDict()
         self._prefill_graphs: OrderedDict[tuple, _PrefillGraph] = OrderedDict()
+        self._draft_graphs: OrderedDict[tuple, _DraftGraph] = OrderedDict()
         self._generation_id = 0
         self._active: CancellationToken | None = None
         self._gen_lock = threading.Lock()
@@ -572,7 +573,8 @@ class CandidateGroupEngine:
         Drafts with logits (drawn from them at the sampling temperature) go
         through aios_amd.sample.verify_drafts, which keeps the candidate's
         distribution; that needs sampling without top_k, top_p and min_new_tokens.  The drafter
-        runs while the engine is locked: it must not call the engine.  Of
+        runs while the engine is locked: it must not call the engine.  Passes of
+        up to MAX_GRAPHED_PREFILL nodes are replayed from graphs.  Of
         ``config``, max_new_tokens, eos_token_id, sampling, seed, min_new_tokens
         and blocked_token_ids count."""
         config = config or CandidateGroupConfig()
@@ -692,23 +694,17 @@ class CandidateGroupEngine:
         parents = [-1, *(p + 1 for p in tree.parents)]
         depths = [0, *tree.depths()]
         n = len(tokens)
-        pages = rt.cache_manager.allocate(n)
+        g = self._draft_graph(cached, n)
+        # (a graph's rows behind the tree write pages too, given back with the rest)
+        pages = rt.cache_manager.allocate(n if g is None else g.nodes)
         stays = [0]
         try:
-            rt.page_table[0, cached : cached + n] = pages
-            req = Req(input_ids=torch.empty(cached + n, dtype=torch.long), cached_len=cached,
-                      output_len=1, uid=0, sampling_params=SamplingParams(max_tokens=1),
-                      table_idx=0)
-            batch = Batch(reqs=[req], phase="prefill")
-            batch.input_ids = torch.tensor(tokens, dtype=torch.long, device=dev)
-            batch.positions = torch.tensor([cached + d for d in depths], dtype=torch.int32,
-                                           device=dev)
-            batch.out_loc = pages
-            batch.return_all_logits = True
-            batch.tree_parents = [parents]
-            rt.model.attn_backend.prepare_metadata(batch)
-            with rt.ctx.forward_batch(batch):
-                logits = rt.model.forward()
+            rt.page_table[0, cached : cached + n] = pages[:n]
+            positions = [cached + d for d in depths]
+            if g is not None:
+                logits, ids = g.run(tokens, positions, parents, cached + n, pages)
+            else:
+                logits, ids = self._draft_forward(tokens, positions, parents, cached, pages)
             sp = config.sampling
             if sp is None or sp.is_greedy or tree.logits is None:
                 picks, raw = self._draft_picks(logits, [n_out + d for d in depths], config)
@@ -726,7 +722,7 @@ class CandidateGroupEngine:
                 par = torch.tensor(parents, dtype=torch.int32, device=dev)
                 # (numbers of their own: not the stream that picks tokens)
                 uni = stateless_uniforms([config.seed + 7_919 * (n_out + 1)], n, dev)[0]
-                r = verify_drafts(logits, batch.input_ids, par,
+                r = verify_drafts(logits, ids, par,
                                   torch.tensor([0, n], dtype=torch.int32, device=dev), uni,
                                   draft_logits=tree.logits, temperature=sp.temperature)
                 took = r.accepted.tolist()
@@ -742,10 +738,44 @@ class CandidateGroupEngine:
         # change places in the table
         keep = pages[torch.tensor(stays, device=dev)]
         rt.page_table[0, cached : cached + len(stays)] = keep
-        gone = [i for i in range(n) if i not in set(stays)]
+        gone = [i for i in range(len(pages)) if i not in set(stays)]
         if gone:
             rt.cache_manager._free(pages[torch.tensor(gone, device=dev)])
         return added, len(path), lps, keep
+
+    def _draft_forward(self, tokens, positions, parents, cached: int, pages: torch.Tensor):
+        """(logits of every node, the nodes' ids on the device), eagerly."""
+        rt, dev = self.rt, self.rt.device
+        req = Req(input_ids=torch.empty(cached + len(tokens), dtype=torch.long), cached_len=cached,
+                  output_len=1, uid=0, sampling_params=SamplingParams(max_tokens=1), table_idx=0)
+        batch = Batch(reqs=[req], phase="prefill")
+        batch.input_ids = torch.tensor(tokens, dtype=torch.long, device=dev)
+        batch.positions = torch.tensor(positions, dtype=torch.int32, device=dev)
+        batch.out_loc = pages
+        batch.return_all_logits = True
+        batch.tree_parents = [parents]
+        rt.model.attn_backend.prepare_metadata(batch)
+        with rt.ctx.forward_batch(batch):
+            return rt.model.forward(), batch.input_ids
+
+    def _draft_graph(self, cached: int, n: int):
+        """The graph for n nodes behind ``cached`` tokens: one per power of two of
+        nodes, up to MAX_GRAPHED_PREFILL, and 256 positions of capacity; None
+        (an eager pass): without graphs, for more nodes, or where the pool does
+        not hold that many pages."""
+        rt = self.rt
+        nodes = 1 << (n - 1).bit_length()
+        kv_cap = min(-(-(cached + nodes) // 256) * 256, rt.max_context)
+        if not self.use_graphs or nodes > min(self.MAX_GRAPHED_PREFILL, kv_cap) or \
+                cached + n > kv_cap or nodes > rt.cache_manager.available_size:
+            return None
+        g = self._draft_graphs.get((nodes, kv_cap))
+        if g is None:
+            while len(self._draft_graphs) >= self.MAX_GRAPHS:
+                self._draft_graphs.popitem(last=False)
+            g = self._draft_graphs[nodes, kv_cap] = _DraftGraph(self, nodes, kv_cap)
+        self._draft_graphs.move_to_end((nodes, kv_cap))
+        return g
 
     # -- prefix ------------------------------------------------------------------
     def _prepare_prefix(self, token_ids, page_table):
@@ -1051,6 +1081,68 @@ class _PrefillGraph:
         cur.wait_stream(stream)
         self.graph = graph
         return out
+
+
+class _DraftGraph:
+    """Fixed buffers and the captured pass over one tree of at most ``nodes``
+    nodes behind page-table row 0's cached tokens, at most ``kv_cap`` positions
+    in all.  A replay takes the ids, positions, parents and lengths out of one
+    buffer, rebuilds masks and page indices, and leaves every node's logits."""
+
+    def __init__(self, eng: "CandidateGroupEngine", nodes: int, kv_cap: int) -> None:
+        rt = eng.rt
+        dev = rt.device
+        self.rt = rt
+        self.nodes = nodes
+        # ids, positions, parents; KV length, nodes of the tree
+        self.given = torch.zeros(3 * nodes + 2, dtype=torch.long, device=dev)
+        self.small = torch.zeros(2 * nodes + 2, dtype=torch.int32, device=dev)
+        self.out_loc = torch.zeros(nodes, dtype=torch.int32, device=dev)
+        self.md = rt.model.attn_backend.prepare_static_prefill(nodes, kv_cap, rt.page_table, 0,
+                                                               trees=True)
+        req = Req(input_ids=torch.empty(nodes, dtype=torch.long), cached_len=0, output_len=1,
+                  uid=0, sampling_params=SamplingParams(max_tokens=1), table_idx=0)
+        self.batch = Batch(reqs=[req], phase="prefill")
+        self.batch.input_ids = self.given[:nodes]
+        self.batch.positions = self.small[:nodes]
+        self.batch.out_loc = self.out_loc
+        self.batch.return_all_logits = True
+        self.batch.attn_metadata = self.md
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self.logits: torch.Tensor | None = None
+
+    def _body(self) -> torch.Tensor:
+        n = self.nodes
+        self.small.copy_(self.given[n:])
+        self.md.refresh(self.small[2 * n : 2 * n + 1], self.small[2 * n + 1 :],
+                        self.small[n : 2 * n])
+        with self.rt.ctx.forward_batch(self.batch):
+            return self.rt.model.forward()
+
+    def run(self, tokens, positions, parents, kv_len: int, pages: torch.Tensor):
+        """(logits of the tree's nodes, overwritten by the next run, and their ids)"""
+        n = len(tokens)
+        if n > self.nodes or kv_len > self.md.max_kv_len or pages.numel() != self.nodes:
+            raise ValueError("draft graph used with more nodes or positions than captured")
+        rest = self.nodes - n
+        self.given.copy_(torch.tensor([*tokens, *([0] * rest), *positions, *([0] * rest), *parents,
+                                       *([-1] * rest), kv_len, n], dtype=torch.long))
+        self.out_loc.copy_(pages)
+        if self.graph is not None:
+            self.graph.replay()
+            return self.logits[:n], self.given[:n]
+        # (first use as in _PrefillGraph)
+        cur = torch.cuda.current_stream(self.rt.device)
+        stream = torch.cuda.Stream(self.rt.device)
+        stream.wait_stream(cur)
+        with torch.cuda.stream(stream):
+            out = self._body()
+        graph = torch.cuda.CUDAGraph()
+        with captured(graph, stream):
+            self.logits = self._body()
+        cur.wait_stream(stream)
+        self.graph = graph
+        return out[:n], self.given[:n]
 
 
 class _DecodeGraph:

@@ -37,11 +37,11 @@ def teardown_function(_):
     torch.cuda.empty_cache()
 
 
-def _engine(config, kv_bits, seed=3, num_pages=512):
+def _engine(config, kv_bits, seed=3, num_pages=512, use_graphs=True):
     w = init_weights(config, seed, "cpu")
     rt = CandidateGroupRuntime(config, weights_to(w, "cuda"), "cuda", num_pages=num_pages,
                                kv_bits=kv_bits)
-    return CandidateGroupEngine(rt), w
+    return CandidateGroupEngine(rt, use_graphs), w
 
 
 def _ids(config, n, seed):
@@ -59,6 +59,30 @@ def _oracle(config, w, rt, ids, pages):
         k, v = _values(*rt.kv_cache.layer(i))
         om.kv.append((torch.from_numpy(k[pages]).float(), torch.from_numpy(v[pages]).float()))
     return om.logits(torch.tensor(ids)[None], 0)[0, -1]
+
+
+def _greedy_up_to_rounding(config, w, prefix, tokens):
+    """Every token's logit is within both sides' errors of the oracle's largest (two
+    launches' logits differ, so their tokens need not be the same)."""
+    n = len(prefix) - 1
+    ref = OracleModel(config, w).logits(torch.tensor(prefix + tokens[:-1])[None], 0)[0, n:]
+    gap = ref.max(-1).values - ref.gather(1, torch.tensor(tokens)[:, None])[:, 0]
+    assert gap.max().item() <= 2 * LOGIT_TOL
+    return ref
+
+
+def _give_logits(rt, table):
+    """The forward runs as ever, and then the logits of position p are row p of a table,
+    so that no launch's rounding enters."""
+    forward = rt.model.forward
+
+    def with_table():
+        b = rt.ctx.batch
+        rows = forward().shape[0]
+        at = b.positions if rows == b.positions.numel() else b.positions[-1:]
+        return table[at.long()]
+
+    rt.model.forward = with_table
 
 
 @CONFIGS
@@ -121,8 +145,9 @@ def test_a_batch_of_trees_gives_every_path_s_logits(config, kv_bits):
 
 @CONFIGS
 @BITS
-def test_greedy_tokens_with_drafts(config, kv_bits):
-    eng, w = _engine(config, kv_bits)
+@pytest.mark.parametrize("use_graphs", [True, False])
+def test_greedy_tokens_with_drafts(config, kv_bits, use_graphs):
+    eng, w = _engine(config, kv_bits, use_graphs=use_graphs)
     rt = eng.rt
     prefix = _ids(config, 33, 9)
     cfg = CandidateGroupConfig(max_new_tokens=9)
@@ -131,13 +156,19 @@ def test_greedy_tokens_with_drafts(config, kv_bits):
     tokens = list(plain.candidate.token_ids)
     assert len(tokens) == 9 and plain.passes == 8 and plain.drafted == 0
     assert plain.candidate.stop_reason == "max_new_tokens"
-    # greedy under the oracle, up to both logits' errors, and its log-probs
-    ref = OracleModel(config, w).logits(torch.tensor(prefix + tokens[:-1])[None], 0)[0, 32:]
     if kv_bits == 16:
-        gap = ref.max(-1).values - ref.gather(1, torch.tensor(tokens)[:, None])[:, 0]
-        assert gap.max().item() <= 2 * LOGIT_TOL
+        ref = _greedy_up_to_rounding(config, w, prefix, tokens)
         lp = ref.log_softmax(-1).gather(1, torch.tensor(tokens)[:, None]).mean().item()
         assert abs(lp - plain.candidate.average_logprob) <= 2 * LOGIT_TOL
+    # an engine whose logits are given, position by position
+    eng.reset_prefix_cache()
+    table = (4 * torch.randn(42, config.vocab_size, generator=torch.Generator().manual_seed(1))
+             ).to("cuda", torch.bfloat16)
+    _give_logits(rt, table)
+    eng = CandidateGroupEngine(rt, use_graphs)
+    plain = eng.complete_drafted(prefix, lambda context, room: None, cfg)
+    tokens = list(plain.candidate.token_ids)
+    assert tokens == table[32:41].argmax(-1).tolist()
     # the same tokens drafted, with others beside them: fewer passes
     wrong = _ids(config, 8, 77)
 
@@ -149,7 +180,7 @@ def test_greedy_tokens_with_drafts(config, kv_bits):
     r = eng.complete_drafted(prefix, drafter, cfg)
     assert list(r.candidate.token_ids) == tokens and r.reused_prefix_tokens == len(prefix)
     assert r.passes == 2 and r.accepted == 6 and r.drafted > 6  # 1 + (4 + 1) + (2 + 1)
-    assert abs(r.candidate.average_logprob - plain.candidate.average_logprob) <= 2 * LOGIT_TOL
+    assert abs(r.candidate.average_logprob - plain.candidate.average_logprob) < 1e-5
     assert rt.cache_manager.available_size == rt.num_pages - len(prefix)
     r = eng.complete_drafted(prefix, PhraseDrafter([prefix[-3:] + tokens, wrong]), cfg)
     assert list(r.candidate.token_ids) == tokens and r.passes == 1
@@ -162,14 +193,12 @@ def test_greedy_tokens_with_drafts(config, kv_bits):
 
 
 @BITS
-def test_sampled_tokens_do_not_depend_on_the_drafts(kv_bits):
-    """Drafts without logits: the candidate's own draws, whatever is drafted.
-
-    The forward runs as ever, and then the logits of position p are row p of a
-    table, so that no launch's rounding enters: a draw depends on the order of the
-    probabilities, and random weights leave neighbours closer than a bf16 step, so
-    the tokens of two launches' own logits need not be the same."""
-    eng, _ = _engine(IME, kv_bits)
+@pytest.mark.parametrize("use_graphs", [True, False])
+def test_sampled_tokens_do_not_depend_on_the_drafts(kv_bits, use_graphs):
+    """Drafts without logits: the candidate's own draws, whatever is drafted (on given
+    logits: a draw depends on the order of the probabilities, and random weights leave
+    neighbours closer than a bf16 step)."""
+    eng, _ = _engine(IME, kv_bits, use_graphs=use_graphs)
     rt = eng.rt
     prefix = _ids(IME, 20, 4)
     cfg = CandidateGroupConfig(max_new_tokens=8, min_new_tokens=3, blocked_token_ids=(5, 9),
@@ -177,15 +206,7 @@ def test_sampled_tokens_do_not_depend_on_the_drafts(kv_bits):
     table = 4 * torch.randn(28, IME.vocab_size, generator=torch.Generator().manual_seed(0))
     table[:, [5, 9]] = 30.0  # what the ban keeps out, and would be drawn without it
     table = table.to("cuda", torch.bfloat16)
-    forward = rt.model.forward
-
-    def with_table():
-        b = rt.ctx.batch
-        rows = forward().shape[0]
-        at = b.positions if rows == b.positions.numel() else b.positions[-1:]
-        return table[at.long()]
-
-    rt.model.forward = with_table
+    _give_logits(rt, table)
     uni = stateless_uniforms([cfg.seed], 8, "cuda")
     ban = torch.tensor(cfg.blocked_ids(), dtype=torch.int32, device="cuda")
     want, lps = [], []
@@ -274,3 +295,77 @@ def test_groups_before_and_behind_a_drafted_completion(kv_bits):
                                                             before.raw_candidates]
     assert [s.logprobs for s in eng.score(prefix, [[1, 2, 3], [4]])] == [s.logprobs for s in scores]
     assert eng.rt.cache_manager.available_size == eng.rt.num_pages - 24
+
+
+@CONFIGS
+@BITS
+def test_a_captured_pass_gives_every_path_s_logits(config, kv_bits):
+    """One graph, replayed with trees and lengths of its size and of smaller ones, other
+    work between: every node's logits, and no page written but those handed over."""
+    eng, w = _engine(config, kv_bits)
+    rt = eng.rt
+    ids = _ids(config, 90, 31)
+    for shift, n in ((0, 8), (37, 8), (5, 6), (0, 5), (37, 7)):
+        cached = 40 + shift
+        eng.reset_prefix_cache()
+        eng.score(ids[:cached], [[1, 2]])  # (fills page-table row 0)
+        prefix_pages = eng._prefix_pages
+        g = torch.Generator().manual_seed(shift + n)
+        parents = [-1] + [int(torch.randint(i, (1,), generator=g)) for i in range(1, n)]
+        tokens = _ids(config, n, 50 + n)
+        paths = []
+        for i in range(n):
+            path = [i]
+            while parents[path[0]] >= 0:
+                path.insert(0, parents[path[0]])
+            paths.append(path)
+        graph = eng._draft_graph(cached, n)
+        assert graph is eng._draft_graph(cached + 1, 8) and graph.nodes == 8
+        pages = rt.cache_manager.allocate(8)
+        rt.page_table[0, cached : cached + n] = pages[:n]
+        pool = rt.kv_cache.k_cache(0) if kv_bits == 16 else rt.kv_cache.layer(0)[0].view(torch.uint8)
+        before = pool.clone()
+        with torch.inference_mode():
+            logits, fed = graph.run(tokens, [cached + len(p) - 1 for p in paths], parents,
+                                    cached + n, pages)
+        assert fed.tolist() == tokens
+        logits = logits.float().cpu()
+        other = torch.ones(before.shape[0], dtype=torch.bool, device="cuda")
+        other[pages.long()] = False
+        assert torch.equal(before[other], pool[other])
+        for row, path in enumerate(paths):
+            at = torch.cat((prefix_pages, pages[torch.tensor(path, device="cuda")])).long().cpu()
+            want = _oracle(config, w, rt, ids[:cached] + [tokens[i] for i in path], at)
+            assert (logits[row] - want).abs().max() <= LOGIT_TOL
+        rt.cache_manager._free(pages)
+    assert len(eng._draft_graphs) == 1
+
+
+def test_passes_that_no_graph_holds():
+    """More nodes than a graph takes, more pages than are left, and a kept number of
+    graphs."""
+    eng, w = _engine(IME, 16, num_pages=200)
+    rt = eng.rt
+    assert eng._draft_graph(30, 65) is None and eng._draft_graph(30, 64).nodes == 64
+    prefix = _ids(IME, 30, 2)
+    cfg = CandidateGroupConfig(max_new_tokens=12)
+    tokens = list(eng.complete_drafted(prefix, lambda context, room: None, cfg)
+                  .candidate.token_ids)
+    wide = [[tokens[0] + 1 + i] for i in range(100)]
+    r = eng.complete_drafted(prefix, lambda context, room: draft_tree(
+        wide + [tokens[len(context) - 30 :]], 120), cfg)
+    assert r.drafted > 100
+    _greedy_up_to_rounding(IME, w, prefix, list(r.candidate.token_ids))
+    # 12 nodes: a graph would take 16 pages
+    graphs = list(eng._draft_graphs)
+    held = rt.cache_manager.allocate(rt.cache_manager.available_size - 15)
+    r = eng.complete_drafted(prefix, lambda context, room: draft_tree(
+        [tokens[len(context) - 30 :]]), cfg)
+    assert len(r.candidate.token_ids) == 12 and graphs[0] == list(eng._draft_graphs)[0]
+    _greedy_up_to_rounding(IME, w, prefix, list(r.candidate.token_ids))
+    rt.cache_manager._free(held)
+    assert rt.cache_manager.available_size == rt.num_pages - 30
+    for n in (1, 2, 4, 8, 16, 32, 64):
+        for cached in (10, 300, 600):
+            eng._draft_graph(cached, n)
+    assert len(eng._draft_graphs) == eng.MAX_GRAPHS
