@@ -572,11 +572,11 @@ class CandidateGroupEngine:
         :meth:`complete`'s candidate 0, but for the rounding of other launches.
         Drafts with logits (drawn from them at the sampling temperature) go
         through aios_amd.sample.verify_drafts, which keeps the candidate's
-        distribution; that needs sampling without top_k, top_p and min_new_tokens.  The drafter
-        runs while the engine is locked: it must not call the engine.  Passes of
-        up to MAX_GRAPHED_PREFILL nodes are replayed from graphs.  Of
-        ``config``, max_new_tokens, eos_token_id, sampling, seed, min_new_tokens
-        and blocked_token_ids count."""
+        distribution; that needs sampling without top_k, top_p and
+        min_new_tokens.  The drafter runs while the engine is locked: it must not
+        call the engine.  Passes of up to MAX_GRAPHED_PREFILL nodes are replayed
+        from graphs.  Of ``config``, max_new_tokens, eos_token_id, sampling, seed,
+        min_new_tokens and blocked_token_ids count."""
         config = config or CandidateGroupConfig()
         cancellation = cancellation or self.new_generation()
         config.validate()
