@@ -1937,6 +1937,7 @@ int aios_verify_drafts(const void* logits, int64_t row_stride, const void* draft
   if (row_stride < 0 || (row_stride > 0 && row_stride < vocab) ||
       (draft && (draft_stride < 0 || (draft_stride > 0 && draft_stride < vocab))))
     return fail(AIOS_ERR_INVALID, "verify_drafts: row stride smaller than the vocabulary");
+  if (batch == 0 && total > 0) return fail(AIOS_ERR_INVALID, "verify_drafts: nodes without a request");
   if (batch == 0) return AIOS_OK;
   if (total > (1ll << 24) || vocab > (1 << 30))
     return fail(AIOS_ERR_UNSUPPORTED, "verify_drafts: more than 2^24 nodes or 2^30 ids");

@@ -1308,7 +1308,10 @@ int64_t verify_workspace(int32_t batch, int64_t total, int32_t vocab, bool drawn
 
 bool verify_fits(int32_t batch, int64_t total, int32_t vocab, bool drawn) {
   const Layout l = layout(batch, total, vocab, drawn);
-  return total * 2 * l.segments < 0x7fffffffll && (int64_t)batch * l.walk_wgs < 0x7fffffffll;
+  // (threads of the largest launches: below 2^32)
+  const int64_t most = 0xffffffffll / kVThreads;
+  return total * (drawn ? 2 : 1) * l.segments <= most && (int64_t)batch * l.walk_wgs <= most &&
+         batch <= 0xffffffffll / kVRestThreads;
 }
 
 hipError_t verify_drafts(VerifyArgs a, double temperature, double draft_temperature,

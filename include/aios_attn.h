@@ -759,8 +759,9 @@ int aios_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, in
  * no finite maximum nothing is accepted and the added token is -1 (NaN); with
  * such draft_logits nothing is accepted and the added token is drawn from p.
  * A request without nodes has count 0 and -1 twice; nodes of no request are
- * not accepted, NaN.  Sums and tests in 64 bits.  workspace: 16-byte aligned,
- * aios_verify_workspace(...) bytes (drawn: whether draft_logits are given).
+ * not accepted, NaN (nodes and no request at all: AIOS_ERR_INVALID).  Sums and
+ * tests in 64 bits.  workspace: 16-byte aligned, aios_verify_workspace(...) bytes
+ * (drawn: whether draft_logits are given).
  */
 #define AIOS_VERIFY_MAX_NODES 256
 int64_t aios_verify_workspace(int32_t batch_size, int64_t total_nodes, int32_t vocab,

@@ -69,7 +69,12 @@ def test_c_refusals():
     big = dict(vocab=151936, stride=151936, dstride=151936)
     for kw in ({"ws": None}, {"ws": 72}, {"ws_bytes": 100}):
         assert _call(**big, **kw) == _lib.AIOS_ERR_WORKSPACE, kw
-    assert _call(batch=0, logits=None, ws=None) == OK
+    assert _call(batch=0, total=0, logits=None, ws=None) == OK
+    assert _call(batch=0) == INVALID  # (nodes that no request owns, and no launch to say so)
+    # launches of 2^32 threads and more
+    assert _call(total=1 << 24) == UNSUPPORTED
+    assert _call(total=1 << 23, draft=None, ws=None) == _lib.AIOS_ERR_WORKSPACE
+    assert _call(batch=1 << 23, draft=None) == UNSUPPORTED
 
 
 def test_workspace_sizes():
