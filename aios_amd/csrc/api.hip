@@ -1707,6 +1707,8 @@ struct TreeCost {
   int32_t round;              // a further round of workgroups
   int32_t join, part, state;  // combine, a part of it, 10^5 elements of states
 };
+// (workgroups of 256 threads: below 2^32 threads a launch)
+constexpr int64_t kTreeMostWgs = 0xffffff;
 static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int32_t* cu_k,
                             bool bits8, int32_t cus, int64_t ws_bytes) {
   const int32_t q_tile = p->prefill_q_tile, hkv = p->num_kv_heads, d = p->head_dim;
@@ -1725,7 +1727,7 @@ static void plan_tree_parts(aios_attn_plan_t* p, const int32_t* cu_q, const int3
     const int64_t parts = slots * n;
     const int64_t o_bytes = align_up(parts * rows * d * 2, 256);
     const int64_t bytes = n > 1 ? o_bytes + align_up(parts * rows * 8, 256) : 0;
-    if (bytes > ws_bytes || parts > 0x3fffffff) break;
+    if (bytes > ws_bytes || parts > kTreeMostWgs) break;
     int64_t wgs = 0;
     for (int32_t b = 0; b < p->batch_size; ++b) {
       const int32_t nodes = cu_q[b + 1] - cu_q[b], kv = cu_k[b + 1] - cu_k[b];
@@ -1759,6 +1761,8 @@ int aios_attn_plan_tree(const int32_t* cu_q, const int32_t* cu_k, int32_t batch,
   if (p->max_q_len > aios::kTreeMaxNodes)
     return fail(AIOS_ERR_UNSUPPORTED, "plan_tree: %d nodes exceed the %d of a request",
                 p->max_q_len, aios::kTreeMaxNodes);
+  if ((int64_t)batch * p->num_q_tiles * hkv > kTreeMostWgs)
+    return fail(AIOS_ERR_UNSUPPORTED, "plan_tree: too many tiles for one launch");
   p->phase = kv_bits == 8 ? AIOS_PHASE_TREE8 : AIOS_PHASE_TREE;
   if (p->max_q_len == 0) return AIOS_OK;
   // the fewest tiles of at most 128 MFMA rows, of equal size

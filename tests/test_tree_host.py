@@ -46,6 +46,9 @@ def test_plan_refusals():
     assert _plan([3], [5], hq=15)[0] == INVALID
     assert _plan([3], [5], d=80)[0] == UNSUPPORTED
     assert _plan([3], [-1])[0] == INVALID  # fewer positions than nodes
+    many = torch.arange((1 << 21) + 1, dtype=torch.int32)  # 2^24 tiles: 2^32 threads
+    with pytest.raises(ValueError, match="too many tiles"):
+        paged.plan("tree", many, many, 8, 8, 64)
     for kw in ({"shared_prefix_len": 4}, {"prefix_chunk_len": 64}, {"suffix_split_len": 64}):
         with pytest.raises(ValueError, match="takes no shared prefix"):
             paged.plan("tree", [0, 3], [0, 8], 16, 8, 128, **kw)
