@@ -408,3 +408,26 @@ def test_values_nobody_sees_in_a_shared_part(bits):
         k, v = k.copy(), np.where(np.isfinite(v), v, 0.0)
     c.check(out, k, v)
     assert torch.isfinite(out).all()
+
+
+@BITS
+def test_pages_at_the_end_of_the_largest_pool(bits):
+    """Rows next to 4 GiB into a layer's cache: offsets past 31 bits."""
+    c = Case([9, 5], [300, 40], 16, 8, 128, bits, seed=5)
+    small, k, v = c.cache()
+    pages = (2_097_000 if bits == 16 else 4_194_000)
+    assert pages * 8 * 128 * (2 if bits == 16 else 1) > 0.999 * 2 ** 32
+    at = pages - c.pages
+    cache = []
+    for t in small[:2]:
+        big = torch.empty((pages, *t.shape[1:]), dtype=t.dtype, device=DEV)
+        big[at:] = t
+        cache.append(big)
+    if bits == 8:
+        scales = torch.empty((8, pages, 2), dtype=torch.bfloat16, device=DEV)
+        scales[:, at:] = small[2]
+        cache.append(scales)
+    c.indices += at
+    out = c.call(cache)
+    c.indices -= at
+    c.check(out, k, v)

@@ -365,3 +365,14 @@ def test_the_first_token_is_distributed_as_the_target_s(mode, kids):
     freq = torch.bincount(first, minlength=vocab).double() / b
     assert ((freq - p).abs() <= 5 * (p * (1 - p) / b).sqrt()).all(), (freq, p)
     assert 0.05 < (last > 0).double().mean() < 1
+
+
+@MODES
+@pytest.mark.parametrize("vocab", [5003, 40009])
+def test_rows_past_32_bits(mode, vocab):
+    c = Case([4, 2], 1, vocab, BF16, mode, seed=vocab)
+    step = 700_000_000  # the last row is 3.5e9 elements behind the first
+    far = lambda x: torch.empty(5 * step + vocab, dtype=x.dtype, device=DEV).as_strided(
+        (6, vocab), (step, 1)).copy_(x)
+    kw = {} if c.draft is None else {"draft_logits": far(c.draft)}
+    c.check(c.call(logits=far(c.logits), **kw))
